@@ -51,6 +51,10 @@ extern "C" {
 #define QDL_BORN_E_TABLE (-10)
 #define QDL_BORN_E_ROPEDIM (-11)
 #define QDL_BORN_E_SCRATCH (-12)
+#define QDL_BORN_E_HEADS (-13)
+#define QDL_BORN_E_STRIDE (-14)
+#define QDL_BORN_E_PAGE (-15)
+#define QDL_BORN_E_BUDGET (-16)
 
 /* Size of the fixed device array qdl_flash_born_bwd_noalloc takes its
  * workspace from (one per GPU): 16 MiB, enough for B * H * T up to about
@@ -331,6 +335,163 @@ int qdl_flash_born_fwd_qk_prologue(int dtype, int64_t B, int64_t H, int64_t T,
                                    float *z, void *q_out, void *k_out,
                                    float *q_rinv, float *k_rinv,
                                    qdl_stream_t stream);
+
+/*
+ * Packed sequences with grouped heads: q, out, dout, dq are (n_q, H, D) rows of
+ * tokens, k, v, dk, dv (n_k, h_kv, D), and `sequences` sequences share them:
+ * sequence s owns the query rows cu_q[s] .. cu_q[s+1] - 1 and the key rows
+ * cu_k[s] .. cu_k[s+1] - 1 (sequences + 1 int32 starts each in device memory,
+ * never decreasing, the first 0, values past the rows are cut).  H is a
+ * multiple of h_kv; query head h reads key head h / (H / h_kv).  Query i of a
+ * sequence of len_q queries and len_k keys stands at position
+ * i + len_k - len_q: causality shows it the keys up to its position, a window
+ * those less than window_size before it.  Rows that see no key, and rows behind
+ * the last sequence, have zero outputs and gradients.
+ *
+ * q, k, v, dout have unit stride along D and *_strides (token, head) in
+ * elements, multiples of 16 bytes (a token's at least D, under 2^24 bytes);
+ * out, dq, dk, dv are contiguous; z is (H, n_q) fp32.  scale == NULL takes
+ * scale_value.  The weights of fp16 rows are scaled by a power of two of the
+ * row's own, so overlaps of any size keep their weight.
+ * The backward's dk and dv are summed over the heads of a group in a fixed
+ * order; dscale == NULL: not wanted.  struct_bytes: sizeof the block.
+ */
+typedef struct qdl_born_packed_call {
+    int64_t struct_bytes;
+    int64_t dtype, sequences, n_q, n_k, H, h_kv, D;
+    const void *q, *k, *v;
+    int64_t q_strides[2], k_strides[2], v_strides[2];
+    void *out; /* written by the forward, read by the backward */
+    float *z;
+    const int32_t *cu_q, *cu_k;
+    const float *scale;
+    int64_t n_scale;
+    double scale_value;
+    int64_t is_causal, window_size;
+    double eps;
+    /* backward */
+    const void *dout;
+    int64_t dout_strides[2];
+    void *dq, *dk, *dv;
+    float *dscale;
+    void *workspace;
+    int64_t workspace_bytes;
+} qdl_born_packed_call;
+
+int qdl_flash_born_packed_forward_call(const qdl_born_packed_call *call, qdl_stream_t stream);
+int64_t qdl_flash_born_packed_workspace_size(int64_t n_q, int64_t H);
+int qdl_flash_born_packed_backward_call(const qdl_born_packed_call *call, qdl_stream_t stream);
+
+/*
+ * A paged cache: k_cache, v_cache hold cache_pages pages of page_size tokens of
+ * h_kv heads of D values, *_cache_strides (page, token, head) in elements,
+ * multiples of 16 bytes, unit stride along D.  Key j of sequence b is token
+ * j % page_size of page block_table[b * table_ld + j / page_size] (int32 in
+ * device memory, `pages` columns).  A table entry outside [0, cache_pages) is a
+ * missing page: its keys are not seen, nothing is written to it.
+ * cache_lens: int32 tokens of each sequence, cut to what its table holds.
+ */
+
+/*
+ * Attention of one new token per sequence: q (B, H, D) with strides (sequence,
+ * head), out (B, H, D) contiguous.  The token is the last of its sequence's
+ * cache_lens keys and sees all of them, or the last window_size.  The keys are
+ * split over workgroups and joined in order; the workspace's size is the size
+ * function's for the same block.
+ * key_weight != NULL: (B, h_kv, weight_len) fp32 with weight_strides (sequence,
+ * head), to which the sum over the group's heads of p_j / Z is added for every
+ * visible key j < weight_len.
+ */
+typedef struct qdl_born_paged_call {
+    int64_t struct_bytes;
+    int64_t dtype, B, H, h_kv, D;
+    const void *q;
+    int64_t q_strides[2];
+    void *out;
+    const void *k_cache, *v_cache;
+    int64_t k_cache_strides[3], v_cache_strides[3];
+    int64_t cache_pages, page_size;
+    const int32_t *block_table;
+    int64_t pages, table_ld;
+    const int32_t *cache_lens;
+    const float *scale;
+    int64_t n_scale;
+    double scale_value;
+    int64_t window_size;
+    double eps;
+    float *key_weight;
+    int64_t weight_strides[2], weight_len;
+    void *workspace;
+    int64_t workspace_bytes;
+} qdl_born_paged_call;
+
+int64_t qdl_flash_born_paged_workspace_size(const qdl_born_paged_call *call);
+int qdl_flash_born_paged_forward_call(const qdl_born_paged_call *call, qdl_stream_t stream);
+
+/*
+ * Append: n tokens' queries (n, H, D), keys and values (n, h_kv, D), strides
+ * (token, head).  The queries and keys are rotated by row positions[t] of the
+ * tables (NULL: the token's slot; rows past the tables take their last) and
+ * normalised, x' = y / sqrt(sum y^2 + eps), in fp32 and rounded once; q_out is
+ * (n, H, D) contiguous, the keys and the values go to their slots of the cache.
+ * cu_seqlens: B + 1 starts of the sequences' new tokens, or NULL: one each
+ * (n == B).  cache_lens counts the new tokens, so token t of sequence s goes to
+ * slot cache_lens[s] - (cu_seqlens[s+1] - t).  Tokens of no sequence have zero
+ * queries; slots without a page are not written.  cos_table NULL: no rotation;
+ * tables and n_freq as for the Q/K prologue, table_rows rows.  D: a multiple of 8.
+ */
+typedef struct qdl_born_append_call {
+    int64_t struct_bytes;
+    int64_t dtype, n, B, H, h_kv, D;
+    const void *q, *k, *v;
+    int64_t q_strides[2], k_strides[2], v_strides[2];
+    void *q_out;
+    void *k_cache, *v_cache;
+    int64_t k_cache_strides[3], v_cache_strides[3];
+    int64_t cache_pages, page_size;
+    const int32_t *block_table;
+    int64_t pages, table_ld;
+    const int32_t *cache_lens, *cu_seqlens;
+    const float *cos_table, *sin_table;
+    int64_t table_rows, n_freq, freq_ld;
+    const int32_t *positions;
+    double eps;
+} qdl_born_append_call;
+
+int qdl_flash_born_cache_append_call(const qdl_born_append_call *call, qdl_stream_t stream);
+
+/*
+ * Evict: every sequence longer than `budget` keeps, for each key head, its last
+ * min(recent, budget) keys and of the others those with the greatest
+ * key_weight, budget in all, ties to the lowest index (NaN above all numbers;
+ * keys at weight_len and after have weight 0).  They keep their order.
+ * kept (B, h_kv, budget): the kept keys' old slots, -1 behind the last;
+ * weight_out (B, h_kv, weight_len): their weights, 0 behind the last;
+ * lens_out (B): min(cache_lens, budget).
+ * The kept rows of K and V move to slots 0, 1, ... of out_table's pages
+ * (out_pages columns), none of which may be a page of block_table, or, with
+ * out_table NULL, of block_table's own.  Rows behind the last kept one stay as
+ * they were; a row kept from a missing page arrives as zeros.
+ */
+typedef struct qdl_born_evict_call {
+    int64_t struct_bytes;
+    int64_t dtype, B, h_kv, D;
+    void *k_cache, *v_cache;
+    int64_t k_cache_strides[3], v_cache_strides[3];
+    int64_t cache_pages, page_size;
+    const int32_t *block_table;
+    int64_t pages, table_ld;
+    const int32_t *cache_lens;
+    const float *key_weight;
+    int64_t weight_strides[2], weight_len;
+    int64_t budget, recent;
+    const int32_t *out_table;
+    int64_t out_pages, out_table_ld;
+    float *weight_out;
+    int32_t *lens_out, *kept;
+} qdl_born_evict_call;
+
+int qdl_flash_born_cache_evict_call(const qdl_born_evict_call *call, qdl_stream_t stream);
 
 #ifdef __cplusplus
 }

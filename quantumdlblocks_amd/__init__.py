@@ -9,10 +9,14 @@ from .kernels import (
     HAS_HIP_KERNELS,
     HAS_TRITON,
     IS_HIP,
+    born_cache_evict,
     flash_born_attention,
+    flash_born_attention_packed,
+    flash_born_attention_paged,
     flash_born_attention_qk_prologue,
     flash_purified_born_attention,
     fused_qk_rope_l2_normalize,
+    fused_qk_rope_l2_normalize_append,
     get_flash_born_launch_meta,
     get_mi355x_launch_meta,
     get_rdna4_autotune_configs,
@@ -25,11 +29,15 @@ __all__ = [
     "HAS_TRITON",
     "IS_HIP",
     "apply_unitary_rope",
+    "born_cache_evict",
     "compute_document_ids",
     "flash_born_attention",
+    "flash_born_attention_packed",
+    "flash_born_attention_paged",
     "flash_born_attention_qk_prologue",
     "flash_purified_born_attention",
     "fused_qk_rope_l2_normalize",
+    "fused_qk_rope_l2_normalize_append",
     "get_flash_born_launch_meta",
     "get_mi355x_launch_meta",
     "get_rdna4_autotune_configs",

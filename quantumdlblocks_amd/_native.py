@@ -42,6 +42,13 @@ EXPORTED_SYMBOLS = (
     "qdl_flash_born_qk_prologue_fwd",
     "qdl_flash_born_qk_prologue_bwd",
     "qdl_flash_born_fwd_qk_prologue",
+    "qdl_flash_born_packed_forward_call",
+    "qdl_flash_born_packed_workspace_size",
+    "qdl_flash_born_packed_backward_call",
+    "qdl_flash_born_paged_workspace_size",
+    "qdl_flash_born_paged_forward_call",
+    "qdl_flash_born_cache_append_call",
+    "qdl_flash_born_cache_evict_call",
 )
 
 
@@ -64,6 +71,21 @@ def pack_call(dtype, B, H, T, D, q, k, v, out, z, scale, n_scale, scale_value, d
     return _CALL.pack(_CALL.size, dtype, B, H, T, D, q, k, v, out, z, scale, n_scale, scale_value, doc, causal, window,
                       eps, purified, tau, n_tau, tau_value, eps_base, out16, param_grads, dout, dq, dk, dv, dscale, dtau, workspace,
                       workspace_bytes, *prologue)
+
+
+class _Block(struct.Struct):
+    """An argument block of the packed, paged and cache entry points: every
+    field 8 bytes ("q" integers and addresses, "d" doubles), its size first."""
+
+    def __call__(self, *fields) -> bytes:
+        return self.pack(self.size, *fields)
+
+
+# Fields in the order of include/qdl_flash_born.h.
+packed_call = _Block("@" + "q" * 8 + "q" * 3 + "q" * 6 + "qq" + "qq" + "qqd" + "qq" + "d" + "q" * 3 + "q" * 3 + "q" * 3)
+paged_call = _Block("@" + "q" * 6 + "q" * 4 + "q" * 8 + "qq" + "qqq" + "q" + "qqd" + "qd" + "q" * 4 + "qq")
+append_call = _Block("@" + "q" * 7 + "q" * 3 + "q" * 6 + "q" + "q" * 8 + "qq" + "qqq" + "qq" + "q" * 5 + "qd")
+evict_call = _Block("@" + "q" * 5 + "q" * 8 + "qq" + "qqq" + "q" + "q" * 4 + "qq" + "qqq" + "qqq")
 
 
 _lock = threading.Lock()
@@ -112,6 +134,15 @@ def _bind(lib: ctypes.CDLL) -> None:
     for call in (lib.qdl_flash_born_forward_call, lib.qdl_flash_born_backward_call):
         call.restype = _int
         call.argtypes = [ctypes.c_char_p, _ptr]  # the packed qdl_born_call, stream
+    for call in (lib.qdl_flash_born_packed_forward_call, lib.qdl_flash_born_packed_backward_call,
+                 lib.qdl_flash_born_paged_forward_call, lib.qdl_flash_born_cache_append_call,
+                 lib.qdl_flash_born_cache_evict_call):
+        call.restype = _int
+        call.argtypes = [ctypes.c_char_p, _ptr]  # the packed argument block, stream
+    lib.qdl_flash_born_packed_workspace_size.restype = _i64
+    lib.qdl_flash_born_packed_workspace_size.argtypes = [_i64, _i64]
+    lib.qdl_flash_born_paged_workspace_size.restype = _i64
+    lib.qdl_flash_born_paged_workspace_size.argtypes = [ctypes.c_char_p]
     lib.qdl_flash_purified_born_fwd.restype = _int
     lib.qdl_flash_purified_born_fwd.argtypes = [
         _int, _i64, _i64, _i64, _i64,      # dtype, B, H, T, D

@@ -1,0 +1,433 @@
+// The paged key-value cache: appending a step's keys and values, with the
+// rotation and normalisation of its queries and keys, and evicting the keys
+// that the accumulated attention weighs least.
+#pragma once
+
+#include <type_traits>
+
+#include "born_common.h"
+#include "born_packed.h"
+
+namespace qdl {
+
+// ---------------------------------------------------------------------------
+// Append.  A row (one head of one token) belongs to a group of `lpr` lanes, a
+// power of two; lane i of it owns VEC columns of the first half and the
+// matching ones of the second, both members of its rotation pairs:
+//   y1 = x1 c - x2 s, y2 = x1 s + x2 c, out = y / sqrt(sum y^2 + eps),
+// in fp32 from the 16-bit inputs on, rounded once.  Bound by memory: rows read
+// and written once.  A group takes ROWS rows of one token, so that the token's
+// angles are read once for them; single tokens take one row each (ROWS = 1),
+// where lanes and not bytes are short.
+// ---------------------------------------------------------------------------
+struct AppendArgs {
+    const void *q, *k, *v;
+    void *q_out, *k_cache, *v_cache;
+    const float *cos, *sin;
+    const int32_t* positions;  // (N) rows of the tables, or nullptr: the slot
+    const int32_t* table;
+    const int32_t* lens;       // (B), the appended tokens included
+    const int32_t* cu;         // B + 1 starts, or nullptr: one token per sequence
+    int N, B, H, Hkv, D;
+    int pages, page, page_shift;
+    int64_t table_ld, cache_pages;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, kp, kt, kh, vp, vt, vh;  // bytes
+    int table_rows, n_freq;
+    int64_t freq_ld;
+    float eps;
+    int lpr;
+};
+
+template <class E, int VEC>
+struct RowVec {
+    static constexpr int W = VEC * kItem<E> / 4;  // dwords
+    uint32_t u[W];
+    __device__ __forceinline__ void load(const uint8_t* p) {
+        if constexpr (W == 4) {
+            const u32x4 x = ldg16(p);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) u[i] = x[i];
+        } else {
+            const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+            u[0] = x[0];
+            u[1] = x[1];
+        }
+    }
+    __device__ __forceinline__ void store(uint8_t* p) const {
+        if constexpr (W == 4) {
+            const u32x4 x = {u[0], u[1], u[2], u[3]};
+            *reinterpret_cast<u32x4*>(p) = x;
+        } else {
+            const u32x2 x = {u[0], u[1]};
+            *reinterpret_cast<u32x2*>(p) = x;
+        }
+    }
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (std::is_same<E, F32>::value) return __uint_as_float(u[i]);
+        else return (i & 1) ? E::hi(u[i >> 1]) : E::lo(u[i >> 1]);
+    }
+    __device__ __forceinline__ void set(const float (&x)[VEC]) {
+        if constexpr (std::is_same<E, F32>::value) {
+#pragma unroll
+            for (int i = 0; i < VEC; ++i) u[i] = __float_as_uint(x[i]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < VEC / 2; ++i) u[i] = E::pack(x[2 * i], x[2 * i + 1]);
+        }
+    }
+};
+
+template <class E, int VEC, int ROWS>
+__global__ __launch_bounds__(256) void born_append_kernel(AppendArgs p) {
+    const int all = p.H + 2 * p.Hkv, groups = (all + ROWS - 1) / ROWS;
+    const int64_t item = (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr;
+    const int lane = threadIdx.x & (p.lpr - 1);
+    if (item >= (int64_t)p.N * groups) return;
+    const int t = (int)(item / groups), r0 = (int)(item % groups) * ROWS;
+    const int half = p.D >> 1;
+    const bool own = lane * VEC < half;  // lanes of a group past the row's chunks
+    const int o1 = lane * VEC * kItem<E>, o2 = o1 + half * kItem<E>;
+
+    // The token's sequence, slot and row of the cache.
+    int s = t, first = t, last = t + 1;
+    bool in = t < p.B;
+    if (p.cu != nullptr) {
+        int lo = 0, hi = p.B;  // the last start at or before t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.cu[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        s = lo;
+        in = p.B > 0;
+        if (in) {
+            first = max(p.cu[s], 0);
+            last = p.cu[s + 1];
+            in = t >= first && t < last;
+        }
+    }
+    int64_t slot = -1, page = -1;
+    int row = 0;
+    if (in) {
+        slot = (int64_t)p.lens[s] - (last - t);
+        if (slot >= 0 && slot < (int64_t)p.pages * p.page) {
+            const int i = p.page_shift >= 0 ? (int)slot >> p.page_shift : (int)slot / p.page;
+            row = (int)slot - i * p.page;
+            page = p.table[(int64_t)s * p.table_ld + i];
+        }
+    }
+    const bool kept = page >= 0 && page < p.cache_pages;
+
+    float c[VEC], sn[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c[i] = 1.f, sn[i] = 0.f;
+    if (p.cos != nullptr && own && r0 < p.H + p.Hkv) {
+        int64_t at = p.positions != nullptr ? p.positions[t] : slot;
+        at = min(max(at, (int64_t)0), (int64_t)p.table_rows - 1) * p.freq_ld;  // rows past the tables: their last
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int f = lane * VEC + i;
+            if (f < p.n_freq) c[i] = p.cos[at + f], sn[i] = p.sin[at + f];
+        }
+    }
+    RowVec<E, VEC> x1[ROWS], x2[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i;
+        if (r >= all || !own) continue;
+        const uint8_t* src = r < p.H          ? (const uint8_t*)p.q + (int64_t)t * p.q_st + (int64_t)r * p.q_sh
+                             : r < p.H + p.Hkv ? (const uint8_t*)p.k + (int64_t)t * p.k_st + (int64_t)(r - p.H) * p.k_sh
+                                               : (const uint8_t*)p.v + (int64_t)t * p.v_st + (int64_t)(r - p.H - p.Hkv) * p.v_sh;
+        x1[i].load(src + o1);
+        x2[i].load(src + o2);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        const int r = r0 + i;
+        if (r >= all) continue;  // uniform in the group
+        if (r >= p.H + p.Hkv) {
+            if (kept && own) {
+                uint8_t* to = (uint8_t*)p.v_cache + page * p.vp + (int64_t)row * p.vt + (int64_t)(r - p.H - p.Hkv) * p.vh;
+                x1[i].store(to + o1);
+                x2[i].store(to + o2);
+            }
+            continue;
+        }
+        float y1[VEC], y2[VEC], ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float a = own ? x1[i].get(e) : 0.f, b = own ? x2[i].get(e) : 0.f;
+            y1[e] = a * c[e] - b * sn[e];
+            y2[e] = a * sn[e] + b * c[e];
+            ss = fmaf(y1[e], y1[e], fmaf(y2[e], y2[e], ss));
+        }
+        for (int o = 1; o < p.lpr; o <<= 1) ss += __shfl_xor(ss, o);
+        float f = 1.0f / sqrtf(ss + p.eps);
+        uint8_t* to;
+        bool write = own;
+        if (r < p.H) {
+            to = (uint8_t*)p.q_out + ((int64_t)t * p.H + r) * p.D * kItem<E>;
+        } else {
+            to = (uint8_t*)p.k_cache + page * p.kp + (int64_t)row * p.kt + (int64_t)(r - p.H) * p.kh;
+            write = write && kept;
+        }
+        if (!write) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            // A token of no sequence has a zero query.
+            y1[e] = in ? y1[e] * f : 0.f;
+            y2[e] = in ? y2[e] * f : 0.f;
+        }
+        x1[i].set(y1);
+        x2[i].set(y2);
+        x1[i].store(to + o1);
+        x2[i].store(to + o2);
+    }
+}
+
+// ---------------------------------------------------------------------------
+// Evict.  Two launches: the selection, one workgroup for a (sequence, key
+// head), and the move of the kept rows.
+//
+// Selection: the `want` greatest weights among the keys before the recent
+// ones, ties to the lowest index: a radix selection over the order-preserving
+// 32-bit forms of the weights, four histograms of 8 bits, then one pass that
+// counts the kept ones before each key.  A thread holds 16 weights, so up to
+// 16384 keys are read once.
+// ---------------------------------------------------------------------------
+struct EvictArgs {
+    void *k, *v;
+    const int32_t *table, *to;  // (B, pages), (B, to_pages)
+    const int32_t* lens;
+    const float* weight;
+    float* weight_out;          // (B, Hkv, w_len)
+    int32_t *lens_out, *kept;   // (B), (B, Hkv, budget)
+    int B, Hkv, D, item;
+    int pages, to_pages, page, page_shift;
+    int64_t table_ld, to_ld, cache_pages;
+    int64_t kp, kt, kh, vp, vt, vh;  // bytes
+    int64_t w_sb, w_sh;              // elements
+    int w_len, budget, recent;
+};
+
+__device__ __forceinline__ int evict_len(const EvictArgs& p, int b) {
+    return (int)min((int64_t)max(p.lens[b], 0), (int64_t)p.pages * p.page);
+}
+
+// Unsigned order of floats; every NaN above all numbers, -0 equal to 0.
+__device__ __forceinline__ uint32_t evict_key(float x) {
+    const uint32_t u = __float_as_uint(x + 0.f);
+    if ((u & 0x7fffffffu) > 0x7f800000u) return 0xffffffffu;
+    return (u & 0x80000000u) ? ~u : u | 0x80000000u;
+}
+
+constexpr int kEvictThreads = 1024, kEvictPer = 16, kEvictSpan = kEvictThreads * kEvictPer;
+
+template <int>
+__global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictArgs p) {
+    constexpr int NW = kEvictThreads / 64;
+    __shared__ uint32_t hist[NW][256];
+    __shared__ uint32_t s_prefix, s_left;
+    __shared__ uint32_t counts[kEvictPer * NW];  // kept for sure | ties << 16, per 64 keys
+    __shared__ uint32_t s_total;
+    const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int n = evict_len(p, b), m = min(n, p.budget);
+    const float* w = p.weight + (int64_t)b * p.w_sb + (int64_t)hk * p.w_sh;
+    float* wo = p.weight_out + ((int64_t)b * p.Hkv + hk) * p.w_len;
+    int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
+    if (hk == 0 && tid == 0) p.lens_out[b] = m;
+    for (int i = m + tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
+    for (int i = m + tid; i < p.w_len; i += kEvictThreads) wo[i] = 0.f;
+    const int tail = n > m ? min(p.recent, m) : m;
+    const int old = n - tail, want = m - tail;  // of the `old` first keys, `want` stay
+    for (int i = tid; i < tail; i += kEvictThreads) {
+        kept[want + i] = old + i;
+        if (want + i < p.w_len) wo[want + i] = old + i < p.w_len ? w[old + i] : 0.f;
+    }
+    if (want == 0) return;
+
+    const int spans = (old + kEvictSpan - 1) / kEvictSpan;
+    float x[kEvictPer];
+    uint32_t key[kEvictPer];
+    auto load = [&](int span) {
+#pragma unroll
+        for (int i = 0; i < kEvictPer; ++i) {
+            const int j = span * kEvictSpan + i * kEvictThreads + tid;
+            x[i] = j < old && j < p.w_len ? w[j] : 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < kEvictPer; ++i) key[i] = evict_key(x[i]);
+    };
+    load(0);
+    if (tid == 0) s_prefix = 0, s_left = want;
+    // The want-th greatest key, 8 bits at a time.
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        for (int i = tid; i < NW * 256; i += kEvictThreads) hist[i >> 8][i & 255] = 0;
+        __syncthreads();
+        const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+        for (int sp = 0; sp < spans; ++sp) {
+            if (spans > 1) load(sp);
+#pragma unroll
+            for (int i = 0; i < kEvictPer; ++i) {
+                const int j = sp * kEvictSpan + i * kEvictThreads + tid;
+                if (j < old && (key[i] & mask) == prefix) atomicAdd(&hist[wave][(key[i] >> shift) & 255u], 1u);
+            }
+        }
+        __syncthreads();
+        if (wave == 0) {
+            // Lane l: bins 255 - 4 l .. 252 - 4 l, from the greatest down.
+            uint32_t c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                c[i] = 0;
+                for (int v = 0; v < NW; ++v) c[i] += hist[v][255 - 4 * lane - i];
+                sum += c[i];
+            }
+            uint32_t above = sum;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(above, o);
+                if (lane >= o) above += y;
+            }
+            above -= sum;
+            const uint32_t left = s_left;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                if (above < left && left <= above + c[i]) {
+                    s_prefix = prefix | ((uint32_t)(255 - 4 * lane - i) << shift);
+                    s_left = left - above;
+                }
+                above += c[i];
+            }
+        }
+        __syncthreads();
+    }
+    const uint32_t cut = s_prefix, ties = s_left;  // keys above the cut stay, and the first `ties` equal to it
+
+    uint32_t before_gt = 0, before_eq = 0;
+    for (int sp = 0; sp < spans; ++sp) {
+        if (spans > 1) load(sp);
+        uint64_t gt[kEvictPer], eq[kEvictPer];
+#pragma unroll
+        for (int i = 0; i < kEvictPer; ++i) {
+            const int j = sp * kEvictSpan + i * kEvictThreads + tid;
+            gt[i] = __ballot(j < old && key[i] > cut);
+            eq[i] = __ballot(j < old && key[i] == cut);
+            if (lane == 0) counts[i * NW + wave] = (uint32_t)__popcll(gt[i]) | ((uint32_t)__popcll(eq[i]) << 16);
+        }
+        __syncthreads();
+        if (wave == 0) {  // exclusive sums, 4 counts a lane (sums up to 16384 fit 16 bits)
+            uint32_t c[4], sum = 0;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) c[i] = counts[4 * lane + i], sum += c[i];
+            uint32_t run = sum;
+            for (int o = 1; o < 64; o <<= 1) {
+                const uint32_t y = __shfl_up(run, o);
+                if (lane >= o) run += y;
+            }
+            if (lane == 63) s_total = run;
+            run -= sum;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                counts[4 * lane + i] = run;
+                run += c[i];
+            }
+        }
+        __syncthreads();
+        const uint64_t below = (1ull << lane) - 1;
+#pragma unroll
+        for (int i = 0; i < kEvictPer; ++i) {
+            const int j = sp * kEvictSpan + i * kEvictThreads + tid;
+            const uint32_t c = counts[i * NW + wave];
+            const uint32_t g = before_gt + (c & 0xffffu) + (uint32_t)__popcll(gt[i] & below);
+            const uint32_t e = before_eq + (c >> 16) + (uint32_t)__popcll(eq[i] & below);
+            const bool is_gt = (gt[i] >> lane) & 1, is_eq = (eq[i] >> lane) & 1;
+            if (is_gt || (is_eq && e < ties)) {
+                const int to = (int)(g + min(e, ties));
+                kept[to] = j;
+                if (to < p.w_len) wo[to] = x[i];
+            }
+        }
+        before_gt += s_total & 0xffffu;
+        before_eq += s_total >> 16;
+        __syncthreads();
+    }
+}
+
+static_assert(kEvictPer * (kEvictThreads / 64) == 256, "the counts of one span are scanned by one wave");
+
+__device__ __forceinline__ int64_t evict_at(const EvictArgs& p, const int32_t* table, int pages, int j, int64_t sp, int64_t st) {
+    const int i = p.page_shift >= 0 ? j >> p.page_shift : j / p.page;
+    const int64_t page = i < pages ? table[i] : -1;
+    return page >= 0 && page < p.cache_pages ? page * sp + (int64_t)(j - i * p.page) * st : -1;
+}
+
+// The kept rows to other pages: 16 bytes a lane, K and V of kEvictRows rows
+// per workgroup.  A row whose page is missing arrives as zeros.
+constexpr int kEvictRows = 64;
+
+template <int>
+__global__ __launch_bounds__(256) void born_evict_move_kernel(EvictArgs p) {
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
+    const int b = rest % p.B, tile = rest / p.B;
+    const int m = min(evict_len(p, b), p.budget);
+    const int cpr = p.D * p.item / 16;
+    const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
+    const int32_t *from = p.table + (int64_t)b * p.table_ld, *to = p.to + (int64_t)b * p.to_ld;
+    const int r1 = min(kEvictRows, m - tile * kEvictRows);
+    for (int x = threadIdx.x; x < r1 * cpr; x += 256) {
+        const int i = tile * kEvictRows + x / cpr, o = 16 * (x % cpr);
+        const int j = kept[i];
+#pragma unroll
+        for (int which = 0; which < 2; ++which) {
+            uint8_t* cache = (uint8_t*)(which ? p.v : p.k) + (int64_t)hk * (which ? p.vh : p.kh) + o;
+            const int64_t sp = which ? p.vp : p.kp, st = which ? p.vt : p.kt;
+            const int64_t a = evict_at(p, from, p.pages, j, sp, st), d = evict_at(p, to, p.to_pages, i, sp, st);
+            u32x4 y = {0u, 0u, 0u, 0u};
+            if (a >= 0) y = ldg16(cache + a);
+            if (d >= 0) *reinterpret_cast<u32x4*>(cache + d) = y;
+        }
+    }
+}
+
+// The kept rows to the front of their own pages.  Rows only move down and keep
+// their order, so one workgroup per (sequence, key head, K or V) walks them
+// upwards: a batch is read whole before any of it is written, and what it
+// writes lies below every row still to be read.
+template <int>
+__global__ __launch_bounds__(1024) void born_evict_compact_kernel(EvictArgs p) {
+    constexpr int U = 4;
+    const int which = blockIdx.x & 1, hk = (blockIdx.x >> 1) % p.Hkv, b = (blockIdx.x >> 1) / p.Hkv;
+    const int m = min(evict_len(p, b), p.budget);
+    const int cpr = p.D * p.item / 16, rows = 1024 / cpr;  // whole rows per round of the workgroup
+    const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
+    const int32_t* table = p.table + (int64_t)b * p.table_ld;
+    const int mine = threadIdx.x / cpr, o = 16 * (threadIdx.x % cpr);
+    uint8_t* cache = (uint8_t*)(which ? p.v : p.k) + (int64_t)hk * (which ? p.vh : p.kh) + o;
+    const int64_t sp = which ? p.vp : p.kp, st = which ? p.vt : p.kt;
+    for (int i0 = 0; i0 < m; i0 += U * rows) {
+        u32x4 y[U];
+        int64_t d[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * rows + mine;
+            d[u] = -1;
+            y[u] = u32x4{0u, 0u, 0u, 0u};
+            if (mine < rows && i < m) {
+                const int j = kept[i];
+                if (j != i) {
+                    d[u] = evict_at(p, table, p.pages, i, sp, st);
+                    const int64_t a = evict_at(p, table, p.pages, j, sp, st);
+                    if (a >= 0) y[u] = ldg16(cache + a);
+                }
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (d[u] >= 0) *reinterpret_cast<u32x4*>(cache + d[u]) = y[u];
+        __syncthreads();
+    }
+}
+
+}  // namespace qdl

@@ -106,6 +106,10 @@ const char* qdl_flash_born_strerror(int code) {
         case QDL_BORN_E_SCRATCH:
             return "problem needs more backward workspace than the fixed 16 MiB array of "
                    "qdl_flash_born_bwd_noalloc (use qdl_flash_born_bwd with a caller workspace)";
+        case QDL_BORN_E_HEADS: return "the query heads must be a multiple of the key heads";
+        case QDL_BORN_E_STRIDE: return "row strides must be multiples of 16 bytes, at least a row and under 2^24 bytes";
+        case QDL_BORN_E_PAGE: return "page size, table or cache size out of range";
+        case QDL_BORN_E_BUDGET: return "budget and recent must be at least 0 and within 2^30";
         default: break;
     }
     if (code > 0) return hipGetErrorString((hipError_t)code);

@@ -1,0 +1,15 @@
+// Packed Born attention, F32 inputs.
+#include "born_packed.h"
+
+namespace qdl {
+
+template <>
+hipError_t packed_fwd<F32>(const PackedArgs& a, hipStream_t st) {
+    return launch_packed_fwd<F32>(a, st);
+}
+template <>
+hipError_t packed_bwd<F32>(const PackedArgs& a, hipStream_t st) {
+    return launch_packed_bwd<F32>(a, st);
+}
+
+}  // namespace qdl

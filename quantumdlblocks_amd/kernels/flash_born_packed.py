@@ -1,0 +1,206 @@
+"""Flash-Born attention over packed sequences with grouped heads, forward and
+backward: the ragged form of ``flash_born_attention``.
+
+Several sequences of different lengths share rows of tokens, ``q`` (N, H, D) and
+``k``, ``v`` (M, Hkv, D) with ``H`` a multiple of ``Hkv``: sequence s owns query
+rows ``cu_seqlens_q[s] : cu_seqlens_q[s + 1]`` and key rows likewise, and query
+head h reads key head ``h // (H // Hkv)``.  Per sequence, with len_q queries
+standing at the last len_q of len_k positions,
+
+    a_ij = max(0, scale_h * q_i . k_j) * M_ij,   p_ij = a_ij ** 2
+    O_i  = sum_j p_ij v_j / (sum_j p_ij + eps)
+    M_ij = [causal => j <= i + len_k - len_q]
+           & [window_size > 0 => i + len_k - len_q - j < window_size]
+
+Rows that see no key are zero, and so are their gradients.
+
+GPU tensors with head dim <= 256 run the HIP kernels; CPU tensors and larger
+head dims the formulation in torch operations.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from .. import _native
+from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _apply, _autocast_dtype, _pad_head, _parameter, _run_call
+
+__all__ = ["flash_born_attention_packed"]
+
+
+def _token_rows(t: torch.Tensor, dtype: torch.dtype, dp: int):
+    """``t`` (N, heads, D) in ``dtype``, zero-padded to ``dp`` columns, and its
+    (token, head) strides, read in place where the kernels can: unit stride
+    along D, 16-byte pieces, tokens that do not overlap."""
+    if t.dtype != dtype:
+        t = t.to(dtype)
+    t = _pad_head(t, dp)
+    n, h, _ = t.shape
+    item = t.element_size()
+    st, sh = (t.stride(0) if n > 1 else h * dp), (t.stride(1) if h > 1 else 0)
+    if (t.stride(2) != 1 or t.data_ptr() % 16 or st * item % 16 or sh * item % 16 or st < dp or sh < 0
+            or st * item >= 1 << 24):
+        t = t.contiguous()
+        if t.data_ptr() % 16:
+            t = t.clone()
+        st, sh = h * dp, dp
+    return t, st, sh
+
+
+def _starts(cu: torch.Tensor, device: torch.device) -> torch.Tensor:
+    if cu.dtype != torch.int32 or cu.device != device:
+        cu = cu.to(device=device, dtype=torch.int32)
+    return cu.contiguous()
+
+
+def _check(q, k, v, n_scale, cu_q, cu_k):
+    if q.dim() != 3:
+        raise ValueError(f"q must be (tokens, heads, head_dim), got shape {tuple(q.shape)}")
+    if k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+        raise ValueError(f"k and v must share one (tokens, key_heads, head_dim) shape with q's head_dim, got "
+                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
+    H, Hkv = q.shape[1], k.shape[1]
+    if Hkv < 1 or H < 1 or H % Hkv or q.shape[2] < 1:
+        raise ValueError(f"the {H} query heads must be a multiple of the {Hkv} key heads, and head_dim positive")
+    if n_scale not in (1, H):
+        raise ValueError(f"scale must hold 1 value or H={H} per-head values, got {n_scale}")
+    for name, cu in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
+        if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
+            raise ValueError(f"{name} must be a 1-D int32 or int64 tensor of sequences + 1 starts, got "
+                             f"{cu.dtype} {tuple(cu.shape)}")
+    if cu_q.numel() != cu_k.numel():
+        raise ValueError(f"cu_seqlens_q and cu_seqlens_k name {cu_q.numel() - 1} and {cu_k.numel() - 1} sequences")
+    if not q.device == k.device == v.device:
+        raise ValueError(f"q, k, v must be on one device, got {q.device}, {k.device}, {v.device}")
+
+
+class _FlashBornPackedFn(torch.autograd.Function):
+    """forward: computes in the autocast dtype (CUDA autocast active) else
+    ``v.dtype``; saves the rows, ``out``, Z (fp32) and the starts.  backward:
+    dq, dk, dv in the inputs' dtypes, dscale in the scale's shape and dtype."""
+
+    @staticmethod
+    def forward(ctx, q, k, v, scale, cu_q, cu_k, is_causal, eps, window):
+        lib = _native.load()
+        target = _autocast_dtype(q) or v.dtype
+        if target not in _DTYPE_CODE:
+            raise TypeError(f"flash_born_attention_packed: unsupported dtype {target}")
+        dev = q.device
+        scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
+        N, H, D = q.shape
+        M, Hkv, _ = k.shape
+        dp = (D + 7) // 8 * 8
+        q_c, *qs = _token_rows(q, target, dp)
+        k_c, *ks = _token_rows(k, target, dp)
+        v_c, *vs = _token_rows(v, target, dp)
+        cu_q, cu_k = _starts(cu_q, dev), _starts(cu_k, dev)
+        out = torch.empty((N, H, dp), dtype=target, device=dev)
+        z = torch.empty((H, N), dtype=torch.float32, device=dev)
+        head = (_DTYPE_CODE[target], cu_q.numel() - 1, N, M, H, Hkv, dp, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(),
+                *qs, *ks, *vs, out.data_ptr(), z.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), scale_p, n_scale, scale_value,
+                1 if is_causal else 0, window, float(eps))
+        _run_call(lib.qdl_flash_born_packed_forward_call, "qdl_flash_born_packed_forward_call", dev,
+                  _native.packed_call(*head, *(0,) * 9))
+        ctx.save_for_backward(q_c, k_c, v_c, out, z, scale_flat, cu_q, cu_k)
+        ctx.head = head
+        ctx.head_dim = D
+        if scale_flat is not None:
+            ctx.scale_shape, ctx.scale_dtype = scale.shape, scale.dtype
+        ctx.dtypes = (q.dtype, k.dtype, v.dtype)
+        return out if dp == D else out[..., :D].contiguous()
+
+    @staticmethod
+    def backward(ctx, do):
+        lib = _native.load()
+        q_c, k_c, v_c, out, z, scale_flat, cu_q, cu_k = ctx.saved_tensors
+        N, H, dp = out.shape
+        M, Hkv = k_c.shape[:2]
+        D, dev = ctx.head_dim, q_c.device
+        do_c, *ds = _token_rows(do, out.dtype, dp)
+        dq = torch.empty((N, H, dp), dtype=out.dtype, device=dev)
+        dk = torch.empty((M, Hkv, dp), dtype=out.dtype, device=dev)
+        dv = torch.empty_like(dk)
+        n_scale = 1 if scale_flat is None else scale_flat.numel()
+        # The scale's gradient costs launches of its own: only where wanted.
+        dscale = torch.empty(n_scale, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
+        size = int(lib.qdl_flash_born_packed_workspace_size(N, H))
+        ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        _run_call(lib.qdl_flash_born_packed_backward_call, "qdl_flash_born_packed_backward_call", dev,
+                  _native.packed_call(*ctx.head, do_c.data_ptr(), *ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
+                                      0 if dscale is None else dscale.data_ptr(), ws.data_ptr(), size))
+        if dp != D:
+            dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
+        qd, kd, vd = ctx.dtypes
+        return (dq.to(qd), dk.to(kd), dv.to(vd),
+                None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype),
+                None, None, None, None, None)
+
+
+def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
+    """The formulas in torch operations, in fp32 (fp64 for fp64 values), one
+    sequence at a time."""
+    cq, ck = cu_q.tolist(), cu_k.tolist()
+    for name, c, n in (("cu_seqlens_q", cq, q.shape[0]), ("cu_seqlens_k", ck, k.shape[0])):
+        if c[0] != 0 or c[-1] > n or any(a > b for a, b in zip(c, c[1:])):
+            raise ValueError(f"{name} must start at 0, never decrease and end within the {n} rows, got {c}")
+    H, Hkv = q.shape[1], k.shape[1]
+    G = H // Hkv
+    wide = torch.float64 if v.dtype == torch.float64 else torch.float32
+    s = scale_t.to(device=q.device, dtype=wide).reshape(-1).expand(H).view(Hkv, G, 1, 1)
+    outs = []
+    for a0, a1, b0, b1 in zip(cq, cq[1:], ck, ck[1:]):
+        nq, nk = a1 - a0, b1 - b0
+        qs = q[a0:a1].to(wide).view(nq, Hkv, G, q.shape[2]).permute(1, 2, 0, 3)
+        ks, vs = (x[b0:b1].to(wide).permute(1, 0, 2).unsqueeze(1) for x in (k, v))
+        lag = (torch.arange(nq, device=q.device) + nk - nq).view(-1, 1) - torch.arange(nk, device=q.device).view(1, -1)
+        keep = torch.ones_like(lag, dtype=torch.bool)
+        if is_causal:
+            keep = keep & (lag >= 0)
+        if window > 0:
+            keep = keep & (lag < window)
+        p = torch.relu(torch.matmul(qs, ks.transpose(-1, -2)) * s).square() * keep
+        den = p.sum(-1, keepdim=True) + eps
+        # Rows without weight are zero, with eps == 0 too.
+        w = p / torch.where(den > 0, den, torch.ones_like(den))
+        outs.append(torch.matmul(w, vs).permute(2, 0, 1, 3).reshape(nq, H, q.shape[2]))
+    outs.append(torch.zeros((q.shape[0] - cq[-1], H, v.shape[2]), dtype=wide, device=q.device))
+    return torch.cat(outs).to(v.dtype)
+
+
+def flash_born_attention_packed(
+    q: torch.Tensor,
+    k: torch.Tensor,
+    v: torch.Tensor,
+    scale: float | torch.Tensor,
+    cu_seqlens_q: torch.Tensor,
+    cu_seqlens_k: torch.Tensor | None = None,
+    is_causal: bool = True,
+    eps: float = 1e-12,
+    window_size: int = 0,
+) -> torch.Tensor:
+    """Born attention over packed sequences; returns (N, H, D) in the compute dtype.
+
+    ``q`` (N, H, D), ``k`` and ``v`` (M, Hkv, D): rows of tokens, any strides
+    with unit stride along D are read in place.  ``scale``: a float or a tensor
+    of 1 or H values.  ``cu_seqlens_q``, ``cu_seqlens_k`` (default: the
+    queries'): the sequences' S + 1 starts, int32 (int64 is converted), the
+    first 0, never decreasing, the last at most the rows; they stay on the
+    device, so on the GPU values that break this are not reported: such calls
+    read and write nothing outside the tensors, and their outputs are undefined.
+    Rows behind the last sequence come out as zeros.  ``is_causal`` and
+    ``window_size`` count positions from the sequences' ends: fewer queries than
+    keys are the last ones (a prompt's next part behind its cache).
+    Differentiable in q, k, v and scale; the sums over a group's heads are taken
+    in a fixed order.
+    """
+    if cu_seqlens_k is None:
+        cu_seqlens_k = cu_seqlens_q
+    n_scale = scale.numel() if isinstance(scale, torch.Tensor) else 1
+    _check(q, k, v, n_scale, cu_seqlens_q, cu_seqlens_k)
+    window = max(int(window_size), 0)
+    if not float(eps) >= 0.0:
+        raise ValueError(f"eps must be at least 0, got {eps}")
+    if q.is_cuda and q.shape[2] <= MAX_HEAD_DIM:
+        return _apply(_FlashBornPackedFn, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
+    scale_t = scale if isinstance(scale, torch.Tensor) else torch.tensor(float(scale), dtype=torch.float64)
+    return _eager_packed(q, k, v, scale_t, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
