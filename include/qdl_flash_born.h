@@ -350,8 +350,8 @@ int qdl_flash_born_fwd_qk_prologue(int dtype, int64_t B, int64_t H, int64_t T,
  *
  * q, k, v, dout have unit stride along D and *_strides (token, head) in
  * elements, multiples of 16 bytes (a token's at least D, under 2^24 bytes);
- * out, dq, dk, dv are contiguous; z is (H, n_q) fp32.  scale == NULL takes
- * scale_value.  The weights of fp16 rows are scaled by a power of two of the
+ * out, dq, dk, dv are contiguous; z is (H, n_q) fp32, NULL in the forward if no
+ * backward follows.  scale == NULL takes scale_value.  The weights of fp16 rows are scaled by a power of two of the
  * row's own, so overlaps of any size keep their weight.
  * The backward's dk and dv are summed over the heads of a group in a fixed
  * order; dscale == NULL: not wanted.  struct_bytes: sizeof the block.
@@ -397,7 +397,7 @@ int qdl_flash_born_packed_backward_call(const qdl_born_packed_call *call, qdl_st
  * head), out (B, H, D) contiguous.  The token is the last of its sequence's
  * cache_lens keys and sees all of them, or the last window_size.  The keys are
  * split over workgroups and joined in order; the workspace's size is the size
- * function's for the same block.
+ * function's for the same sizes (weighed: key_weight != NULL).
  * key_weight != NULL: (B, h_kv, weight_len) fp32 with weight_strides (sequence,
  * head), to which the sum over the group's heads of p_j / Z is added for every
  * visible key j < weight_len.
@@ -425,7 +425,8 @@ typedef struct qdl_born_paged_call {
     int64_t workspace_bytes;
 } qdl_born_paged_call;
 
-int64_t qdl_flash_born_paged_workspace_size(const qdl_born_paged_call *call);
+int64_t qdl_flash_born_paged_workspace_size(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages,
+                                            int64_t page_size, int64_t window_size, int weighed);
 int qdl_flash_born_paged_forward_call(const qdl_born_paged_call *call, qdl_stream_t stream);
 
 /*

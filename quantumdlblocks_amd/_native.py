@@ -142,7 +142,7 @@ def _bind(lib: ctypes.CDLL) -> None:
     lib.qdl_flash_born_packed_workspace_size.restype = _i64
     lib.qdl_flash_born_packed_workspace_size.argtypes = [_i64, _i64]
     lib.qdl_flash_born_paged_workspace_size.restype = _i64
-    lib.qdl_flash_born_paged_workspace_size.argtypes = [ctypes.c_char_p]
+    lib.qdl_flash_born_paged_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]
     lib.qdl_flash_purified_born_fwd.restype = _int
     lib.qdl_flash_purified_born_fwd.argtypes = [
         _int, _i64, _i64, _i64, _i64,      # dtype, B, H, T, D

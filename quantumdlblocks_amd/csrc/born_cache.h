@@ -221,12 +221,15 @@ __device__ __forceinline__ uint32_t evict_key(float x) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-constexpr int kEvictThreads = 1024, kEvictPer = 16, kEvictSpan = kEvictThreads * kEvictPer;
+// NT threads, 16 weights each: 256 for caches of up to 4096 keys, where the
+// barriers are what the launch waits for, else 1024.
+constexpr int kEvictPer = 16;
 
-template <int>
-__global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictArgs p) {
-    constexpr int NW = kEvictThreads / 64;
-    __shared__ uint32_t hist[NW][256];
+template <int NT>
+__global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
+    constexpr int NW = NT / 64, SPAN = NT * kEvictPer;
+    constexpr int CL = kEvictPer * NW / 64;  // counts that a lane of one wave scans
+    __shared__ uint32_t hist[256];
     __shared__ uint32_t s_prefix, s_left;
     __shared__ uint32_t counts[kEvictPer * NW];  // kept for sure | ties << 16, per 64 keys
     __shared__ uint32_t s_total;
@@ -236,42 +239,53 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
     const float* w = p.weight + (int64_t)b * p.w_sb + (int64_t)hk * p.w_sh;
     float* wo = p.weight_out + ((int64_t)b * p.Hkv + hk) * p.w_len;
     int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
-    if (hk == 0 && tid == 0) p.lens_out[b] = m;
-    for (int i = m + tid; i < p.budget; i += kEvictThreads) kept[i] = -1;
-    for (int i = m + tid; i < p.w_len; i += kEvictThreads) wo[i] = 0.f;
     const int tail = n > m ? min(p.recent, m) : m;
     const int old = n - tail, want = m - tail;  // of the `old` first keys, `want` stay
-    for (int i = tid; i < tail; i += kEvictThreads) {
-        kept[want + i] = old + i;
-        if (want + i < p.w_len) wo[want + i] = old + i < p.w_len ? w[old + i] : 0.f;
-    }
-    if (want == 0) return;
 
-    const int spans = (old + kEvictSpan - 1) / kEvictSpan;
+    const int spans = (old + SPAN - 1) / SPAN;
     float x[kEvictPer];
     uint32_t key[kEvictPer];
     auto load = [&](int span) {
 #pragma unroll
         for (int i = 0; i < kEvictPer; ++i) {
-            const int j = span * kEvictSpan + i * kEvictThreads + tid;
+            const int j = span * SPAN + i * NT + tid;
             x[i] = j < old && j < p.w_len ? w[j] : 0.f;
         }
 #pragma unroll
         for (int i = 0; i < kEvictPer; ++i) key[i] = evict_key(x[i]);
     };
-    load(0);
+    if (want > 0) load(0);
+    if (hk == 0 && tid == 0) p.lens_out[b] = m;
+    for (int i = m + tid; i < p.budget; i += NT) kept[i] = -1;
+    for (int i = m + tid; i < p.w_len; i += NT) wo[i] = 0.f;
+    for (int i = tid; i < tail; i += NT) {
+        kept[want + i] = old + i;
+        if (want + i < p.w_len) wo[want + i] = old + i < p.w_len ? w[old + i] : 0.f;
+    }
+    if (want == 0) return;
+
     if (tid == 0) s_prefix = 0, s_left = want;
     // The want-th greatest key, 8 bits at a time.
     for (int shift = 24; shift >= 0; shift -= 8) {
-        for (int i = tid; i < NW * 256; i += kEvictThreads) hist[i >> 8][i & 255] = 0;
+        if (tid < 256) hist[tid] = 0;
         __syncthreads();
         const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
         for (int sp = 0; sp < spans; ++sp) {
             if (spans > 1) load(sp);
 #pragma unroll
             for (int i = 0; i < kEvictPer; ++i) {
-                const int j = sp * kEvictSpan + i * kEvictThreads + tid;
-                if (j < old && (key[i] & mask) == prefix) atomicAdd(&hist[wave][(key[i] >> shift) & 255u], 1u);
+                const int j = sp * SPAN + i * NT + tid;
+                const bool in = j < old && (key[i] & mask) == prefix;
+                const uint64_t active = __ballot(in);
+                if (active == 0) continue;
+                // The lanes of the first one's bin add as one: keys that were
+                // never weighed are all in one bin.
+                const uint32_t bin = (key[i] >> shift) & 255u;
+                const int first = __ffsll((long long)active) - 1;
+                const uint32_t lead = __builtin_amdgcn_readlane(bin, first);
+                const uint64_t same = __ballot(in && bin == lead);
+                if (lane == first) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
+                else if (in && bin != lead) atomicAdd(&hist[bin], 1u);
             }
         }
         __syncthreads();
@@ -279,12 +293,9 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
             // Lane l: bins 255 - 4 l .. 252 - 4 l, from the greatest down.
             uint32_t c[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                c[i] = 0;
-                for (int v = 0; v < NW; ++v) c[i] += hist[v][255 - 4 * lane - i];
-                sum += c[i];
-            }
+            for (int i = 0; i < 4; ++i) c[i] = hist[255 - 4 * lane - i], sum += c[i];
             uint32_t above = sum;
+#pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const uint32_t y = __shfl_up(above, o);
                 if (lane >= o) above += y;
@@ -310,17 +321,18 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
         uint64_t gt[kEvictPer], eq[kEvictPer];
 #pragma unroll
         for (int i = 0; i < kEvictPer; ++i) {
-            const int j = sp * kEvictSpan + i * kEvictThreads + tid;
+            const int j = sp * SPAN + i * NT + tid;
             gt[i] = __ballot(j < old && key[i] > cut);
             eq[i] = __ballot(j < old && key[i] == cut);
             if (lane == 0) counts[i * NW + wave] = (uint32_t)__popcll(gt[i]) | ((uint32_t)__popcll(eq[i]) << 16);
         }
         __syncthreads();
-        if (wave == 0) {  // exclusive sums, 4 counts a lane (sums up to 16384 fit 16 bits)
-            uint32_t c[4], sum = 0;
+        if (wave == 0) {  // exclusive sums (up to 16384, which fits 16 bits)
+            uint32_t c[CL], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = counts[4 * lane + i], sum += c[i];
+            for (int i = 0; i < CL; ++i) c[i] = counts[CL * lane + i], sum += c[i];
             uint32_t run = sum;
+#pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
                 const uint32_t y = __shfl_up(run, o);
                 if (lane >= o) run += y;
@@ -328,8 +340,8 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
             if (lane == 63) s_total = run;
             run -= sum;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                counts[4 * lane + i] = run;
+            for (int i = 0; i < CL; ++i) {
+                counts[CL * lane + i] = run;
                 run += c[i];
             }
         }
@@ -337,7 +349,7 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
         const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
         for (int i = 0; i < kEvictPer; ++i) {
-            const int j = sp * kEvictSpan + i * kEvictThreads + tid;
+            const int j = sp * SPAN + i * NT + tid;
             const uint32_t c = counts[i * NW + wave];
             const uint32_t g = before_gt + (c & 0xffffu) + (uint32_t)__popcll(gt[i] & below);
             const uint32_t e = before_eq + (c >> 16) + (uint32_t)__popcll(eq[i] & below);
@@ -354,40 +366,59 @@ __global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictA
     }
 }
 
-static_assert(kEvictPer * (kEvictThreads / 64) == 256, "the counts of one span are scanned by one wave");
-
 __device__ __forceinline__ int64_t evict_at(const EvictArgs& p, const int32_t* table, int pages, int j, int64_t sp, int64_t st) {
     const int i = p.page_shift >= 0 ? j >> p.page_shift : j / p.page;
     const int64_t page = i < pages ? table[i] : -1;
     return page >= 0 && page < p.cache_pages ? page * sp + (int64_t)(j - i * p.page) * st : -1;
 }
 
-// The kept rows to other pages: 16 bytes a lane, K and V of kEvictRows rows
-// per workgroup.  A row whose page is missing arrives as zeros.
-constexpr int kEvictRows = 64;
+// The kept rows to other pages: 16 bytes a lane, K and V of four rows in flight
+// for each.  A row whose page is missing arrives as zeros.
+constexpr int kEvictUnroll = 4;
+inline __host__ __device__ int evict_rows(int cpr) { return 256 / cpr * kEvictUnroll; }  // per workgroup
 
 template <int>
 __global__ __launch_bounds__(256) void born_evict_move_kernel(EvictArgs p) {
     const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
     const int b = rest % p.B, tile = rest / p.B;
     const int m = min(evict_len(p, b), p.budget);
-    const int cpr = p.D * p.item / 16;
+    const int cpr = p.D * p.item / 16, rows = 256 / cpr;
     const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
     const int32_t *from = p.table + (int64_t)b * p.table_ld, *to = p.to + (int64_t)b * p.to_ld;
-    const int r1 = min(kEvictRows, m - tile * kEvictRows);
-    for (int x = threadIdx.x; x < r1 * cpr; x += 256) {
-        const int i = tile * kEvictRows + x / cpr, o = 16 * (x % cpr);
-        const int j = kept[i];
+    const int mine = threadIdx.x / cpr, o = 16 * (threadIdx.x % cpr);
+    const int i0 = tile * evict_rows(cpr) + mine;
+    if (mine >= rows || i0 >= m) return;
+    uint8_t *kc = (uint8_t*)p.k + (int64_t)hk * p.kh + o, *vc = (uint8_t*)p.v + (int64_t)hk * p.vh + o;
+    int j[kEvictUnroll];
 #pragma unroll
-        for (int which = 0; which < 2; ++which) {
-            uint8_t* cache = (uint8_t*)(which ? p.v : p.k) + (int64_t)hk * (which ? p.vh : p.kh) + o;
-            const int64_t sp = which ? p.vp : p.kp, st = which ? p.vt : p.kt;
-            const int64_t a = evict_at(p, from, p.pages, j, sp, st), d = evict_at(p, to, p.to_pages, i, sp, st);
-            u32x4 y = {0u, 0u, 0u, 0u};
-            if (a >= 0) y = ldg16(cache + a);
-            if (d >= 0) *reinterpret_cast<u32x4*>(cache + d) = y;
+    for (int u = 0; u < kEvictUnroll; ++u) j[u] = i0 + u * rows < m ? kept[i0 + u * rows] : -1;
+    // Page and row of the row's old and new slots; page -1: none.
+    int pf[kEvictUnroll], rf[kEvictUnroll], pt[kEvictUnroll], rt[kEvictUnroll];
+#pragma unroll
+    for (int u = 0; u < kEvictUnroll; ++u) {
+        const int i = i0 + u * rows, jj = max(j[u], 0);
+        const int a = p.page_shift >= 0 ? jj >> p.page_shift : jj / p.page;
+        const int d = p.page_shift >= 0 ? i >> p.page_shift : i / p.page;
+        rf[u] = jj - a * p.page;
+        rt[u] = i - d * p.page;
+        pf[u] = j[u] >= 0 && a < p.pages ? from[a] : -1;
+        pt[u] = j[u] >= 0 && d < p.to_pages ? to[d] : -1;
+    }
+    u32x4 y[kEvictUnroll][2];
+#pragma unroll
+    for (int u = 0; u < kEvictUnroll; ++u) {
+        y[u][0] = y[u][1] = u32x4{0u, 0u, 0u, 0u};
+        if (pf[u] >= 0 && pf[u] < p.cache_pages) {
+            y[u][0] = ldg16(kc + pf[u] * p.kp + rf[u] * p.kt);
+            y[u][1] = ldg16(vc + pf[u] * p.vp + rf[u] * p.vt);
         }
     }
+#pragma unroll
+    for (int u = 0; u < kEvictUnroll; ++u)
+        if (pt[u] >= 0 && pt[u] < p.cache_pages) {
+            *reinterpret_cast<u32x4*>(kc + pt[u] * p.kp + rt[u] * p.kt) = y[u][0];
+            *reinterpret_cast<u32x4*>(vc + pt[u] * p.vp + rt[u] * p.vt) = y[u][1];
+        }
 }
 
 // The kept rows to the front of their own pages.  Rows only move down and keep

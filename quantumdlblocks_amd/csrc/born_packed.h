@@ -45,7 +45,7 @@ constexpr int kItem = std::is_same<E, F32>::value ? 4 : 2;
 struct PackedArgs {
     const void *q, *k, *v, *o, *dout;
     void *out, *dq, *dk, *dv;
-    float* z;       // (H, Nq)
+    float* z;       // (H, Nq), or nullptr: no backward follows
     float* ndelta;  // (H, Nq) workspace: -(dO . O)
     float* zs;      // (H, Nq) workspace: s^2 / Z
     const float* scale;  // 1 or H values, or nullptr: scale_value
@@ -390,7 +390,7 @@ void born_packed_fwd_kernel(PackedArgs p) {
     const float inv = den > 0.f && sc != 0.f ? 1.0f / den : 0.f;
     if (!ok) return;
     packed_store_row<E>((uint8_t*)p.out + ((size_t)(sq.q0 + row) * p.H + h) * D * kItem<E>, acc, inv, D, g);
-    if (g == 0) p.z[(size_t)h * p.Nq + sq.q0 + row] = s2 * z + p.eps;
+    if (g == 0 && p.z != nullptr) p.z[(size_t)h * p.Nq + sq.q0 + row] = s2 * z + p.eps;
 }
 
 // ---------------------------------------------------------------------------

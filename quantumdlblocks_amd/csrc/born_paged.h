@@ -53,6 +53,7 @@ struct PagedArgs {
     int64_t w_sb, w_sh;    // elements
     int w_len;             // columns of weights
     float* raw;            // (B, H, raw_ld) workspace: p without s^2, where weights are kept
+    float* inv;            // (B, H) workspace: 1 / (Z without s^2), likewise
     int64_t raw_ld;
 };
 
@@ -77,9 +78,13 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& p, int b) {
     return {p.window > 0 ? max(0, n - p.window) : 0, n};
 }
 
+// Page table entries and scalars that never change during a launch, read as
+// scalar loads where the index is uniform.
+typedef const __attribute__((address_space(4))) int32_t* ConstIntPtr;
+
 // Row of key j: page and row in it; false for keys outside [first, n) and for
 // pages that are none of the cache's.
-__device__ __forceinline__ bool paged_row(const PagedArgs& p, const int32_t* table, PagedSpan sp, int j, int64_t& page, int& row) {
+__device__ __forceinline__ bool paged_row(const PagedArgs& p, ConstIntPtr table, PagedSpan sp, int j, int64_t& page, int& row) {
     const bool in = j >= sp.first && j < sp.n;
     const int jj = in ? j : 0;
     const int i = p.page_shift >= 0 ? jj >> p.page_shift : jj / p.page;
@@ -101,15 +106,45 @@ __device__ __forceinline__ u32x4 paged_column(const u32x4 (&x)[8], int e) {
     return a;
 }
 
-// DP: 64, 128 or 256 columns; WEIGH: the raw weights are written too.
-template <class E, int DP, bool WEIGH>
-__global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
-    constexpr bool k32 = std::is_same<E, F32>::value;
-    constexpr int IT = kItem<E>, NW = 4;
+template <class E, int DP>
+struct PagedCfg {
+    static constexpr bool k32 = std::is_same<E, F32>::value;
+    static constexpr int IT = kItem<E>;
     // K: 16-byte chunks of a row, four lanes of a key taking chunks 4 ks + j.
-    constexpr int KS = DP * IT / 64;
+    static constexpr int KS = DP * IT / 64;
     // V: columns per lane and load (VC), blocks of 16 VC columns.
-    constexpr int VC = k32 ? 4 : DP == 64 ? 4 : 8, VB = DP / (16 * VC), NO = VB * VC;
+    static constexpr int VC = k32 ? 4 : DP == 64 ? 4 : 8, VB = DP / (16 * VC), NO = VB * VC;
+    static constexpr int VW = VC * IT / 4;  // dwords of a V load
+    // Two sets of 32 keys in registers, one loading while the other is used,
+    // where two fit beside the accumulators.
+    static constexpr int NBUF = 2 * 4 * KS + 8 * VW * VB <= 64 ? 2 : 1;
+    static constexpr int WPE = IT * DP <= 256 ? 2 : 1;
+};
+
+// A wave's 32 keys.
+template <class E, int DP>
+struct PagedKeys {
+    using C = PagedCfg<E, DP>;
+    u32x4 k[2][C::KS];
+    u32x4 v[C::VB][8];
+    bool full, there[2];  // all 32 visible; the pages of each 16
+};
+
+__device__ __forceinline__ u32x4 paged_ldg(const uint8_t* p, int words) {
+    if (words == 4) return ldg16(p);
+    const u32x2 y = *reinterpret_cast<const u32x2*>(p);
+    return u32x4{y[0], y[1], 0u, 0u};
+}
+
+// DP: 64, 128 or 256 columns; WEIGH: the raw weights are written too; P16:
+// pages of a multiple of 16 tokens, so that 16 keys from a multiple of 16 lie in
+// one page and their addresses are one scalar base and a lane's offset.
+template <class E, int DP, bool WEIGH, bool P16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(PagedCfg<E, DP>::WPE)))
+void born_paged_kernel(PagedArgs p) {
+    using C = PagedCfg<E, DP>;
+    constexpr bool k32 = C::k32;
+    constexpr int IT = C::IT, NW = 4, KS = C::KS, VC = C::VC, VB = C::VB, NO = C::NO, VW = C::VW;
     __shared__ float red[NW][16][DP + 4];
     __shared__ float zred[NW][16];
 
@@ -123,9 +158,26 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
     const int base = sp.first & ~31;  // splits count from here
     const int s0 = base + split * p.chunk, s1 = min(sp.n, s0 + p.chunk);
     if (s0 >= s1 && split > 0) return;  // the join reads the filled splits only
-    const int32_t* table = p.table + (int64_t)b * p.table_ld;
+    const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.table + (int64_t)b * p.table_ld);
     const uint8_t* const kc = (const uint8_t*)p.k + (int64_t)hk * p.kh;
     const uint8_t* const vc = (const uint8_t*)p.v + (int64_t)hk * p.vh;
+
+    // A lane's chunks of K and columns of V; past D they are read from the
+    // row's start, K's made zeros and V's columns never stored.
+    int ko[KS], vo[VB];
+    uint32_t kmask[KS];
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks) {
+        const int at = 16 * (4 * ks + j4);
+        kmask[ks] = at < IT * p.D ? ~0u : 0u;
+        ko[ks] = at < IT * p.D ? at : 0;
+    }
+#pragma unroll
+    for (int vb = 0; vb < VB; ++vb) {
+        const int col = 16 * VC * vb + VC * m;
+        vo[vb] = col < p.D ? IT * col : 0;
+    }
+    const bool whole = p.D == DP;
 
     // Query head h0 + m in the columns of S^T.
     const bool okh = m < heads;
@@ -134,20 +186,51 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
     u32x4 qr[KS];
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        const int at = 16 * (4 * ks + j4);
         u32x4 x = {0u, 0u, 0u, 0u};
-        if (okh && at < IT * p.D) x = ldg16((const uint8_t*)p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + m) * p.q_sh + at);
-        qr[ks] = x ^ flip;
+        if (okh && kmask[ks]) x = ldg16((const uint8_t*)p.q + (int64_t)b * p.q_sb + (int64_t)(h0 + m) * p.q_sh + ko[ks]) ^ flip;
+        qr[ks] = x;
     }
     f32x4v acc[NO];
 #pragma unroll
     for (int i = 0; i < NO; ++i) acc[i] = f32x4v{0.f, 0.f, 0.f, 0.f};
     float z = 0.f, cf = std::is_same<E, F16>::value ? kF16Start : 1.f;
 
-    for (int key0 = s0 + 32 * wave; key0 < s1; key0 += 32 * NW) {
-        // Keys of this lane: rows key0 + m and + 16 for K, key0 + 4 j4 + i and
-        // + 16 for V.
-        u32x4 kx[2][KS];
+    // Keys key0 + 16 t + m for K, key0 + 16 t + 4 j4 + i for V.
+    auto load = [&](PagedKeys<E, DP>& x, int key0) __attribute__((always_inline)) {
+        if constexpr (P16) {
+            // Keys outside [first, n) and missing pages: the loads go to the
+            // nearest visible key, or to page 0, and use() drops what they bring.
+            const uint8_t *kp[2], *vp[2];
+            int first[2];
+            x.full = key0 >= sp.first && key0 + 32 <= sp.n;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int j = min(max(key0 + 16 * t, sp.first), sp.n - 1);
+                const int i = __builtin_amdgcn_readfirstlane(p.page_shift >= 0 ? j >> p.page_shift : j / p.page);
+                const int32_t page = table[i];
+                x.there[t] = page >= 0 && page < p.cache_pages;
+                x.full = x.full && x.there[t];
+                const int64_t at = x.there[t] ? page : 0;
+                kp[t] = kc + at * p.kp;
+                vp[t] = vc + at * p.vp;
+                first[t] = i * p.page;
+            }
+            auto row = [&](int t, int r) { return (uint32_t)(min(max(key0 + 16 * t + r, sp.first), sp.n - 1) - first[t]); };
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const uint32_t o = row(t, m) * (uint32_t)p.kt;
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) x.k[t][ks] = ldg16(kp[t] + (o + (uint32_t)ko[ks]));
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const uint32_t o = row(i >> 2, 4 * j4 + (i & 3)) * (uint32_t)p.vt;
+#pragma unroll
+                for (int vb = 0; vb < VB; ++vb) x.v[vb][i] = paged_ldg(vp[i >> 2] + (o + (uint32_t)vo[vb]), VW);
+            }
+            return;
+        }
+        x.full = true;
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
             int64_t page;
@@ -156,13 +239,11 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
             const uint8_t* at = kc + page * p.kp + (int64_t)row * p.kt;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const int o = 16 * (4 * ks + j4);
-                u32x4 x = {0u, 0u, 0u, 0u};
-                if (ok && o < IT * p.D) x = ldg16(at + o);
-                kx[t][ks] = x;
+                u32x4 y = {0u, 0u, 0u, 0u};
+                if (ok) y = ldg16(at + ko[ks]);
+                x.k[t][ks] = y;
             }
         }
-        u32x4 vx[VB][8];
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
             int64_t page;
@@ -171,19 +252,18 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
             const uint8_t* at = vc + page * p.vp + (int64_t)row * p.vt;
 #pragma unroll
             for (int vb = 0; vb < VB; ++vb) {
-                const int col = 16 * VC * vb + VC * m;
-                u32x4 x = {0u, 0u, 0u, 0u};
-                if (ok && col < p.D) {
-                    if constexpr (VC * IT == 16) {
-                        x = ldg16(at + IT * col);
-                    } else {
-                        const u32x2 y = *reinterpret_cast<const u32x2*>(at + IT * col);
-                        x[0] = y[0];
-                        x[1] = y[1];
-                    }
-                }
-                vx[vb][i] = x;
+                u32x4 y = {0u, 0u, 0u, 0u};
+                if (ok) y = paged_ldg(at + vo[vb], VW);
+                x.v[vb][i] = y;
             }
+        }
+    };
+    auto use = [&](PagedKeys<E, DP>& x, int key0) __attribute__((always_inline)) {
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) x.k[t][ks] &= kmask[ks];
         }
         f32x4v s[2];
 #pragma unroll
@@ -193,10 +273,20 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
             for (int ks = 0; ks < KS; ++ks) {
                 if constexpr (k32) {
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) s[t] = mfma16_f32(__uint_as_float(kx[t][ks][i]), __uint_as_float(qr[ks][i]), s[t]);
+                    for (int i = 0; i < 4; ++i) s[t] = mfma16_f32(__uint_as_float(x.k[t][ks][i]), __uint_as_float(qr[ks][i]), s[t]);
                 } else {
-                    s[t] = mfma16<E>(kx[t][ks], qr[ks], s[t]);
+                    s[t] = mfma16<E>(x.k[t][ks], qr[ks], s[t]);
                 }
+            }
+        }
+        if (P16 && !x.full) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int key = key0 + 16 * (i >> 2) + 4 * j4 + (i & 3);
+                const bool seen = x.there[i >> 2] && key >= sp.first && key < sp.n;
+                if (!seen) s[i >> 2][i & 3] = 0.f;
+#pragma unroll
+                for (int vb = 0; vb < VB; ++vb) x.v[vb][i] &= seen ? ~0u : 0u;
             }
         }
         // Weights: relu(r)^2, keys 16 t + 4 j4 + r of the 32.
@@ -227,8 +317,8 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
                 for (int t = 0; t < 2; ++t) {
                     const int key = key0 + 16 * t + 4 * j4;
                     float* to = p.raw + ((int64_t)b * p.H + h0 + m) * p.raw_ld + key;
-                    const f32x4v x = {w[4 * t] * back, w[4 * t + 1] * back, w[4 * t + 2] * back, w[4 * t + 3] * back};
-                    if (key < p.raw_ld) *reinterpret_cast<f32x4v*>(to) = x;  // raw_ld: a multiple of 32
+                    const f32x4v y = {w[4 * t] * back, w[4 * t + 1] * back, w[4 * t + 2] * back, w[4 * t + 3] * back};
+                    if (key < p.raw_ld) *reinterpret_cast<f32x4v*>(to) = y;  // raw_ld: a multiple of 32
                 }
             }
         }
@@ -240,7 +330,7 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
                 for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
                     for (int e = 0; e < VC; ++e)
-                        acc[vb * VC + e] = mfma16_f32(__uint_as_float(vx[vb][i][e]), w[i], acc[vb * VC + e]);
+                        acc[vb * VC + e] = mfma16_f32(__uint_as_float(x.v[vb][i][e]), w[i], acc[vb * VC + e]);
             }
         } else {
             u32x4 pk;
@@ -252,7 +342,25 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
 #pragma unroll
             for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-                for (int e = 0; e < VC; ++e) acc[vb * VC + e] = mfma16<E>(paged_column(vx[vb], e), pk, acc[vb * VC + e]);
+                for (int e = 0; e < VC; ++e) acc[vb * VC + e] = mfma16<E>(paged_column(x.v[vb], e), pk, acc[vb * VC + e]);
+        }
+    };
+    const int step = 32 * NW, key0 = s0 + 32 * wave;
+    if constexpr (C::NBUF == 2) {
+        PagedKeys<E, DP> x, y;
+        if (key0 < s1) load(x, key0);
+        for (int key = key0; key < s1; key += 2 * step) {
+            if (key + step < s1) load(y, key + step);
+            use(x, key);
+            if (key + step >= s1) break;
+            if (key + 2 * step < s1) load(x, key + 2 * step);
+            use(y, key + step);
+        }
+    } else {
+        PagedKeys<E, DP> x;
+        for (int key = key0; key < s1; key += step) {
+            load(x, key);
+            use(x, key);
         }
     }
     // The wave's sums, without the fp16 factor.
@@ -296,29 +404,45 @@ __global__ __launch_bounds__(256) void born_paged_kernel(PagedArgs p) {
     }
 }
 
-// Splits joined in order.  One workgroup per (sequence, head).
+// Splits joined in a fixed order: one workgroup per (sequence, head), `ncol`
+// threads over the columns, 256 / ncol groups of them over the splits.
 template <class E>
-__global__ __launch_bounds__(64) void born_paged_join_kernel(PagedArgs p) {
+__global__ __launch_bounds__(256) void born_paged_join_kernel(PagedArgs p, int ncol) {
+    __shared__ f32x4v red[256];
+    __shared__ float zred[256];
     const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
+    const int col = threadIdx.x % ncol, group = threadIdx.x / ncol, groups = 256 / ncol;
     const PagedSpan sp = paged_span(p, b);
     const int n = max(1, (sp.n - (sp.first & ~31) + p.chunk - 1) / p.chunk);
     const float* part = p.part + ((int64_t)b * p.H + h) * p.nsplit * (p.D + 4);
-    const float s = arg_scale(p, h);
+    const bool ok = 4 * col < p.D;
+    f32x4v x = {0.f, 0.f, 0.f, 0.f};
     float z = 0.f;
-    for (int i = 0; i < n; ++i) z += part[(int64_t)i * (p.D + 4)];
-    const float den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
+#pragma unroll 4
+    for (int i = group; i < n; i += groups) {
+        const float* at = part + (int64_t)i * (p.D + 4);
+        z += at[0];
+        if (ok) x += *reinterpret_cast<const f32x4v*>(at + 4 + 4 * col);
+    }
+    red[threadIdx.x] = x;
+    zred[threadIdx.x] = z;
+    __syncthreads();
+    if (group != 0) return;
+    for (int i = 1; i < groups; ++i) {
+        x += red[i * ncol + col];
+        z += zred[i * ncol + col];
+    }
+    const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
     const float inv = den > 0.f && s != 0.f ? 1.0f / den : 0.f;
-    for (int col = 4 * threadIdx.x; col < p.D; col += 256) {
-        f32x4v x = {0.f, 0.f, 0.f, 0.f};
-        for (int i = 0; i < n; ++i) x += *reinterpret_cast<const f32x4v*>(part + (int64_t)i * (p.D + 4) + 4 + col);
-        x *= inv;
-        uint8_t* to = (uint8_t*)p.out + (((int64_t)b * p.H + h) * p.D + col) * kItem<E>;
-        if constexpr (std::is_same<E, F32>::value) {
-            *reinterpret_cast<f32x4v*>(to) = x;
-        } else {
-            const u32x2 y = {E::pack(x[0], x[1]), E::pack(x[2], x[3])};
-            *reinterpret_cast<u32x2*>(to) = y;
-        }
+    if (p.raw != nullptr && col == 0) p.inv[(int64_t)b * p.H + h] = inv;
+    if (!ok) return;
+    x *= inv;
+    uint8_t* to = (uint8_t*)p.out + (((int64_t)b * p.H + h) * p.D + 4 * col) * kItem<E>;
+    if constexpr (std::is_same<E, F32>::value) {
+        *reinterpret_cast<f32x4v*>(to) = x;
+    } else {
+        const u32x2 y = {E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+        *reinterpret_cast<u32x2*>(to) = y;
     }
 }
 
@@ -326,53 +450,47 @@ __global__ __launch_bounds__(64) void born_paged_join_kernel(PagedArgs p) {
 // keys per workgroup.
 template <int>
 __global__ __launch_bounds__(256) void born_paged_weigh_kernel(PagedArgs p) {
-    __shared__ float inv[256];
     const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
     const int b = rest % p.B, block = rest / p.B;
     const PagedSpan sp = paged_span(p, b);
-    const int base = sp.first & ~31;
-    const int j = base + block * 256 + threadIdx.x;
-    if (base + block * 256 >= sp.n) return;
-    const int n = max(1, (sp.n - base + p.chunk - 1) / p.chunk);
+    const int j = (sp.first & ~31) + block * 256 + threadIdx.x;
+    if (j < sp.first || j >= sp.n || j >= p.w_len) return;
+    const int64_t h0 = (int64_t)b * p.H + hk * p.G;
+    const float* raw = p.raw + h0 * p.raw_ld + j;
     float sum = 0.f;
-    for (int g0 = 0; g0 < p.G; g0 += 256) {
-        const int gn = min(256, p.G - g0);
-        if ((int)threadIdx.x < gn) {
-            const int h = hk * p.G + g0 + threadIdx.x;
-            const float* part = p.part + ((int64_t)b * p.H + h) * p.nsplit * (p.D + 4);
-            const float s = arg_scale(p, h);
-            float z = 0.f;
-            for (int i = 0; i < n; ++i) z += part[(int64_t)i * (p.D + 4)];
-            const float den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
-            inv[threadIdx.x] = den > 0.f && s != 0.f ? 1.0f / den : 0.f;
-        }
-        __syncthreads();
-        if (j >= sp.first && j < sp.n && j < p.w_len) {
-            const float* raw = p.raw + ((int64_t)b * p.H + hk * p.G + g0) * p.raw_ld + j;
-            for (int i = 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], inv[i], sum);
-        }
-        __syncthreads();
-    }
-    if (j >= sp.first && j < sp.n && j < p.w_len) p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
+#pragma unroll 4
+    for (int i = 0; i < p.G; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], p.inv[h0 + i], sum);
+    p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
 }
 
 template <class E>
 hipError_t paged_fwd(const PagedArgs& a, hipStream_t st);
 
-template <class E, bool WEIGH>
-hipError_t launch_paged_dp(const PagedArgs& a, hipStream_t st) {
+template <class E, bool WEIGH, bool P16>
+void launch_paged_dp(const PagedArgs& a, hipStream_t st) {
     const dim3 grid((unsigned)(a.B * a.nsplit * a.Hkv * a.gblocks));
-    if (a.D <= 64) hipLaunchKernelGGL((born_paged_kernel<E, 64, WEIGH>), grid, dim3(256), 0, st, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((born_paged_kernel<E, 128, WEIGH>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((born_paged_kernel<E, 256, WEIGH>), grid, dim3(256), 0, st, a);
-    return hipGetLastError();
+    if (a.D <= 64) hipLaunchKernelGGL((born_paged_kernel<E, 64, WEIGH, P16>), grid, dim3(256), 0, st, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_paged_kernel<E, 128, WEIGH, P16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((born_paged_kernel<E, 256, WEIGH, P16>), grid, dim3(256), 0, st, a);
 }
 
 template <class E>
 hipError_t launch_paged(const PagedArgs& a, hipStream_t st) {
-    hipError_t e = a.raw != nullptr ? launch_paged_dp<E, true>(a, st) : launch_paged_dp<E, false>(a, st);
+    // Offsets within a page in 32 bits; a page 0 to send masked loads to.
+    const bool p16 = a.page % 16 == 0 && a.cache_pages > 0 && a.page * a.kt < ((int64_t)1 << 31) && a.page * a.vt < ((int64_t)1 << 31);
+    if (a.raw != nullptr) {
+        if (p16) launch_paged_dp<E, true, true>(a, st);
+        else launch_paged_dp<E, true, false>(a, st);
+    } else if (p16) {
+        launch_paged_dp<E, false, true>(a, st);
+    } else {
+        launch_paged_dp<E, false, false>(a, st);
+    }
+    hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.part == nullptr) return e;
-    hipLaunchKernelGGL((born_paged_join_kernel<E>), dim3((unsigned)(a.B * a.H)), dim3(64), 0, st, a);
+    int ncol = 2;
+    while (4 * ncol < a.D) ncol *= 2;
+    hipLaunchKernelGGL((born_paged_join_kernel<E>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, st, a, ncol);
     e = hipGetLastError();
     if (e != hipSuccess || a.raw == nullptr) return e;
     const int64_t span = a.window > 0 && a.window + 32 < a.raw_ld ? a.window + 32 : a.raw_ld;

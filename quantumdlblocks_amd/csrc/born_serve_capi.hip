@@ -67,7 +67,7 @@ int check_packed(const qdl_born_packed_call* c) {
     if (c->window_size < 0 || c->window_size > (int64_t)1 << 30) return QDL_BORN_E_WINDOW;
     if (!(c->eps >= 0.0)) return QDL_BORN_E_SHAPE;
     if (!c->cu_q || !c->cu_k) return QDL_BORN_E_NULL;
-    if ((c->n_q > 0 && (!c->q || !c->out || !c->z)) || (c->n_k > 0 && (!c->k || !c->v))) return QDL_BORN_E_NULL;
+    if ((c->n_q > 0 && (!c->q || !c->out)) || (c->n_k > 0 && (!c->k || !c->v))) return QDL_BORN_E_NULL;
     if (!aligned16(c->q) || !aligned16(c->k) || !aligned16(c->v) || !aligned16(c->out)) return QDL_BORN_E_ALIGN;
     const int64_t it = item(c->dtype);
     if (!rows_ok(c->q_strides, it, c->D) || !rows_ok(c->k_strides, it, c->D) || !rows_ok(c->v_strides, it, c->D))
@@ -117,28 +117,34 @@ qdl::PackedArgs packed_args(const qdl_born_packed_call* c) {
 int64_t packed_stats(int64_t n_q, int64_t H) { return (H * n_q * 4 + 15) / 16 * 16; }
 
 // Splits of a paged launch: enough workgroups for four a compute unit, none
-// under 128 keys (a wave's 32), and at most 256 keys a wave.
+// under 128 keys (a wave's 32) or over 512.
 struct PagedPlan {
-    int64_t chunk, nsplit, span, gblocks, raw_ld, part_bytes, raw_bytes;
+    int64_t chunk, nsplit, gblocks, raw_ld, part_bytes, raw_bytes, inv_bytes;
+    int64_t bytes() const { return part_bytes + raw_bytes + inv_bytes; }
 };
-PagedPlan paged_plan(const qdl_born_paged_call* c) {
+PagedPlan paged_plan(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window, bool weigh) {
     PagedPlan r = {};
-    const int64_t room = c->pages * c->page_size;
-    r.span = c->window_size > 0 && c->window_size + 31 < room ? c->window_size + 31 : room;
-    if (r.span < 1) r.span = 1;
-    r.gblocks = (c->H / c->h_kv + 15) / 16;
-    const int64_t units = c->B * c->h_kv * r.gblocks;
+    const int64_t room = pages * page;
+    int64_t span = window > 0 && window + 31 < room ? window + 31 : room;
+    if (span < 1) span = 1;
+    r.gblocks = (H / h_kv + 15) / 16;
+    const int64_t units = B * h_kv * r.gblocks;
     const int64_t want = units > 0 ? (1024 + units - 1) / units : 1;
-    int64_t chunk = (r.span + want - 1) / want;
+    int64_t chunk = (span + want - 1) / want;
     chunk = (chunk + 127) / 128 * 128;
-    if (chunk > 1024) chunk = 1024;
+    if (chunk > 512) chunk = 512;
     r.chunk = chunk;
-    r.nsplit = (r.span + chunk - 1) / chunk;
-    const bool weigh = c->key_weight != nullptr;
+    r.nsplit = (span + chunk - 1) / chunk;
     r.raw_ld = (room + 31) / 32 * 32;
-    r.part_bytes = r.nsplit > 1 || weigh ? c->B * c->H * r.nsplit * (c->D + 4) * 4 : 0;
-    r.raw_bytes = weigh ? c->B * c->H * r.raw_ld * 4 : 0;
+    if (r.nsplit > 1 || weigh) r.part_bytes = B * H * r.nsplit * (D + 4) * 4;
+    if (weigh) {
+        r.raw_bytes = B * H * r.raw_ld * 4;
+        r.inv_bytes = (B * H * 4 + 15) / 16 * 16;
+    }
     return r;
+}
+PagedPlan paged_plan(const qdl_born_paged_call* c) {
+    return paged_plan(c->B, c->H, c->h_kv, c->D, c->pages, c->page_size, c->window_size, c->key_weight != nullptr);
 }
 
 int check_paged(const qdl_born_paged_call* c) {
@@ -193,7 +199,7 @@ int64_t qdl_flash_born_packed_workspace_size(int64_t n_q, int64_t H) {
 int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_stream_t stream) {
     const int rc = check_packed(c);
     if (rc != QDL_BORN_OK) return rc;
-    if ((c->n_q > 0 && (!c->dout || !c->dq)) || (c->n_k > 0 && (!c->dk || !c->dv))) return QDL_BORN_E_NULL;
+    if ((c->n_q > 0 && (!c->dout || !c->dq || !c->z)) || (c->n_k > 0 && (!c->dk || !c->dv))) return QDL_BORN_E_NULL;
     if (!aligned16(c->dout) || !aligned16(c->dq) || !aligned16(c->dk) || !aligned16(c->dv)) return QDL_BORN_E_ALIGN;
     if (c->n_q > 0 && !rows_ok(c->dout_strides, item(c->dtype), c->D)) return QDL_BORN_E_STRIDE;
     if (c->workspace_bytes < qdl_flash_born_packed_workspace_size(c->n_q, c->H) || !c->workspace || !aligned16(c->workspace))
@@ -218,10 +224,12 @@ int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_strea
     return hip_status(hipGetLastError());
 }
 
-int64_t qdl_flash_born_paged_workspace_size(const qdl_born_paged_call* c) {
-    if (check_paged(c) != QDL_BORN_OK || c->B == 0) return 0;
-    const PagedPlan r = paged_plan(c);
-    return r.part_bytes + r.raw_bytes;
+int64_t qdl_flash_born_paged_workspace_size(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page_size,
+                                            int64_t window_size, int weighed) {
+    if (B <= 0 || B > kMostHeads || H <= 0 || H > kMostHeads || h_kv <= 0 || H % h_kv != 0 || D <= 0 || D > 256 || pages < 0 ||
+        page_size < 1 || page_size > (int64_t)1 << 24 || pages > (int64_t)1 << 30 || pages * page_size > (int64_t)1 << 30 || window_size < 0)
+        return 0;
+    return paged_plan(B, H, h_kv, D, pages, page_size, window_size, weighed != 0).bytes();
 }
 
 int qdl_flash_born_paged_forward_call(const qdl_born_paged_call* c, qdl_stream_t stream) {
@@ -233,8 +241,7 @@ int qdl_flash_born_paged_forward_call(const qdl_born_paged_call* c, qdl_stream_t
     const int64_t it = item(c->dtype);
     if (!stride_ok(c->q_strides[0], it) || !stride_ok(c->q_strides[1], it)) return QDL_BORN_E_STRIDE;
     const PagedPlan r = paged_plan(c);
-    if (r.part_bytes + r.raw_bytes > 0 &&
-        (!c->workspace || !aligned16(c->workspace) || c->workspace_bytes < r.part_bytes + r.raw_bytes))
+    if (r.bytes() > 0 && (!c->workspace || !aligned16(c->workspace) || c->workspace_bytes < r.bytes()))
         return QDL_BORN_E_WORKSPACE;
     qdl::PagedArgs a = {};
     a.q = c->q;
@@ -274,6 +281,7 @@ int qdl_flash_born_paged_forward_call(const qdl_born_paged_call* c, qdl_stream_t
     if (r.raw_bytes > 0) {
         a.raw = reinterpret_cast<float*>(ws + r.part_bytes);
         a.raw_ld = r.raw_ld;
+        a.inv = reinterpret_cast<float*>(ws + r.part_bytes + r.raw_bytes);
         a.weights = c->key_weight;
         a.w_sb = c->weight_strides[0];
         a.w_sh = c->weight_strides[1];
@@ -376,7 +384,7 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call* c, qdl_stream_t s
     if (c->struct_bytes != (int64_t)sizeof(qdl_born_evict_call)) return QDL_BORN_E_SHAPE;
     int rc = check_heads(c->dtype, c->h_kv, c->h_kv, c->D);
     if (rc != QDL_BORN_OK) return rc;
-    if (c->B < 0 || c->B > kMostRows || c->B * c->h_kv > kMostBlocks / 4) return QDL_BORN_E_SHAPE;
+    if (c->B < 0 || c->B > kMostRows || c->B * c->h_kv > kMostBlocks / 8) return QDL_BORN_E_SHAPE;
     rc = check_cache(c->dtype, c->k_cache_strides, c->v_cache_strides, c->cache_pages, c->page_size, c->k_cache, c->v_cache,
                      c->block_table, c->pages, c->table_ld);
     if (rc != QDL_BORN_OK) return rc;
@@ -388,7 +396,7 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call* c, qdl_stream_t s
         return QDL_BORN_E_NULL;
     const int64_t it = item(c->dtype);
     const int64_t most = c->budget < c->pages * c->page_size ? c->budget : c->pages * c->page_size;  // kept rows
-    const int64_t tiles = (most + qdl::kEvictRows - 1) / qdl::kEvictRows;
+    const int64_t per = qdl::evict_rows((int)(c->D * it / 16)), tiles = (most + per - 1) / per;
     if (c->out_table && tiles * c->B * c->h_kv > kMostBlocks) return QDL_BORN_E_SHAPE;
     qdl::EvictArgs a = {};
     a.k = c->k_cache;
@@ -424,7 +432,8 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call* c, qdl_stream_t s
     a.recent = (int)c->recent;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const unsigned units = (unsigned)(c->B * c->h_kv);
-    hipLaunchKernelGGL((qdl::born_evict_select_kernel<0>), dim3(units), dim3(qdl::kEvictThreads), 0, s, a);
+    if (c->pages * c->page_size <= 256 * qdl::kEvictPer) hipLaunchKernelGGL((qdl::born_evict_select_kernel<256>), dim3(units), dim3(256), 0, s, a);
+    else hipLaunchKernelGGL((qdl::born_evict_select_kernel<1024>), dim3(units), dim3(1024), 0, s, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || most == 0 || c->cache_pages == 0) return hip_status(e);
     if (c->out_table) hipLaunchKernelGGL((qdl::born_evict_move_kernel<0>), dim3((unsigned)tiles * units), dim3(256), 0, s, a);

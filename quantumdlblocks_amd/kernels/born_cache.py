@@ -21,6 +21,8 @@ tensors that a gradient is recorded for.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _native
@@ -29,73 +31,96 @@ from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
 __all__ = ["born_cache_evict", "flash_born_attention_paged", "fused_qk_rope_l2_normalize_append"]
 
 _LIMIT = 1 << 30
+_INDEX = (torch.int32, torch.int64)
 
 
 def _no_grad(what: str, *tensors) -> None:
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
-        raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
+    for t in tensors:
+        if isinstance(t, torch.Tensor) and t.requires_grad:
+            raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
+
+
+def _bad_cache(name: str, c: torch.Tensor):
+    return ValueError(f"{name} needs unit stride along head_dim, other strides that are multiples of 16 bytes and a 16-byte "
+                      f"aligned base, got strides {c.stride()}")
 
 
 def _check_cache(k_cache, v_cache, block_table, cache_lens, B, written: bool):
-    """The caches' (page, token, head) strides."""
-    if k_cache.dim() != 4 or k_cache.shape != v_cache.shape or k_cache.dtype != v_cache.dtype:
+    """The caches' (page, token, head) strides on the GPU.  Decoding calls this
+    for every layer and token: plain tests in a row, no loops over tensors."""
+    shape, dt = k_cache.shape, k_cache.dtype
+    if len(shape) != 4 or shape != v_cache.shape or v_cache.dtype != dt:
         raise ValueError(f"k_cache and v_cache must share one (pages, page_size, key_heads, head_dim) shape and dtype, got "
-                         f"{k_cache.dtype} {tuple(k_cache.shape)}, {v_cache.dtype} {tuple(v_cache.shape)}")
-    P, page, Hkv, D = k_cache.shape
+                         f"{dt} {tuple(shape)}, {v_cache.dtype} {tuple(v_cache.shape)}")
+    P, page, Hkv, D = shape
     if page < 1 or Hkv < 1 or D < 1:
-        raise ValueError(f"page_size, key_heads and head_dim must be positive, got {tuple(k_cache.shape)}")
-    if block_table.dim() != 2 or block_table.shape[0] != B or block_table.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"block_table must be (B={B}, pages) int32, got {block_table.dtype} {tuple(block_table.shape)}")
-    if tuple(cache_lens.shape) != (B,) or cache_lens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"cache_lens must be (B={B},) int32, got {cache_lens.dtype} {tuple(cache_lens.shape)}")
-    if block_table.shape[1] * page > _LIMIT:
-        raise ValueError(f"block_table holds {block_table.shape[1]} pages of {page}: more than 2^30 keys a sequence")
-    for name, t in (("v_cache", v_cache), ("block_table", block_table), ("cache_lens", cache_lens)):
-        if t.device != k_cache.device:
-            raise ValueError(f"{name} must be on the caches' device {k_cache.device}, got {t.device}")
-    strides = []
-    for name, c in (("k_cache", k_cache), ("v_cache", v_cache)):
-        if written and any(n > 1 and s == 0 for n, s in zip(c.shape, c.stride())):
-            raise ValueError(f"{name} is written and must not overlap itself, got strides {c.stride()}")
-        if k_cache.is_cuda:
-            if D % 8 or D > MAX_HEAD_DIM or c.dtype not in _DTYPE_CODE:
-                raise NotImplementedError(f"paged caches take fp32, fp16 or bf16 and head dims that are multiples of 8 up to "
-                                          f"{MAX_HEAD_DIM}, got {c.dtype} and {D}")
-            st = [s if n > 1 else 0 for n, s in zip(c.shape, c.stride())]
-            if c.stride(3) != 1 or c.data_ptr() % 16 or any(s * c.element_size() % 16 for s in st[:3]):
-                raise ValueError(f"{name} needs unit stride along head_dim, other strides that are multiples of 16 bytes "
-                                 f"and a 16-byte aligned base, got strides {c.stride()}")
-            strides += st[:3]
-    return strides
+        raise ValueError(f"page_size, key_heads and head_dim must be positive, got {tuple(shape)}")
+    tshape, lshape = block_table.shape, cache_lens.shape
+    if len(tshape) != 2 or tshape[0] != B or block_table.dtype not in _INDEX:
+        raise ValueError(f"block_table must be (B={B}, pages) int32, got {block_table.dtype} {tuple(tshape)}")
+    if len(lshape) != 1 or lshape[0] != B or cache_lens.dtype not in _INDEX:
+        raise ValueError(f"cache_lens must be (B={B},) int32, got {cache_lens.dtype} {tuple(lshape)}")
+    if tshape[1] * page > _LIMIT:
+        raise ValueError(f"block_table holds {tshape[1]} pages of {page}: more than 2^30 keys a sequence")
+    dev = k_cache.get_device()
+    if v_cache.get_device() != dev or block_table.get_device() != dev or cache_lens.get_device() != dev:
+        raise ValueError(f"k_cache, v_cache, block_table and cache_lens must be on one device, got {k_cache.device}, "
+                         f"{v_cache.device}, {block_table.device}, {cache_lens.device}")
+    ks, vs = k_cache.stride(), v_cache.stride()
+    if written:
+        for name, st in (("k_cache", ks), ("v_cache", vs)):
+            if (st[0] == 0 and P > 1) or (st[1] == 0 and page > 1) or (st[2] == 0 and Hkv > 1) or (st[3] == 0 and D > 1):
+                raise ValueError(f"{name} is written and must not overlap itself, got strides {st}")
+    if dev < 0:
+        return ()
+    if D % 8 or D > MAX_HEAD_DIM or dt not in _DTYPE_CODE:
+        raise NotImplementedError(f"paged caches take fp32, fp16 or bf16 and head dims that are multiples of 8 up to "
+                                  f"{MAX_HEAD_DIM}, got {dt} and {D}")
+    pieces = 4 if dt is torch.float32 else 8  # elements of 16 bytes
+    k0, k1, k2 = ks[0] if P > 1 else 0, ks[1] if page > 1 else 0, ks[2] if Hkv > 1 else 0
+    v0, v1, v2 = vs[0] if P > 1 else 0, vs[1] if page > 1 else 0, vs[2] if Hkv > 1 else 0
+    if ks[3] != 1 or k0 % pieces or k1 % pieces or k2 % pieces or k_cache.data_ptr() % 16:
+        raise _bad_cache("k_cache", k_cache)
+    if vs[3] != 1 or v0 % pieces or v1 % pieces or v2 % pieces or v_cache.data_ptr() % 16:
+        raise _bad_cache("v_cache", v_cache)
+    return k0, k1, k2, v0, v1, v2
 
 
 def _index(t: torch.Tensor) -> torch.Tensor:
-    if t.dtype != torch.int32:
+    """1-D int32, contiguous."""
+    if t.dtype is not torch.int32:
         t = t.to(torch.int32)
-    return t if t.numel() == 0 or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
+    return t if t.is_contiguous() else t.contiguous()
 
 
-def _table_ld(t: torch.Tensor) -> int:
-    return t.stride(0) if t.shape[0] > 1 else t.shape[1]
-
-
-def _table(t: torch.Tensor) -> torch.Tensor:
-    t = _index(t)
-    return t if t.shape[0] <= 1 or t.stride(0) >= t.shape[1] else t.contiguous()
+def _table(t: torch.Tensor):
+    """int32 rows of unit stride, and their distance."""
+    if t.dtype is not torch.int32:
+        t = t.to(torch.int32)
+    if t.is_contiguous():
+        return t, t.shape[1]
+    if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:
+        t = t.contiguous()
+    return t, t.stride(0) if t.shape[0] > 1 else t.shape[1]
 
 
 def _heads(t: torch.Tensor, dtype: torch.dtype):
     """(n, heads, D) rows in ``dtype`` and their (row, head) strides."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         t = t.to(dtype)
-    item = t.element_size()
-    st = [s if n > 1 else 0 for n, s in zip(t.shape, t.stride())]
-    if t.stride(2) != 1 or t.data_ptr() % 16 or any(s * item % 16 or s < 0 for s in st[:2]):
+    n, h, _ = t.shape
+    s0, s1, s2 = t.stride()
+    pieces = 4 if dtype is torch.float32 else 8
+    if n <= 1:
+        s0 = 0
+    if h <= 1:
+        s1 = 0
+    if s2 != 1 or s0 % pieces or s1 % pieces or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
-        st = list(t.stride())
-    return t, st[0], st[1]
+        s0, s1, _ = t.stride()
+    return t, s0, s1
 
 
 def _slots(block_table, page, slots):
@@ -111,6 +136,11 @@ def _slots(block_table, page, slots):
 # ---------------------------------------------------------------------------
 # One new token per sequence
 # ---------------------------------------------------------------------------
+@functools.lru_cache(maxsize=256)
+def _paged_workspace(*sizes) -> int:
+    return int(_native.load().qdl_flash_born_paged_workspace_size(*sizes))
+
+
 def _eager_paged(q, k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight):
     B, H, D = q.shape
     P, page, Hkv, _ = k_cache.shape
@@ -165,7 +195,8 @@ def flash_born_attention_paged(
     Lengths past the table's pages are cut to them; a sequence without visible
     keys gets zeros.
     """
-    _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
+    if torch.is_grad_enabled():
+        _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
     if q.dim() != 3:
         raise ValueError(f"q must be (B, heads, head_dim), got shape {tuple(q.shape)}")
     B, H, D = q.shape
@@ -173,40 +204,43 @@ def flash_born_attention_paged(
     P, page, Hkv, Dk = k_cache.shape
     if Dk != D or H < 1 or H % Hkv:
         raise ValueError(f"q {tuple(q.shape)} does not fit caches of {Hkv} key heads of {Dk}")
-    if q.device != k_cache.device:
+    if q.get_device() != k_cache.get_device():
         raise ValueError(f"q must be on the caches' device {k_cache.device}, got {q.device}")
-    n_scale = scale.numel() if isinstance(scale, torch.Tensor) else 1
-    if n_scale not in (1, H):
-        raise ValueError(f"scale must hold 1 value or H={H} per-head values, got {n_scale}")
-    if not float(eps) >= 0.0:
+    dev, eps = q.device, float(eps)
+    # A scale tensor is kept alive here until the call: the block holds addresses.
+    if isinstance(scale, torch.Tensor):
+        if scale.numel() not in (1, H):
+            raise ValueError(f"scale must hold 1 value or H={H} per-head values, got {scale.numel()}")
+        scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
+    else:
+        scale_flat, scale_p, n_scale, scale_value = None, 0, 1, float(scale)
+    if not eps >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
     window = min(max(int(window_size), 0), _LIMIT)
     w_ptr = w_sb = w_sh = w_len = 0
     if key_weight is not None:
         if (key_weight.dim() != 3 or tuple(key_weight.shape[:2]) != (B, Hkv) or key_weight.dtype != torch.float32
-                or key_weight.device != k_cache.device or (key_weight.numel() and key_weight.shape[2] > 1 and key_weight.stride(2) != 1)
+                or key_weight.device != dev or (key_weight.numel() and key_weight.shape[2] > 1 and key_weight.stride(2) != 1)
                 or any(n > 1 and s == 0 for n, s in zip(key_weight.shape, key_weight.stride()))):
-            raise ValueError(f"key_weight must be (B={B}, key_heads={Hkv}, keys) fp32 on {k_cache.device} with unit stride along "
+            raise ValueError(f"key_weight must be (B={B}, key_heads={Hkv}, keys) fp32 on {dev} with unit stride along "
                              f"the keys, got {key_weight.dtype} {tuple(key_weight.shape)} on {key_weight.device}, strides "
                              f"{key_weight.stride()}")
         w_ptr, w_sb, w_sh, w_len = key_weight.data_ptr(), key_weight.stride(0), key_weight.stride(1), key_weight.shape[2]
     if not q.is_cuda:
-        scale_t = scale if isinstance(scale, torch.Tensor) else torch.tensor(float(scale), dtype=torch.float64)
-        return _eager_paged(q.detach(), k_cache, v_cache, block_table, cache_lens, scale_t.detach(), float(eps), window, key_weight)
+        scale_t = scale.detach() if isinstance(scale, torch.Tensor) else torch.tensor(scale_value, dtype=torch.float64)
+        return _eager_paged(q.detach(), k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight)
     lib = _native.load()
-    dev = q.device
-    # Kept alive here until the call: the block holds addresses.
-    scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
-    q_c, sb, sh = _heads(q.detach(), k_cache.dtype)
-    table, lens = _table(block_table), _index(cache_lens)
-    out = torch.empty((B, H, D), dtype=k_cache.dtype, device=dev)
-    head = (_DTYPE_CODE[k_cache.dtype], B, H, Hkv, D, q_c.data_ptr(), sb, sh, out.data_ptr(), k_cache.data_ptr(),
-            v_cache.data_ptr(), *strides, P, page, table.data_ptr(), table.shape[1], _table_ld(table), lens.data_ptr(),
-            scale_p, n_scale, scale_value, window, float(eps), w_ptr, w_sb, w_sh, w_len)
-    size = int(lib.qdl_flash_born_paged_workspace_size(_native.paged_call(*head, 0, 0)))
+    dt = k_cache.dtype
+    q_c, sb, sh = _heads(q, dt)
+    (table, ld), lens = _table(block_table), _index(cache_lens)
+    pages = table.shape[1]
+    out = torch.empty((B, H, D), dtype=dt, device=dev)
+    size = _paged_workspace(B, H, Hkv, D, pages, page, window, w_ptr != 0)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
-    _run_call(lib.qdl_flash_born_paged_forward_call, "qdl_flash_born_paged_forward_call", dev,
-              _native.paged_call(*head, 0 if ws is None else ws.data_ptr(), size))
+    _run_call(lib.qdl_flash_born_paged_forward_call, "qdl_flash_born_paged_forward_call", dev, _native.paged_call(
+        _DTYPE_CODE[dt], B, H, Hkv, D, q_c.data_ptr(), sb, sh, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *strides,
+        P, page, table.data_ptr(), pages, ld, lens.data_ptr(), scale_p, n_scale, scale_value, window, eps, w_ptr, w_sb, w_sh, w_len,
+        0 if ws is None else ws.data_ptr(), size))
     return out
 
 
@@ -214,7 +248,11 @@ def flash_born_attention_paged(
 # New tokens
 # ---------------------------------------------------------------------------
 def _tables(cos, sin, half, device):
-    """(rows, n) fp32 tables with n = min(width, half)."""
+    """(rows, n) fp32 tables with n = min(width, half), and their row stride."""
+    if (cos.dim() == 2 and cos.shape == sin.shape and cos.shape[1] <= half and cos.shape[0] > 0 and cos.dtype is torch.float32
+            and sin.dtype is torch.float32 and cos.device == device and sin.device == device and cos.is_contiguous()
+            and sin.is_contiguous()):
+        return cos, sin, cos.shape[1]  # the usual tables: as they are
     out = []
     for t in (cos, sin):
         t = t.detach()
@@ -231,7 +269,9 @@ def _tables(cos, sin, half, device):
     n = out[0].shape[1]
     same = out[0].stride() == out[1].stride() and (n <= 1 or out[0].stride(1) == 1) and (
         out[0].shape[0] == 1 or out[0].stride(0) >= n)
-    return out if same else [t.contiguous() for t in out]
+    if not same:
+        out = [t.contiguous() for t in out]
+    return *out, out[0].stride(0) if out[0].shape[0] > 1 else n
 
 
 def _eager_append(q, k, v, tables, k_cache, v_cache, block_table, cache_lens, cu, positions, eps):
@@ -257,7 +297,7 @@ def _eager_append(q, k, v, tables, k_cache, v_cache, block_table, cache_lens, cu
     else:
         at = (slot if positions is None else positions.long()).clamp(0, tables[0].shape[0] - 1)
         pad = (0, half - tables[0].shape[1])
-        cos, sin = (torch.nn.functional.pad(x.to(wide)[at], pad, value=one).unsqueeze(1) for x, one in zip(tables, (1.0, 0.0)))
+        cos, sin = (torch.nn.functional.pad(x.to(wide)[at], pad, value=one).unsqueeze(1) for x, one in zip(tables[:2], (1.0, 0.0)))
 
     def turned(x):
         x1, x2 = x.to(wide)[..., :half], x.to(wide)[..., half:]
@@ -305,52 +345,58 @@ def fused_qk_rope_l2_normalize_append(
     16 bits as the reference does.  Values that no sequence owns come out as
     zero queries; slots without a page are not written.
     """
-    what = "fused_qk_rope_l2_normalize_append"
-    _no_grad(what, q, k, v, k_cache, v_cache)
-    if q.dim() != 3 or k.dim() != 3 or k.shape != v.shape or k.shape[0] != q.shape[0] or k.shape[2] != q.shape[2]:
+    if torch.is_grad_enabled():
+        _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, k_cache, v_cache)
+    kshape = k.shape
+    if q.dim() != 3 or len(kshape) != 3 or kshape != v.shape or kshape[0] != q.shape[0] or kshape[2] != q.shape[2]:
         raise ValueError(f"q must be (N, heads, head_dim) and k, v (N, key_heads, head_dim), got {tuple(q.shape)}, "
-                         f"{tuple(k.shape)}, {tuple(v.shape)}")
+                         f"{tuple(kshape)}, {tuple(v.shape)}")
     N, H, D = q.shape
     B = block_table.shape[0] if block_table.dim() == 2 else -1
     strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
     P, page, Hkv, Dk = k_cache.shape
-    if Dk != D or k.shape[1] != Hkv or H < 1 or H % Hkv or D % 2:
-        raise ValueError(f"q {tuple(q.shape)} and k {tuple(k.shape)} do not fit caches of {Hkv} key heads of {Dk}, or "
+    if Dk != D or kshape[1] != Hkv or H < 1 or H % Hkv or D % 2:
+        raise ValueError(f"q {tuple(q.shape)} and k {tuple(kshape)} do not fit caches of {Hkv} key heads of {Dk}, or "
                          f"head_dim is odd")
+    dev, at = k_cache.device, k_cache.get_device()
+    if q.get_device() != at or k.get_device() != at or v.get_device() != at:
+        raise ValueError(f"q, k and v must be on the caches' device {dev}, got {q.device}, {k.device}, {v.device}")
     if cu_seqlens is None:
         if N != B:
             raise ValueError(f"without cu_seqlens there is one token per sequence, got {N} tokens and {B} sequences")
-    elif tuple(cu_seqlens.shape) != (B + 1,) or cu_seqlens.dtype not in (torch.int32, torch.int64):
-        raise ValueError(f"cu_seqlens must be (B + 1 = {B + 1},) int32, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)}")
-    if positions is not None and (tuple(positions.shape) != (N,) or positions.dtype not in (torch.int32, torch.int64)):
-        raise ValueError(f"positions must be (N={N},) int32, got {positions.dtype} {tuple(positions.shape)}")
+    elif cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1 or cu_seqlens.dtype not in _INDEX or cu_seqlens.get_device() != at:
+        raise ValueError(f"cu_seqlens must be (B + 1 = {B + 1},) int32 on {dev}, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} "
+                         f"on {cu_seqlens.device}")
+    if positions is not None and (positions.dim() != 1 or positions.shape[0] != N or positions.dtype not in _INDEX
+                                  or positions.get_device() != at):
+        raise ValueError(f"positions must be (N={N},) int32 on {dev}, got {positions.dtype} {tuple(positions.shape)} on "
+                         f"{positions.device}")
     if (cos is None) != (sin is None):
         raise ValueError("cos and sin come together")
-    if not float(eps) >= 0.0:
+    eps = float(eps)
+    if not eps >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
-    dev = k_cache.device
-    for name, t in (("q", q), ("k", k), ("v", v), ("cu_seqlens", cu_seqlens), ("positions", positions)):
-        if t is not None and t.device != dev:
-            raise ValueError(f"{name} must be on the caches' device {dev}, got {t.device}")
     tables = None if cos is None else _tables(cos, sin, D // 2, dev)
-    if not q.is_cuda:
+    if at < 0:
         return _eager_append(q.detach(), k.detach(), v.detach(), tables, k_cache, v_cache, block_table, cache_lens, cu_seqlens,
-                             positions, float(eps))
+                             positions, eps)
     lib = _native.load()
     dt = k_cache.dtype
-    (q_c, *qs), (k_c, *ks), (v_c, *vs) = (_heads(x.detach(), dt) for x in (q, k, v))
-    table, lens = _table(block_table), _index(cache_lens)
-    cu, pos = (None if x is None else _index(x) for x in (cu_seqlens, positions))
+    q_c, q0, q1 = _heads(q, dt)
+    k_c, k0, k1 = _heads(k, dt)
+    v_c, v0, v1 = _heads(v, dt)
+    (table, ld), lens = _table(block_table), _index(cache_lens)
+    cu = None if cu_seqlens is None else _index(cu_seqlens)
+    pos = None if positions is None else _index(positions)
     out = torch.empty((N, H, D), dtype=dt, device=dev)
     if tables is None:
         rot = (0, 0, 0, 0, 0)
     else:
-        c, s = tables
-        rot = (c.data_ptr(), s.data_ptr(), c.shape[0], c.shape[1], c.stride(0) if c.shape[0] > 1 else c.shape[1])
+        rot = (tables[0].data_ptr(), tables[1].data_ptr(), *tables[0].shape, tables[2])
     _run_call(lib.qdl_flash_born_cache_append_call, "qdl_flash_born_cache_append_call", dev, _native.append_call(
-        _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), *qs, *ks, *vs, out.data_ptr(),
-        k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(), table.shape[1], _table_ld(table),
-        lens.data_ptr(), 0 if cu is None else cu.data_ptr(), *rot, 0 if pos is None else pos.data_ptr(), float(eps)))
+        _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
+        k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(), table.shape[1], ld, lens.data_ptr(),
+        0 if cu is None else cu.data_ptr(), *rot, 0 if pos is None else pos.data_ptr(), eps))
     return out
 
 
@@ -419,42 +465,45 @@ def born_cache_evict(
     behind the last.  Keys stay rotated by the positions that they were appended
     at: pass ``positions`` to the next append.
     """
-    _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
+    if torch.is_grad_enabled():
+        _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
     strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
     P, page, Hkv, D = k_cache.shape
+    dev, at = k_cache.device, k_cache.get_device()
     budget, recent = int(budget), int(recent)
     if not 0 <= budget <= _LIMIT or not 0 <= recent <= _LIMIT:
         raise ValueError(f"budget and recent must be at least 0 and within 2^30, got {budget} and {recent}")
-    if (key_weight.dim() != 3 or tuple(key_weight.shape[:2]) != (B, Hkv) or key_weight.dtype != torch.float32
-            or key_weight.device != k_cache.device):
-        raise ValueError(f"key_weight must be (B={B}, key_heads={Hkv}, keys) fp32 on {k_cache.device}, got {key_weight.dtype} "
-                         f"{tuple(key_weight.shape)} on {key_weight.device}")
-    most = min(budget, block_table.shape[1] * page)
+    wshape = key_weight.shape
+    if len(wshape) != 3 or wshape[0] != B or wshape[1] != Hkv or key_weight.dtype is not torch.float32 or key_weight.get_device() != at:
+        raise ValueError(f"key_weight must be (B={B}, key_heads={Hkv}, keys) fp32 on {dev}, got {key_weight.dtype} "
+                         f"{tuple(wshape)} on {key_weight.device}")
     if out_block_table is not None:
-        if (out_block_table.dim() != 2 or out_block_table.shape[0] != B or out_block_table.dtype not in (torch.int32, torch.int64)
-                or out_block_table.device != k_cache.device):
-            raise ValueError(f"out_block_table must be (B={B}, pages) int32 on {k_cache.device}, got {out_block_table.dtype} "
-                             f"{tuple(out_block_table.shape)} on {out_block_table.device}")
-        if out_block_table.shape[1] * page < most:
-            raise ValueError(f"out_block_table holds {out_block_table.shape[1]} pages of {page}: fewer than the {most} keys kept")
-        if out_block_table.shape[1] * page > _LIMIT:
-            raise ValueError(f"out_block_table holds {out_block_table.shape[1]} pages of {page}: more than 2^30 keys a sequence")
-        if out_block_table.numel() and out_block_table.data_ptr() == block_table.data_ptr():
+        tshape = out_block_table.shape
+        if len(tshape) != 2 or tshape[0] != B or out_block_table.dtype not in _INDEX or out_block_table.get_device() != at:
+            raise ValueError(f"out_block_table must be (B={B}, pages) int32 on {dev}, got {out_block_table.dtype} {tuple(tshape)} "
+                             f"on {out_block_table.device}")
+        most = min(budget, block_table.shape[1] * page)
+        if tshape[1] * page < most:
+            raise ValueError(f"out_block_table holds {tshape[1]} pages of {page}: fewer than the {most} keys kept")
+        if tshape[1] * page > _LIMIT:
+            raise ValueError(f"out_block_table holds {tshape[1]} pages of {page}: more than 2^30 keys a sequence")
+        if tshape[1] and B and out_block_table.data_ptr() == block_table.data_ptr():
             raise ValueError("out_block_table is block_table itself: leave it out to compact in place")
-    if not k_cache.is_cuda:
+    if at < 0:
         return _eager_evict(k_cache, v_cache, block_table, cache_lens, key_weight, budget, recent, out_block_table)
     lib = _native.load()
-    dev = k_cache.device
-    w = key_weight if key_weight.numel() == 0 or key_weight.shape[2] <= 1 or key_weight.stride(2) == 1 else key_weight.contiguous()
-    table, lens = _table(block_table), _index(cache_lens)
-    to = None if out_block_table is None else _table(out_block_table)
-    weight = torch.empty((B, Hkv, w.shape[2]), dtype=torch.float32, device=dev)
+    w = key_weight
+    if not w.is_contiguous() and wshape[2] > 1 and w.stride(2) != 1:
+        w = w.contiguous()
+    (table, ld), lens = _table(block_table), _index(cache_lens)
+    to, to_ld = (None, 0) if out_block_table is None else _table(out_block_table)
+    weight = torch.empty(wshape, dtype=torch.float32, device=dev)
     new_lens = torch.empty(B, dtype=torch.int32, device=dev)
     kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
     _run_call(lib.qdl_flash_born_cache_evict_call, "qdl_flash_born_cache_evict_call", dev, _native.evict_call(
         _DTYPE_CODE[k_cache.dtype], B, Hkv, D, k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(),
-        table.shape[1], _table_ld(table), lens.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1), w.shape[2], budget, recent,
-        0 if to is None else to.data_ptr(), 0 if to is None else to.shape[1], 0 if to is None else _table_ld(to),
+        table.shape[1], ld, lens.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1), wshape[2], budget, recent,
+        0 if to is None else to.data_ptr(), 0 if to is None else to.shape[1], to_ld,
         weight.data_ptr(), new_lens.data_ptr(), kept.data_ptr()))
     return new_lens, weight, kept

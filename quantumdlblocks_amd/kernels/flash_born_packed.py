@@ -32,14 +32,18 @@ def _token_rows(t: torch.Tensor, dtype: torch.dtype, dp: int):
     """``t`` (N, heads, D) in ``dtype``, zero-padded to ``dp`` columns, and its
     (token, head) strides, read in place where the kernels can: unit stride
     along D, 16-byte pieces, tokens that do not overlap."""
-    if t.dtype != dtype:
+    if t.dtype is not dtype:
         t = t.to(dtype)
-    t = _pad_head(t, dp)
-    n, h, _ = t.shape
-    item = t.element_size()
-    st, sh = (t.stride(0) if n > 1 else h * dp), (t.stride(1) if h > 1 else 0)
-    if (t.stride(2) != 1 or t.data_ptr() % 16 or st * item % 16 or sh * item % 16 or st < dp or sh < 0
-            or st * item >= 1 << 24):
+    n, h, d = t.shape
+    if d != dp:
+        t = _pad_head(t, dp)
+    st, sh, sd = t.stride()
+    if n <= 1:
+        st = h * dp
+    if h <= 1:
+        sh = 0
+    pieces = 4 if dtype is torch.float32 else 8  # elements of 16 bytes
+    if sd != 1 or st % pieces or sh % pieces or st < dp or st >= pieces << 20 or t.data_ptr() % 16:
         t = t.contiguous()
         if t.data_ptr() % 16:
             t = t.clone()
@@ -48,30 +52,72 @@ def _token_rows(t: torch.Tensor, dtype: torch.dtype, dp: int):
 
 
 def _starts(cu: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if cu.dtype != torch.int32 or cu.device != device:
+    if cu.dtype is not torch.int32 or cu.device != device:
         cu = cu.to(device=device, dtype=torch.int32)
-    return cu.contiguous()
+    return cu if cu.is_contiguous() else cu.contiguous()
+
+
+def _bad_starts(name, cu):
+    return ValueError(f"{name} must be a 1-D int32 or int64 tensor of sequences + 1 starts, got {cu.dtype} {tuple(cu.shape)}")
 
 
 def _check(q, k, v, n_scale, cu_q, cu_k):
-    if q.dim() != 3:
-        raise ValueError(f"q must be (tokens, heads, head_dim), got shape {tuple(q.shape)}")
-    if k.dim() != 3 or k.shape != v.shape or k.shape[2] != q.shape[2]:
+    qs, ks = q.shape, k.shape
+    if len(qs) != 3:
+        raise ValueError(f"q must be (tokens, heads, head_dim), got shape {tuple(qs)}")
+    if len(ks) != 3 or ks != v.shape or ks[2] != qs[2]:
         raise ValueError(f"k and v must share one (tokens, key_heads, head_dim) shape with q's head_dim, got "
-                         f"{tuple(q.shape)}, {tuple(k.shape)}, {tuple(v.shape)}")
-    H, Hkv = q.shape[1], k.shape[1]
-    if Hkv < 1 or H < 1 or H % Hkv or q.shape[2] < 1:
+                         f"{tuple(qs)}, {tuple(ks)}, {tuple(v.shape)}")
+    H, Hkv = qs[1], ks[1]
+    if Hkv < 1 or H < 1 or H % Hkv or qs[2] < 1:
         raise ValueError(f"the {H} query heads must be a multiple of the {Hkv} key heads, and head_dim positive")
-    if n_scale not in (1, H):
+    if n_scale != 1 and n_scale != H:
         raise ValueError(f"scale must hold 1 value or H={H} per-head values, got {n_scale}")
-    for name, cu in (("cu_seqlens_q", cu_q), ("cu_seqlens_k", cu_k)):
-        if cu.dim() != 1 or cu.numel() < 1 or cu.dtype not in (torch.int32, torch.int64):
-            raise ValueError(f"{name} must be a 1-D int32 or int64 tensor of sequences + 1 starts, got "
-                             f"{cu.dtype} {tuple(cu.shape)}")
-    if cu_q.numel() != cu_k.numel():
-        raise ValueError(f"cu_seqlens_q and cu_seqlens_k name {cu_q.numel() - 1} and {cu_k.numel() - 1} sequences")
-    if not q.device == k.device == v.device:
+    if cu_q.dim() != 1 or cu_q.shape[0] < 1 or cu_q.dtype not in (torch.int32, torch.int64):
+        raise _bad_starts("cu_seqlens_q", cu_q)
+    if cu_k is not cu_q:
+        if cu_k.dim() != 1 or cu_k.shape[0] < 1 or cu_k.dtype not in (torch.int32, torch.int64):
+            raise _bad_starts("cu_seqlens_k", cu_k)
+        if cu_q.shape[0] != cu_k.shape[0]:
+            raise ValueError(f"cu_seqlens_q and cu_seqlens_k name {cu_q.shape[0] - 1} and {cu_k.shape[0] - 1} sequences")
+    at = q.get_device()
+    if k.get_device() != at or v.get_device() != at:
         raise ValueError(f"q, k, v must be on one device, got {q.device}, {k.device}, {v.device}")
+
+
+def _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, train):
+    """The call: (output, argument block's head, what the backward needs)."""
+    lib = _native.load()
+    target = _autocast_dtype(q) or v.dtype
+    if target not in _DTYPE_CODE:
+        raise TypeError(f"flash_born_attention_packed: unsupported dtype {target}")
+    dev = q.device
+    scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
+    N, H, D = q.shape
+    M, Hkv, _ = k.shape
+    dp = (D + 7) // 8 * 8
+    q_c, q0, q1 = _token_rows(q, target, dp)
+    k_c, k0, k1 = _token_rows(k, target, dp)
+    v_c, v0, v1 = _token_rows(v, target, dp)
+    cs_q = _starts(cu_q, dev)
+    cs_k = cs_q if cu_k is cu_q else _starts(cu_k, dev)
+    out = torch.empty((N, H, dp), dtype=target, device=dev)
+    z = torch.empty((H, N), dtype=torch.float32, device=dev) if train else None
+    head = (_DTYPE_CODE[target], cs_q.shape[0] - 1, N, M, H, Hkv, dp, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(),
+            q0, q1, k0, k1, v0, v1, out.data_ptr(), z.data_ptr() if train else 0, cs_q.data_ptr(), cs_k.data_ptr(), scale_p,
+            n_scale, scale_value, 1 if is_causal else 0, window, eps)
+    _run_call(lib.qdl_flash_born_packed_forward_call, "qdl_flash_born_packed_forward_call", dev,
+              _native.packed_call(*head, 0, 0, 0, 0, 0, 0, 0, 0, 0))
+    return out if dp == D else out[..., :D].contiguous(), head, (q_c, k_c, v_c, out, z, scale_flat, cs_q, cs_k)
+
+
+@torch.compiler.disable
+def _call_uncompiled(fn, args):
+    return fn(*args)
+
+
+def _uncompiled(fn, *args):
+    return _call_uncompiled(fn, args) if torch.compiler.is_compiling() else fn(*args)
 
 
 class _FlashBornPackedFn(torch.autograd.Function):
@@ -81,33 +127,13 @@ class _FlashBornPackedFn(torch.autograd.Function):
 
     @staticmethod
     def forward(ctx, q, k, v, scale, cu_q, cu_k, is_causal, eps, window):
-        lib = _native.load()
-        target = _autocast_dtype(q) or v.dtype
-        if target not in _DTYPE_CODE:
-            raise TypeError(f"flash_born_attention_packed: unsupported dtype {target}")
-        dev = q.device
-        scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
-        N, H, D = q.shape
-        M, Hkv, _ = k.shape
-        dp = (D + 7) // 8 * 8
-        q_c, *qs = _token_rows(q, target, dp)
-        k_c, *ks = _token_rows(k, target, dp)
-        v_c, *vs = _token_rows(v, target, dp)
-        cu_q, cu_k = _starts(cu_q, dev), _starts(cu_k, dev)
-        out = torch.empty((N, H, dp), dtype=target, device=dev)
-        z = torch.empty((H, N), dtype=torch.float32, device=dev)
-        head = (_DTYPE_CODE[target], cu_q.numel() - 1, N, M, H, Hkv, dp, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(),
-                *qs, *ks, *vs, out.data_ptr(), z.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), scale_p, n_scale, scale_value,
-                1 if is_causal else 0, window, float(eps))
-        _run_call(lib.qdl_flash_born_packed_forward_call, "qdl_flash_born_packed_forward_call", dev,
-                  _native.packed_call(*head, *(0,) * 9))
-        ctx.save_for_backward(q_c, k_c, v_c, out, z, scale_flat, cu_q, cu_k)
-        ctx.head = head
-        ctx.head_dim = D
-        if scale_flat is not None:
+        out, ctx.head, saved = _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, True)
+        ctx.save_for_backward(*saved)
+        ctx.head_dim = q.shape[2]
+        if isinstance(scale, torch.Tensor):
             ctx.scale_shape, ctx.scale_dtype = scale.shape, scale.dtype
         ctx.dtypes = (q.dtype, k.dtype, v.dtype)
-        return out if dp == D else out[..., :D].contiguous()
+        return out
 
     @staticmethod
     def backward(ctx, do):
@@ -201,6 +227,9 @@ def flash_born_attention_packed(
     if not float(eps) >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
     if q.is_cuda and q.shape[2] <= MAX_HEAD_DIM:
-        return _apply(_FlashBornPackedFn, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
+        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                        or (isinstance(scale, torch.Tensor) and scale.requires_grad)):
+            return _apply(_FlashBornPackedFn, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
+        return _uncompiled(_forward, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window, False)[0]
     scale_t = scale if isinstance(scale, torch.Tensor) else torch.tensor(float(scale), dtype=torch.float64)
     return _eager_packed(q, k, v, scale_t, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)

@@ -261,7 +261,8 @@ def test_empty_calls_launch_nothing():
     assert lib.qdl_flash_born_paged_forward_call(_paged_block(B=0), None) == 0
     assert lib.qdl_flash_born_cache_append_call(_append_block(n=0, B=0), None) == 0
     assert lib.qdl_flash_born_cache_evict_call(_evict_block(B=0), None) == 0
-    assert lib.qdl_flash_born_paged_workspace_size(_paged_block(B=0)) == 0
+    assert lib.qdl_flash_born_paged_workspace_size(0, 4, 2, 64, 4, 16, 0, 0) == 0
+    assert lib.qdl_flash_born_paged_workspace_size(2, 4, 3, 64, 4, 16, 0, 0) == 0
     for call in (lib.qdl_flash_born_paged_forward_call, lib.qdl_flash_born_cache_append_call, lib.qdl_flash_born_cache_evict_call):
         assert call(None, None) == -5
         assert call(b"\x08" + bytes(511), None) == -2

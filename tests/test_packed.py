@@ -87,7 +87,7 @@ def _packed_block(**over):
 
 @pytest.mark.parametrize("over,code", [
     (dict(dtype=5), -1), (dict(n_q=-1), -2), (dict(sequences=1 << 27), -2), (dict(eps=-1.0), -2), (dict(eps=float("nan")), -2),
-    (dict(D=12), -3), (dict(D=264), -3), (dict(q=8), -4), (dict(out=8), -4), (dict(k=0), -5), (dict(cu_q=0), -5), (dict(z=0), -5),
+    (dict(D=12), -3), (dict(D=264), -3), (dict(q=8), -4), (dict(out=8), -4), (dict(k=0), -5), (dict(cu_q=0), -5),
     (dict(scale=16, n_scale=3), -6), (dict(window=-1), -7), (dict(window=1 << 31), -7), (dict(H=3), -13), (dict(h_kv=0), -13),
     (dict(qs0=32), -14), (dict(qs0=257), -14), (dict(ks1=-64), -14), (dict(vs0=1 << 23), -14), (dict(H=1 << 20, h_kv=2), -2),
 ])
@@ -103,6 +103,7 @@ def test_backward_block_checks():
     assert call(_packed_block(ws=0), None) == -8
     assert call(_packed_block(dout=0), None) == -5
     assert call(_packed_block(dk=0), None) == -5
+    assert call(_packed_block(z=0), None) == -5
     assert call(_packed_block(dq=8), None) == -4
     assert call(_packed_block(ds0=16), None) == -14
     assert call(None, None) == -5
