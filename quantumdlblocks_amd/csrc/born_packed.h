@@ -13,13 +13,15 @@
 //   dK_j = 2 sign(s) sum_i u_ij q_i,  dV_j = sum_i relu(r_ij)^2 zs_i dO_i,
 // the last two over the queries of all G heads of the group, in a fixed order.
 //
-// What bounds them: the matrix pipe.  A workgroup's four waves own 32
-// stationary rows each (queries in the forward and dQ, keys in dK/dV) and
-// share the tiles of the streamed operands, which LDS-DMA loads bring into a
-// ring of stages, one barrier per tile.  The weights of a row have no running
-// maximum, so nothing but the sums passes from tile to tile.
+// What bounds them: the matrix pipe.  A workgroup's four waves share the tiles
+// of the streamed operands, which LDS-DMA loads bring into a ring of two stages,
+// one barrier per tile.  Each wave owns 32 stationary rows (queries in the
+// forward and dQ, keys in dK/dV); the weights of a row have no running maximum,
+// so waves may also share stationary rows and take different rows of each tile
+// (SPLIT of them), their sums meeting in LDS once, at the end: fewer rows per
+// block, so more and shorter blocks.
 //
-// Blocks: sequence s takes the block slots from cu[s] / BM + s on.  Since
+// Blocks of BM rows: sequence s takes the block slots from cu[s] / BM + s on.  Since
 // ceil(len / BM) <= cu[s+1] / BM - cu[s] / BM + 1 they never overlap, so the
 // grid follows from N and S alone (no copy of the lengths to the host, no list
 // made by another launch), and a block finds its sequence by a 64-way search.
@@ -47,7 +49,7 @@ struct PackedArgs {
     void *out, *dq, *dk, *dv;
     float* z;       // (H, Nq), or nullptr: no backward follows
     float* ndelta;  // (H, Nq) workspace: -(dO . O)
-    float* zs;      // (H, Nq) workspace: s^2 / Z
+    float* zs;      // (H, Nq) workspace: sign(s) s^2 / Z (fp16: times kUp)
     const float* scale;  // 1 or H values, or nullptr: scale_value
     float scale_value;
     int per_head_scale;
@@ -59,7 +61,7 @@ struct PackedArgs {
 };
 
 constexpr int kPackedWaves = 4;
-constexpr int kPackedRows = 32 * kPackedWaves;  // stationary rows per workgroup
+constexpr int packed_rows(int split) { return 32 * kPackedWaves / split; }  // stationary rows per workgroup
 
 // A sequence's rows: queries q0 .. q0 + nq - 1, keys k0 .. k0 + nk - 1.
 struct PackedSeq {
@@ -71,26 +73,50 @@ __device__ __forceinline__ int packed_start(const int32_t* cu, int s, int N) {
     return s == 0 ? 0 : min(max(cu[s], 0), N);
 }
 
-// The sequence and tile of block slot x, slots counted along `cu` (N rows).
-__device__ __forceinline__ int packed_find(const int32_t* cu, int S, int N, int x) {
-    const int lane = threadIdx.x & 63;
-    int lo = 0, hi = S + 1;
-    while (hi - lo > 1) {
-        const int step = (hi - lo + 63) / 64;
-        const int s = lo + (lane + 1) * step;
-        const bool below = s < hi && packed_start(cu, s, N) / kPackedRows + s <= x;
-        lo += (int)__popcll(__ballot(below)) * step;
-        hi = min(hi, lo + step);
-    }
-    return __builtin_amdgcn_readfirstlane(lo);
-}
-
-template <bool KEYS>
+// Block x of the launch: a tile of BM query rows or (KEYS) key rows.  Slots are
+// counted along `cu`; the sequence is found by a 64-way search.  Under plain
+// causality, with few enough sequences for a lane each, the blocks go in the
+// order of their work instead, over all sequences (a block's tiles are those
+// before its queries or behind its keys): a launch ends with short blocks
+// (packed training step of 8 sequences, 16384 tokens: dK/dV 600 -> 505 us).
+template <bool KEYS, int BM>
 __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
     const int32_t* cu = KEYS ? p.cu_k : p.cu_q;
-    const int N = KEYS ? p.Nk : p.Nq;
-    const int s = packed_find(cu, p.S, N, x);
+    const int N = KEYS ? p.Nk : p.Nq, lane = threadIdx.x & 63;
     PackedSeq r;
+    int s;
+    if (p.S < 64 && p.lower == 0 && p.upper == 1 << 30) {
+        const int a = lane <= p.S ? packed_start(cu, lane, N) : 0;
+        const int e = lane < p.S ? max(packed_start(cu, lane + 1, N), a) : lane == p.S ? N : 0;
+        const int tiles = (e - a + BM - 1) / BM;
+        int left = tiles;  // the most work of any block, then one less
+        for (int o = 1; o < 64; o <<= 1) left = max(left, __shfl_xor(left, o));
+        left = __builtin_amdgcn_readfirstlane(left);
+        uint64_t have = 0;
+        for (; left > 0; --left) {
+            have = __ballot(tiles >= left);
+            const int n = (int)__popcll(have);
+            if (x < n) break;
+            x -= n;
+        }
+        // The x-th of them.
+        const bool mine = ((have >> lane) & 1) != 0 && (int)__popcll(have & ((1ull << lane) - 1)) == x;
+        const uint64_t at = __ballot(left > 0 && mine);
+        s = at != 0 ? __ffsll((long long)at) - 1 : p.S;
+        r.tile = at != 0 ? (KEYS ? __builtin_amdgcn_readlane(tiles, s) - left : left - 1) : (1 << 22);
+    } else {
+        if (!KEYS) x = N / BM + p.S - x;  // a sequence's last queries first
+        int lo = 0, hi = p.S + 1;
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 63) / 64;
+            const int i = lo + (lane + 1) * step;
+            const bool below = i < hi && packed_start(cu, i, N) / BM + i <= x;
+            lo += (int)__popcll(__ballot(below)) * step;
+            hi = min(hi, lo + step);
+        }
+        s = __builtin_amdgcn_readfirstlane(lo);
+        r.tile = x - (packed_start(cu, s, N) / BM + s);
+    }
     r.q0 = r.k0 = r.nq = r.nk = 0;
     if (s < p.S) {
         r.q0 = packed_start(p.cu_q, s, p.Nq);
@@ -104,7 +130,6 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
         r.q0 = packed_start(cu, s, N);
         r.nq = N - r.q0;
     }
-    r.tile = x - (packed_start(cu, s, N) / kPackedRows + s);
     return r;
 }
 
@@ -260,68 +285,177 @@ __device__ __forceinline__ float f16_factor(float largest) {
     return __uint_as_float((uint32_t)(min(max(6 - e, -126), 127) + 127) << 23);
 }
 
-// fp16 gradients' operands: p / Z is at most 1 and the factor of dS has no
-// bound; these powers of two keep small ones in fp16's normal range.
+// fp16 gradients' operands, p / Z and the factor of dS, are scaled by this power
+// of two: what rounding then takes from a small one lies below the step of a
+// small fp16 output, and one overflows only where the gradient nearly does.
 template <class E>
-constexpr float kUpW = std::is_same<E, F16>::value ? 1024.f : 1.f;
-template <class E>
-constexpr float kUpU = std::is_same<E, F16>::value ? 64.f : 1.f;
+constexpr float kUp = std::is_same<E, F16>::value ? 16.f : 1.f;
 
-template <class E, int DP>
+// 32 rows of a wave's accumulators to its share of the reduction buffer, rows of
+// DP + 4 floats, and another wave's share added to a wave's own.
+template <int DB>
+__device__ __forceinline__ void packed_put(float* red, const f32x16 (&acc)[DB], int c, int g) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 w = {acc[db][4 * j], acc[db][4 * j + 1], acc[db][4 * j + 2], acc[db][4 * j + 3]};
+            *reinterpret_cast<f32x4*>(red + c * (32 * DB + 4) + 32 * db + 8 * j + 4 * g) = w;
+        }
+}
+template <int DB>
+__device__ __forceinline__ void packed_add(f32x16 (&acc)[DB], const float* red, int c, int g) {
+#pragma unroll
+    for (int db = 0; db < DB; ++db)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 w = *reinterpret_cast<const f32x4*>(red + c * (32 * DB + 4) + 32 * db + 8 * j + 4 * g);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) acc[db][4 * j + e] += w[e];
+        }
+}
+
+// A wave's tiles 0 .. n - 1, whose rows start at first + u step and number w,
+// against the positions that it sees: those from a0 to a1 by some of its rows,
+// from b0 to b1 by all.  [0, ta): none visible; [ta, tf) and [tg, tv): some
+// pairs masked; [tf, tg): none masked; [tv, n): none visible.  Each run has a
+// loop of its own: a masked and an unmasked body behind one branch would move
+// the accumulators on every tile, or spill.
+struct PackedRuns {
+    int ta, tf, tg, tv;
+    __device__ __forceinline__ PackedRuns(int n, int first, int step, int w, int a0, int a1, int b0, int b1) {
+        auto from = [&](int x) {  // the first tile that starts at x or behind
+            const int d = x - first;
+            return __builtin_amdgcn_readfirstlane(d <= 0 ? 0 : min((d + step - 1) / step, n));
+        };
+        ta = from(a0 - w + 1);
+        tv = max(from(a1 + 1), ta);
+        tf = min(max(from(b0), ta), tv);
+        tg = min(max(from(b1 - w + 2), tf), tv);
+    }
+};
+typedef std::integral_constant<int, 0> PackedIdle;
+typedef std::integral_constant<int, 1> PackedFull;
+typedef std::integral_constant<int, 2> PackedCut;
+
+// A block's shape.  SPLIT waves share 32 stationary rows and take SUB 32-row
+// parts of each tile in turn.
+template <class E, int DP, int SPLIT>
 struct PackedCfg {
-    static constexpr bool k16 = kItem<E> == 2;
-    static constexpr int BN = k16 && DP <= 128 ? 64 : 32;  // streamed rows per tile
     static constexpr int RB = kItem<E> * DP;
-    static constexpr int STAGE = 2 * BN * RB;              // two operands
-    // 16-bit up to head dim 128: two workgroups per CU; above and fp32, one.
-    static constexpr int NST = 2;
-    static constexpr int WPE = RB <= 256 ? 2 : 1;
+    static constexpr int SUB = SPLIT == 1 ? (kItem<E> == 2 && DP <= 128 ? 2 : 1) : SPLIT == 2 && RB <= 256 ? 2 : 1;
+    static constexpr int BN = 32 * SUB * SPLIT;  // streamed rows per tile
+    static constexpr int BM = packed_rows(SPLIT), GROUPS = kPackedWaves / SPLIT;
+    static constexpr int STAGE = 2 * BN * RB, NST = 2;  // two operands
+    static constexpr int RING = NST * STAGE, REDUCE = (SPLIT - 1) * GROUPS * 32 * (DP + 4) * 4;
+    static constexpr int SMEM = RING > REDUCE ? RING : REDUCE;
+    static_assert(SMEM <= 160 * 1024 - 4096, "LDS");
+    // Forward and dQ: two workgroups per CU where the ring and the registers
+    // let them; above, one.
+    static constexpr int WPE = RB <= 256 && SMEM <= 78 * 1024 ? 2 : 1;
+};
+
+// A block of the forward or dQ: its rows, the keys that they see, their loads.
+template <class E, int DP, int SPLIT>
+struct PackedQueries {
+    using C = PackedCfg<E, DP, SPLIT>;
+    using Tile = PackedTile<E, DP, C::BN>;
+    PackedSeq sq;
+    int hk, h, m0, off, t0, n;
+    int lane, wave, c, g, group, part;  // the wave's rows among the block's, its part of each tile
+    int rw, row;                        // its first row, the lane's
+    bool ok;
+    const uint8_t *kb, *vb;
+    int koff[Tile::LPW], voff[Tile::LPW];
+
+    __device__ __forceinline__ bool init(const PackedArgs& p) {
+        hk = blockIdx.x % p.Hkv;
+        const int rest = blockIdx.x / p.Hkv;
+        h = hk * p.G + rest % p.G;
+        sq = packed_seq<false, C::BM>(p, rest / p.G);
+        m0 = sq.tile * C::BM;
+        if (m0 >= sq.nq) return false;
+        lane = threadIdx.x & 63;
+        wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+        c = lane & 31;
+        g = lane >> 5;
+        group = wave % C::GROUPS;
+        part = wave / C::GROUPS;
+        off = sq.nk - sq.nq;
+        const int m1 = min(sq.nq, m0 + C::BM);
+        const int jlo = max(0, m0 + off - p.upper + 1), jhi = min(sq.nk - 1, m1 - 1 + off - p.lower);
+        t0 = jlo / C::BN;
+        n = jhi >= jlo ? jhi / C::BN - t0 + 1 : 0;
+        kb = (const uint8_t*)p.k + (int64_t)sq.k0 * p.k_st + (int64_t)hk * p.k_sh;
+        vb = (const uint8_t*)p.v + (int64_t)sq.k0 * p.v_st + (int64_t)hk * p.v_sh;
+        Tile::offsets(koff, (int)p.k_st, p.D, wave, lane);
+        Tile::offsets(voff, (int)p.v_st, p.D, wave, lane);
+        rw = m0 + 32 * group;
+        row = rw + c;
+        ok = row < sq.nq;
+        return true;
+    }
+    __device__ __forceinline__ static Tile kt(uint8_t* ring, int st) { return Tile{ring + st * C::STAGE}; }
+    __device__ __forceinline__ static Tile vt(uint8_t* ring, int st) { return Tile{ring + st * C::STAGE + Tile::BYTES}; }
+    __device__ __forceinline__ void issue(const PackedArgs& p, uint8_t* ring, int u, int st) const {
+        const int key0 = (t0 + u) * C::BN;
+        kt(ring, st).issue(kb + (int64_t)key0 * p.k_st, sq.nk - key0, (int)p.k_st, p.D, koff, wave);
+        vt(ring, st).issue(vb + (int64_t)key0 * p.v_st, sq.nk - key0, (int)p.v_st, p.D, voff, wave);
+    }
+    // The wave's tiles: u's keys from key0(u) on.
+    __device__ __forceinline__ int key0(int u) const { return (t0 + u) * C::BN + 32 * C::SUB * part; }
+    __device__ __forceinline__ PackedRuns runs(const PackedArgs& p) const {
+        return PackedRuns(n, key0(0), C::BN, 32 * C::SUB, rw + off - p.upper + 1, rw + 31 + off - p.lower,
+                          rw + 31 + off - p.upper + 1, rw + off - p.lower);
+    }
+    // Every tile in turn: tile(u, stage, kind) where the wave sees any of it.
+    template <class F>
+    __device__ __forceinline__ void tiles(const PackedArgs& p, uint8_t* ring, F&& tile) const {
+        const PackedRuns r = runs(p);
+        if (n > 0) issue(p, ring, 0, 0);
+        int u = 0;
+        auto run = [&](int end, auto kind) __attribute__((always_inline)) {
+            for (; u < end; ++u) {
+                wait_vmcnt<0>();
+                __syncthreads();
+                if (u + 1 < n) issue(p, ring, u + 1, (u + 1) % C::NST);
+                if constexpr (kind.value != 0) tile(u, u % C::NST, kind);
+            }
+        };
+        run(r.ta, PackedIdle{});
+        run(r.tf, PackedCut{});
+        run(r.tg, PackedFull{});
+        run(r.tv, PackedCut{});
+        run(n, PackedIdle{});
+    }
+    // Zeroes a lane's overlaps with keys that its row does not see.
+    __device__ __forceinline__ void mask(const PackedArgs& p, f32x16& s, int key0) const {
+        const int d = row + off - key0 - p.lower, span = p.upper - p.lower;
+#pragma unroll
+        for (int r = 0; r < 16; ++r)
+            if ((uint32_t)(d - acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+    }
 };
 
 // ---------------------------------------------------------------------------
 // Forward: S^T = K Q^T per 32 keys, the weights in place, O^T += V^T P^T.
 // ---------------------------------------------------------------------------
-template <class E, int DP>
-__global__ __launch_bounds__(64 * kPackedWaves) __attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP>::WPE, PackedCfg<E, DP>::WPE)))
+template <class E, int DP, int SPLIT>
+__global__ __launch_bounds__(64 * kPackedWaves)
+__attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP, SPLIT>::WPE, PackedCfg<E, DP, SPLIT>::WPE)))
 void born_packed_fwd_kernel(PackedArgs p) {
-    using C = PackedCfg<E, DP>;
-    using Tile = PackedTile<E, DP, C::BN>;
-    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, BM = kPackedRows;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[NST * C::STAGE];
+    using C = PackedCfg<E, DP, SPLIT>;
+    using Q = PackedQueries<E, DP, SPLIT>;
+    constexpr int KS = Q::Tile::KS, DB = Q::Tile::DB;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[C::SMEM];
+    __shared__ float zred[SPLIT][kPackedWaves / SPLIT][32];
+    Q b;
+    if (!b.init(p)) return;
+    const int lane = b.lane, c = b.c, g = b.g, D = p.D;
+    const float sc = arg_scale(p, b.h);
 
-    const int slots = p.Nq / BM + p.S + 1;
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
-    const int h = hk * p.G + rest % p.G;
-    const PackedSeq sq = packed_seq<false>(p, slots - 1 - rest / p.G);
-    const int m0 = sq.tile * BM;
-    if (m0 >= sq.nq) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 31, g = lane >> 5;
-    const int D = p.D, off = sq.nk - sq.nq;
-    const float sc = arg_scale(p, h);
-
-    // Keys that the block's rows see, as tiles of BN.
-    const int m1 = min(sq.nq, m0 + BM);
-    const int jlo = max(0, m0 + off - p.upper + 1), jhi = min(sq.nk - 1, m1 - 1 + off - p.lower);
-    const int t0 = jlo / BN, n = jhi >= jlo ? jhi / BN - t0 + 1 : 0;
-
-    const uint8_t* const kb = (const uint8_t*)p.k + (int64_t)sq.k0 * p.k_st + (int64_t)hk * p.k_sh;
-    const uint8_t* const vb = (const uint8_t*)p.v + (int64_t)sq.k0 * p.v_st + (int64_t)hk * p.v_sh;
-    int koff[Tile::LPW], voff[Tile::LPW];
-    Tile::offsets(koff, (int)p.k_st, D, wave, lane);
-    Tile::offsets(voff, (int)p.v_st, D, wave, lane);
-    auto kt = [&](int st) { return Tile{ring + st * C::STAGE}; };
-    auto vt = [&](int st) { return Tile{ring + st * C::STAGE + Tile::BYTES}; };
-    auto issue = [&](int u, int st) __attribute__((always_inline)) {
-        const int key0 = (t0 + u) * BN;
-        kt(st).issue(kb + (int64_t)key0 * p.k_st, sq.nk - key0, (int)p.k_st, D, koff, wave);
-        vt(st).issue(vb + (int64_t)key0 * p.v_st, sq.nk - key0, (int)p.v_st, D, voff, wave);
-    };
-
-    const int rw = m0 + 32 * wave, row = rw + c;
-    const bool ok = row < sq.nq;
     u32x4 qr[KS];
-    packed_load_row<E>(qr, (const uint8_t*)p.q + (int64_t)(sq.q0 + row) * p.q_st + (int64_t)h * p.q_sh, ok, D, g);
+    packed_load_row<E>(qr, (const uint8_t*)p.q + (int64_t)(b.sq.q0 + b.row) * p.q_st + (int64_t)b.h * p.q_sh, b.ok, D, g);
     const uint32_t flip = packed_flip<E>(sc);
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
@@ -332,27 +466,17 @@ void born_packed_fwd_kernel(PackedArgs p) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
     float z = 0.f, cf = kF16Start;
-    const int pos = row + off, span = p.upper - p.lower;
 
-    if (n > 0) issue(0, 0);
-    for (int u = 0; u < n; ++u) {
-        const int st = u % NST, key0 = (t0 + u) * BN;
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (u + 1 < n) issue(u + 1, (u + 1) % NST);
-        const bool none = key0 > rw + 31 + off - p.lower || key0 + BN <= rw + off - p.upper + 1;
-        if (none) continue;
-        const bool cut = key0 + BN - 1 > rw + off - p.lower || key0 < rw + 31 + off - p.upper + 1;
+    const int r0 = 32 * C::SUB * b.part;  // this wave's part of every tile
+    b.tiles(p, ring, [&](int u, int st, auto kind) __attribute__((always_inline)) {
+        const int key0 = b.key0(u);
+        const auto kt = Q::kt(ring, st), vt = Q::vt(ring, st);
 #pragma unroll
-        for (int nb = 0; nb < BN / 32; ++nb) {
+        for (int nb = 0; nb < C::SUB; ++nb) {
             f32x16 s = zero16();
 #pragma unroll
-            for (int ks = 0; ks < KS; ++ks) s = packed_step<E>(kt(st).row(32 * nb + c, ks, g), qr[ks], s);
-            if (cut) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((uint32_t)(pos - (key0 + 32 * nb + acc_row(r, g)) - p.lower) >= (uint32_t)span) s[r] = 0.f;
-            }
+            for (int ks = 0; ks < KS; ++ks) s = packed_step<E>(kt.row(r0 + 32 * nb + c, ks, g), qr[ks], s);
+            if constexpr (kind.value == 2) b.mask(p, s, key0 + 32 * nb);
             PackedWeights<E> w;
             if constexpr (std::is_same<E, F32>::value) {
 #pragma unroll
@@ -380,83 +504,79 @@ void born_packed_fwd_kernel(PackedArgs p) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w.w[j] = born_weight_pair<BF16>(s[2 * j], s[2 * j + 1], 1.f, z);
             }
-            packed_columns<E>(vt(st), 32 * nb, w, acc, lane);
+            packed_columns<E>(vt, r0 + 32 * nb, w, acc, lane);
         }
-    }
+    });
 
     z += __shfl_xor(z, 32);
-    const float s1 = std::is_same<E, F16>::value ? sc / cf : sc, s2 = s1 * s1;
+    float s1 = std::is_same<E, F16>::value && SPLIT == 1 ? sc / cf : sc;
+    if constexpr (SPLIT > 1) {
+        if constexpr (std::is_same<E, F16>::value) {  // without the waves' own factors
+            const float back = 1.f / (cf * cf);
+            z *= back;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= back;
+        }
+        float* const red = reinterpret_cast<float*>(ring);
+        auto share = [&](int part) { return red + ((part - 1) * C::GROUPS + b.group) * 32 * (DP + 4); };
+        __syncthreads();
+        if (g == 0) zred[b.part][b.group][c] = z;
+        if (b.part > 0) packed_put(share(b.part), acc, c, g);
+        __syncthreads();
+        if (b.part > 0) return;
+#pragma unroll
+        for (int i = 1; i < SPLIT; ++i) {
+            packed_add(acc, share(i), c, g);
+            z += zred[i][b.group][c];
+        }
+    }
+    if (!b.ok) return;
+    const float s2 = s1 * s1;
     const float den = z + (p.eps == 0.f ? 0.f : p.eps / s2);
     const float inv = den > 0.f && sc != 0.f ? 1.0f / den : 0.f;
-    if (!ok) return;
-    packed_store_row<E>((uint8_t*)p.out + ((size_t)(sq.q0 + row) * p.H + h) * D * kItem<E>, acc, inv, D, g);
-    if (g == 0 && p.z != nullptr) p.z[(size_t)h * p.Nq + sq.q0 + row] = s2 * z + p.eps;
+    packed_store_row<E>((uint8_t*)p.out + ((size_t)(b.sq.q0 + b.row) * p.H + b.h) * D * kItem<E>, acc, inv, D, g);
+    if (g == 0 && p.z != nullptr) p.z[(size_t)b.h * p.Nq + b.sq.q0 + b.row] = s2 * z + p.eps;
 }
 
 // ---------------------------------------------------------------------------
-// dQ; also -delta and s^2 / Z per row for the dK/dV kernel.
+// dQ; also -delta and sign(s) s^2 / Z per row for the dK/dV kernel.
 // ---------------------------------------------------------------------------
-template <class E, int DP>
-__global__ __launch_bounds__(64 * kPackedWaves) __attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP>::WPE, PackedCfg<E, DP>::WPE)))
+template <class E, int DP, int SPLIT>
+__global__ __launch_bounds__(64 * kPackedWaves)
+__attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP, SPLIT>::WPE, PackedCfg<E, DP, SPLIT>::WPE)))
 void born_packed_dq_kernel(PackedArgs p) {
-    using C = PackedCfg<E, DP>;
-    using Tile = PackedTile<E, DP, C::BN>;
-    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, BM = kPackedRows, IT = kItem<E>;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[NST * C::STAGE];
+    using C = PackedCfg<E, DP, SPLIT>;
+    using Q = PackedQueries<E, DP, SPLIT>;
+    constexpr int KS = Q::Tile::KS, DB = Q::Tile::DB, IT = kItem<E>;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[C::SMEM];
+    Q b;
+    if (!b.init(p)) return;
+    const int lane = b.lane, c = b.c, g = b.g, D = p.D;
+    const float sc = arg_scale(p, b.h);
 
-    const int slots = p.Nq / BM + p.S + 1;
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
-    const int h = hk * p.G + rest % p.G;
-    const PackedSeq sq = packed_seq<false>(p, slots - 1 - rest / p.G);
-    const int m0 = sq.tile * BM;
-    if (m0 >= sq.nq) return;
-    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const int c = lane & 31, g = lane >> 5;
-    const int D = p.D, off = sq.nk - sq.nq;
-    const float sc = arg_scale(p, h);
-
-    const int m1 = min(sq.nq, m0 + BM);
-    const int jlo = max(0, m0 + off - p.upper + 1), jhi = min(sq.nk - 1, m1 - 1 + off - p.lower);
-    const int t0 = jlo / BN, n = jhi >= jlo ? jhi / BN - t0 + 1 : 0;
-
-    const uint8_t* const kb = (const uint8_t*)p.k + (int64_t)sq.k0 * p.k_st + (int64_t)hk * p.k_sh;
-    const uint8_t* const vb = (const uint8_t*)p.v + (int64_t)sq.k0 * p.v_st + (int64_t)hk * p.v_sh;
-    int koff[Tile::LPW], voff[Tile::LPW];
-    Tile::offsets(koff, (int)p.k_st, D, wave, lane);
-    Tile::offsets(voff, (int)p.v_st, D, wave, lane);
-    auto kt = [&](int st) { return Tile{ring + st * C::STAGE}; };
-    auto vt = [&](int st) { return Tile{ring + st * C::STAGE + Tile::BYTES}; };
-    auto issue = [&](int u, int st) __attribute__((always_inline)) {
-        const int key0 = (t0 + u) * BN;
-        kt(st).issue(kb + (int64_t)key0 * p.k_st, sq.nk - key0, (int)p.k_st, D, koff, wave);
-        vt(st).issue(vb + (int64_t)key0 * p.v_st, sq.nk - key0, (int)p.v_st, D, voff, wave);
-    };
-
-    const int rw = m0 + 32 * wave, row = rw + c;
-    const bool ok = row < sq.nq;
     u32x4 qr[KS], dr[KS];
-    packed_load_row<E>(qr, (const uint8_t*)p.q + (int64_t)(sq.q0 + row) * p.q_st + (int64_t)h * p.q_sh, ok, D, g);
-    packed_load_row<E>(dr, (const uint8_t*)p.dout + (int64_t)(sq.q0 + row) * p.do_st + (int64_t)h * p.do_sh, ok, D, g);
-    const size_t at = ((size_t)(sq.q0 + row) * p.H + h) * D * IT;  // contiguous (Nq, H, D)
+    packed_load_row<E>(qr, (const uint8_t*)p.q + (int64_t)(b.sq.q0 + b.row) * p.q_st + (int64_t)b.h * p.q_sh, b.ok, D, g);
+    packed_load_row<E>(dr, (const uint8_t*)p.dout + (int64_t)(b.sq.q0 + b.row) * p.do_st + (int64_t)b.h * p.do_sh, b.ok, D, g);
+    const size_t at = ((size_t)(b.sq.q0 + b.row) * p.H + b.h) * D * IT;  // contiguous (Nq, H, D)
     float delta = 0.f;
 #pragma unroll
     for (int ks = 0; ks < KS; ++ks) {
-        const int b = 32 * ks + 16 * g;
-        if (!ok || b >= IT * D) continue;
-        const u32x4 o = ldg16((const uint8_t*)p.o + at + b);
+        const int o = 32 * ks + 16 * g;
+        if (!b.ok || o >= IT * D) continue;
+        const u32x4 x = ldg16((const uint8_t*)p.o + at + o);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            if constexpr (std::is_same<E, F32>::value) delta = fmaf(__uint_as_float(o[j]), __uint_as_float(dr[ks][j]), delta);
-            else delta += E::lo(o[j]) * E::lo(dr[ks][j]) + E::hi(o[j]) * E::hi(dr[ks][j]);
+            if constexpr (std::is_same<E, F32>::value) delta = fmaf(__uint_as_float(x[j]), __uint_as_float(dr[ks][j]), delta);
+            else delta += E::lo(x[j]) * E::lo(dr[ks][j]) + E::hi(x[j]) * E::hi(dr[ks][j]);
         }
     }
     delta += __shfl_xor(delta, 32);
-    const size_t stat = (size_t)h * p.Nq + sq.q0 + row;
-    const float zr = ok ? p.z[stat] : 1.f;
-    const float zs = zr > 0.f ? sc * sc / zr : 0.f;
-    if (ok && g == 0) {
+    const size_t stat = (size_t)b.h * p.Nq + b.sq.q0 + b.row;
+    const float zr = b.ok ? p.z[stat] : 1.f;
+    const float zs = zr > 0.f ? sc * fabsf(sc) / zr : 0.f;
+    if (b.ok && g == 0 && b.part == 0) {
         p.ndelta[stat] = -delta;
-        p.zs[stat] = zs;
+        p.zs[stat] = kUp<E> * zs;
     }
     const uint32_t flip = packed_flip<E>(sc);
 #pragma unroll
@@ -468,34 +588,24 @@ void born_packed_dq_kernel(PackedArgs p) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
     // fp16 scales each operand into its range; otherwise zs is a row's factor.
-    const float pre = std::is_same<E, F16>::value ? kUpU<E> * zs : 1.f;
-    const int pos = row + off, span = p.upper - p.lower;
+    const float pre = std::is_same<E, F16>::value ? kUp<E> * zs : 1.f;
     asm volatile("" : "+v"(delta));
 
-    if (n > 0) issue(0, 0);
-    for (int u = 0; u < n; ++u) {
-        const int st = u % NST, key0 = (t0 + u) * BN;
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (u + 1 < n) issue(u + 1, (u + 1) % NST);
-        const bool none = key0 > rw + 31 + off - p.lower || key0 + BN <= rw + off - p.upper + 1;
-        if (none) continue;
-        const bool cut = key0 + BN - 1 > rw + off - p.lower || key0 < rw + 31 + off - p.upper + 1;
+    const int r0 = 32 * C::SUB * b.part;  // this wave's part of every tile
+    b.tiles(p, ring, [&](int u, int st, auto kind) __attribute__((always_inline)) {
+        const int key0 = b.key0(u);
+        const auto kt = Q::kt(ring, st), vt = Q::vt(ring, st);
 #pragma unroll
-        for (int nb = 0; nb < BN / 32; ++nb) {
+        for (int nb = 0; nb < C::SUB; ++nb) {
             f32x16 s = zero16(), t;
 #pragma unroll
             for (int r = 0; r < 16; ++r) t[r] = -delta;
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                s = packed_step<E>(kt(st).row(32 * nb + c, ks, g), qr[ks], s);
-                t = packed_step<E>(vt(st).row(32 * nb + c, ks, g), dr[ks], t);
+                s = packed_step<E>(kt.row(r0 + 32 * nb + c, ks, g), qr[ks], s);
+                t = packed_step<E>(vt.row(r0 + 32 * nb + c, ks, g), dr[ks], t);
             }
-            if (cut) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((uint32_t)(pos - (key0 + 32 * nb + acc_row(r, g)) - p.lower) >= (uint32_t)span) s[r] = 0.f;
-            }
+            if constexpr (kind.value == 2) b.mask(p, s, key0 + 32 * nb);
             PackedWeights<E> w;
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
@@ -507,38 +617,58 @@ void born_packed_dq_kernel(PackedArgs p) {
                 }
                 w.set(j, x[0], x[1]);
             }
-            packed_columns<E>(kt(st), 32 * nb, w, acc, lane);
+            packed_columns<E>(kt, r0 + 32 * nb, w, acc, lane);
         }
+    });
+    if constexpr (SPLIT > 1) {
+        float* const red = reinterpret_cast<float*>(ring);
+        auto share = [&](int part) { return red + ((part - 1) * C::GROUPS + b.group) * 32 * (DP + 4); };
+        __syncthreads();
+        if (b.part > 0) packed_put(share(b.part), acc, c, g);
+        __syncthreads();
+        if (b.part > 0) return;
+#pragma unroll
+        for (int i = 1; i < SPLIT; ++i) packed_add(acc, share(i), c, g);
     }
-    if (!ok) return;
-    const float f = (sc < 0.f ? -2.f : 2.f) * (std::is_same<E, F16>::value ? 1.f / kUpU<E> : zs);
-    packed_store_row<E>((uint8_t*)p.dq + at, acc, f, D, g);
+    if (!b.ok) return;
+    packed_store_row<E>((uint8_t*)p.dq + at, acc, std::is_same<E, F16>::value ? 2.f / kUp<E> : 2.f * zs, D, g);
 }
 
 // ---------------------------------------------------------------------------
 // dK / dV: 32 keys per wave, the queries of all heads of the group streamed.
+//
+// One wave per SIMD (the accumulators and the stationary rows of both take half
+// of its registers) leaves nothing to hide a wave's LDS latency behind but its
+// own work, so two 32-row parts of a tile run as four fenced phases, the
+// operands of each read one phase earlier:
+//   1: S, dP of part 0                        reads the rows of part 1
+//   2: S, dP of part 1 | elementwise(part 0)  reads the columns of part 0
+//   3: dV, dK += part 0 | elementwise(part 1) reads the columns of part 1
+//   4: dV, dK += part 1
 // fp32 above head dim 128 takes one launch for each (the registers hold the
 // operands of both or the accumulators of both).
 // ---------------------------------------------------------------------------
-template <class E, int DP, bool DK, bool DV>
+template <class E, int DP, int SPLIT, bool DK, bool DV>
 __global__ __launch_bounds__(64 * kPackedWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
 void born_packed_dkdv_kernel(PackedArgs p) {
-    using C = PackedCfg<E, DP>;
+    using C = PackedCfg<E, DP, SPLIT>;
     using Tile = PackedTile<E, DP, C::BN>;
-    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, BM = kPackedRows, IT = kItem<E>;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[NST * C::STAGE];
+    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, SUB = C::SUB, IT = kItem<E>;
+    constexpr bool kPhased = SUB == 2 && IT == 2 && DK && DV;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[C::SMEM];
     __shared__ __attribute__((aligned(16))) float stats[NST][2][BN];  // -delta, zs
 
     const int hk = blockIdx.x % p.Hkv;
-    const PackedSeq sq = packed_seq<true>(p, blockIdx.x / p.Hkv);
-    const int k0 = sq.tile * BM;
+    const PackedSeq sq = packed_seq<true, C::BM>(p, blockIdx.x / p.Hkv);
+    const int k0 = sq.tile * C::BM;
     if (k0 >= sq.nk) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int c = lane & 31, g = lane >> 5;
+    const int group = wave % C::GROUPS, part = wave / C::GROUPS;
     const int D = p.D, off = sq.nk - sq.nq;
 
     // Queries that see the block's keys, as tiles of BN, for each head.
-    const int k1 = min(sq.nk, k0 + BM);
+    const int k1 = min(sq.nk, k0 + C::BM);
     const int ilo = max(0, k0 - off + p.lower), ihi = min(sq.nq - 1, k1 - 1 - off + p.upper - 1);
     const int t0 = ilo / BN, nt = ihi >= ilo ? ihi / BN - t0 + 1 : 0, n = nt * p.G;
 
@@ -561,7 +691,7 @@ void born_packed_dkdv_kernel(PackedArgs p) {
         }
     };
 
-    const int kw = k0 + 32 * wave, key = kw + c;
+    const int kw = k0 + 32 * group, key = kw + c;
     const bool ok = key < sq.nk;
     u32x4 kr[KS], vr[DK ? KS : 1];
     packed_load_row<E>(kr, (const uint8_t*)p.k + (int64_t)(sq.k0 + key) * p.k_st + (int64_t)hk * p.k_sh, ok, D, g);
@@ -580,67 +710,193 @@ void born_packed_dkdv_kernel(PackedArgs p) {
     }
     const int span = p.upper - p.lower;
 
-    int gi = 0, t = 0, ni = 0, nx = 0;  // this tile's and the next one's head of the group and tile
-    if (n > 0) issue(hk * p.G, 0, 0);
-    for (int u = 0; u < n; ++u) {
-        const int st = u % NST, i0 = (t0 + t) * BN;
-        const float sc = arg_scale(p, hk * p.G + gi);
-        nx = t + 1, ni = gi;
-        if (nx == nt) nx = 0, ++ni;
-        wait_vmcnt<0>();
-        __syncthreads();
-        if (u + 1 < n) issue(hk * p.G + ni, nx, (u + 1) % NST);
-        t = nx, gi = ni;
-        const bool none = i0 + BN - 1 + off - kw < p.lower || i0 + off - (kw + 31) >= p.upper;
-        if (none) continue;
-        const bool cut = i0 + off - (kw + 31) < p.lower || i0 + BN - 1 + off - kw >= p.upper;
-        const float sign = sc < 0.f ? -1.f : 1.f;
+    // Row values r0 + 8 j + 4 g + e.
+    auto values = [&](const float* x, int r0) __attribute__((always_inline)) {
+        f32x16 y;
 #pragma unroll
-        for (int nb = 0; nb < BN / 32; ++nb) {
-            f32x16 s = zero16(), dp, zi;
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(x + r0 + 8 * j + 4 * g);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[st][0][32 * nb + 8 * j + 4 * g]);
-                const f32x4 b = *reinterpret_cast<const f32x4*>(&stats[st][1][32 * nb + 8 * j + 4 * g]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e) dp[4 * j + e] = a[e], zi[4 * j + e] = b[e];
-            }
-#pragma unroll
-            for (int ks = 0; ks < KS; ++ks) {
-                s = packed_step<E>(qt(st).row(32 * nb + c, ks, g), kr[ks], s);
-                if constexpr (DK) dp = packed_step<E>(dt(st).row(32 * nb + c, ks, g), vr[ks], dp);
-            }
-            if (cut) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r)
-                    if ((uint32_t)(i0 + 32 * nb + acc_row(r, g) + off - key - p.lower) >= (uint32_t)span) s[r] = 0.f;
-            }
-            PackedWeights<E> w, x;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float ww[2], uu[2];
-#pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const int r = 2 * j + e;
-                    const float a = relu_f32(s[r] * sign), tz = a * zi[r];
-                    ww[e] = kUpW<E> * tz * a;
-                    uu[e] = kUpU<E> * sign * tz * dp[r];
-                }
-                w.set(j, ww[0], ww[1]);
-                x.set(j, uu[0], uu[1]);
-            }
-            if constexpr (DV) packed_columns<E>(dt(st), 32 * nb, w, dv, lane);
-            if constexpr (DK) packed_columns<E>(qt(st), 32 * nb, x, dk, lane);
+            for (int e = 0; e < 4; ++e) y[4 * j + e] = a[e];
         }
+        return y;
+    };
+    // p / Z and the factor of dS of 32 queries from i0 + r0, from S and dP.
+    auto elementwise = [&](int st, int i0, int r0, f32x16& s, const f32x16& dp, PackedWeights<E>& w, PackedWeights<E>& x,
+                           auto kind) __attribute__((always_inline)) {
+        if constexpr (kind.value == 2) {
+            const int d = i0 + r0 + off - key - p.lower;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((uint32_t)(d + acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+        }
+        const f32x16 zi = values(stats[st][1], r0);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            float ww[2], uu[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+                const int r = 2 * j + e;
+                const float a = relu_f32(s[r]), t = a * zi[r];
+                ww[e] = fabsf(t) * a;  // zs carries the sign of s
+                uu[e] = t * dp[r];
+            }
+            if constexpr (DV) w.set(j, ww[0], ww[1]);
+            if constexpr (DK) x.set(j, uu[0], uu[1]);
+        }
+    };
+
+    const int r0 = 32 * SUB * part;  // this wave's part of every tile
+    auto tile = [&](int t, int st, auto kind) __attribute__((always_inline)) {
+        const int i0 = (t0 + t) * BN;
+        const Tile q = qt(st), d = dt(st);
+        if constexpr (kPhased) {
+            auto rows = [&](const Tile& tile, int nb, u32x4 (&x)[KS]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) x[ks] = tile.row(r0 + 32 * nb + c, ks, g);
+            };
+            auto cols = [&](const Tile& tile, int nb, u32x4 (&x)[2][DB]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) x[hh][db] = tile.transposed(r0 + 32 * nb + 16 * hh, db, lane);
+            };
+            auto overlaps = [&](const u32x4 (&a)[KS], const u32x4 (&b)[KS], f32x16& s, f32x16& dp) __attribute__((always_inline)) {
+                s = zero16();
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    s = E::mfma(a[ks], kr[ks], s);
+                    dp = E::mfma(b[ks], vr[ks], dp);
+                }
+            };
+            auto sums = [&](const u32x4 (&td)[2][DB], const u32x4 (&tq)[2][DB], const PackedWeights<E>& w,
+                            const PackedWeights<E>& x) __attribute__((always_inline)) {
+#pragma unroll
+                for (int hh = 0; hh < 2; ++hh) {
+                    const u32x4 bw = {w.w[4 * hh], w.w[4 * hh + 1], w.w[4 * hh + 2], w.w[4 * hh + 3]};
+                    const u32x4 bx = {x.w[4 * hh], x.w[4 * hh + 1], x.w[4 * hh + 2], x.w[4 * hh + 3]};
+#pragma unroll
+                    for (int db = 0; db < DB; ++db) {
+                        dv[db] = E::mfma(td[hh][db], bw, dv[db]);
+                        dk[db] = E::mfma(tq[hh][db], bx, dk[db]);
+                    }
+                }
+            };
+            u32x4 rq0[KS], rd0[KS], rq1[KS], rd1[KS], tq0[2][DB], td0[2][DB], tq1[2][DB], td1[2][DB];
+            f32x16 s0, s1, dp0, dp1;
+            PackedWeights<E> w0, w1, x0, x1;
+            rows(q, 0, rq0);
+            rows(d, 0, rd0);
+            dp0 = values(stats[st][0], r0);
+            dp1 = values(stats[st][0], r0 + 32);
+            // 1
+            __builtin_amdgcn_s_setprio(1);
+            rows(q, 1, rq1);
+            rows(d, 1, rd1);
+            overlaps(rq0, rd0, s0, dp0);
+            __builtin_amdgcn_sched_barrier(0);
+            // 2
+            __builtin_amdgcn_s_setprio(0);
+            cols(q, 0, tq0);
+            cols(d, 0, td0);
+            overlaps(rq1, rd1, s1, dp1);
+            elementwise(st, i0, r0, s0, dp0, w0, x0, kind);
+#pragma unroll
+            for (int i = 0; i < 2 * KS; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS read
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // 3
+            cols(q, 1, tq1);
+            cols(d, 1, td1);
+            sums(td0, tq0, w0, x0);
+            elementwise(st, i0, r0 + 32, s1, dp1, w1, x1, kind);
+#pragma unroll
+            for (int i = 0; i < 4 * DB; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
+                __builtin_amdgcn_sched_group_barrier(0x002, 6, 1);
+                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+            // 4
+            __builtin_amdgcn_s_setprio(1);
+            sums(td1, tq1, w1, x1);
+            __builtin_amdgcn_sched_barrier(0);
+            __builtin_amdgcn_s_setprio(0);
+        } else {
+#pragma unroll
+            for (int nb = 0; nb < SUB; ++nb) {
+                const int rr = r0 + 32 * nb;
+                f32x16 s = zero16(), dp = values(stats[st][0], rr);
+#pragma unroll
+                for (int ks = 0; ks < KS; ++ks) {
+                    s = packed_step<E>(q.row(rr + c, ks, g), kr[ks], s);
+                    if constexpr (DK) dp = packed_step<E>(d.row(rr + c, ks, g), vr[ks], dp);
+                }
+                PackedWeights<E> w, x;
+                elementwise(st, i0, rr, s, dp, w, x, kind);
+                if constexpr (DV) packed_columns<E>(d, rr, w, dv, lane);
+                if constexpr (DK) packed_columns<E>(q, rr, x, dk, lane);
+            }
+        }
+    };
+
+    // Positions of the queries from the wave's first key on.
+    const PackedRuns runs(nt, t0 * BN + r0 + off - kw, BN, 32 * SUB, p.lower, p.upper + 30, p.lower + 31, p.upper - 1);
+    uint32_t flip = 0;  // the scale's sign, folded into K
+    int u = 0;          // tiles so far
+    if (n > 0) issue(hk * p.G, 0, 0);
+    for (int gi = 0; gi < p.G; ++gi) {
+        const uint32_t fl = packed_flip<E>(arg_scale(p, hk * p.G + gi));
+        if (fl != flip) {
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) kr[ks] ^= fl ^ flip;
+            flip = fl;
+        }
+        int t = 0;
+        auto run = [&](int end, auto kind) __attribute__((always_inline)) {
+            for (; t < end; ++t, ++u) {
+                wait_vmcnt<0>();
+                __syncthreads();
+                if (u + 1 < n) {
+                    const bool last = t + 1 == nt;
+                    issue(hk * p.G + gi + (last ? 1 : 0), last ? 0 : t + 1, (u + 1) % NST);
+                }
+                if constexpr (kind.value != 0) tile(t, u % NST, kind);
+            }
+        };
+        run(runs.ta, PackedIdle{});
+        run(runs.tf, PackedCut{});
+        run(runs.tg, PackedFull{});
+        run(runs.tv, PackedCut{});
+        run(nt, PackedIdle{});
+    }
+    if constexpr (SPLIT > 1) {
+        float* const red = reinterpret_cast<float*>(ring);
+        auto share = [&](int i) { return red + ((i - 1) * C::GROUPS + group) * 32 * (DP + 4); };
+        auto join = [&](f32x16 (&acc)[DB]) __attribute__((always_inline)) {
+            __syncthreads();
+            if (part > 0) packed_put(share(part), acc, c, g);
+            __syncthreads();
+            if (part == 0) {
+#pragma unroll
+                for (int i = 1; i < SPLIT; ++i) packed_add(acc, share(i), c, g);
+            }
+        };
+        if constexpr (DK) join(dk);
+        if constexpr (DV) join(dv);
+        if (part > 0) return;
     }
     if (!ok) return;
     const size_t at = ((size_t)(sq.k0 + key) * p.Hkv + hk) * D * IT;  // contiguous (Nk, Hkv, D)
-    if constexpr (DK) packed_store_row<E>((uint8_t*)p.dk + at, dk, 2.f / kUpU<E>, D, g);
-    if constexpr (DV) packed_store_row<E>((uint8_t*)p.dv + at, dv, 1.f / kUpW<E>, D, g);
+    if constexpr (DK) packed_store_row<E>((uint8_t*)p.dk + at, dk, 2.f / kUp<E>, D, g);
+    if constexpr (DV) packed_store_row<E>((uint8_t*)p.dv + at, dv, 1.f / kUp<E>, D, g);
 }
 
 // ---------------------------------------------------------------------------
-// dscale_h = (2 / s) sum_i delta_i eps / Z_i = (2 eps / s^3) sum_i delta_i zs_i:
+// dscale_h = (2 / s) sum_i delta_i eps / Z_i = (2 eps / |s|^3) sum_i delta_i zs_i:
 // 32 partial sums per head in 64 bits, then their sums in order.
 // ---------------------------------------------------------------------------
 constexpr int kPackedParts = 32;
@@ -661,13 +917,13 @@ __global__ __launch_bounds__(256) void born_packed_dscale_part_kernel(PackedArgs
 }
 
 template <int>
-__global__ __launch_bounds__(64) void born_packed_dscale_kernel(PackedArgs p, const double* part, float* dscale, int n_scale) {
+__global__ __launch_bounds__(64) void born_packed_dscale_kernel(PackedArgs p, const double* part, float* dscale, int n_scale, double up) {
     double total = 0.0;
     for (int h = threadIdx.x; h < p.H; h += 64) {
         double x = 0.0;
         for (int i = 0; i < kPackedParts; ++i) x += part[(size_t)h * kPackedParts + i];
-        const double s = (double)arg_scale(p, h);
-        x = s != 0.0 ? 2.0 * (double)p.eps / (s * s * s) * x : 0.0;
+        const double s = fabs((double)arg_scale(p, h));
+        x = s != 0.0 ? 2.0 * (double)p.eps / (s * s * s * up) * x : 0.0;
         if (n_scale > 1) dscale[h] = (float)x;
         total += x;
     }
@@ -679,49 +935,73 @@ __global__ __launch_bounds__(64) void born_packed_dscale_kernel(PackedArgs p, co
 // ---------------------------------------------------------------------------
 // Launches.
 // ---------------------------------------------------------------------------
-inline unsigned packed_blocks(int N, int S) { return (unsigned)(N / kPackedRows + S + 1); }
+inline unsigned packed_blocks(int N, int S, int split) { return (unsigned)(N / packed_rows(split) + S + 1); }
 
-#define QDL_PACKED_DP(D, BODY)                            \
+// Waves that share a block's rows: the most that the ring has room for.
+template <class E, int DP>
+constexpr int kPackedMaxSplit = kItem<E> * DP <= 256 ? 4 : kItem<E> * DP <= 512 ? 2 : 1;
+
+// Forward and dQ: unsplit blocks unless they are too few to fill the chip.
+inline bool packed_split(int N, int S, int heads) { return (int64_t)packed_blocks(N, S, 1) * heads < 512; }
+
+#define QDL_PACKED_DP(D, ...)                             \
     if ((D) <= 64) {                                      \
         constexpr int DPV = 64;                           \
-        BODY                                              \
+        __VA_ARGS__                                            \
     } else if ((D) <= 96) {                               \
         constexpr int DPV = 96;                           \
-        BODY                                              \
+        __VA_ARGS__                                            \
     } else if ((D) <= 128) {                              \
         constexpr int DPV = 128;                          \
-        BODY                                              \
+        __VA_ARGS__                                            \
     } else {                                              \
         constexpr int DPV = 256;                          \
-        BODY                                              \
+        __VA_ARGS__                                            \
     }
+
+template <class E, int DP, int SPLIT>
+void launch_packed_fwd_as(const PackedArgs& a, hipStream_t st) {
+    const dim3 grid(packed_blocks(a.Nq, a.S, SPLIT) * (unsigned)a.H), block(64 * kPackedWaves);
+    hipLaunchKernelGGL((born_packed_fwd_kernel<E, DP, SPLIT>), grid, block, 0, st, a);
+}
+template <class E, int DP, int SPLIT>
+void launch_packed_dq_as(const PackedArgs& a, hipStream_t st) {
+    const dim3 grid(packed_blocks(a.Nq, a.S, SPLIT) * (unsigned)a.H), block(64 * kPackedWaves);
+    hipLaunchKernelGGL((born_packed_dq_kernel<E, DP, SPLIT>), grid, block, 0, st, a);
+}
+template <class E, int DP, int SPLIT, bool DK, bool DV>
+void launch_packed_dkdv_as(const PackedArgs& a, hipStream_t st) {
+    const dim3 grid(packed_blocks(a.Nk, a.S, SPLIT) * (unsigned)a.Hkv), block(64 * kPackedWaves);
+    hipLaunchKernelGGL((born_packed_dkdv_kernel<E, DP, SPLIT, DK, DV>), grid, block, 0, st, a);
+}
 
 template <class E>
 hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t st) {
-    const dim3 grid(packed_blocks(a.Nq, a.S) * (unsigned)a.H), block(64 * kPackedWaves);
-    QDL_PACKED_DP(a.D, { hipLaunchKernelGGL((born_packed_fwd_kernel<E, DPV>), grid, block, 0, st, a); })
+    QDL_PACKED_DP(a.D, {
+        if (kPackedMaxSplit<E, DPV> > 1 && packed_split(a.Nq, a.S, a.H)) launch_packed_fwd_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
+        else launch_packed_fwd_as<E, DPV, 1>(a, st);
+    })
     return hipGetLastError();
 }
 
 // dQ first: it forms the rows' -delta and s^2 / Z.
 template <class E>
 hipError_t launch_packed_bwd(const PackedArgs& a, hipStream_t st) {
-    const dim3 grid(packed_blocks(a.Nq, a.S) * (unsigned)a.H), block(64 * kPackedWaves);
-    const dim3 kgrid(packed_blocks(a.Nk, a.S) * (unsigned)a.Hkv);
     QDL_PACKED_DP(a.D, {
         if (a.Nq > 0) {
-            hipLaunchKernelGGL((born_packed_dq_kernel<E, DPV>), grid, block, 0, st, a);
+            if (kPackedMaxSplit<E, DPV> > 1 && packed_split(a.Nq, a.S, a.H)) launch_packed_dq_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
+            else launch_packed_dq_as<E, DPV, 1>(a, st);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
         if (a.Nk > 0) {
-            if constexpr (kItem<E> * DPV > 512) {
-                hipLaunchKernelGGL((born_packed_dkdv_kernel<E, DPV, true, false>), kgrid, block, 0, st, a);
-                const hipError_t e = hipGetLastError();
-                if (e != hipSuccess) return e;
-                hipLaunchKernelGGL((born_packed_dkdv_kernel<E, DPV, false, true>), kgrid, block, 0, st, a);
+            if constexpr (kPackedMaxSplit<E, DPV> == 1) {
+                launch_packed_dkdv_as<E, DPV, 1, true, false>(a, st);
+                launch_packed_dkdv_as<E, DPV, 1, false, true>(a, st);
+            } else if (kPackedMaxSplit<E, DPV> > 2 && packed_split(a.Nk, a.S, a.Hkv)) {
+                launch_packed_dkdv_as<E, DPV, kPackedMaxSplit<E, DPV>, true, true>(a, st);
             } else {
-                hipLaunchKernelGGL((born_packed_dkdv_kernel<E, DPV, true, true>), kgrid, block, 0, st, a);
+                launch_packed_dkdv_as<E, DPV, 2, true, true>(a, st);
             }
         }
     })

@@ -60,8 +60,8 @@ int check_packed(const qdl_born_packed_call* c) {
     if (rc != QDL_BORN_OK) return rc;
     if (c->sequences < 0 || c->n_q < 0 || c->n_k < 0 || c->n_q > kMostRows || c->n_k > kMostRows || c->sequences > kMostRows)
         return QDL_BORN_E_SHAPE;
-    if ((c->n_q / qdl::kPackedRows + c->sequences + 1) * c->H > kMostBlocks ||
-        (c->n_k / qdl::kPackedRows + c->sequences + 1) * c->h_kv > kMostBlocks)
+    if ((c->n_q / qdl::packed_rows(4) + c->sequences + 1) * c->H > kMostBlocks ||
+        (c->n_k / qdl::packed_rows(4) + c->sequences + 1) * c->h_kv > kMostBlocks)
         return QDL_BORN_E_SHAPE;
     if (c->scale && c->n_scale != 1 && c->n_scale != c->H) return QDL_BORN_E_SCALE;
     if (c->window_size < 0 || c->window_size > (int64_t)1 << 30) return QDL_BORN_E_WINDOW;
@@ -220,7 +220,8 @@ int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_strea
     hipLaunchKernelGGL((qdl::born_packed_dscale_part_kernel<0>), dim3((unsigned)a.H, qdl::kPackedParts), dim3(256), 0, s, a, part);
     e = hipGetLastError();
     if (e != hipSuccess) return (int)e;
-    hipLaunchKernelGGL((qdl::born_packed_dscale_kernel<0>), dim3(1), dim3(64), 0, s, a, part, c->dscale, a.per_head_scale ? a.H : 1);
+    hipLaunchKernelGGL((qdl::born_packed_dscale_kernel<0>), dim3(1), dim3(64), 0, s, a, part, c->dscale,
+                       a.per_head_scale ? a.H : 1, c->dtype == QDL_BORN_DTYPE_F16 ? (double)qdl::kUp<qdl::F16> : 1.0);
     return hip_status(hipGetLastError());
 }
 

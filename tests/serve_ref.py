@@ -63,8 +63,9 @@ def head(q, k, v, s, keep, eps, dt, grad=None):
     ef = 2 * s2 / zz * (da * (t.abs() + et) + a * et) + f.abs() * (up + dz + 8 * U32)
     ew = dw + w * (dz + up)
     if dt == torch.float16:
-        ef = ef + 2 * 2.0 ** -25 / 64 * keep
-        ew = ew + 2.0 ** -25 / 1024 * keep
+        # Half of fp16's smallest step, in operands that are scaled up by 16.
+        ef = ef + 2 * 2.0 ** -25 / 16 * keep
+        ew = ew + 2.0 ** -25 / 16 * keep
     dq, dk, dv = torch.mm(f, k), torch.mm(f.t(), q), torch.mm(w.t(), grad)
     edq = torch.mm(ef, k.abs()) + (m + 16) * U32 * torch.mm(f.abs(), k.abs())
     edk = torch.mm(ef.t(), q.abs()) + (n + 16) * U32 * torch.mm(f.abs().t(), q.abs())
