@@ -379,7 +379,7 @@ typedef struct qdl_born_packed_call {
 } qdl_born_packed_call;
 
 int qdl_flash_born_packed_forward_call(const qdl_born_packed_call *call, qdl_stream_t stream);
-int64_t qdl_flash_born_packed_workspace_size(int64_t n_q, int64_t H);
+int64_t qdl_flash_born_packed_workspace_size(const qdl_born_packed_call *call); /* the backward's; 0 for an invalid block */
 int qdl_flash_born_packed_backward_call(const qdl_born_packed_call *call, qdl_stream_t stream);
 
 /*

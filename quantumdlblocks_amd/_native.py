@@ -140,7 +140,7 @@ def _bind(lib: ctypes.CDLL) -> None:
         call.restype = _int
         call.argtypes = [ctypes.c_char_p, _ptr]  # the packed argument block, stream
     lib.qdl_flash_born_packed_workspace_size.restype = _i64
-    lib.qdl_flash_born_packed_workspace_size.argtypes = [_i64, _i64]
+    lib.qdl_flash_born_packed_workspace_size.argtypes = [ctypes.c_char_p]
     lib.qdl_flash_born_paged_workspace_size.restype = _i64
     lib.qdl_flash_born_paged_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]
     lib.qdl_flash_purified_born_fwd.restype = _int

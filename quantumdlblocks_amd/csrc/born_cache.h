@@ -221,18 +221,20 @@ __device__ __forceinline__ uint32_t evict_key(float x) {
     return (u & 0x80000000u) ? ~u : u | 0x80000000u;
 }
 
-// NT threads, 16 weights each: 256 for caches of up to 4096 keys, where the
-// barriers are what the launch waits for, else 1024.
-constexpr int kEvictPer = 16;
+// 1024 threads with PER weights each: what the launch waits for is the
+// instructions of one wave, so the caches' capacity picks the fewest.
+constexpr int kEvictThreads = 1024, kEvictMost = 16;
 
-template <int NT>
-__global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
-    constexpr int NW = NT / 64, SPAN = NT * kEvictPer;
-    constexpr int CL = kEvictPer * NW / 64;  // counts that a lane of one wave scans
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t s_prefix, s_left;
-    __shared__ uint32_t counts[kEvictPer * NW];  // kept for sure | ties << 16, per 64 keys
-    __shared__ uint32_t s_total;
+template <int PER>
+__global__ __launch_bounds__(kEvictThreads) void born_evict_select_kernel(EvictArgs p) {
+    constexpr int NT = kEvictThreads, NW = NT / 64, SPAN = NT * PER, COPIES = 4;
+    constexpr int CL = (PER * NW + 63) / 64;  // counts that a lane of one wave scans
+    constexpr uint32_t kZero = 0x80000000u;   // the key of 0
+    // Weights lie close together: four copies of each bin, one for every fourth lane.
+    __shared__ __attribute__((aligned(16))) uint32_t hist[256 * COPIES];
+    __shared__ uint32_t s_prefix, s_left, s_all;
+    __shared__ uint32_t counts[64 * CL];  // kept for sure | ties << 16, per 64 keys
+    __shared__ uint32_t s_total, s_zeros;
     const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int n = evict_len(p, b), m = min(n, p.budget);
@@ -243,16 +245,16 @@ __global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
     const int old = n - tail, want = m - tail;  // of the `old` first keys, `want` stay
 
     const int spans = (old + SPAN - 1) / SPAN;
-    float x[kEvictPer];
-    uint32_t key[kEvictPer];
+    float x[PER];
+    uint32_t key[PER];  // 0, below every number's, where there is no key
     auto load = [&](int span) {
 #pragma unroll
-        for (int i = 0; i < kEvictPer; ++i) {
+        for (int i = 0; i < PER; ++i) {
             const int j = span * SPAN + i * NT + tid;
             x[i] = j < old && j < p.w_len ? w[j] : 0.f;
         }
 #pragma unroll
-        for (int i = 0; i < kEvictPer; ++i) key[i] = evict_key(x[i]);
+        for (int i = 0; i < PER; ++i) key[i] = span * SPAN + i * NT + tid < old ? evict_key(x[i]) : 0u;
     };
     if (want > 0) load(0);
     if (hk == 0 && tid == 0) p.lens_out[b] = m;
@@ -264,36 +266,37 @@ __global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
     }
     if (want == 0) return;
 
-    if (tid == 0) s_prefix = 0, s_left = want;
-    // The want-th greatest key, 8 bits at a time.
+    if (tid == 0) s_prefix = 0, s_left = want, s_all = 0, s_zeros = 0;
+    hist[tid] = 0;
+    for (int i = tid; i < 64 * CL; i += NT) counts[i] = 0;
+    __syncthreads();
+    // The want-th greatest key, 8 bits at a time.  Keys that were never weighed
+    // would all meet in one bin: they are counted by wave, in the first round.
     for (int shift = 24; shift >= 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
-        __syncthreads();
         const uint32_t prefix = s_prefix, mask = shift == 24 ? 0u : 0xffffffffu << (shift + 8);
+        uint32_t zeros = 0;
         for (int sp = 0; sp < spans; ++sp) {
             if (spans > 1) load(sp);
 #pragma unroll
-            for (int i = 0; i < kEvictPer; ++i) {
-                const int j = sp * SPAN + i * NT + tid;
-                const bool in = j < old && (key[i] & mask) == prefix;
-                const uint64_t active = __ballot(in);
-                if (active == 0) continue;
-                // The lanes of the first one's bin add as one: keys that were
-                // never weighed are all in one bin.
-                const uint32_t bin = (key[i] >> shift) & 255u;
-                const int first = __ffsll((long long)active) - 1;
-                const uint32_t lead = __builtin_amdgcn_readlane(bin, first);
-                const uint64_t same = __ballot(in && bin == lead);
-                if (lane == first) atomicAdd(&hist[lead], (uint32_t)__popcll(same));
-                else if (in && bin != lead) atomicAdd(&hist[bin], 1u);
+            for (int i = 0; i < PER; ++i) {
+                if (shift == 24) zeros += (uint32_t)__popcll(__ballot(key[i] == kZero));
+                if (key[i] != 0 && key[i] != kZero && (key[i] & mask) == prefix)
+                    atomicAdd(&hist[((key[i] >> shift) & 255u) * COPIES + (lane & (COPIES - 1))], 1u);
             }
         }
+        if (shift == 24 && lane == 0) atomicAdd(&s_zeros, zeros);
         __syncthreads();
         if (wave == 0) {
             // Lane l: bins 255 - 4 l .. 252 - 4 l, from the greatest down.
             uint32_t c[4], sum = 0;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) c[i] = hist[255 - 4 * lane - i], sum += c[i];
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t bin = 255 - 4 * lane - i;
+                const u32x4 h = *reinterpret_cast<const u32x4*>(&hist[bin * COPIES]);
+                c[i] = h[0] + h[1] + h[2] + h[3];
+                if ((kZero & mask) == prefix && ((kZero >> shift) & 255u) == bin) c[i] += s_zeros;
+                sum += c[i];
+            }
             uint32_t above = sum;
 #pragma unroll
             for (int o = 1; o < 64; o <<= 1) {
@@ -307,23 +310,27 @@ __global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
                 if (above < left && left <= above + c[i]) {
                     s_prefix = prefix | ((uint32_t)(255 - 4 * lane - i) << shift);
                     s_left = left - above;
+                    s_all = left == above + c[i];  // the whole bin stays: nothing left to find
                 }
                 above += c[i];
             }
         }
         __syncthreads();
+        if (s_all) break;
+        hist[tid] = 0;
+        __syncthreads();
     }
-    const uint32_t cut = s_prefix, ties = s_left;  // keys above the cut stay, and the first `ties` equal to it
+    // Keys above the cut stay, and the first `ties` equal to it.
+    const uint32_t cut = s_all ? s_prefix - 1 : s_prefix, ties = s_all ? 0u : s_left;
 
     uint32_t before_gt = 0, before_eq = 0;
     for (int sp = 0; sp < spans; ++sp) {
         if (spans > 1) load(sp);
-        uint64_t gt[kEvictPer], eq[kEvictPer];
+        uint64_t gt[PER], eq[PER];
 #pragma unroll
-        for (int i = 0; i < kEvictPer; ++i) {
-            const int j = sp * SPAN + i * NT + tid;
-            gt[i] = __ballot(j < old && key[i] > cut);
-            eq[i] = __ballot(j < old && key[i] == cut);
+        for (int i = 0; i < PER; ++i) {
+            gt[i] = __ballot(key[i] > cut);
+            eq[i] = __ballot(key[i] == cut);
             if (lane == 0) counts[i * NW + wave] = (uint32_t)__popcll(gt[i]) | ((uint32_t)__popcll(eq[i]) << 16);
         }
         __syncthreads();
@@ -348,22 +355,29 @@ __global__ __launch_bounds__(NT) void born_evict_select_kernel(EvictArgs p) {
         __syncthreads();
         const uint64_t below = (1ull << lane) - 1;
 #pragma unroll
-        for (int i = 0; i < kEvictPer; ++i) {
-            const int j = sp * SPAN + i * NT + tid;
+        for (int i = 0; i < PER; ++i) {
             const uint32_t c = counts[i * NW + wave];
             const uint32_t g = before_gt + (c & 0xffffu) + (uint32_t)__popcll(gt[i] & below);
             const uint32_t e = before_eq + (c >> 16) + (uint32_t)__popcll(eq[i] & below);
-            const bool is_gt = (gt[i] >> lane) & 1, is_eq = (eq[i] >> lane) & 1;
-            if (is_gt || (is_eq && e < ties)) {
+            if (key[i] > cut || (key[i] == cut && e < ties)) {
                 const int to = (int)(g + min(e, ties));
-                kept[to] = j;
+                kept[to] = sp * SPAN + i * NT + tid;
                 if (to < p.w_len) wo[to] = x[i];
             }
         }
+        if (spans == 1) break;
         before_gt += s_total & 0xffffu;
         before_eq += s_total >> 16;
         __syncthreads();
     }
+}
+
+inline void launch_evict_select(const EvictArgs& a, unsigned units, int64_t room, hipStream_t st) {
+    const dim3 grid(units), block(kEvictThreads);
+    if (room <= 2 * kEvictThreads) hipLaunchKernelGGL((born_evict_select_kernel<2>), grid, block, 0, st, a);
+    else if (room <= 4 * kEvictThreads) hipLaunchKernelGGL((born_evict_select_kernel<4>), grid, block, 0, st, a);
+    else if (room <= 8 * kEvictThreads) hipLaunchKernelGGL((born_evict_select_kernel<8>), grid, block, 0, st, a);
+    else hipLaunchKernelGGL((born_evict_select_kernel<kEvictMost>), grid, block, 0, st, a);
 }
 
 __device__ __forceinline__ int64_t evict_at(const EvictArgs& p, const int32_t* table, int pages, int j, int64_t sp, int64_t st) {

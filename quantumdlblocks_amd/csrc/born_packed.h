@@ -56,6 +56,8 @@ struct PackedArgs {
     const int32_t *cu_q, *cu_k;  // S + 1 starts
     int S, Nq, Nk, H, Hkv, G, D;
     int lower, upper;  // visible: lower <= query position - key < upper
+    int head_splits;   // dK/dV: workgroups that share a group's heads
+    float* part;       // their fp32 sums, (2, head_splits, Nk, Hkv, D), where there are several
     float eps;
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh, do_st, do_sh;
 };
@@ -138,12 +140,12 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
 // consecutive rows, 64 bytes each) meets a bank twice: rows that all start on
 // bank 0 by all four bits of the row, rows of alternating halves by lds_swz,
 // rows on four starts by the row's upper bits.
-template <class E, int DP, int ROWS>
+template <class E, int DP, int ROWS, int NW = kPackedWaves>
 struct PackedTile {
     static constexpr int IT = kItem<E>, RB = IT * DP, CPR = RB / 16, BYTES = ROWS * RB;
-    static constexpr int LPW = BYTES / (1024 * kPackedWaves);  // 1-KiB loads per wave
+    static constexpr int LOADS = BYTES / 1024, LPW = (LOADS + NW - 1) / NW;  // 1-KiB loads, dealt to the waves
     static constexpr int KS = RB / 32, DB = DP / 32;
-    static_assert(BYTES % (1024 * kPackedWaves) == 0, "whole loads per wave");
+    static_assert(BYTES % 1024 == 0, "whole loads");
     uint8_t* lds;
     __device__ __forceinline__ static int swz(int row) {
         if constexpr (RB % 256 == 0) return ((row & 3) << 2) | ((row >> 2) & 3);
@@ -155,7 +157,7 @@ struct PackedTile {
     __device__ __forceinline__ static void offsets(int (&off)[LPW], int stride, int D, int wave, int lane) {
 #pragma unroll
         for (int i = 0; i < LPW; ++i) {
-            const int slot = (wave * LPW + i) * 64 + lane, row = slot / CPR, chunk = (slot % CPR) ^ swz(row);
+            const int slot = (i * NW + wave) * 64 + lane, row = slot / CPR, chunk = (slot % CPR) ^ swz(row);
             off[i] = 16 * chunk < IT * D ? row * stride + 16 * chunk : kBufOOB;
         }
     }
@@ -166,7 +168,8 @@ struct PackedTile {
 #pragma unroll
         for (int i = 0; i < 4; ++i) rs[i] = __builtin_amdgcn_readfirstlane(rs[i]);
 #pragma unroll
-        for (int i = 0; i < LPW; ++i) dma_load16(rs, lds_addr(lds + (wave * LPW + i) * 1024), off[i]);
+        for (int i = 0; i < LPW; ++i)
+            if (LOADS % NW == 0 || i * NW + wave < LOADS) dma_load16(rs, lds_addr(lds + (i * NW + wave) * 1024), off[i]);
     }
     // A operand of a contraction over the head dim: row, chunk 2 ks + g.
     __device__ __forceinline__ u32x4 row(int r, int ks, int g) const {
@@ -282,14 +285,43 @@ __device__ __forceinline__ void packed_store_row(uint8_t* row, const f32x16 (&ac
 constexpr float kF16Start = 0x1p60f;
 __device__ __forceinline__ float f16_factor(float largest) {
     const int e = (int)((__float_as_uint(largest) >> 23) & 255u) - 127;
-    return __uint_as_float((uint32_t)(min(max(6 - e, -126), 127) + 127) << 23);
+    return __uint_as_float((uint32_t)(min(max(6 - e, -126), 60) + 127) << 23);
 }
 
-// fp16 gradients' operands, p / Z and the factor of dS, are scaled by this power
-// of two: what rounding then takes from a small one lies below the step of a
-// small fp16 output, and one overflows only where the gradient nearly does.
+// fp16 gradients' operands.  p / Z is at most 1: times 16, what rounding takes
+// from a small one lies below the step of a small fp16 output.  The factor u of
+// dS has no bound (a row whose overlaps are all small divides by their sum), so
+// it is kept in fp16's range like the weights: by a power of two per column of
+// its product, which drops where a part would pass the bound, with what that
+// column has summed.
 template <class E>
 constexpr float kUp = std::is_same<E, F16>::value ? 16.f : 1.f;
+template <class E, int DB>
+__device__ __forceinline__ void packed_fit(float (&u)[16], float& f, f32x16 (&acc)[DB]) {
+    if constexpr (std::is_same<E, F16>::value) {
+        float m = 0.f;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) m = fmaxf(m, fabsf(u[r]));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        if (__ballot(m * f > 61440.f) != 0) {
+            const float to = m * f > 61440.f ? f16_factor(m) * 256.f : f, by = to / f;  // to [2^14, 2^15)
+            f = to;
+#pragma unroll
+            for (int db = 0; db < DB; ++db) acc[db] *= by;
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) u[r] *= f;
+    }
+}
+template <class E, int DB>
+__device__ __forceinline__ void packed_unfit(float& f, f32x16 (&acc)[DB]) {
+    if constexpr (std::is_same<E, F16>::value) {
+        const float by = 1.f / f;
+        f = 1.f;
+#pragma unroll
+        for (int db = 0; db < DB; ++db) acc[db] *= by;
+    }
+}
 
 // 32 rows of a wave's accumulators to its share of the reduction buffer, rows of
 // DP + 4 floats, and another wave's share added to a wave's own.
@@ -351,8 +383,11 @@ struct PackedCfg {
     static constexpr int SMEM = RING > REDUCE ? RING : REDUCE;
     static_assert(SMEM <= 160 * 1024 - 4096, "LDS");
     // Forward and dQ: two workgroups per CU where the ring and the registers
-    // let them; above, one.
+    // let them; above, one.  The 16-bit forward up to head dim 64, whose
+    // products are short beside its weights, has room for four (8 prompts of
+    // 2048 tokens, 16 heads: 97 us with two, 91 with three, 87 with four).
     static constexpr int WPE = RB <= 256 && SMEM <= 78 * 1024 ? 2 : 1;
+    static constexpr int FWD_WPE = RB == 128 && SPLIT == 1 ? 4 : WPE;
 };
 
 // A block of the forward or dQ: its rows, the keys that they see, their loads.
@@ -442,7 +477,7 @@ struct PackedQueries {
 // ---------------------------------------------------------------------------
 template <class E, int DP, int SPLIT>
 __global__ __launch_bounds__(64 * kPackedWaves)
-__attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP, SPLIT>::WPE, PackedCfg<E, DP, SPLIT>::WPE)))
+__attribute__((amdgpu_waves_per_eu(PackedCfg<E, DP, SPLIT>::FWD_WPE, PackedCfg<E, DP, SPLIT>::FWD_WPE)))
 void born_packed_fwd_kernel(PackedArgs p) {
     using C = PackedCfg<E, DP, SPLIT>;
     using Q = PackedQueries<E, DP, SPLIT>;
@@ -587,8 +622,7 @@ void born_packed_dq_kernel(PackedArgs p) {
     f32x16 acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
-    // fp16 scales each operand into its range; otherwise zs is a row's factor.
-    const float pre = std::is_same<E, F16>::value ? kUp<E> * zs : 1.f;
+    float f = std::is_same<E, F16>::value ? kF16Start : 1.f;
     asm volatile("" : "+v"(delta));
 
     const int r0 = 32 * C::SUB * b.part;  // this wave's part of every tile
@@ -606,21 +640,19 @@ void born_packed_dq_kernel(PackedArgs p) {
                 t = packed_step<E>(vt.row(r0 + 32 * nb + c, ks, g), dr[ks], t);
             }
             if constexpr (kind.value == 2) b.mask(p, s, key0 + 32 * nb);
+            // Without zs, the row's factor.
             PackedWeights<E> w;
+            float x[16];
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                float x[2];
+            for (int r = 0; r < 16; ++r) x[r] = relu_f32(s[r]) * t[r];
+            packed_fit<E>(x, f, acc);
 #pragma unroll
-                for (int e = 0; e < 2; ++e) {
-                    const float a = relu_f32(s[2 * j + e]);
-                    x[e] = (std::is_same<E, F16>::value ? a * pre : a) * t[2 * j + e];
-                }
-                w.set(j, x[0], x[1]);
-            }
+            for (int j = 0; j < 8; ++j) w.set(j, x[2 * j], x[2 * j + 1]);
             packed_columns<E>(kt, r0 + 32 * nb, w, acc, lane);
         }
     });
     if constexpr (SPLIT > 1) {
+        packed_unfit<E>(f, acc);
         float* const red = reinterpret_cast<float*>(ring);
         auto share = [&](int part) { return red + ((part - 1) * C::GROUPS + b.group) * 32 * (DP + 4); };
         __syncthreads();
@@ -631,7 +663,55 @@ void born_packed_dq_kernel(PackedArgs p) {
         for (int i = 1; i < SPLIT; ++i) packed_add(acc, share(i), c, g);
     }
     if (!b.ok) return;
-    packed_store_row<E>((uint8_t*)p.dq + at, acc, std::is_same<E, F16>::value ? 2.f / kUp<E> : 2.f * zs, D, g);
+    packed_store_row<E>((uint8_t*)p.dq + at, acc, std::is_same<E, F16>::value ? 2.f * zs * (1.f / f) : 2.f * zs, D, g);
+}
+
+// A dK/dV workgroup's key head, block and heads g0 .. g1 - 1 of the group.
+struct PackedHeads {
+    int hk, block, split, g0, g1;
+    __device__ __forceinline__ PackedHeads(const PackedArgs& p) {
+        hk = blockIdx.x % p.Hkv;
+        const int rest = blockIdx.x / p.Hkv;
+        split = rest % p.head_splits;
+        block = rest / p.head_splits;
+        g0 = p.G * split / p.head_splits;
+        g1 = p.G * (split + 1) / p.head_splits;
+    }
+};
+
+// A key's row of dK (which = 0) or dV (1): the output, or this workgroup's part.
+template <class E, int DB>
+__device__ __forceinline__ void packed_store_keys(const PackedArgs& p, void* out, int which, int split, size_t at,
+                                                  const f32x16 (&acc)[DB], float f, int g) {
+    if (p.head_splits > 1) {
+        const size_t whole = (size_t)p.Nk * p.Hkv * p.D;
+        packed_store_row<F32>((uint8_t*)(p.part + (which * p.head_splits + split) * whole + at), acc, f, p.D, g);
+    } else {
+        packed_store_row<E>((uint8_t*)out + at * kItem<E>, acc, f, p.D, g);
+    }
+}
+
+// The parts' sums, in order: 8 values a thread, dK and then dV.
+template <class E>
+__global__ __launch_bounds__(256) void born_packed_dkdv_join_kernel(PackedArgs p) {
+    const size_t whole = (size_t)p.Nk * p.Hkv * p.D, i = ((size_t)blockIdx.x * 256 + threadIdx.x) * 8;
+    if (i >= 2 * whole) return;
+    const int which = i >= whole;
+    const size_t at = i - which * whole;
+    const float* src = p.part + which * p.head_splits * whole + at;
+    f32x4 x = *reinterpret_cast<const f32x4*>(src), y = *reinterpret_cast<const f32x4*>(src + 4);
+    for (int k = 1; k < p.head_splits; ++k) {
+        x += *reinterpret_cast<const f32x4*>(src + k * whole);
+        y += *reinterpret_cast<const f32x4*>(src + k * whole + 4);
+    }
+    uint8_t* out = (uint8_t*)(which ? p.dv : p.dk) + at * kItem<E>;
+    if constexpr (std::is_same<E, F32>::value) {
+        *reinterpret_cast<f32x4*>(out) = x;
+        *reinterpret_cast<f32x4*>(out + 16) = y;
+    } else {
+        const u32x4 w = {E::pack(x[0], x[1]), E::pack(x[2], x[3]), E::pack(y[0], y[1]), E::pack(y[2], y[3])};
+        *reinterpret_cast<u32x4*>(out) = w;
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -653,13 +733,14 @@ __global__ __launch_bounds__(64 * kPackedWaves) __attribute__((amdgpu_waves_per_
 void born_packed_dkdv_kernel(PackedArgs p) {
     using C = PackedCfg<E, DP, SPLIT>;
     using Tile = PackedTile<E, DP, C::BN>;
-    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, SUB = C::SUB, IT = kItem<E>;
-    constexpr bool kPhased = SUB == 2 && IT == 2 && DK && DV;
+    constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, SUB = C::SUB;
+    constexpr bool kPhased = SUB == 2 && kItem<E> == 2 && DK && DV;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[C::SMEM];
     __shared__ __attribute__((aligned(16))) float stats[NST][2][BN];  // -delta, zs
 
-    const int hk = blockIdx.x % p.Hkv;
-    const PackedSeq sq = packed_seq<true, C::BM>(p, blockIdx.x / p.Hkv);
+    const PackedHeads hd(p);
+    const int hk = hd.hk;
+    const PackedSeq sq = packed_seq<true, C::BM>(p, hd.block);
     const int k0 = sq.tile * C::BM;
     if (k0 >= sq.nk) return;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -670,7 +751,7 @@ void born_packed_dkdv_kernel(PackedArgs p) {
     // Queries that see the block's keys, as tiles of BN, for each head.
     const int k1 = min(sq.nk, k0 + C::BM);
     const int ilo = max(0, k0 - off + p.lower), ihi = min(sq.nq - 1, k1 - 1 - off + p.upper - 1);
-    const int t0 = ilo / BN, nt = ihi >= ilo ? ihi / BN - t0 + 1 : 0, n = nt * p.G;
+    const int t0 = ilo / BN, nt = ihi >= ilo ? ihi / BN - t0 + 1 : 0, n = nt * (hd.g1 - hd.g0);
 
     int qoff[Tile::LPW], doff[Tile::LPW];
     Tile::offsets(qoff, (int)p.q_st, D, wave, lane);
@@ -708,6 +789,7 @@ void born_packed_dkdv_kernel(PackedArgs p) {
         if constexpr (DK) dk[db] = zero16();
         if constexpr (DV) dv[db] = zero16();
     }
+    float f = std::is_same<E, F16>::value ? kF16Start : 1.f;
     const int span = p.upper - p.lower;
 
     // Row values r0 + 8 j + 4 g + e.
@@ -731,18 +813,23 @@ void born_packed_dkdv_kernel(PackedArgs p) {
                 if ((uint32_t)(d + acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
         }
         const f32x16 zi = values(stats[st][1], r0);
+        float u[16];
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            float ww[2], uu[2];
+            float ww[2];
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
                 const int r = 2 * j + e;
                 const float a = relu_f32(s[r]), t = a * zi[r];
                 ww[e] = fabsf(t) * a;  // zs carries the sign of s
-                uu[e] = t * dp[r];
+                u[r] = t * dp[r];
             }
             if constexpr (DV) w.set(j, ww[0], ww[1]);
-            if constexpr (DK) x.set(j, uu[0], uu[1]);
+        }
+        if constexpr (DK) {
+            packed_fit<E>(u, f, dk);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) x.set(j, u[2 * j], u[2 * j + 1]);
         }
     };
 
@@ -847,8 +934,8 @@ void born_packed_dkdv_kernel(PackedArgs p) {
     const PackedRuns runs(nt, t0 * BN + r0 + off - kw, BN, 32 * SUB, p.lower, p.upper + 30, p.lower + 31, p.upper - 1);
     uint32_t flip = 0;  // the scale's sign, folded into K
     int u = 0;          // tiles so far
-    if (n > 0) issue(hk * p.G, 0, 0);
-    for (int gi = 0; gi < p.G; ++gi) {
+    if (n > 0) issue(hk * p.G + hd.g0, 0, 0);
+    for (int gi = hd.g0; gi < hd.g1; ++gi) {
         const uint32_t fl = packed_flip<E>(arg_scale(p, hk * p.G + gi));
         if (fl != flip) {
 #pragma unroll
@@ -885,14 +972,184 @@ void born_packed_dkdv_kernel(PackedArgs p) {
                 for (int i = 1; i < SPLIT; ++i) packed_add(acc, share(i), c, g);
             }
         };
-        if constexpr (DK) join(dk);
+        if constexpr (DK) {
+            packed_unfit<E>(f, dk);
+            join(dk);
+        }
         if constexpr (DV) join(dv);
         if (part > 0) return;
     }
     if (!ok) return;
-    const size_t at = ((size_t)(sq.k0 + key) * p.Hkv + hk) * D * IT;  // contiguous (Nk, Hkv, D)
-    if constexpr (DK) packed_store_row<E>((uint8_t*)p.dk + at, dk, 2.f / kUp<E>, D, g);
-    if constexpr (DV) packed_store_row<E>((uint8_t*)p.dv + at, dv, 1.f / kUp<E>, D, g);
+    const size_t at = ((size_t)(sq.k0 + key) * p.Hkv + hk) * D;  // contiguous (Nk, Hkv, D)
+    if constexpr (DK) packed_store_keys<E>(p, p.dk, 0, hd.split, at, dk, std::is_same<E, F16>::value ? 2.f / kUp<E> * (1.f / f) : 2.f, g);
+    if constexpr (DV) packed_store_keys<E>(p, p.dv, 1, hd.split, at, dv, 1.f / kUp<E>, g);
+}
+
+// ---------------------------------------------------------------------------
+// dK / dV of long blocks (16-bit, up to head dim 128): eight waves, two on each
+// SIMD, over 128 keys.  The stationary rows stay in LDS beside the ring, which
+// leaves a wave the registers of its accumulators; four waves take 32 keys each
+// of a tile's first half, four of its second.  Every tile feeds 128 keys, so
+// the tiles' way from L2, which bounds 64-key blocks, is half as long.
+// ---------------------------------------------------------------------------
+template <class E, int DP>
+__global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
+void born_packed_dkdv8_kernel(PackedArgs p) {
+    constexpr int NW = 8, BM = 128, BN = 64, NST = 2;
+    using Tile = PackedTile<E, DP, BN, NW>;
+    using Keys = PackedTile<E, DP, BM, NW>;
+    constexpr int KS = Tile::KS, DB = Tile::DB, STAGE = 2 * Tile::BYTES;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[NST * STAGE + 2 * Keys::BYTES];  // and K, V
+    uint8_t* const keys = ring + NST * STAGE;
+    __shared__ __attribute__((aligned(16))) float stats[NST][2][BN];  // -delta, zs
+
+    const PackedHeads hd(p);
+    const int hk = hd.hk;
+    const PackedSeq sq = packed_seq<true, BM>(p, hd.block);
+    const int k0 = sq.tile * BM;
+    if (k0 >= sq.nk) return;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int c = lane & 31, g = lane >> 5, group = wave & 3, part = wave >> 2;
+    const int D = p.D, off = sq.nk - sq.nq;
+
+    const int k1 = min(sq.nk, k0 + BM);
+    const int ilo = max(0, k0 - off + p.lower), ihi = min(sq.nq - 1, k1 - 1 - off + p.upper - 1);
+    const int t0 = ilo / BN, nt = ihi >= ilo ? ihi / BN - t0 + 1 : 0, n = nt * (hd.g1 - hd.g0);
+
+    int qoff[Tile::LPW], doff[Tile::LPW];
+    Tile::offsets(qoff, (int)p.q_st, D, wave, lane);
+    Tile::offsets(doff, (int)p.do_st, D, wave, lane);
+    auto issue = [&](int h, int t, int st) __attribute__((always_inline)) {
+        const int i0 = (t0 + t) * BN, left = sq.nq - i0;
+        const int64_t r = sq.q0 + i0;
+        const Tile q{ring + st * STAGE}, d{ring + st * STAGE + Tile::BYTES};
+        q.issue((const uint8_t*)p.q + r * p.q_st + (int64_t)h * p.q_sh, left, (int)p.q_st, D, qoff, wave);
+        d.issue((const uint8_t*)p.dout + r * p.do_st + (int64_t)h * p.do_sh, left, (int)p.do_st, D, doff, wave);
+        if (wave < 2) {
+            const float* v = (wave == 0 ? p.ndelta : p.zs) + (size_t)h * p.Nq + r;
+            i32x4 rs = buffer_rsrc(v, (uint32_t)(4 * max(0, min(left, BN))));
+#pragma unroll
+            for (int i = 0; i < 4; ++i) rs[i] = __builtin_amdgcn_readfirstlane(rs[i]);
+            if (lane < BN / 4) dma_load16(rs, lds_addr(stats[st][wave]), 16 * lane);
+        }
+    };
+    const Keys kt{keys}, vt{keys + Keys::BYTES};
+    {
+        int koff[Keys::LPW];
+        const int64_t r = sq.k0 + k0;
+        Keys::offsets(koff, (int)p.k_st, D, wave, lane);
+        kt.issue((const uint8_t*)p.k + r * p.k_st + (int64_t)hk * p.k_sh, sq.nk - k0, (int)p.k_st, D, koff, wave);
+        Keys::offsets(koff, (int)p.v_st, D, wave, lane);
+        vt.issue((const uint8_t*)p.v + r * p.v_st + (int64_t)hk * p.v_sh, sq.nk - k0, (int)p.v_st, D, koff, wave);
+    }
+    const int kw = k0 + 32 * group, key = kw + c, r0 = 32 * part;
+    f32x16 dk[DB], dv[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) dk[db] = zero16(), dv[db] = zero16();
+    float f = std::is_same<E, F16>::value ? kF16Start : 1.f;
+    const int span = p.upper - p.lower;
+
+    auto tile = [&](int t, int st, auto kind) __attribute__((always_inline)) {
+        const Tile q{ring + st * STAGE}, d{ring + st * STAGE + Tile::BYTES};
+        f32x16 s = zero16(), dp;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 a = *reinterpret_cast<const f32x4*>(&stats[st][0][r0 + 8 * j + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) dp[4 * j + e] = a[e];
+        }
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) {
+            s = E::mfma(q.row(r0 + c, ks, g), kt.row(32 * group + c, ks, g), s);
+            dp = E::mfma(d.row(r0 + c, ks, g), vt.row(32 * group + c, ks, g), dp);
+        }
+        if constexpr (kind.value == 2) {
+            const int x = (t0 + t) * BN + r0 + off - key - p.lower;
+#pragma unroll
+            for (int r = 0; r < 16; ++r)
+                if ((uint32_t)(x + acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+        }
+        PackedWeights<E> w, x;
+        float uu[16];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const f32x4 zi = *reinterpret_cast<const f32x4*>(&stats[st][1][r0 + 8 * j + 4 * g]);
+#pragma unroll
+            for (int e = 0; e < 4; e += 2) {
+                float ww[2];
+#pragma unroll
+                for (int i = 0; i < 2; ++i) {
+                    const int r = 4 * j + e + i;
+                    const float a = relu_f32(s[r]), y = a * zi[e + i];
+                    ww[i] = fabsf(y) * a;  // zs carries the sign of s
+                    uu[r] = y * dp[r];
+                }
+                w.set(2 * j + e / 2, ww[0], ww[1]);
+            }
+        }
+        packed_fit<E>(uu, f, dk);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x.set(j, uu[2 * j], uu[2 * j + 1]);
+#pragma unroll
+        for (int hh = 0; hh < 2; ++hh) {
+            const u32x4 bw = {w.w[4 * hh], w.w[4 * hh + 1], w.w[4 * hh + 2], w.w[4 * hh + 3]};
+            const u32x4 bx = {x.w[4 * hh], x.w[4 * hh + 1], x.w[4 * hh + 2], x.w[4 * hh + 3]};
+#pragma unroll
+            for (int db = 0; db < DB; ++db) {
+                dv[db] = E::mfma(d.transposed(r0 + 16 * hh, db, lane), bw, dv[db]);
+                dk[db] = E::mfma(q.transposed(r0 + 16 * hh, db, lane), bx, dk[db]);
+            }
+        }
+    };
+
+    // Positions of the queries from the wave's first key on.
+    const PackedRuns runs(nt, t0 * BN + r0 + off - kw, BN, 32, p.lower, p.upper + 30, p.lower + 31, p.upper - 1);
+    uint32_t flip = 0;  // the scale's sign, folded into K
+    int u = 0;          // tiles so far
+    if (n > 0) issue(hk * p.G + hd.g0, 0, 0);
+    for (int gi = hd.g0; gi < hd.g1; ++gi) {
+        const uint32_t fl = packed_flip<E>(arg_scale(p, hk * p.G + gi));
+        if (fl != flip) {
+            wait_vmcnt<0>();
+            __syncthreads();  // K has arrived, and the last head's tiles are done
+            for (int i = threadIdx.x; i < Keys::BYTES / 16; i += 64 * NW) reinterpret_cast<u32x4*>(keys)[i] ^= fl ^ flip;
+            flip = fl;
+        }
+        int t = 0;
+        auto run = [&](int end, auto kind) __attribute__((always_inline)) {
+            for (; t < end; ++t, ++u) {
+                wait_vmcnt<0>();
+                __syncthreads();
+                if (u + 1 < n) {
+                    const bool last = t + 1 == nt;
+                    issue(hk * p.G + gi + (last ? 1 : 0), last ? 0 : t + 1, (u + 1) % NST);
+                }
+                if constexpr (kind.value != 0) tile(t, u % NST, kind);
+            }
+        };
+        run(runs.ta, PackedIdle{});
+        run(runs.tf, PackedCut{});
+        run(runs.tg, PackedFull{});
+        run(runs.tv, PackedCut{});
+        run(nt, PackedIdle{});
+    }
+    // The second half's sums to the first's waves, dK and then dV.
+    static_assert(4 * 32 * (DP + 4) * 4 <= NST * STAGE + 2 * Keys::BYTES, "room for the shares");
+    wait_vmcnt<0>();
+    float* const red = reinterpret_cast<float*>(ring) + group * 32 * (DP + 4);
+    auto join = [&](f32x16 (&acc)[DB]) __attribute__((always_inline)) {
+        __syncthreads();
+        if (part > 0) packed_put(red, acc, c, g);
+        __syncthreads();
+        if (part == 0) packed_add(acc, red, c, g);
+    };
+    packed_unfit<E>(f, dk);
+    join(dk);
+    join(dv);
+    if (part > 0 || key >= sq.nk) return;
+    const size_t at = ((size_t)(sq.k0 + key) * p.Hkv + hk) * D;  // contiguous (Nk, Hkv, D)
+    packed_store_keys<E>(p, p.dk, 0, hd.split, at, dk, 2.f / kUp<E>, g);
+    packed_store_keys<E>(p, p.dv, 1, hd.split, at, dv, 1.f / kUp<E>, g);
 }
 
 // ---------------------------------------------------------------------------
@@ -941,8 +1198,49 @@ inline unsigned packed_blocks(int N, int S, int split) { return (unsigned)(N / p
 template <class E, int DP>
 constexpr int kPackedMaxSplit = kItem<E> * DP <= 256 ? 4 : kItem<E> * DP <= 512 ? 2 : 1;
 
-// Forward and dQ: unsplit blocks unless they are too few to fill the chip.
-inline bool packed_split(int N, int S, int heads) { return (int64_t)packed_blocks(N, S, 1) * heads < 512; }
+// How a launch of few blocks is divided.  The lengths are on the device, so the
+// longest sequence is taken for half as long again as the mean.
+struct PackedPlan {
+    bool split_q, split_k;  // 32-row blocks of four waves: forward and dQ, dK/dV
+    int head_splits;
+};
+inline PackedPlan packed_plan(int item, int64_t Nq, int64_t Nk, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t window) {
+    const int64_t rb = D <= 64 ? 64 * item : D <= 96 ? 96 * item : D <= 128 ? 128 * item : 256 * item;
+    const double seqs = S > 0 ? (double)S : 1.0;
+    PackedPlan r = {};
+    // A block costs its start, its tiles and its end; a is the first and last
+    // in 64-row tiles (fp32's are four times as long).  Split blocks walk a
+    // quarter of the tiles, a third slower each, and above 128-byte rows have a
+    // CU to themselves.  Measured, us unsplit and split: fp32 3 sequences of
+    // 1000 tokens, 8 heads D64, forward 42 and 18, dQ 57 and 24; fp16 5
+    // sequences of 3125 tokens, 6 heads D96, a window of 384: 17 and 26, 19 and 30.
+    if (rb <= 512) {
+        const double a = item == 2 ? 6.0 : 1.5, share = rb <= 256 ? 4.0 : 2.0;
+        double longest = 1.5 * (double)Nk / seqs;
+        if (longest > (double)Nk) longest = (double)Nk;
+        if (window > 0 && longest > window + 128.0) longest = window + 128.0;
+        const double c = longest / 64.0;
+        const double whole = (double)packed_blocks((int)Nq, (int)S, 1) * H / (rb <= 256 ? 512.0 : 256.0);
+        const double parts = (double)packed_blocks((int)Nq, (int)S, (int)share) * H / (rb == 128 ? 512.0 : 256.0);
+        r.split_q = (parts > 1.0 ? parts : 1.0) * (a + 1.33 * c / share) < (whole > 1.0 ? whole : 1.0) * (a + c);
+    }
+    const int64_t few = (int64_t)packed_blocks((int)Nk, (int)S, 4) * Hkv;
+    r.split_k = rb <= 256 && few <= 512;
+    // Heads of a group are shared out while the launch has too few blocks to
+    // even out their lengths and a block has tiles to share.  Each share costs
+    // its sums in fp32, written and read again.
+    const int64_t G = H / Hkv, blocks = r.split_k ? few : (int64_t)packed_blocks((int)Nk, (int)S, rb <= 256 && item == 2 ? 1 : 2) * Hkv;
+    double rows = 1.5 * (double)Nq / seqs;
+    if (rows > (double)Nq) rows = (double)Nq;
+    if (window > 0 && rows > window + 128.0) rows = window + 128.0;
+    int64_t hs = 1;
+    while (2 * hs <= G && blocks * hs < (r.split_k ? 192 : 1024) && (double)(G / hs) * rows / 64.0 >= 32.0) hs *= 2;
+    r.head_splits = (int)hs;
+    return r;
+}
+inline int64_t packed_part_bytes(const PackedPlan& r, int64_t Nk, int64_t Hkv, int64_t D) {
+    return r.head_splits > 1 ? 2 * r.head_splits * Nk * Hkv * D * 4 : 0;
+}
 
 #define QDL_PACKED_DP(D, ...)                             \
     if ((D) <= 64) {                                      \
@@ -971,14 +1269,14 @@ void launch_packed_dq_as(const PackedArgs& a, hipStream_t st) {
 }
 template <class E, int DP, int SPLIT, bool DK, bool DV>
 void launch_packed_dkdv_as(const PackedArgs& a, hipStream_t st) {
-    const dim3 grid(packed_blocks(a.Nk, a.S, SPLIT) * (unsigned)a.Hkv), block(64 * kPackedWaves);
+    const dim3 grid(packed_blocks(a.Nk, a.S, SPLIT) * (unsigned)(a.Hkv * a.head_splits)), block(64 * kPackedWaves);
     hipLaunchKernelGGL((born_packed_dkdv_kernel<E, DP, SPLIT, DK, DV>), grid, block, 0, st, a);
 }
 
 template <class E>
-hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t st) {
+hipError_t launch_packed_fwd(const PackedArgs& a, const PackedPlan& plan, hipStream_t st) {
     QDL_PACKED_DP(a.D, {
-        if (kPackedMaxSplit<E, DPV> > 1 && packed_split(a.Nq, a.S, a.H)) launch_packed_fwd_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
+        if (kPackedMaxSplit<E, DPV> > 1 && plan.split_q) launch_packed_fwd_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
         else launch_packed_fwd_as<E, DPV, 1>(a, st);
     })
     return hipGetLastError();
@@ -986,10 +1284,10 @@ hipError_t launch_packed_fwd(const PackedArgs& a, hipStream_t st) {
 
 // dQ first: it forms the rows' -delta and s^2 / Z.
 template <class E>
-hipError_t launch_packed_bwd(const PackedArgs& a, hipStream_t st) {
+hipError_t launch_packed_bwd(const PackedArgs& a, const PackedPlan& plan, hipStream_t st) {
     QDL_PACKED_DP(a.D, {
         if (a.Nq > 0) {
-            if (kPackedMaxSplit<E, DPV> > 1 && packed_split(a.Nq, a.S, a.H)) launch_packed_dq_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
+            if (kPackedMaxSplit<E, DPV> > 1 && plan.split_q) launch_packed_dq_as<E, DPV, kPackedMaxSplit<E, DPV>>(a, st);
             else launch_packed_dq_as<E, DPV, 1>(a, st);
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
@@ -998,20 +1296,29 @@ hipError_t launch_packed_bwd(const PackedArgs& a, hipStream_t st) {
             if constexpr (kPackedMaxSplit<E, DPV> == 1) {
                 launch_packed_dkdv_as<E, DPV, 1, true, false>(a, st);
                 launch_packed_dkdv_as<E, DPV, 1, false, true>(a, st);
-            } else if (kPackedMaxSplit<E, DPV> > 2 && packed_split(a.Nk, a.S, a.Hkv)) {
-                launch_packed_dkdv_as<E, DPV, kPackedMaxSplit<E, DPV>, true, true>(a, st);
+            } else if constexpr (kPackedMaxSplit<E, DPV> == 2) {
+                launch_packed_dkdv_as<E, DPV, 2, true, true>(a, st);
+            } else if (plan.split_k) {
+                launch_packed_dkdv_as<E, DPV, 4, true, true>(a, st);
+            } else if constexpr (kItem<E> == 2) {
+                const dim3 grid(packed_blocks(a.Nk, a.S, 1) * (unsigned)(a.Hkv * a.head_splits));
+                hipLaunchKernelGGL((born_packed_dkdv8_kernel<E, DPV>), grid, dim3(512), 0, st, a);
             } else {
                 launch_packed_dkdv_as<E, DPV, 2, true, true>(a, st);
             }
         }
     })
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || a.Nk == 0 || a.head_splits == 1) return e;
+    const int64_t pieces = (int64_t)a.Nk * a.Hkv * a.D / 4;  // of 8 values, dK and dV
+    hipLaunchKernelGGL((born_packed_dkdv_join_kernel<E>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();
 }
 
 // Entry points of the per-dtype translation units.
 template <class E>
-hipError_t packed_fwd(const PackedArgs& a, hipStream_t st);
+hipError_t packed_fwd(const PackedArgs& a, const PackedPlan& plan, hipStream_t st);
 template <class E>
-hipError_t packed_bwd(const PackedArgs& a, hipStream_t st);
+hipError_t packed_bwd(const PackedArgs& a, const PackedPlan& plan, hipStream_t st);
 
 }  // namespace qdl

@@ -61,7 +61,7 @@ int check_packed(const qdl_born_packed_call* c) {
     if (c->sequences < 0 || c->n_q < 0 || c->n_k < 0 || c->n_q > kMostRows || c->n_k > kMostRows || c->sequences > kMostRows)
         return QDL_BORN_E_SHAPE;
     if ((c->n_q / qdl::packed_rows(4) + c->sequences + 1) * c->H > kMostBlocks ||
-        (c->n_k / qdl::packed_rows(4) + c->sequences + 1) * c->h_kv > kMostBlocks)
+        (c->n_k / qdl::packed_rows(4) + c->sequences + 1) * c->H > kMostBlocks || c->n_k * c->h_kv * c->D > (int64_t)1 << 33)
         return QDL_BORN_E_SHAPE;
     if (c->scale && c->n_scale != 1 && c->n_scale != c->H) return QDL_BORN_E_SCALE;
     if (c->window_size < 0 || c->window_size > (int64_t)1 << 30) return QDL_BORN_E_WINDOW;
@@ -102,6 +102,7 @@ qdl::PackedArgs packed_args(const qdl_born_packed_call* c) {
     a.D = (int)c->D;
     a.lower = c->is_causal ? 0 : -kFar;
     a.upper = c->window_size > 0 ? (int)c->window_size : kFar;
+    a.head_splits = 1;
     a.eps = (float)c->eps;
     a.q_st = c->q_strides[0] * it;
     a.q_sh = c->q_strides[1] * it;
@@ -116,8 +117,17 @@ qdl::PackedArgs packed_args(const qdl_born_packed_call* c) {
 
 int64_t packed_stats(int64_t n_q, int64_t H) { return (H * n_q * 4 + 15) / 16 * 16; }
 
+qdl::PackedPlan packed_plan(const qdl_born_packed_call* c) {
+    return qdl::packed_plan((int)item(c->dtype), c->n_q, c->n_k, c->sequences, c->H, c->h_kv, c->D, c->window_size);
+}
+// The backward's workspace: the rows' two values, dscale's parts, and the sums
+// of head splits.
+int64_t packed_workspace(const qdl_born_packed_call* c) {
+    return 2 * packed_stats(c->n_q, c->H) + c->H * qdl::kPackedParts * 8 + qdl::packed_part_bytes(packed_plan(c), c->n_k, c->h_kv, c->D);
+}
+
 // Splits of a paged launch: enough workgroups for four a compute unit, none
-// under 128 keys (a wave's 32) or over 512.
+// under 128 keys (a wave's 32) or over 1024.
 struct PagedPlan {
     int64_t chunk, nsplit, gblocks, raw_ld, part_bytes, raw_bytes, inv_bytes;
     int64_t bytes() const { return part_bytes + raw_bytes + inv_bytes; }
@@ -132,7 +142,7 @@ PagedPlan paged_plan(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t page
     const int64_t want = units > 0 ? (1024 + units - 1) / units : 1;
     int64_t chunk = (span + want - 1) / want;
     chunk = (chunk + 127) / 128 * 128;
-    if (chunk > 512) chunk = 512;
+    if (chunk > 1024) chunk = 1024;
     r.chunk = chunk;
     r.nsplit = (span + chunk - 1) / chunk;
     r.raw_ld = (room + 31) / 32 * 32;
@@ -185,15 +195,14 @@ int qdl_flash_born_packed_forward_call(const qdl_born_packed_call* c, qdl_stream
     const qdl::PackedArgs a = packed_args(c);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (c->dtype) {
-        case QDL_BORN_DTYPE_BF16: return hip_status(qdl::packed_fwd<qdl::BF16>(a, s));
-        case QDL_BORN_DTYPE_F16: return hip_status(qdl::packed_fwd<qdl::F16>(a, s));
-        default: return hip_status(qdl::packed_fwd<qdl::F32>(a, s));
+        case QDL_BORN_DTYPE_BF16: return hip_status(qdl::packed_fwd<qdl::BF16>(a, packed_plan(c), s));
+        case QDL_BORN_DTYPE_F16: return hip_status(qdl::packed_fwd<qdl::F16>(a, packed_plan(c), s));
+        default: return hip_status(qdl::packed_fwd<qdl::F32>(a, packed_plan(c), s));
     }
 }
 
-int64_t qdl_flash_born_packed_workspace_size(int64_t n_q, int64_t H) {
-    if (n_q < 0 || H < 0 || n_q > kMostRows || H > kMostHeads) return 0;
-    return 2 * packed_stats(n_q, H) + H * qdl::kPackedParts * 8;
+int64_t qdl_flash_born_packed_workspace_size(const qdl_born_packed_call* c) {
+    return check_packed(c) == QDL_BORN_OK ? packed_workspace(c) : 0;
 }
 
 int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_stream_t stream) {
@@ -202,19 +211,22 @@ int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_strea
     if ((c->n_q > 0 && (!c->dout || !c->dq || !c->z)) || (c->n_k > 0 && (!c->dk || !c->dv))) return QDL_BORN_E_NULL;
     if (!aligned16(c->dout) || !aligned16(c->dq) || !aligned16(c->dk) || !aligned16(c->dv)) return QDL_BORN_E_ALIGN;
     if (c->n_q > 0 && !rows_ok(c->dout_strides, item(c->dtype), c->D)) return QDL_BORN_E_STRIDE;
-    if (c->workspace_bytes < qdl_flash_born_packed_workspace_size(c->n_q, c->H) || !c->workspace || !aligned16(c->workspace))
+    if (c->workspace_bytes < packed_workspace(c) || !c->workspace || !aligned16(c->workspace))
         return QDL_BORN_E_WORKSPACE;
     qdl::PackedArgs a = packed_args(c);
     uint8_t* ws = static_cast<uint8_t*>(c->workspace);
     a.ndelta = reinterpret_cast<float*>(ws);
     a.zs = reinterpret_cast<float*>(ws + packed_stats(c->n_q, c->H));
     double* part = reinterpret_cast<double*>(ws + 2 * packed_stats(c->n_q, c->H));
+    const qdl::PackedPlan plan = packed_plan(c);
+    a.head_splits = plan.head_splits;
+    if (plan.head_splits > 1) a.part = reinterpret_cast<float*>(part + c->H * qdl::kPackedParts);
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     hipError_t e;
     switch (c->dtype) {
-        case QDL_BORN_DTYPE_BF16: e = qdl::packed_bwd<qdl::BF16>(a, s); break;
-        case QDL_BORN_DTYPE_F16: e = qdl::packed_bwd<qdl::F16>(a, s); break;
-        default: e = qdl::packed_bwd<qdl::F32>(a, s); break;
+        case QDL_BORN_DTYPE_BF16: e = qdl::packed_bwd<qdl::BF16>(a, plan, s); break;
+        case QDL_BORN_DTYPE_F16: e = qdl::packed_bwd<qdl::F16>(a, plan, s); break;
+        default: e = qdl::packed_bwd<qdl::F32>(a, plan, s); break;
     }
     if (e != hipSuccess || !c->dscale) return hip_status(e);
     hipLaunchKernelGGL((qdl::born_packed_dscale_part_kernel<0>), dim3((unsigned)a.H, qdl::kPackedParts), dim3(256), 0, s, a, part);
@@ -433,8 +445,7 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call* c, qdl_stream_t s
     a.recent = (int)c->recent;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     const unsigned units = (unsigned)(c->B * c->h_kv);
-    if (c->pages * c->page_size <= 256 * qdl::kEvictPer) hipLaunchKernelGGL((qdl::born_evict_select_kernel<256>), dim3(units), dim3(256), 0, s, a);
-    else hipLaunchKernelGGL((qdl::born_evict_select_kernel<1024>), dim3(units), dim3(1024), 0, s, a);
+    qdl::launch_evict_select(a, units, c->pages * c->page_size, s);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || most == 0 || c->cache_pages == 0) return hip_status(e);
     if (c->out_table) hipLaunchKernelGGL((qdl::born_evict_move_kernel<0>), dim3((unsigned)tiles * units), dim3(256), 0, s, a);

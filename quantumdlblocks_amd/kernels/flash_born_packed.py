@@ -20,6 +20,8 @@ head dims the formulation in torch operations.
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from .. import _native
@@ -120,6 +122,15 @@ def _uncompiled(fn, *args):
     return _call_uncompiled(fn, args) if torch.compiler.is_compiling() else fn(*args)
 
 
+@functools.lru_cache(maxsize=256)
+def _workspace(dtype, sequences, N, M, H, Hkv, dp, window) -> int:
+    """Bytes of the backward's workspace, by sizes alone (the block's addresses and strides are not looked at)."""
+    piece = 16
+    block = _native.packed_call(dtype, sequences, N, M, H, Hkv, dp, piece, piece, piece, H * dp, dp, Hkv * dp, dp, Hkv * dp, dp, piece,
+                                piece, piece, piece, 0, 1, 1.0, 1, window, 0.0, 0, 0, 0, 0, 0, 0, 0, 0, 0)
+    return int(_native.load().qdl_flash_born_packed_workspace_size(block))
+
+
 class _FlashBornPackedFn(torch.autograd.Function):
     """forward: computes in the autocast dtype (CUDA autocast active) else
     ``v.dtype``; saves the rows, ``out``, Z (fp32) and the starts.  backward:
@@ -128,6 +139,7 @@ class _FlashBornPackedFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, cu_q, cu_k, is_causal, eps, window):
         out, ctx.head, saved = _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, True)
+        ctx.workspace = _workspace(*ctx.head[:7], window)
         ctx.save_for_backward(*saved)
         ctx.head_dim = q.shape[2]
         if isinstance(scale, torch.Tensor):
@@ -149,7 +161,7 @@ class _FlashBornPackedFn(torch.autograd.Function):
         n_scale = 1 if scale_flat is None else scale_flat.numel()
         # The scale's gradient costs launches of its own: only where wanted.
         dscale = torch.empty(n_scale, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
-        size = int(lib.qdl_flash_born_packed_workspace_size(N, H))
+        size = ctx.workspace
         ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
         _run_call(lib.qdl_flash_born_packed_backward_call, "qdl_flash_born_packed_backward_call", dev,
                   _native.packed_call(*ctx.head, do_c.data_ptr(), *ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),

@@ -69,6 +69,27 @@ def test_groups(cuda_device, dtype, H, Hkv):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 96, 128, 256])
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 60)])
+def test_heads_of_a_group_shared_out(cuda_device, dtype, D, causal, window):
+    # Few blocks, many heads on one key head: dK and dV are summed from parts.
+    q, k, v, do, cq, ck = _inputs([700, 1, 333], 0, 12, 1, D, DT[dtype], cuda_device, seed=16)
+    scale = torch.tensor([2.0, -1.0, 3.0] * 4, device=cuda_device)
+    _check(q, k, v, do, scale, cq, ck, causal, 1e-12, window)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+@pytest.mark.parametrize("D", [64, 96, 128])
+@pytest.mark.parametrize("causal,window", MASKS)
+def test_long_blocks(cuda_device, dtype, D, causal, window):
+    # Enough key blocks for the eight-wave dK/dV kernel.
+    lens = [300, 129, 1, 40] * 9
+    q, k, v, do, cq, ck = _inputs(lens, 3, 8, 4, D, DT[dtype], cuda_device, seed=17)
+    scale = torch.tensor([2.0, -1.0, 3.0, 1.0, -2.0, -3.0, 1.0, 1.0], device=cuda_device)
+    _check(q, k, v, do, scale, cq, ck, causal, 1e-12, window)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("past", [1, 63, 300])
 @pytest.mark.parametrize("causal,window", MASKS)
 def test_more_keys_than_queries(cuda_device, dtype, past, causal, window):

@@ -110,4 +110,5 @@ def test_backward_block_checks():
     assert lib.qdl_flash_born_packed_forward_call(_packed_block(n_q=0), None) == 0
     short = _packed_block()
     assert lib.qdl_flash_born_packed_forward_call(b"\x08" + short[1:], None) == -2
-    assert lib.qdl_flash_born_packed_workspace_size(5, 4) >= 2 * 5 * 4 * 4
+    assert lib.qdl_flash_born_packed_workspace_size(_packed_block()) >= 2 * 4 * 4 * 4
+    assert lib.qdl_flash_born_packed_workspace_size(_packed_block(D=12)) == 0
