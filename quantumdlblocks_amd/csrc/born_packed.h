@@ -715,18 +715,10 @@ __global__ __launch_bounds__(256) void born_packed_dkdv_join_kernel(PackedArgs p
 }
 
 // ---------------------------------------------------------------------------
-// dK / dV: 32 keys per wave, the queries of all heads of the group streamed.
-//
-// One wave per SIMD (the accumulators and the stationary rows of both take half
-// of its registers) leaves nothing to hide a wave's LDS latency behind but its
-// own work, so two 32-row parts of a tile run as four fenced phases, the
-// operands of each read one phase earlier:
-//   1: S, dP of part 0                        reads the rows of part 1
-//   2: S, dP of part 1 | elementwise(part 0)  reads the columns of part 0
-//   3: dV, dK += part 0 | elementwise(part 1) reads the columns of part 1
-//   4: dV, dK += part 1
-// fp32 above head dim 128 takes one launch for each (the registers hold the
-// operands of both or the accumulators of both).
+// dK / dV of fp32, and of 16 bits above head dim 128: 32 keys per wave, whose
+// rows stay in registers, one wave per SIMD; the queries of all heads of the
+// group streamed.  fp32 above head dim 128 takes one launch for each (the
+// registers hold the operands of both or the accumulators of both).
 // ---------------------------------------------------------------------------
 template <class E, int DP, int SPLIT, bool DK, bool DV>
 __global__ __launch_bounds__(64 * kPackedWaves) __attribute__((amdgpu_waves_per_eu(1, 1)))
@@ -734,7 +726,6 @@ void born_packed_dkdv_kernel(PackedArgs p) {
     using C = PackedCfg<E, DP, SPLIT>;
     using Tile = PackedTile<E, DP, C::BN>;
     constexpr int KS = Tile::KS, DB = Tile::DB, BN = C::BN, NST = C::NST, SUB = C::SUB;
-    constexpr bool kPhased = SUB == 2 && kItem<E> == 2 && DK && DV;
     __shared__ __attribute__((aligned(1024))) uint8_t ring[C::SMEM];
     __shared__ __attribute__((aligned(16))) float stats[NST][2][BN];  // -delta, zs
 
@@ -837,96 +828,19 @@ void born_packed_dkdv_kernel(PackedArgs p) {
     auto tile = [&](int t, int st, auto kind) __attribute__((always_inline)) {
         const int i0 = (t0 + t) * BN;
         const Tile q = qt(st), d = dt(st);
-        if constexpr (kPhased) {
-            auto rows = [&](const Tile& tile, int nb, u32x4 (&x)[KS]) __attribute__((always_inline)) {
 #pragma unroll
-                for (int ks = 0; ks < KS; ++ks) x[ks] = tile.row(r0 + 32 * nb + c, ks, g);
-            };
-            auto cols = [&](const Tile& tile, int nb, u32x4 (&x)[2][DB]) __attribute__((always_inline)) {
+        for (int nb = 0; nb < SUB; ++nb) {
+            const int rr = r0 + 32 * nb;
+            f32x16 s = zero16(), dp = values(stats[st][0], rr);
 #pragma unroll
-                for (int hh = 0; hh < 2; ++hh)
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) x[hh][db] = tile.transposed(r0 + 32 * nb + 16 * hh, db, lane);
-            };
-            auto overlaps = [&](const u32x4 (&a)[KS], const u32x4 (&b)[KS], f32x16& s, f32x16& dp) __attribute__((always_inline)) {
-                s = zero16();
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    s = E::mfma(a[ks], kr[ks], s);
-                    dp = E::mfma(b[ks], vr[ks], dp);
-                }
-            };
-            auto sums = [&](const u32x4 (&td)[2][DB], const u32x4 (&tq)[2][DB], const PackedWeights<E>& w,
-                            const PackedWeights<E>& x) __attribute__((always_inline)) {
-#pragma unroll
-                for (int hh = 0; hh < 2; ++hh) {
-                    const u32x4 bw = {w.w[4 * hh], w.w[4 * hh + 1], w.w[4 * hh + 2], w.w[4 * hh + 3]};
-                    const u32x4 bx = {x.w[4 * hh], x.w[4 * hh + 1], x.w[4 * hh + 2], x.w[4 * hh + 3]};
-#pragma unroll
-                    for (int db = 0; db < DB; ++db) {
-                        dv[db] = E::mfma(td[hh][db], bw, dv[db]);
-                        dk[db] = E::mfma(tq[hh][db], bx, dk[db]);
-                    }
-                }
-            };
-            u32x4 rq0[KS], rd0[KS], rq1[KS], rd1[KS], tq0[2][DB], td0[2][DB], tq1[2][DB], td1[2][DB];
-            f32x16 s0, s1, dp0, dp1;
-            PackedWeights<E> w0, w1, x0, x1;
-            rows(q, 0, rq0);
-            rows(d, 0, rd0);
-            dp0 = values(stats[st][0], r0);
-            dp1 = values(stats[st][0], r0 + 32);
-            // 1
-            __builtin_amdgcn_s_setprio(1);
-            rows(q, 1, rq1);
-            rows(d, 1, rd1);
-            overlaps(rq0, rd0, s0, dp0);
-            __builtin_amdgcn_sched_barrier(0);
-            // 2
-            __builtin_amdgcn_s_setprio(0);
-            cols(q, 0, tq0);
-            cols(d, 0, td0);
-            overlaps(rq1, rd1, s1, dp1);
-            elementwise(st, i0, r0, s0, dp0, w0, x0, kind);
-#pragma unroll
-            for (int i = 0; i < 2 * KS; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);  // MFMA
-                __builtin_amdgcn_sched_group_barrier(0x002, 6, 0);  // VALU
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 0);  // DS read
+            for (int ks = 0; ks < KS; ++ks) {
+                s = packed_step<E>(q.row(rr + c, ks, g), kr[ks], s);
+                if constexpr (DK) dp = packed_step<E>(d.row(rr + c, ks, g), vr[ks], dp);
             }
-            __builtin_amdgcn_sched_barrier(0);
-            // 3
-            cols(q, 1, tq1);
-            cols(d, 1, td1);
-            sums(td0, tq0, w0, x0);
-            elementwise(st, i0, r0 + 32, s1, dp1, w1, x1, kind);
-#pragma unroll
-            for (int i = 0; i < 4 * DB; ++i) {
-                __builtin_amdgcn_sched_group_barrier(0x008, 1, 1);
-                __builtin_amdgcn_sched_group_barrier(0x002, 6, 1);
-                __builtin_amdgcn_sched_group_barrier(0x100, 2, 1);
-            }
-            __builtin_amdgcn_sched_barrier(0);
-            // 4
-            __builtin_amdgcn_s_setprio(1);
-            sums(td1, tq1, w1, x1);
-            __builtin_amdgcn_sched_barrier(0);
-            __builtin_amdgcn_s_setprio(0);
-        } else {
-#pragma unroll
-            for (int nb = 0; nb < SUB; ++nb) {
-                const int rr = r0 + 32 * nb;
-                f32x16 s = zero16(), dp = values(stats[st][0], rr);
-#pragma unroll
-                for (int ks = 0; ks < KS; ++ks) {
-                    s = packed_step<E>(q.row(rr + c, ks, g), kr[ks], s);
-                    if constexpr (DK) dp = packed_step<E>(d.row(rr + c, ks, g), vr[ks], dp);
-                }
-                PackedWeights<E> w, x;
-                elementwise(st, i0, rr, s, dp, w, x, kind);
-                if constexpr (DV) packed_columns<E>(d, rr, w, dv, lane);
-                if constexpr (DK) packed_columns<E>(q, rr, x, dk, lane);
-            }
+            PackedWeights<E> w, x;
+            elementwise(st, i0, rr, s, dp, w, x, kind);
+            if constexpr (DV) packed_columns<E>(d, rr, w, dv, lane);
+            if constexpr (DK) packed_columns<E>(q, rr, x, dk, lane);
         }
     };
 
@@ -986,11 +900,13 @@ void born_packed_dkdv_kernel(PackedArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// dK / dV of long blocks (16-bit, up to head dim 128): eight waves, two on each
-// SIMD, over 128 keys.  The stationary rows stay in LDS beside the ring, which
-// leaves a wave the registers of its accumulators; four waves take 32 keys each
-// of a tile's first half, four of its second.  Every tile feeds 128 keys, so
-// the tiles' way from L2, which bounds 64-key blocks, is half as long.
+// dK / dV of 16 bits up to head dim 128: eight waves, two on each SIMD, over 128
+// keys.  The stationary rows stay in LDS beside the ring, which leaves a wave
+// the registers of its accumulators; four waves take 32 keys each of a tile's
+// first half, four of its second.  Every tile feeds 128 keys: with 64, the
+// tiles' way from L2 bounds the launch (one wave on a SIMD over 64 or 128 keys
+// in registers: 553 and 550 us where this takes 482, 16384 tokens in 8
+// sequences, 16 heads over 4, D128).
 // ---------------------------------------------------------------------------
 template <class E, int DP>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
@@ -1201,7 +1117,7 @@ constexpr int kPackedMaxSplit = kItem<E> * DP <= 256 ? 4 : kItem<E> * DP <= 512 
 // How a launch of few blocks is divided.  The lengths are on the device, so the
 // longest sequence is taken for half as long again as the mean.
 struct PackedPlan {
-    bool split_q, split_k;  // 32-row blocks of four waves: forward and dQ, dK/dV
+    bool split_q, split_k;  // 32-row blocks of four waves: forward and dQ, fp32's dK/dV
     int head_splits;
 };
 inline PackedPlan packed_plan(int item, int64_t Nq, int64_t Nk, int64_t S, int64_t H, int64_t Hkv, int64_t D, int64_t window) {
@@ -1224,17 +1140,22 @@ inline PackedPlan packed_plan(int item, int64_t Nq, int64_t Nk, int64_t S, int64
         const double parts = (double)packed_blocks((int)Nq, (int)S, (int)share) * H / (rb == 128 ? 512.0 : 256.0);
         r.split_q = (parts > 1.0 ? parts : 1.0) * (a + 1.33 * c / share) < (whole > 1.0 ? whole : 1.0) * (a + c);
     }
+    // fp32's dK/dV: 32-key blocks while 64-key ones would be under one a CU.
     const int64_t few = (int64_t)packed_blocks((int)Nk, (int)S, 4) * Hkv;
-    r.split_k = rb <= 256 && few <= 512;
-    // Heads of a group are shared out while the launch has too few blocks to
-    // even out their lengths and a block has tiles to share.  Each share costs
-    // its sums in fp32, written and read again.
-    const int64_t G = H / Hkv, blocks = r.split_k ? few : (int64_t)packed_blocks((int)Nk, (int)S, rb <= 256 && item == 2 ? 1 : 2) * Hkv;
+    r.split_k = item == 4 && rb <= 256 && few <= 512;
+    // Heads of a group are shared out while that leaves a launch under four
+    // blocks a CU, to even out their lengths, and a share some tiles.  Each
+    // share costs its sums in fp32, written and read again.  Measured, us of
+    // dK/dV and join by shares 1, 2, 4, 8: 2 sequences of 4096, 8 heads over 1,
+    // D128, 776, 416, 241, 182; 4 of up to 3000, 32 heads over 8, D64, 253, 237,
+    // 275; 8 of 2048, 16 heads over 4, D64 (548 blocks), 176, 202.
+    const int split = rb > 512 || (rb <= 256 && item == 2) ? 1 : r.split_k ? 4 : 2;
+    const int64_t G = H / Hkv, blocks = (int64_t)packed_blocks((int)Nk, (int)S, split) * Hkv;
     double rows = 1.5 * (double)Nq / seqs;
     if (rows > (double)Nq) rows = (double)Nq;
     if (window > 0 && rows > window + 128.0) rows = window + 128.0;
     int64_t hs = 1;
-    while (2 * hs <= G && blocks * hs < (r.split_k ? 192 : 1024) && (double)(G / hs) * rows / 64.0 >= 32.0) hs *= 2;
+    while (2 * hs <= G && 2 * hs * blocks <= 1024 && (double)(G / (2 * hs)) * rows / 64.0 >= 5.0) hs *= 2;
     r.head_splits = (int)hs;
     return r;
 }
@@ -1293,16 +1214,16 @@ hipError_t launch_packed_bwd(const PackedArgs& a, const PackedPlan& plan, hipStr
             if (e != hipSuccess) return e;
         }
         if (a.Nk > 0) {
-            if constexpr (kPackedMaxSplit<E, DPV> == 1) {
+            if constexpr (kItem<E> == 2 && DPV <= 128) {
+                const dim3 grid(packed_blocks(a.Nk, a.S, 1) * (unsigned)(a.Hkv * a.head_splits));
+                hipLaunchKernelGGL((born_packed_dkdv8_kernel<E, DPV>), grid, dim3(512), 0, st, a);
+            } else if constexpr (kPackedMaxSplit<E, DPV> == 1) {
                 launch_packed_dkdv_as<E, DPV, 1, true, false>(a, st);
                 launch_packed_dkdv_as<E, DPV, 1, false, true>(a, st);
             } else if constexpr (kPackedMaxSplit<E, DPV> == 2) {
                 launch_packed_dkdv_as<E, DPV, 2, true, true>(a, st);
             } else if (plan.split_k) {
                 launch_packed_dkdv_as<E, DPV, 4, true, true>(a, st);
-            } else if constexpr (kItem<E> == 2) {
-                const dim3 grid(packed_blocks(a.Nk, a.S, 1) * (unsigned)(a.Hkv * a.head_splits));
-                hipLaunchKernelGGL((born_packed_dkdv8_kernel<E, DPV>), grid, dim3(512), 0, st, a);
             } else {
                 launch_packed_dkdv_as<E, DPV, 2, true, true>(a, st);
             }
