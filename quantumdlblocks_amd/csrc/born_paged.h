@@ -53,7 +53,6 @@ struct PagedArgs {
     int64_t w_sb, w_sh;    // elements
     int w_len;             // columns of weights
     float* raw;            // (B, H, raw_ld) workspace: p without s^2, where weights are kept
-    float* inv;            // (B, H) workspace: 1 / (Z without s^2), likewise
     int64_t raw_ld;
 };
 
@@ -92,6 +91,12 @@ __device__ __forceinline__ bool paged_row(const PagedArgs& p, ConstIntPtr table,
     const int32_t t = in ? table[i] : -1;
     page = t;
     return t >= 0 && t < p.cache_pages;
+}
+
+// 1 / Z, without the s^2 of both; 0 for rows without weight.
+__device__ __forceinline__ float paged_inverse(const PagedArgs& p, int h, float z) {
+    const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
+    return den > 0.f && s != 0.f ? 1.0f / den : 0.f;
 }
 
 // A operands of V^T: 16-bit, lane's 8 keys x 8 columns (x[k][...]) -> the keys
@@ -391,8 +396,7 @@ void born_paged_kernel(PagedArgs p) {
             *reinterpret_cast<f32x4v*>(to + 4 + col) = x;
             if (col == 0) to[0] = zz;
         } else {
-            const float s = arg_scale(p, h), den = zz + (p.eps == 0.f ? 0.f : p.eps / (s * s));
-            x *= den > 0.f && s != 0.f ? 1.0f / den : 0.f;
+            x *= paged_inverse(p, h, zz);
             uint8_t* to = (uint8_t*)p.out + (((int64_t)b * p.H + h) * p.D + col) * IT;
             if constexpr (k32) {
                 *reinterpret_cast<f32x4v*>(to) = x;
@@ -404,39 +408,71 @@ void born_paged_kernel(PagedArgs p) {
     }
 }
 
+// Numerators and denominators of a (sequence, head)'s splits.
+struct PagedParts {
+    const float* at;
+    int n;
+    __device__ __forceinline__ PagedParts(const PagedArgs& p, const PagedSpan& sp, int64_t bh)
+        : at(p.part + bh * p.nsplit * (p.D + 4)), n(max(1, (sp.n - (sp.first & ~31) + p.chunk - 1) / p.chunk)) {}
+};
 // Splits joined in a fixed order: one workgroup per (sequence, head), `ncol`
 // threads over the columns, 256 / ncol groups of them over the splits.
-template <class E>
+// WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the
+// sum over the group of p_j / Z, the heads in order, is added to its weights
+// (a launch of their own behind the join took 4 us of 28, 16 sequences of up
+// to 8192 keys).
+template <class E, bool WEIGH>
 __global__ __launch_bounds__(256) void born_paged_join_kernel(PagedArgs p, int ncol) {
     __shared__ f32x4v red[256];
     __shared__ float zred[256];
+    if (WEIGH && (int)blockIdx.x >= p.B * p.H) {
+        const int x = blockIdx.x - p.B * p.H, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
+        const PagedSpan sp = paged_span(p, b);
+        const int j0 = (sp.first & ~31) + block * 256, j = j0 + threadIdx.x;
+        if (j0 >= sp.n) return;
+        const bool seen = j >= sp.first && j < sp.n && j < p.w_len;
+        float sum = 0.f;
+        for (int g0 = 0; g0 < p.G; g0 += 256) {
+            const int h0 = hk * p.G + g0, gn = min(256, p.G - g0);
+            if ((int)threadIdx.x < gn) {
+                const PagedParts part(p, sp, (int64_t)b * p.H + h0 + threadIdx.x);
+                float z = 0.f;
+#pragma unroll 8
+                for (int i = 0; i < part.n; ++i) z += part.at[(int64_t)i * (p.D + 4)];
+                zred[threadIdx.x] = paged_inverse(p, h0 + threadIdx.x, z);
+            }
+            __syncthreads();
+            if (seen) {
+                const float* raw = p.raw + ((int64_t)b * p.H + h0) * p.raw_ld + j;
+#pragma unroll 4
+                for (int i = 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
+            }
+            __syncthreads();
+        }
+        if (seen) p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
+        return;
+    }
     const int h = blockIdx.x % p.H, b = blockIdx.x / p.H;
     const int col = threadIdx.x % ncol, group = threadIdx.x / ncol, groups = 256 / ncol;
-    const PagedSpan sp = paged_span(p, b);
-    const int n = max(1, (sp.n - (sp.first & ~31) + p.chunk - 1) / p.chunk);
-    const float* part = p.part + ((int64_t)b * p.H + h) * p.nsplit * (p.D + 4);
+    const PagedParts part(p, paged_span(p, b), (int64_t)b * p.H + h);
     const bool ok = 4 * col < p.D;
     f32x4v x = {0.f, 0.f, 0.f, 0.f};
     float z = 0.f;
 #pragma unroll 4
-    for (int i = group; i < n; i += groups) {
-        const float* at = part + (int64_t)i * (p.D + 4);
+    for (int i = group; i < part.n; i += groups) {
+        const float* at = part.at + (int64_t)i * (p.D + 4);
         z += at[0];
         if (ok) x += *reinterpret_cast<const f32x4v*>(at + 4 + 4 * col);
     }
     red[threadIdx.x] = x;
     zred[threadIdx.x] = z;
     __syncthreads();
-    if (group != 0) return;
+    if (group != 0 || !ok) return;
     for (int i = 1; i < groups; ++i) {
         x += red[i * ncol + col];
         z += zred[i * ncol + col];
     }
-    const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
-    const float inv = den > 0.f && s != 0.f ? 1.0f / den : 0.f;
-    if (p.raw != nullptr && col == 0) p.inv[(int64_t)b * p.H + h] = inv;
-    if (!ok) return;
-    x *= inv;
+    x *= paged_inverse(p, h, z);
     uint8_t* to = (uint8_t*)p.out + (((int64_t)b * p.H + h) * p.D + 4 * col) * kItem<E>;
     if constexpr (std::is_same<E, F32>::value) {
         *reinterpret_cast<f32x4v*>(to) = x;
@@ -444,23 +480,6 @@ __global__ __launch_bounds__(256) void born_paged_join_kernel(PagedArgs p, int n
         const u32x2 y = {E::pack(x[0], x[1]), E::pack(x[2], x[3])};
         *reinterpret_cast<u32x2*>(to) = y;
     }
-}
-
-// weights[b][hk][j] += sum over the group of p_j / Z, the heads in order, 256
-// keys per workgroup.
-template <int>
-__global__ __launch_bounds__(256) void born_paged_weigh_kernel(PagedArgs p) {
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
-    const int b = rest % p.B, block = rest / p.B;
-    const PagedSpan sp = paged_span(p, b);
-    const int j = (sp.first & ~31) + block * 256 + threadIdx.x;
-    if (j < sp.first || j >= sp.n || j >= p.w_len) return;
-    const int64_t h0 = (int64_t)b * p.H + hk * p.G;
-    const float* raw = p.raw + h0 * p.raw_ld + j;
-    float sum = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < p.G; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], p.inv[h0 + i], sum);
-    p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
 }
 
 template <class E>
@@ -490,11 +509,14 @@ hipError_t launch_paged(const PagedArgs& a, hipStream_t st) {
     if (e != hipSuccess || a.part == nullptr) return e;
     int ncol = 2;
     while (4 * ncol < a.D) ncol *= 2;
-    hipLaunchKernelGGL((born_paged_join_kernel<E>), dim3((unsigned)(a.B * a.H)), dim3(256), 0, st, a, ncol);
-    e = hipGetLastError();
-    if (e != hipSuccess || a.raw == nullptr) return e;
-    const int64_t span = a.window > 0 && a.window + 32 < a.raw_ld ? a.window + 32 : a.raw_ld;
-    hipLaunchKernelGGL((born_paged_weigh_kernel<0>), dim3((unsigned)((span + 255) / 256 * a.B * a.Hkv)), dim3(256), 0, st, a);
+    const unsigned join = (unsigned)(a.B * a.H);
+    if (a.raw != nullptr) {
+        const int64_t span = a.window > 0 && a.window + 32 < a.raw_ld ? a.window + 32 : a.raw_ld;
+        const unsigned weigh = (unsigned)((span + 255) / 256 * a.B * a.Hkv);
+        hipLaunchKernelGGL((born_paged_join_kernel<E, true>), dim3(join + weigh), dim3(256), 0, st, a, ncol);
+    } else {
+        hipLaunchKernelGGL((born_paged_join_kernel<E, false>), dim3(join), dim3(256), 0, st, a, ncol);
+    }
     return hipGetLastError();
 }
 

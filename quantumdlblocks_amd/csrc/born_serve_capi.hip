@@ -129,8 +129,8 @@ int64_t packed_workspace(const qdl_born_packed_call* c) {
 // Splits of a paged launch: enough workgroups for four a compute unit, none
 // under 128 keys (a wave's 32) or over 1024.
 struct PagedPlan {
-    int64_t chunk, nsplit, gblocks, raw_ld, part_bytes, raw_bytes, inv_bytes;
-    int64_t bytes() const { return part_bytes + raw_bytes + inv_bytes; }
+    int64_t chunk, nsplit, gblocks, raw_ld, part_bytes, raw_bytes;
+    int64_t bytes() const { return part_bytes + raw_bytes; }
 };
 PagedPlan paged_plan(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window, bool weigh) {
     PagedPlan r = {};
@@ -147,10 +147,7 @@ PagedPlan paged_plan(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t page
     r.nsplit = (span + chunk - 1) / chunk;
     r.raw_ld = (room + 31) / 32 * 32;
     if (r.nsplit > 1 || weigh) r.part_bytes = B * H * r.nsplit * (D + 4) * 4;
-    if (weigh) {
-        r.raw_bytes = B * H * r.raw_ld * 4;
-        r.inv_bytes = (B * H * 4 + 15) / 16 * 16;
-    }
+    if (weigh) r.raw_bytes = B * H * r.raw_ld * 4;
     return r;
 }
 PagedPlan paged_plan(const qdl_born_paged_call* c) {
@@ -170,7 +167,8 @@ int check_paged(const qdl_born_paged_call* c) {
                      c->block_table, c->pages, c->table_ld);
     if (rc != QDL_BORN_OK) return rc;
     const PagedPlan r = paged_plan(c);
-    if (c->B * c->h_kv * r.gblocks * r.nsplit > kMostBlocks || (c->key_weight && c->B * c->h_kv * (r.raw_ld / 256 + 1) > kMostBlocks))
+    if (c->B * c->h_kv * r.gblocks * r.nsplit > kMostBlocks ||
+        (c->key_weight && c->B * (c->H + c->h_kv * (r.raw_ld / 256 + 1)) > kMostBlocks))
         return QDL_BORN_E_SHAPE;
     if (c->key_weight && (c->weight_len < 0 || c->weight_len > INT32_MAX)) return QDL_BORN_E_SHAPE;
     return QDL_BORN_OK;
@@ -294,7 +292,6 @@ int qdl_flash_born_paged_forward_call(const qdl_born_paged_call* c, qdl_stream_t
     if (r.raw_bytes > 0) {
         a.raw = reinterpret_cast<float*>(ws + r.part_bytes);
         a.raw_ld = r.raw_ld;
-        a.inv = reinterpret_cast<float*>(ws + r.part_bytes + r.raw_bytes);
         a.weights = c->key_weight;
         a.w_sb = c->weight_strides[0];
         a.w_sh = c->weight_strides[1];
