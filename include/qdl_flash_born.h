@@ -354,7 +354,8 @@ int qdl_flash_born_fwd_qk_prologue(int dtype, int64_t B, int64_t H, int64_t T,
  * backward follows.  scale == NULL takes scale_value.  The weights of fp16 rows are scaled by a power of two of the
  * row's own, so overlaps of any size keep their weight.
  * The backward's dk and dv are summed over the heads of a group in a fixed
- * order; dscale == NULL: not wanted.  struct_bytes: sizeof the block.
+ * order; dk == dv == NULL, dscale == NULL: not wanted.  struct_bytes: sizeof
+ * the block.
  */
 typedef struct qdl_born_packed_call {
     int64_t struct_bytes;

@@ -80,7 +80,7 @@ __device__ __forceinline__ int packed_start(const int32_t* cu, int s, int N) {
 // causality, with few enough sequences for a lane each, the blocks go in the
 // order of their work instead, over all sequences (a block's tiles are those
 // before its queries or behind its keys): a launch ends with short blocks
-// (packed training step of 8 sequences, 16384 tokens: dK/dV 600 -> 505 us).
+// (packed training step of 8 sequences, 16384 tokens: dK/dV 600 -> 560 us).
 template <bool KEYS, int BM>
 __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
     const int32_t* cu = KEYS ? p.cu_k : p.cu_q;
@@ -1213,7 +1213,7 @@ hipError_t launch_packed_bwd(const PackedArgs& a, const PackedPlan& plan, hipStr
             const hipError_t e = hipGetLastError();
             if (e != hipSuccess) return e;
         }
-        if (a.Nk > 0) {
+        if (a.Nk > 0 && a.dk != nullptr) {
             if constexpr (kItem<E> == 2 && DPV <= 128) {
                 const dim3 grid(packed_blocks(a.Nk, a.S, 1) * (unsigned)(a.Hkv * a.head_splits));
                 hipLaunchKernelGGL((born_packed_dkdv8_kernel<E, DPV>), grid, dim3(512), 0, st, a);
@@ -1230,7 +1230,7 @@ hipError_t launch_packed_bwd(const PackedArgs& a, const PackedPlan& plan, hipStr
         }
     })
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.Nk == 0 || a.head_splits == 1) return e;
+    if (e != hipSuccess || a.Nk == 0 || a.dk == nullptr || a.head_splits == 1) return e;
     const int64_t pieces = (int64_t)a.Nk * a.Hkv * a.D / 4;  // of 8 values, dK and dV
     hipLaunchKernelGGL((born_packed_dkdv_join_kernel<E>), dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st, a);
     return hipGetLastError();

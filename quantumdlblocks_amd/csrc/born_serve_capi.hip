@@ -127,7 +127,12 @@ int64_t packed_workspace(const qdl_born_packed_call* c) {
 }
 
 // Splits of a paged launch: enough workgroups for four a compute unit, none
-// under 128 keys (a wave's 32) or over 1024.
+// under 128 keys (a wave's 32) or over 1024.  Eight a unit cut the chunks finer
+// and mostly pay more in partial sums than they level: us at four and at eight,
+// bf16, 64 sequences of 1024 keys, 8 key heads, D64 42.2 and 44.8, D128 66.4 and
+// 70.8; 16 of 512..8192, 4 key heads, D64 23.7 and 23.9, D128 36.5 and 39.5.
+// One ragged batch with the keys' weights gained (fp16 D64: 35.1 and 31.8),
+// another of its shape did not (bf16: 32.0 and 32.2).
 struct PagedPlan {
     int64_t chunk, nsplit, gblocks, raw_ld, part_bytes, raw_bytes;
     int64_t bytes() const { return part_bytes + raw_bytes; }
@@ -206,7 +211,7 @@ int64_t qdl_flash_born_packed_workspace_size(const qdl_born_packed_call* c) {
 int qdl_flash_born_packed_backward_call(const qdl_born_packed_call* c, qdl_stream_t stream) {
     const int rc = check_packed(c);
     if (rc != QDL_BORN_OK) return rc;
-    if ((c->n_q > 0 && (!c->dout || !c->dq || !c->z)) || (c->n_k > 0 && (!c->dk || !c->dv))) return QDL_BORN_E_NULL;
+    if ((c->n_q > 0 && (!c->dout || !c->dq || !c->z)) || (c->n_k > 0 && !c->dk != !c->dv)) return QDL_BORN_E_NULL;
     if (!aligned16(c->dout) || !aligned16(c->dq) || !aligned16(c->dk) || !aligned16(c->dv)) return QDL_BORN_E_ALIGN;
     if (c->n_q > 0 && !rows_ok(c->dout_strides, item(c->dtype), c->D)) return QDL_BORN_E_STRIDE;
     if (c->workspace_bytes < packed_workspace(c) || !c->workspace || !aligned16(c->workspace))

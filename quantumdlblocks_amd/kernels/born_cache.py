@@ -231,10 +231,12 @@ def flash_born_attention_paged(
         return _eager_paged(q.detach(), k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight)
     lib = _native.load()
     dt = k_cache.dtype
+    out = torch.empty((B, H, D), dtype=dt, device=dev)
+    if B == 0:
+        return out
     q_c, sb, sh = _heads(q, dt)
     (table, ld), lens = _table(block_table), _index(cache_lens)
     pages = table.shape[1]
-    out = torch.empty((B, H, D), dtype=dt, device=dev)
     size = _paged_workspace(B, H, Hkv, D, pages, page, window, w_ptr != 0)
     ws = torch.empty(size, dtype=torch.uint8, device=dev) if size else None
     _run_call(lib.qdl_flash_born_paged_forward_call, "qdl_flash_born_paged_forward_call", dev, _native.paged_call(
@@ -382,13 +384,17 @@ def fused_qk_rope_l2_normalize_append(
                              positions, eps)
     lib = _native.load()
     dt = k_cache.dtype
+    out = torch.empty((N, H, D), dtype=dt, device=dev)
+    if N == 0:
+        return out
+    if B == 0:
+        return out.zero_()  # tokens of no sequence
     q_c, q0, q1 = _heads(q, dt)
     k_c, k0, k1 = _heads(k, dt)
     v_c, v0, v1 = _heads(v, dt)
     (table, ld), lens = _table(block_table), _index(cache_lens)
     cu = None if cu_seqlens is None else _index(cu_seqlens)
     pos = None if positions is None else _index(positions)
-    out = torch.empty((N, H, D), dtype=dt, device=dev)
     if tables is None:
         rot = (0, 0, 0, 0, 0)
     else:
@@ -501,6 +507,8 @@ def born_cache_evict(
     weight = torch.empty(wshape, dtype=torch.float32, device=dev)
     new_lens = torch.empty(B, dtype=torch.int32, device=dev)
     kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    if B == 0:
+        return new_lens, weight, kept
     _run_call(lib.qdl_flash_born_cache_evict_call, "qdl_flash_born_cache_evict_call", dev, _native.evict_call(
         _DTYPE_CODE[k_cache.dtype], B, Hkv, D, k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(),
         table.shape[1], ld, lens.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1), wshape[2], budget, recent,

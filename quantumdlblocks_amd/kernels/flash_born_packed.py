@@ -155,23 +155,31 @@ class _FlashBornPackedFn(torch.autograd.Function):
         M, Hkv = k_c.shape[:2]
         D, dev = ctx.head_dim, q_c.device
         do_c, *ds = _token_rows(do, out.dtype, dp)
-        dq = torch.empty((N, H, dp), dtype=out.dtype, device=dev)
-        dk = torch.empty((M, Hkv, dp), dtype=out.dtype, device=dev)
-        dv = torch.empty_like(dk)
+        _, want_k, want_v, want_scale = ctx.needs_input_grad[:4]
+        dq = torch.empty_like(out)
+        # dK and dV come together, and not at all where neither is wanted.
+        dk = dv = None
+        if want_k or want_v:
+            dk = torch.empty((M, Hkv, dp), dtype=out.dtype, device=dev)
+            dv = torch.empty_like(dk)
         n_scale = 1 if scale_flat is None else scale_flat.numel()
         # The scale's gradient costs launches of its own: only where wanted.
-        dscale = torch.empty(n_scale, dtype=torch.float32, device=dev) if ctx.needs_input_grad[3] else None
+        dscale = torch.empty(n_scale, dtype=torch.float32, device=dev) if want_scale else None
         size = ctx.workspace
         ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
         _run_call(lib.qdl_flash_born_packed_backward_call, "qdl_flash_born_packed_backward_call", dev,
-                  _native.packed_call(*ctx.head, do_c.data_ptr(), *ds, dq.data_ptr(), dk.data_ptr(), dv.data_ptr(),
-                                      0 if dscale is None else dscale.data_ptr(), ws.data_ptr(), size))
-        if dp != D:
-            dq, dk, dv = dq[..., :D], dk[..., :D], dv[..., :D]
-        qd, kd, vd = ctx.dtypes
-        return (dq.to(qd), dk.to(kd), dv.to(vd),
-                None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype),
-                None, None, None, None, None)
+                  _native.packed_call(*ctx.head, do_c.data_ptr(), *ds, dq.data_ptr(), 0 if dk is None else dk.data_ptr(),
+                                      0 if dv is None else dv.data_ptr(), 0 if dscale is None else dscale.data_ptr(),
+                                      ws.data_ptr(), size))
+        grads = []
+        for g, dt in zip((dq, dk, dv), ctx.dtypes):
+            if g is not None:
+                if dp != D:
+                    g = g[..., :D]
+                if g.dtype is not dt:
+                    g = g.to(dt)
+            grads.append(g)
+        return (*grads, None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype), None, None, None, None, None)
 
 
 def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):

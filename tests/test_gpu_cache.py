@@ -278,3 +278,23 @@ def test_streams_and_two_graphs(cuda_device):
             other = flash_born_attention_paged(q1, kc, vc, table, n, 2.0)
         torch.cuda.synchronize()
         assert torch.equal(held[0], want[0]) and torch.equal(held[1], want[1]) and torch.equal(other, want[0])
+
+
+def test_batches_without_sequences_or_tokens(cuda_device):
+    for dev in ("cpu", cuda_device):
+        kc, vc = (torch.randn(3, 16, 2, 64, device=dev) for _ in range(2))
+        before = kc.clone(), vc.clone()
+        table, lens = torch.zeros(0, 2, dtype=torch.int32, device=dev), torch.zeros(0, dtype=torch.int32, device=dev)
+        weight = torch.zeros(0, 2, 32, device=dev)
+        x = torch.randn(5, 4, 64, device=dev)
+        assert flash_born_attention_paged(x[:0], kc, vc, table, lens, 1.0, key_weight=weight).shape == (0, 4, 64)
+        cu = torch.zeros(1, dtype=torch.int32, device=dev)
+        q = fused_qk_rope_l2_normalize_append(x, x[:, :2], x[:, :2], None, None, kc, vc, table, lens, cu)
+        assert q.shape == x.shape and not q.any()
+        one, n = torch.ones(1, 2, dtype=torch.int32, device=dev), torch.full((1,), 3, dtype=torch.int32, device=dev)
+        cu = torch.zeros(2, dtype=torch.int32, device=dev)
+        q = fused_qk_rope_l2_normalize_append(x[:0], x[:0, :2], x[:0, :2], None, None, kc, vc, one, n, cu)
+        assert q.shape == (0, 4, 64)
+        lens_out, w, kept = born_cache_evict(kc, vc, table, lens, weight, 8)
+        assert lens_out.shape == (0,) and w.shape == weight.shape and kept.shape == (0, 2, 8)
+        assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])

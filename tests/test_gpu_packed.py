@@ -284,3 +284,18 @@ def test_training_step_in_a_graph(cuda_device):
         torch.cuda.synchronize()
         eager = step([x.detach().clone().requires_grad_() for x in static])
         assert all(torch.equal(a, b) for a, b in zip(held, eager))
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 96, 256])
+def test_gradients_of_some_inputs_only(cuda_device, dtype, D):
+    # Whichever are asked for, each is the one of the whole backward; heads are shared out here too.
+    q, k, v, do, cq, _ = _inputs([200, 1, 65], 0, 8, 1, D, DT[dtype], cuda_device, seed=18)
+    cu, scale = _cu(cq, cuda_device), torch.tensor([2.0], device=cuda_device)
+    leaves = [x.requires_grad_() for x in (q, k, v, scale)]
+    every = torch.autograd.grad(flash_born_attention_packed(*leaves, cu, eps=0.5), leaves, do)
+    for pick in ((0,), (1,), (2,), (3,), (0, 3), (0, 1), (1, 2), (2, 3)):
+        some = [x if i in pick else x.detach() for i, x in enumerate(leaves)]
+        out = flash_born_attention_packed(*some, cu, eps=0.5)
+        for i, g in zip(pick, torch.autograd.grad(out, [leaves[i] for i in pick], do)):
+            assert torch.equal(g, every[i]), (pick, i)
