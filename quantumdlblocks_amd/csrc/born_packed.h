@@ -13,6 +13,19 @@
 //   dK_j = 2 sign(s) sum_i u_ij q_i,  dV_j = sum_i relu(r_ij)^2 zs_i dO_i,
 // the last two over the queries of all G heads of the group, in a fixed order.
 //
+// Roundings.  Scores, sums, statistics and accumulators are fp32.  The 16-bit
+// matrix instructions take 16-bit operands, so the factor that a kernel forms
+// itself is rounded once before each second product: p (forward), p / Z (dV)
+// and u (dQ, dK), half a step each.  bf16's Z adds the rounded p, so numerator
+// and denominator carry the same error; fp16's adds them in fp32.  delta comes
+// from the output as it was rounded: O in fp32 would cost 2 N H D bytes more to
+// write and to read.  Against 64 bits the 16-bit dQ and dK are about twice as
+// far off as gradients whose only rounding is the output's (bf16 3.1e-3 and
+// 1.7e-3, fp16 4.0e-4 and 2.1e-4 in norm).  A simulation in 64 bits of bf16 dQ
+// gives 2.6e-3 from u's and dQ's rounding alone and 2.8e-3 with delta from an
+// unrounded O: only a second product for u's remainder would bring it down.
+// fp32 rounds nothing on the way (3.3e-7, plain fp32 4.8e-7).
+//
 // What bounds them: the matrix pipe.  A workgroup's four waves share the tiles
 // of the streamed operands, which LDS-DMA loads bring into a ring of two stages,
 // one barrier per tile.  Each wave owns 32 stationary rows (queries in the
@@ -80,7 +93,8 @@ __device__ __forceinline__ int packed_start(const int32_t* cu, int s, int N) {
 // causality, with few enough sequences for a lane each, the blocks go in the
 // order of their work instead, over all sequences (a block's tiles are those
 // before its queries or behind its keys): a launch ends with short blocks
-// (packed training step of 8 sequences, 16384 tokens: dK/dV 600 -> 560 us).
+// (8 ragged sequences, 16384 tokens, D128: dK/dV 541 us, in the slots' order
+// 554 to 571).
 template <bool KEYS, int BM>
 __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
     const int32_t* cu = KEYS ? p.cu_k : p.cu_q;
@@ -385,7 +399,7 @@ struct PackedCfg {
     // Forward and dQ: two workgroups per CU where the ring and the registers
     // let them; above, one.  The 16-bit forward up to head dim 64, whose
     // products are short beside its weights, has room for four (8 prompts of
-    // 2048 tokens, 16 heads: 97 us with two, 91 with three, 87 with four).
+    // 2048 tokens, 16 heads: 95 us with two, 88 with three, 86 with four).
     static constexpr int WPE = RB <= 256 && SMEM <= 78 * 1024 ? 2 : 1;
     static constexpr int FWD_WPE = RB == 128 && SPLIT == 1 ? 4 : WPE;
 };
@@ -474,6 +488,9 @@ struct PackedQueries {
 
 // ---------------------------------------------------------------------------
 // Forward: S^T = K Q^T per 32 keys, the weights in place, O^T += V^T P^T.
+// Bound by the matrix pipe at D128, by the weights' elementwise work beside it
+// at D64.  Ragged bf16, 16 heads over 4: 16384 tokens D128 211 us (879 TFLOP/s),
+// 8896 tokens D64 40 us (670); fp32, 1000 tokens, 8 heads D64: 18 us.
 // ---------------------------------------------------------------------------
 template <class E, int DP, int SPLIT>
 __global__ __launch_bounds__(64 * kPackedWaves)
@@ -574,7 +591,9 @@ void born_packed_fwd_kernel(PackedArgs p) {
 }
 
 // ---------------------------------------------------------------------------
-// dQ; also -delta and sign(s) s^2 / Z per row for the dK/dV kernel.
+// dQ; also -delta and sign(s) s^2 / Z per row for the dK/dV kernel.  Three
+// products a tile; bound by the matrix pipe: 300 us (928 TFLOP/s) for the 16384
+// tokens of the forward's D128 figure.
 // ---------------------------------------------------------------------------
 template <class E, int DP, int SPLIT>
 __global__ __launch_bounds__(64 * kPackedWaves)
@@ -904,9 +923,10 @@ void born_packed_dkdv_kernel(PackedArgs p) {
 // keys.  The stationary rows stay in LDS beside the ring, which leaves a wave
 // the registers of its accumulators; four waves take 32 keys each of a tile's
 // first half, four of its second.  Every tile feeds 128 keys: with 64, the
-// tiles' way from L2 bounds the launch (one wave on a SIMD over 64 or 128 keys
-// in registers: 553 and 550 us where this takes 482, 16384 tokens in 8
-// sequences, 16 heads over 4, D128).
+// tiles' way from L2 bounds the launch.  8 ragged sequences, 16384 tokens, 16
+// heads over 4, D128, on one machine: 541 us, one wave on a SIMD over 64 or 128
+// keys in registers 613 and 620.  Machines differ: 486 us (763 TFLOP/s) on
+// another.  Four products a tile and the longest sequence's blocks bound it.
 // ---------------------------------------------------------------------------
 template <class E, int DP>
 __global__ __launch_bounds__(512) __attribute__((amdgpu_waves_per_eu(2)))
@@ -1128,8 +1148,8 @@ inline PackedPlan packed_plan(int item, int64_t Nq, int64_t Nk, int64_t S, int64
     // in 64-row tiles (fp32's are four times as long).  Split blocks walk a
     // quarter of the tiles, a third slower each, and above 128-byte rows have a
     // CU to themselves.  Measured, us unsplit and split: fp32 3 sequences of
-    // 1000 tokens, 8 heads D64, forward 42 and 18, dQ 57 and 24; fp16 5
-    // sequences of 3125 tokens, 6 heads D96, a window of 384: 17 and 26, 19 and 30.
+    // 1000 tokens, 8 heads D64, forward 43 and 18, dQ 58 and 24; fp16 5
+    // sequences of 3125 tokens, 6 heads D96, a window of 384: 17 and 26, 21 and 33.
     if (rb <= 512) {
         const double a = item == 2 ? 6.0 : 1.5, share = rb <= 256 ? 4.0 : 2.0;
         double longest = 1.5 * (double)Nk / seqs;
@@ -1148,7 +1168,10 @@ inline PackedPlan packed_plan(int item, int64_t Nq, int64_t Nk, int64_t S, int64
     // share costs its sums in fp32, written and read again.  Measured, us of
     // dK/dV and join by shares 1, 2, 4, 8: 2 sequences of 4096, 8 heads over 1,
     // D128, 776, 416, 241, 182; 4 of up to 3000, 32 heads over 8, D64, 253, 237,
-    // 275; 8 of 2048, 16 heads over 4, D64 (548 blocks), 176, 202.
+    // 275.  At 548 blocks (16384 tokens, 16 heads over 4) ragged lengths would
+    // still gain (D128, 541 and 509), equal ones lose (8 of 2048: D128 358 and
+    // 407, D64 224 and 257; 32 of 512: 117 and 177): the lengths are not known
+    // here, so the limit lies below.
     const int split = rb > 512 || (rb <= 256 && item == 2) ? 1 : r.split_k ? 4 : 2;
     const int64_t G = H / Hkv, blocks = (int64_t)packed_blocks((int)Nk, (int)S, split) * Hkv;
     double rows = 1.5 * (double)Nq / seqs;

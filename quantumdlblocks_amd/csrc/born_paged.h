@@ -19,6 +19,13 @@
 // free: the m-th row of accumulator e is column 8 m + e.  The weights never
 // leave the registers: the two 16-key products' C layout is the B operand of
 // the 32-key one in the key order that the V loads use.
+//
+// The weights are rounded once to 16 bits, as that product's operand; the
+// denominator and the raw weights for key_weight take them in fp32.  Splits are
+// written and joined in fp32.
+//
+// bf16, 32 sequences of 2048 to 14622 keys, 8 key heads D128: 808 MB in 163 us
+// (5.0 TB/s) and a join of 5; one sequence of 1531 keys: 5.4 us and 3.5.
 #pragma once
 
 #include <type_traits>
