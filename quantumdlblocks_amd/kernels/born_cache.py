@@ -27,6 +27,7 @@ import torch
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
+from .flash_born_packed import _int32
 
 __all__ = ["born_cache_evict", "flash_born_attention_paged", "fused_qk_rope_l2_normalize_append"]
 
@@ -88,15 +89,13 @@ def _check_cache(k_cache, v_cache, block_table, cache_lens, B, written: bool):
 
 def _index(t: torch.Tensor) -> torch.Tensor:
     """1-D int32, contiguous."""
-    if t.dtype is not torch.int32:
-        t = t.to(torch.int32)
+    t = _int32(t)
     return t if t.is_contiguous() else t.contiguous()
 
 
 def _table(t: torch.Tensor):
     """int32 rows of unit stride, and their distance."""
-    if t.dtype is not torch.int32:
-        t = t.to(torch.int32)
+    t = _int32(t)
     if t.is_contiguous():
         return t, t.shape[1]
     if t.shape[1] > 1 and t.stride(1) != 1 or t.shape[0] > 1 and t.stride(0) < t.shape[1]:

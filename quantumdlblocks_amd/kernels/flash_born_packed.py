@@ -53,9 +53,15 @@ def _token_rows(t: torch.Tensor, dtype: torch.dtype, dp: int):
     return t, st, sh
 
 
+def _int32(t: torch.Tensor) -> torch.Tensor:
+    """int32, values outside its range cut to it: what lies outside the tensors stays outside."""
+    return t if t.dtype is torch.int32 else t.clamp(-(1 << 31), (1 << 31) - 1).to(torch.int32)
+
+
 def _starts(cu: torch.Tensor, device: torch.device) -> torch.Tensor:
-    if cu.dtype is not torch.int32 or cu.device != device:
-        cu = cu.to(device=device, dtype=torch.int32)
+    cu = _int32(cu)
+    if cu.device != device:
+        cu = cu.to(device)
     return cu if cu.is_contiguous() else cu.contiguous()
 
 

@@ -266,3 +266,17 @@ def test_empty_calls_launch_nothing():
     for call in (lib.qdl_flash_born_paged_forward_call, lib.qdl_flash_born_cache_append_call, lib.qdl_flash_born_cache_evict_call):
         assert call(None, None) == -5
         assert call(b"\x08" + bytes(511), None) == -2
+
+
+def test_int64_indices_outside_32_bits_are_not_wrapped():
+    # 2^32 is page 0 with its upper half cut off, 2^32 + 5 a length of 5.
+    from quantumdlblocks_amd.kernels import born_cache, flash_born_packed
+
+    table = torch.tensor([[1 << 32, 2, -(1 << 40), (1 << 62) + 1]])
+    got, _ = born_cache._table(table)
+    assert got.dtype is torch.int32 and got[0, 1] == 2
+    assert all(not 0 <= got[0, i] < 1000 for i in (0, 2, 3))
+    lens = born_cache._index(torch.tensor([(1 << 32) + 5, 7, -(1 << 33)]))
+    assert lens[0] == 2 ** 31 - 1 and lens[1] == 7 and lens[2] < 0
+    cu = flash_born_packed._starts(torch.tensor([0, 9, (1 << 32) + 1]), torch.device("cpu"))
+    assert cu.tolist() == [0, 9, 2 ** 31 - 1]
