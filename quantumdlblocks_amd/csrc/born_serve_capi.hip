@@ -63,6 +63,8 @@ int check_packed(const qdl_born_packed_call* c) {
     if ((c->n_q / qdl::packed_rows(4) + c->sequences + 1) * c->H > kMostBlocks ||
         (c->n_k / qdl::packed_rows(4) + c->sequences + 1) * c->H > kMostBlocks || c->n_k * c->h_kv * c->D > (int64_t)1 << 33)
         return QDL_BORN_E_SHAPE;
+    // dK/dV's workgroups have 512 threads.
+    if ((c->n_k / qdl::packed_rows(1) + c->sequences + 1) * c->h_kv > kMostBlocks / 2) return QDL_BORN_E_SHAPE;
     if (c->scale && c->n_scale != 1 && c->n_scale != c->H) return QDL_BORN_E_SCALE;
     if (c->window_size < 0 || c->window_size > (int64_t)1 << 30) return QDL_BORN_E_WINDOW;
     if (!(c->eps >= 0.0)) return QDL_BORN_E_SHAPE;

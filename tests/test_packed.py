@@ -112,3 +112,11 @@ def test_backward_block_checks():
     assert lib.qdl_flash_born_packed_forward_call(b"\x08" + short[1:], None) == -2
     assert lib.qdl_flash_born_packed_workspace_size(_packed_block()) >= 2 * 4 * 4 * 4
     assert lib.qdl_flash_born_packed_workspace_size(_packed_block(D=12)) == 0
+
+
+def test_many_sequences_fit_the_launches_of_both_directions():
+    # dK/dV's workgroups of 512 threads: 2^23 of them leave the 32 bits that count a launch's threads.
+    lib = _native.load()
+    assert lib.qdl_flash_born_packed_workspace_size(_packed_block(H=1, h_kv=1, sequences=(1 << 23) - 4)) > 0
+    assert lib.qdl_flash_born_packed_workspace_size(_packed_block(H=1, h_kv=1, sequences=1 << 23)) == 0
+    assert lib.qdl_flash_born_packed_forward_call(_packed_block(H=1, h_kv=1, sequences=1 << 23), None) == -2
