@@ -181,10 +181,14 @@ int check_paged(const qdl_born_paged_call* c) {
     return QDL_BORN_OK;
 }
 
+int64_t append_blocks(int64_t n, int64_t rows, int lpr, bool many) {
+    const int64_t per = 256 / lpr;
+    return (n * (many ? (rows + 3) / 4 : rows) + per - 1) / per;
+}
+
 template <class E, int VEC>
 void launch_append(const qdl::AppendArgs& a, bool many, hipStream_t st) {
-    const int64_t rows = a.H + 2 * a.Hkv, groups = many ? (rows + 3) / 4 : rows;
-    const int64_t per = 256 / a.lpr, blocks = (a.N * groups + per - 1) / per;
+    const int64_t blocks = append_blocks(a.N, a.H + 2 * a.Hkv, a.lpr, many);
     if (many) hipLaunchKernelGGL((qdl::born_append_kernel<E, VEC, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
     else hipLaunchKernelGGL((qdl::born_append_kernel<E, VEC, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
 }
@@ -380,7 +384,7 @@ int qdl_flash_born_cache_append_call(const qdl_born_append_call* c, qdl_stream_t
     // Groups of four rows where single ones would fill the chip twice over
     // (256 CUs x 32 waves x 64 lanes).
     const bool many = c->n * (c->H + 2 * c->h_kv) * lpr >= (int64_t)1 << 20;
-    if ((c->n * (c->H + 2 * c->h_kv) * lpr) / 256 + 1 > kMostBlocks * (many ? 4 : 1)) return QDL_BORN_E_SHAPE;
+    if (append_blocks(c->n, c->H + 2 * c->h_kv, lpr, many) > kMostBlocks) return QDL_BORN_E_SHAPE;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (c->dtype) {
         case QDL_BORN_DTYPE_BF16:

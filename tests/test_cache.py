@@ -280,3 +280,9 @@ def test_int64_indices_outside_32_bits_are_not_wrapped():
     assert lens[0] == 2 ** 31 - 1 and lens[1] == 7 and lens[2] < 0
     cu = flash_born_packed._starts(torch.tensor([0, 9, (1 << 32) + 1]), torch.device("cpu"))
     assert cu.tolist() == [0, 9, 2 ** 31 - 1]
+
+
+def test_append_counts_the_groups_that_it_launches():
+    # Five rows a token are two groups of four: 2^24 workgroups, where 5 / 4 of a group would pass.
+    over = dict(n=1 << 28, B=1, cu=16, H=3, h_kv=1, D=128, qs0=384, qs1=128, ks0=128, ks1=128, vs0=128, vs1=128)
+    assert _native.load().qdl_flash_born_cache_append_call(_append_block(**over), None) == -2
