@@ -469,7 +469,8 @@ int qdl_flash_born_cache_append_call(const qdl_born_append_call *call, qdl_strea
  * keys at weight_len and after have weight 0).  They keep their order.
  * kept (B, h_kv, budget): the kept keys' old slots, -1 behind the last;
  * weight_out (B, h_kv, weight_len): their weights, 0 behind the last;
- * lens_out (B): min(cache_lens, budget).
+ * lens_out (B): min(cache_lens, budget).  None of the three may overlap an
+ * input.
  * The kept rows of K and V move to slots 0, 1, ... of out_table's pages
  * (out_pages columns), none of which may be a page of block_table, or, with
  * out_table NULL, of block_table's own.  Rows behind the last kept one stay as

@@ -415,6 +415,9 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call* c, qdl_stream_t s
     if (c->B == 0) return QDL_BORN_OK;
     if (!c->cache_lens || !c->lens_out || (c->budget > 0 && !c->kept) || (c->weight_len > 0 && (!c->key_weight || !c->weight_out)))
         return QDL_BORN_E_NULL;
+    // Outputs that other workgroups still read as inputs.
+    if (c->lens_out == c->cache_lens || (c->weight_len > 0 && c->weight_out == c->key_weight)) return QDL_BORN_E_SHAPE;
+    if (c->out_table && c->out_table == c->block_table) return QDL_BORN_E_PAGE;
     const int64_t it = item(c->dtype);
     const int64_t most = c->budget < c->pages * c->page_size ? c->budget : c->pages * c->page_size;  // kept rows
     const int64_t per = qdl::evict_rows((int)(c->D * it / 16)), tiles = (most + per - 1) / per;

@@ -286,3 +286,11 @@ def test_append_counts_the_groups_that_it_launches():
     # Five rows a token are two groups of four: 2^24 workgroups, where 5 / 4 of a group would pass.
     over = dict(n=1 << 28, B=1, cu=16, H=3, h_kv=1, D=128, qs0=384, qs1=128, ks0=128, ks1=128, vs0=128, vs1=128)
     assert _native.load().qdl_flash_born_cache_append_call(_append_block(**over), None) == -2
+
+
+@pytest.mark.parametrize("over,code", [(dict(lens_out=32, lens=32), -2), (dict(weight_out=32, weight=32), -2),
+                                       (dict(to=32, table=32, to_pages=4, to_ld=4), -15)])
+def test_evict_refuses_outputs_that_are_its_inputs(over, code):
+    # Other workgroups still read them.
+    base = dict(lens_out=48, lens=64, weight_out=80, weight=96)
+    assert _native.load().qdl_flash_born_cache_evict_call(_evict_block(**{**base, **over}), None) == code
