@@ -298,3 +298,81 @@ def test_batches_without_sequences_or_tokens(cuda_device):
         lens_out, w, kept = born_cache_evict(kc, vc, table, lens, weight, 8)
         assert lens_out.shape == (0,) and w.shape == weight.shape and kept.shape == (0, 2, 8)
         assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+def test_int64_tables_name_no_other_page(cuda_device):
+    # 2^32 is no page of the cache: nothing is read there, and nothing written.
+    g = torch.Generator().manual_seed(31)
+    kc, vc, x = (torch.randn(*s, generator=g).to(cuda_device) for s in ((4, 16, 2, 64), (4, 16, 2, 64), (1, 4, 64)))
+    before = kc.clone(), vc.clone()
+    lens = torch.tensor([20], device=cuda_device)
+    far = torch.tensor([[1, 1 << 32]], device=cuda_device)
+    near = torch.tensor([[1, -1]], device=cuda_device, dtype=torch.int32)
+    assert torch.equal(flash_born_attention_paged(x, kc, vc, far, lens, 1.0), flash_born_attention_paged(x, kc, vc, near, lens, 1.0))
+    fused_qk_rope_l2_normalize_append(x, x[:, :2], x[:, :2], None, None, kc, vc, far, lens)
+    assert torch.equal(kc, before[0]) and torch.equal(vc, before[1])
+
+
+@pytest.mark.parametrize("page", [16, 24])
+def test_offsets_past_32_bits(cuda_device, page):
+    # The same rows in a cache's first pages and behind its first 4 GiB give the same.
+    B, Hkv, D, n = 2, 8, 128, 100
+    per = -(-n // page)
+    pages = (9 << 29) // (page * Hkv * D * 2) + 4 * per * B  # 4.5 GiB and more of bf16
+    g = torch.Generator().manual_seed(32)
+    kc, vc = (torch.zeros(pages, page, Hkv, D, dtype=torch.bfloat16, device=cuda_device) for _ in range(2))
+    lens = torch.full((B,), n, dtype=torch.int32, device=cuda_device)
+    low = torch.arange(B * per, dtype=torch.int32, device=cuda_device).view(B, per)
+    high = pages - 1 - low
+    to_low, to_high = low + B * per, high - B * per
+    assert int(to_high.min()) * page * Hkv * D * 2 > 1 << 32
+    q, k, v = (torch.randn(B * n, h, D, generator=g).to(device=cuda_device, dtype=torch.bfloat16) for h in (16, Hkv, Hkv))
+    cu = torch.tensor([0, n, 2 * n], dtype=torch.int32, device=cuda_device)
+    weight = torch.rand(B, Hkv, n, generator=g).to(cuda_device)
+    got = []
+    for table, to in ((low, to_low), (high, to_high)):
+        qn = fused_qk_rope_l2_normalize_append(q, k, v, None, None, kc, vc, table, lens, cu)
+        out = flash_born_attention_paged(qn[n - 1 :: n], kc, vc, table, lens, 1.0)
+        cut, _, kept = born_cache_evict(kc, vc, table, lens, weight, 50, 10, to)
+        moved = flash_born_attention_paged(qn[n - 1 :: n], kc, vc, to, cut, 1.0)
+        born_cache_evict(kc, vc, table, lens, weight, 50, 10)
+        own = flash_born_attention_paged(qn[n - 1 :: n], kc, vc, table, cut, 1.0)
+        assert torch.equal(own, moved) and out.any() and moved.any()
+        got.append((out, moved, kept))
+    assert all(torch.equal(a, b) for a, b in zip(*got))
+
+
+def test_evict_over_one_span_of_the_selection(cuda_device):
+    # More keys than the workgroup's threads hold at once, with ties across the spans.
+    n, budget, recent = 40000, 17000, 100
+    g = torch.Generator().manual_seed(33)
+    w = torch.randint(0, 500, (1, 2, n), generator=g).float()
+    w[0, 1, 5000:30000] = 0.0
+    kc, vc, table, lens, _ = make_cache([n], 64, 2, 8, torch.float32, 34)
+    want = born_cache_evict(kc.clone(), vc.clone(), table, lens, w, budget, recent)
+    k2, v2 = kc.to(cuda_device), vc.to(cuda_device)
+    got = born_cache_evict(k2, v2, table.to(cuda_device), lens.to(cuda_device), w.to(cuda_device), budget, recent)
+    k1, v1 = kc.clone(), vc.clone()
+    born_cache_evict(k1, v1, table, lens, w, budget, recent)
+    for a, b in zip((*got, k2, v2), (*want, k1, v1)):
+        assert torch.equal(a.cpu().to(b.dtype), b)
+
+
+def test_two_streams_at_once(cuda_device):
+    # Calls that overlap share nothing: each has its own workspace.
+    cases = [make_cache([3000, 700], 16, 2, 64, torch.float32, s) for s in (35, 36)]
+    sets = []
+    for i, (kc, vc, table, lens, _) in enumerate(cases):
+        q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(37 + i))
+        sets.append([x.to(cuda_device) for x in (q, kc, vc, table, lens)])
+    alone = [flash_born_attention_paged(*s, 1.0) for s in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    outs = [[], []]
+    for _ in range(20):
+        for i, s in enumerate(sets):
+            with torch.cuda.stream(streams[i]):
+                outs[i].append(flash_born_attention_paged(*s, 1.0))
+    torch.cuda.synchronize()
+    for a, many in zip(alone, outs):
+        assert all(torch.equal(a, x) for x in many)

@@ -299,3 +299,35 @@ def test_gradients_of_some_inputs_only(cuda_device, dtype, D):
         out = flash_born_attention_packed(*some, cu, eps=0.5)
         for i, g in zip(pick, torch.autograd.grad(out, [leaves[i] for i in pick], do)):
             assert torch.equal(g, every[i]), (pick, i)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp32"])
+def test_offsets_past_32_bits(cuda_device, dtype):
+    # Token strides of half a step under the limit: rows lie over more than 4 GiB.
+    lens, H, Hkv, D = [500, 200], 2, 1, 64
+    q, k, v, do, cq, _ = _inputs(lens, 0, H, Hkv, D, DT[dtype], cuda_device, seed=19)
+    cu = _cu(cq, cuda_device)
+    stride = (1 << 23) // q.element_size()  # 8 MiB a token
+
+    def far(x):
+        n, h, d = x.shape
+        big = torch.empty((n - 1) * stride + h * d, dtype=x.dtype, device=x.device).as_strided((n, h, d), (stride, d, 1))
+        return big.copy_(x)
+
+    def run(*xs):
+        xs = [x.detach().requires_grad_() for x in xs]
+        out = flash_born_attention_packed(*xs, 2.0, cu)
+        return (out, *torch.autograd.grad(out, xs, do))
+
+    assert 700 * stride * q.element_size() > 1 << 32
+    for a, b in zip(run(q, k, v), run(far(q), far(k), far(v))):
+        assert torch.equal(a, b)
+
+
+def test_keys_without_queries(cuda_device):
+    q, k, v, _, _, _ = _inputs([70], 0, 4, 2, 64, torch.bfloat16, cuda_device, seed=20)
+    none, some = torch.tensor([0, 0], device=cuda_device), torch.tensor([0, 70], device=cuda_device)
+    leaves = [x.requires_grad_() for x in (q[:0].detach(), k, v)]
+    out = flash_born_attention_packed(*leaves, 1.0, none, some)
+    for x, g in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
+        assert g.shape == x.shape and not g.any()
