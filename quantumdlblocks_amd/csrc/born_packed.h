@@ -19,11 +19,14 @@
 // and u (dQ, dK), half a step each.  bf16's Z adds the rounded p, so numerator
 // and denominator carry the same error; fp16's adds them in fp32.  delta comes
 // from the output as it was rounded: O in fp32 would cost 2 N H D bytes more to
-// write and to read.  Against 64 bits the 16-bit dQ and dK are about twice as
-// far off as gradients whose only rounding is the output's (bf16 3.1e-3 and
-// 1.7e-3, fp16 4.0e-4 and 2.1e-4 in norm).  A simulation in 64 bits of bf16 dQ
-// gives 2.6e-3 from u's and dQ's rounding alone and 2.8e-3 with delta from an
-// unrounded O: only a second product for u's remainder would bring it down.
+// write and to read.  Against 64 bits the 16-bit dQ and dK are 1.8 to 2.6 times
+// as far off as gradients whose only rounding is the output's (in norm: bf16
+// 3.0e-3 to 4.2e-3 for 1.7e-3, fp16 4.0e-4 to 5.4e-4 for 2.1e-4), most in short
+// sequences, where delta's error weighs more.  A simulation in 64 bits, bf16
+// D64, sequences of 2048, 64 and 2 tokens: dQ 3.3e-3, 3.5e-3, 4.0e-3, with delta
+// from an unrounded O 3.0e-3, 3.1e-3, 3.1e-3, with exact statistics 2.6e-3,
+// 2.6e-3, 2.2e-3: what is left is u's rounding, which only a second product for
+// its remainder would take away.
 // fp32 rounds nothing on the way (3.3e-7, plain fp32 4.8e-7).
 //
 // What bounds them: the matrix pipe.  A workgroup's four waves share the tiles
