@@ -25,7 +25,7 @@ import functools
 import torch
 
 from .. import _native
-from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _apply, _autocast_dtype, _pad_head, _parameter, _run_call
+from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _aligned, _apply, _autocast_dtype, _pad_head, _parameter, _run_call
 
 __all__ = ["flash_born_attention_packed"]
 
@@ -93,30 +93,37 @@ def _check(q, k, v, n_scale, cu_q, cu_k):
         raise ValueError(f"q, k, v must be on one device, got {q.device}, {k.device}, {v.device}")
 
 
+def _head(dtype, q_rows, k_rows, v_rows, out, z, cu_q, cu_k, scale, is_causal, eps, window):
+    """The argument block's fields up to eps.  ``*_rows``: a tensor and its
+    strides; ``scale``: address, count, value.  The tensors stay with the caller
+    until the call: the block holds addresses."""
+    (q, *qs), (k, *ks), (v, *vs) = q_rows, k_rows, v_rows
+    N, H, dp = out.shape
+    M, Hkv, _ = k.shape
+    return (_DTYPE_CODE[dtype], cu_q.shape[0] - 1, N, M, H, Hkv, dp, q.data_ptr(), k.data_ptr(), v.data_ptr(), *qs, *ks, *vs,
+            out.data_ptr(), 0 if z is None else z.data_ptr(), cu_q.data_ptr(), cu_k.data_ptr(), *scale, 1 if is_causal else 0, window, eps)
+
+
 def _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, train):
-    """The call: (output, argument block's head, what the backward needs)."""
+    """The call: (output, its sizes, what the backward needs)."""
     lib = _native.load()
     target = _autocast_dtype(q) or v.dtype
     if target not in _DTYPE_CODE:
         raise TypeError(f"flash_born_attention_packed: unsupported dtype {target}")
     dev = q.device
-    scale_flat, scale_p, n_scale, scale_value = _parameter(scale, dev)
+    scale_flat, *scale_args = _parameter(scale, dev)
     N, H, D = q.shape
-    M, Hkv, _ = k.shape
     dp = (D + 7) // 8 * 8
-    q_c, q0, q1 = _token_rows(q, target, dp)
-    k_c, k0, k1 = _token_rows(k, target, dp)
-    v_c, v0, v1 = _token_rows(v, target, dp)
+    q_rows, k_rows, v_rows = _token_rows(q, target, dp), _token_rows(k, target, dp), _token_rows(v, target, dp)
     cs_q = _starts(cu_q, dev)
     cs_k = cs_q if cu_k is cu_q else _starts(cu_k, dev)
     out = torch.empty((N, H, dp), dtype=target, device=dev)
     z = torch.empty((H, N), dtype=torch.float32, device=dev) if train else None
-    head = (_DTYPE_CODE[target], cs_q.shape[0] - 1, N, M, H, Hkv, dp, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(),
-            q0, q1, k0, k1, v0, v1, out.data_ptr(), z.data_ptr() if train else 0, cs_q.data_ptr(), cs_k.data_ptr(), scale_p,
-            n_scale, scale_value, 1 if is_causal else 0, window, eps)
+    head = _head(target, q_rows, k_rows, v_rows, out, z, cs_q, cs_k, scale_args, is_causal, eps, window)
     _run_call(lib.qdl_flash_born_packed_forward_call, "qdl_flash_born_packed_forward_call", dev,
               _native.packed_call(*head, 0, 0, 0, 0, 0, 0, 0, 0, 0))
-    return out if dp == D else out[..., :D].contiguous(), head, (q_c, k_c, v_c, out, z, scale_flat, cs_q, cs_k)
+    return (out if dp == D else out[..., :D].contiguous(), head[:7],
+            (q_rows[0], k_rows[0], v_rows[0], out, z, scale_flat, cs_q, cs_k))
 
 
 @torch.compiler.disable
@@ -140,12 +147,18 @@ def _workspace(dtype, sequences, N, M, H, Hkv, dp, window) -> int:
 class _FlashBornPackedFn(torch.autograd.Function):
     """forward: computes in the autocast dtype (CUDA autocast active) else
     ``v.dtype``; saves the rows, ``out``, Z (fp32) and the starts.  backward:
-    dq, dk, dv in the inputs' dtypes, dscale in the scale's shape and dtype."""
+    dq, dk, dv in the inputs' dtypes, dscale in the scale's shape and dtype.
+
+    The context holds no address and no stride: a saved tensor's hook
+    (checkpoints, offloading) gives the backward other tensors than these."""
 
     @staticmethod
     def forward(ctx, q, k, v, scale, cu_q, cu_k, is_causal, eps, window):
-        out, ctx.head, saved = _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, True)
-        ctx.workspace = _workspace(*ctx.head[:7], window)
+        out, sizes, saved = _forward(q, k, v, scale, cu_q, cu_k, is_causal, eps, window, True)
+        ctx.workspace = _workspace(*sizes, window)
+        ctx.dtype = saved[3].dtype
+        ctx.modes = is_causal, eps, window
+        ctx.scale_value = 0.0 if isinstance(scale, torch.Tensor) else float(scale)
         ctx.save_for_backward(*saved)
         ctx.head_dim = q.shape[2]
         if isinstance(scale, torch.Tensor):
@@ -156,34 +169,37 @@ class _FlashBornPackedFn(torch.autograd.Function):
     @staticmethod
     def backward(ctx, do):
         lib = _native.load()
-        q_c, k_c, v_c, out, z, scale_flat, cu_q, cu_k = ctx.saved_tensors
-        N, H, dp = out.shape
-        M, Hkv = k_c.shape[:2]
-        D, dev = ctx.head_dim, q_c.device
-        do_c, *ds = _token_rows(do, out.dtype, dp)
+        q, k, v, out, z, scale_flat, cu_q, cu_k = ctx.saved_tensors
+        D, dev, dt, dp = ctx.head_dim, out.device, ctx.dtype, out.shape[2]
+        q_rows, k_rows, v_rows = _token_rows(q, dt, dp), _token_rows(k, dt, dp), _token_rows(v, dt, dp)
+        out, z, cu_q, cu_k = _aligned(out.to(dt)), _aligned(z.to(torch.float32)), _starts(cu_q, dev), _starts(cu_k, dev)
+        scale_flat, *scale_args = _parameter(ctx.scale_value if scale_flat is None else scale_flat, dev)
+        M, Hkv, _ = k.shape
+        do_c, *ds = _token_rows(do, dt, dp)
         _, want_k, want_v, want_scale = ctx.needs_input_grad[:4]
-        dq = torch.empty_like(out)
+        dq = torch.empty_like(out)  # contiguous, as out is
         # dK and dV come together, and not at all where neither is wanted.
         dk = dv = None
         if want_k or want_v:
-            dk = torch.empty((M, Hkv, dp), dtype=out.dtype, device=dev)
+            dk = torch.empty((M, Hkv, dp), dtype=dt, device=dev)
             dv = torch.empty_like(dk)
         n_scale = 1 if scale_flat is None else scale_flat.numel()
         # The scale's gradient costs launches of its own: only where wanted.
         dscale = torch.empty(n_scale, dtype=torch.float32, device=dev) if want_scale else None
         size = ctx.workspace
         ws = torch.empty(max(size, 16), dtype=torch.uint8, device=dev)
+        head = _head(dt, q_rows, k_rows, v_rows, out, z, cu_q, cu_k, scale_args, *ctx.modes)
         _run_call(lib.qdl_flash_born_packed_backward_call, "qdl_flash_born_packed_backward_call", dev,
-                  _native.packed_call(*ctx.head, do_c.data_ptr(), *ds, dq.data_ptr(), 0 if dk is None else dk.data_ptr(),
+                  _native.packed_call(*head, do_c.data_ptr(), *ds, dq.data_ptr(), 0 if dk is None else dk.data_ptr(),
                                       0 if dv is None else dv.data_ptr(), 0 if dscale is None else dscale.data_ptr(),
                                       ws.data_ptr(), size))
         grads = []
-        for g, dt in zip((dq, dk, dv), ctx.dtypes):
+        for g, want in zip((dq, dk, dv), ctx.dtypes):
             if g is not None:
                 if dp != D:
                     g = g[..., :D]
-                if g.dtype is not dt:
-                    g = g.to(dt)
+                if g.dtype is not want:
+                    g = g.to(want)
             grads.append(g)
         return (*grads, None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype), None, None, None, None, None)
 
