@@ -15,8 +15,8 @@ are missing pages: their keys are not seen and nothing is written to them.
 
 No call copies anything to the host, so a decoding step can be captured into a
 HIP graph; tables and lengths may change between replays.  CPU tensors run the
-same formulas in torch operations.  None of these has a backward: they refuse
-tensors that a gradient is recorded for.
+same formulas in torch operations.  None of these has a derivative: they refuse
+tensors that one is recorded for, backward or forward.
 """
 
 from __future__ import annotations
@@ -27,7 +27,7 @@ import torch
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
-from .flash_born_packed import _int32
+from .flash_born_packed import _int32, _is_dual
 
 __all__ = ["born_cache_evict", "flash_born_attention_paged", "fused_qk_rope_l2_normalize_append"]
 
@@ -36,9 +36,12 @@ _INDEX = (torch.int32, torch.int64)
 
 
 def _no_grad(what: str, *tensors) -> None:
-    for t in tensors:
-        if isinstance(t, torch.Tensor) and t.requires_grad:
-            raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and t.requires_grad:
+                raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
+    if _is_dual(*tensors):
+        raise RuntimeError(f"{what} has no forward-mode derivative: call it with the tensors' primals")
 
 
 def _bad_cache(name: str, c: torch.Tensor):
@@ -194,8 +197,7 @@ def flash_born_attention_paged(
     Lengths past the table's pages are cut to them; a sequence without visible
     keys gets zeros.
     """
-    if torch.is_grad_enabled():
-        _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
+    _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
     if q.dim() != 3:
         raise ValueError(f"q must be (B, heads, head_dim), got shape {tuple(q.shape)}")
     B, H, D = q.shape
@@ -346,8 +348,7 @@ def fused_qk_rope_l2_normalize_append(
     16 bits as the reference does.  Values that no sequence owns come out as
     zero queries; slots without a page are not written.
     """
-    if torch.is_grad_enabled():
-        _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, k_cache, v_cache)
+    _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, cos, sin, k_cache, v_cache)
     kshape = k.shape
     if q.dim() != 3 or len(kshape) != 3 or kshape != v.shape or kshape[0] != q.shape[0] or kshape[2] != q.shape[2]:
         raise ValueError(f"q must be (N, heads, head_dim) and k, v (N, key_heads, head_dim), got {tuple(q.shape)}, "
@@ -470,8 +471,7 @@ def born_cache_evict(
     behind the last.  Keys stay rotated by the positions that they were appended
     at: pass ``positions`` to the next append.
     """
-    if torch.is_grad_enabled():
-        _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
+    _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
     strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
     P, page, Hkv, D = k_cache.shape

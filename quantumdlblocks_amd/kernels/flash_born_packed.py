@@ -23,6 +23,7 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _aligned, _apply, _autocast_dtype, _pad_head, _parameter, _run_call
@@ -144,6 +145,13 @@ def _workspace(dtype, sequences, N, M, H, Hkv, dp, window) -> int:
     return int(_native.load().qdl_flash_born_packed_workspace_size(block))
 
 
+def _is_dual(*values) -> bool:
+    """Whether a forward-mode derivative runs through any of them (the level
+    first: outside of one there are no tangents, and this is all it costs)."""
+    return forward_ad._current_level >= 0 and any(
+        isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in values)
+
+
 class _FlashBornPackedFn(torch.autograd.Function):
     """forward: computes in the autocast dtype (CUDA autocast active) else
     ``v.dtype``; saves the rows, ``out``, Z (fp32) and the starts.  backward:
@@ -202,6 +210,14 @@ class _FlashBornPackedFn(torch.autograd.Function):
                     g = g.to(want)
             grads.append(g)
         return (*grads, None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype), None, None, None, None, None)
+
+
+def _on_gpu(q, k, v, scale, *rest):
+    """Through the autograd function where a derivative is recorded; it refuses a forward-mode one."""
+    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                     or (isinstance(scale, torch.Tensor) and scale.requires_grad))) or _is_dual(q, k, v, scale):
+        return _apply(_FlashBornPackedFn, q, k, v, scale, *rest)
+    return _uncompiled(_forward, q, k, v, scale, *rest, False)[0]
 
 
 def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
@@ -269,9 +285,6 @@ def flash_born_attention_packed(
     if not float(eps) >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
     if q.is_cuda and q.shape[2] <= MAX_HEAD_DIM:
-        if torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                        or (isinstance(scale, torch.Tensor) and scale.requires_grad)):
-            return _apply(_FlashBornPackedFn, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
-        return _uncompiled(_forward, q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window, False)[0]
+        return _on_gpu(q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
     scale_t = scale if isinstance(scale, torch.Tensor) else torch.tensor(float(scale), dtype=torch.float64)
     return _eager_packed(q, k, v, scale_t, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
