@@ -152,6 +152,19 @@ def _is_dual(*values) -> bool:
         isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None for t in values)
 
 
+class _OnlyOnce(torch.autograd.Function):
+    """A gradient of a recorded backward (``create_graph``): the kernels have no
+    second derivative, so to differentiate it again is an error, not a zero."""
+
+    @staticmethod
+    def forward(ctx, grad, anchor):
+        return grad.view_as(grad)
+
+    @staticmethod
+    def backward(ctx, _):
+        raise RuntimeError("flash_born_attention_packed has no second derivative on the GPU")
+
+
 class _FlashBornPackedFn(torch.autograd.Function):
     """forward: computes in the autocast dtype (CUDA autocast active) else
     ``v.dtype``; saves the rows, ``out``, Z (fp32) and the starts.  backward:
@@ -201,7 +214,7 @@ class _FlashBornPackedFn(torch.autograd.Function):
                   _native.packed_call(*head, do_c.data_ptr(), *ds, dq.data_ptr(), 0 if dk is None else dk.data_ptr(),
                                       0 if dv is None else dv.data_ptr(), 0 if dscale is None else dscale.data_ptr(),
                                       ws.data_ptr(), size))
-        grads = []
+        grads, again = [], torch.is_grad_enabled()
         for g, want in zip((dq, dk, dv), ctx.dtypes):
             if g is not None:
                 if dp != D:
@@ -209,7 +222,11 @@ class _FlashBornPackedFn(torch.autograd.Function):
                 if g.dtype is not want:
                     g = g.to(want)
             grads.append(g)
-        return (*grads, None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype), None, None, None, None, None)
+        grads.append(None if dscale is None else dscale.view(ctx.scale_shape).to(ctx.scale_dtype))
+        if again:
+            anchor = torch.empty(0, requires_grad=True)
+            grads = [None if g is None else _OnlyOnce.apply(g, anchor) for g in grads]
+        return (*grads, None, None, None, None, None)
 
 
 def _on_gpu(q, k, v, scale, *rest):

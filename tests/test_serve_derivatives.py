@@ -82,3 +82,21 @@ def test_cache_operators_refuse_recorded_derivatives(op):
             fn(**dict(kw, **{name: leaf}))
     with forward_ad.dual_level():
         fn(**kw)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float64])  # float64: rows that the call casts
+@pytest.mark.parametrize("wrt", range(4))
+def test_packed_second_derivative(calls, dtype, wrt):
+    x, cu = _packed_inputs()
+    leaves = [x["q"].to(dtype), x["k"].to(dtype), x["v"], x["scale"].to(dtype)]
+    leaves = [t.requires_grad_() for t in leaves]
+    out = packed._on_gpu(*leaves, cu, cu, True, 1e-12, 0)
+    (g,) = torch.autograd.grad(out.sum(), leaves[wrt], create_graph=True)
+    with pytest.raises(RuntimeError, match="second derivative"):
+        (g.square().sum() + leaves[0].sum()).backward()
+    # A recorded backward by itself is none.
+    out = packed._on_gpu(*leaves, cu, cu, True, 1e-12, 0)
+    out.sum().backward(create_graph=True)
+    assert all(t.grad.shape == t.shape for t in leaves)
+    for t in leaves:
+        t.grad = None  # with its graph
