@@ -313,7 +313,8 @@ def _eager_append(q, k, v, tables, k_cache, v_cache, block_table, cache_lens, cu
         ok = here & (pages >= 0) & (pages < P)
         k_cache[pages[ok], rows[ok]] = turned(k)[ok].to(k_cache.dtype)
         v_cache[pages[ok], rows[ok]] = v[ok].to(v_cache.dtype)
-    return (turned(q) * here.view(-1, 1, 1)).to(k_cache.dtype)
+    queries = turned(q)
+    return torch.where(here.view(-1, 1, 1), queries, torch.zeros_like(queries)).to(k_cache.dtype)
 
 
 def fused_qk_rope_l2_normalize_append(
