@@ -162,7 +162,7 @@ def _eager_paged(q, k_cache, v_cache, block_table, cache_lens, scale_t, eps, win
         k, v = (torch.where(mask, c[at, rows].to(wide), torch.zeros((), dtype=wide, device=q.device)) for c in (k_cache, v_cache))
     s = scale_t.to(device=q.device, dtype=wide).reshape(-1).expand(H).view(1, Hkv, G, 1)
     r = torch.matmul(q.to(wide).view(B, Hkv, G, D), k.permute(0, 2, 3, 1))
-    p = torch.relu(r * s).square() * keep.view(B, 1, 1, L)
+    p = torch.relu(torch.where(keep.view(B, 1, 1, L), r * s, torch.zeros_like(r))).square()
     den = p.sum(-1, keepdim=True) + eps
     w = p / torch.where(den > 0, den, torch.ones_like(den))
     if key_weight is not None:

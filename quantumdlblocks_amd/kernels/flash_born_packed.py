@@ -259,7 +259,8 @@ def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
             keep = keep & (lag >= 0)
         if window > 0:
             keep = keep & (lag < window)
-        p = torch.relu(torch.matmul(qs, ks.transpose(-1, -2)) * s).square() * keep
+        r = torch.matmul(qs, ks.transpose(-1, -2)) * s
+        p = torch.relu(torch.where(keep, r, torch.zeros_like(r))).square()
         den = p.sum(-1, keepdim=True) + eps
         # Rows without weight are zero, with eps == 0 too.
         w = p / torch.where(den > 0, den, torch.ones_like(den))

@@ -6,7 +6,7 @@ from __future__ import annotations
 import pytest
 import torch
 
-from quantumdlblocks_amd import fused_qk_rope_l2_normalize_append
+from quantumdlblocks_amd import flash_born_attention_packed, flash_born_attention_paged, fused_qk_rope_l2_normalize_append
 
 BAD = [float("nan"), float("inf"), -float("inf")]
 
@@ -30,3 +30,36 @@ def test_tokens_of_no_sequence_are_zero_queries(bad):
     out = fused_qk_rope_l2_normalize_append(zero, zero[:, :1], zero[:, :1], None, None, kc, vc, table, lens * 0,
                                             torch.tensor([0, 0]), eps=0.0)
     assert not out.any() and not out.isnan().any()
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("causal,window", [(True, 0), (False, 2), (True, 2)])
+def test_packed_keys_that_a_row_does_not_see(bad, causal, window):
+    g = torch.Generator().manual_seed(1)
+    q, k, v = (torch.rand(9, h, 8, generator=g) for h in (4, 2, 2))
+    cu = torch.tensor([0, 4, 9])
+    want = flash_born_attention_packed(q, k, v, 2.0, cu, None, causal, 1e-12, window)
+    at = 3 if causal else 0  # seen by the first sequence's last row, or by its first two
+    k[at] = bad
+    out = flash_born_attention_packed(q, k, v, 2.0, cu, None, causal, 1e-12, window)
+    blind = [0, 1, 2, 4, 5, 6, 7, 8] if causal else [2, 3, 4, 5, 6, 7, 8]
+    assert torch.equal(out[blind], want[blind])
+    # Rows that see no key, whatever they hold.
+    q[:2] = bad
+    out = flash_born_attention_packed(q[:4], k[:2], v[:2], 2.0, torch.tensor([0, 4]), torch.tensor([0, 2]), eps=0.0)
+    assert not out[:2].any()
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("window", [0, 3])
+def test_paged_rows_without_keys(bad, window):
+    table = _cache((0, 5, 5))[2]
+    kc, vc = torch.rand(6, 4, 1, 8), torch.rand(6, 4, 1, 8)
+    table[2] = -1
+    q = torch.rand(3, 2, 8)
+    weight = torch.zeros(3, 1, 8)
+    want = flash_born_attention_paged(q, kc, vc, table, torch.tensor([0, 5, 5]), 2.0, 0.0, window, weight.clone())
+    q[0] = q[2] = bad
+    out = flash_born_attention_paged(q, kc, vc, table, torch.tensor([0, 5, 5]), 2.0, 0.0, window, weight)
+    assert torch.equal(out, want) and not out[0].any() and not out[2].any()
+    assert not weight[0].any() and not weight[2].any() and weight[1].isfinite().all()
