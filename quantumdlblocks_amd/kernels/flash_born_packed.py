@@ -237,9 +237,11 @@ def _on_gpu(q, k, v, scale, *rest):
     return _uncompiled(_forward, q, k, v, scale, *rest, False)[0]
 
 
-def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
-    """The formulas in torch operations, in fp32 (fp64 for fp64 values), one
-    sequence at a time."""
+@torch.autocast("cpu", enabled=False)
+@torch.autocast("cuda", enabled=False)
+def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window, target):
+    """The formulas in torch operations, in fp32 (fp64 for fp64 values) under
+    autocast too, one sequence at a time; the output in ``target``."""
     cq, ck = cu_q.tolist(), cu_k.tolist()
     for name, c, n in (("cu_seqlens_q", cq, q.shape[0]), ("cu_seqlens_k", ck, k.shape[0])):
         if c[0] != 0 or c[-1] > n or any(a > b for a, b in zip(c, c[1:])):
@@ -266,7 +268,7 @@ def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
         w = p / torch.where(den > 0, den, torch.ones_like(den))
         outs.append(torch.matmul(w, vs).permute(2, 0, 1, 3).reshape(nq, H, q.shape[2]))
     outs.append(torch.zeros((q.shape[0] - cq[-1], H, v.shape[2]), dtype=wide, device=q.device))
-    return torch.cat(outs).to(v.dtype)
+    return torch.cat(outs).to(target)
 
 
 def flash_born_attention_packed(
@@ -305,4 +307,5 @@ def flash_born_attention_packed(
     if q.is_cuda and q.shape[2] <= MAX_HEAD_DIM:
         return _on_gpu(q, k, v, scale, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
     scale_t = scale if isinstance(scale, torch.Tensor) else torch.tensor(float(scale), dtype=torch.float64)
-    return _eager_packed(q, k, v, scale_t, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window)
+    target = _autocast_dtype(q) or v.dtype
+    return _eager_packed(q, k, v, scale_t, cu_seqlens_q, cu_seqlens_k, bool(is_causal), float(eps), window, target)

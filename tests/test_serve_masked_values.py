@@ -63,3 +63,21 @@ def test_paged_rows_without_keys(bad, window):
     out = flash_born_attention_paged(q, kc, vc, table, torch.tensor([0, 5, 5]), 2.0, 0.0, window, weight)
     assert torch.equal(out, want) and not out[0].any() and not out[2].any()
     assert not weight[0].any() and not weight[2].any() and weight[1].isfinite().all()
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+def test_autocast_leaves_the_formulas_in_fp32(dtype):
+    g = torch.Generator().manual_seed(2)
+    q, k, v = (torch.randn(9, h, 8, generator=g).to(dtype) for h in (4, 2, 2))
+    cu = torch.tensor([0, 4, 9])
+    kc, vc, table, lens = _cache((7,))
+    kc, vc = kc.to(dtype), vc.to(dtype)
+
+    def run(autocast):
+        leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+        with torch.autocast("cpu", dtype=torch.bfloat16, enabled=autocast):
+            out = flash_born_attention_packed(*leaves, 2.0, cu)
+            one = flash_born_attention_paged(q[:1], kc, vc, table, lens, 2.0)
+        return (out, one, *torch.autograd.grad(out, leaves, torch.ones_like(out)))
+
+    assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(run(True), run(False)))
