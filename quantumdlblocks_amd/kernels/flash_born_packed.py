@@ -251,6 +251,8 @@ def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window, target):
     wide = torch.float64 if v.dtype == torch.float64 else torch.float32
     s = scale_t.to(device=q.device, dtype=wide).reshape(-1).expand(H).view(Hkv, G, 1, 1)
     outs = []
+    if len(cq) == 1:  # no sequences: an empty one, for the gradients
+        cq, ck = cq * 2, ck * 2
     for a0, a1, b0, b1 in zip(cq, cq[1:], ck, ck[1:]):
         nq, nk = a1 - a0, b1 - b0
         qs = q[a0:a1].to(wide).view(nq, Hkv, G, q.shape[2]).permute(1, 2, 0, 3)

@@ -81,3 +81,11 @@ def test_autocast_leaves_the_formulas_in_fp32(dtype):
         return (out, one, *torch.autograd.grad(out, leaves, torch.ones_like(out)))
 
     assert all(torch.equal(a, b) and a.dtype == b.dtype for a, b in zip(run(True), run(False)))
+
+
+def test_packed_batches_without_sequences_have_zero_gradients():
+    leaves = [torch.rand(5, h, 8, requires_grad=True) for h in (4, 2, 2)] + [torch.tensor([2.0], requires_grad=True)]
+    out = flash_born_attention_packed(*leaves, torch.zeros(1, dtype=torch.int32))
+    assert not out.any()
+    for x, g in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
+        assert g.shape == x.shape and not g.any()
