@@ -346,7 +346,8 @@ int qdl_flash_born_fwd_qk_prologue(int dtype, int64_t B, int64_t H, int64_t T,
  * sequence of len_q queries and len_k keys stands at position
  * i + len_k - len_q: causality shows it the keys up to its position, a window
  * those less than window_size before it.  Rows that see no key, and rows behind
- * the last sequence, have zero outputs and gradients.
+ * the last sequence, have zero outputs and gradients, and so have rows whose
+ * (sum of weights + eps) / scale^2 lies below fp32's normal range, 2^-126.
  *
  * q, k, v, dout have unit stride along D and *_strides (token, head) in
  * elements, multiples of 16 bytes (a token's at least D, under 2^24 bytes);

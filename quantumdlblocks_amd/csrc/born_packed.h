@@ -268,6 +268,12 @@ __device__ __forceinline__ void packed_load_row(u32x4 (&x)[KS], const uint8_t* r
     }
 }
 
+// 1 / den; 0 for rows without weight, and for sums below fp32's normal range,
+// whose reciprocals may be infinite: a row of zeros times that is not a number.
+// The backward's zs = 1 / den is cut at the same sum, its bound divided by the
+// factor that it is stored with.
+__device__ __forceinline__ float packed_inverse(float den) { return den >= 0x1p-126f ? 1.0f / den : 0.f; }
+
 // 0 or the sign bits of one 32-bit word of E.
 template <class E>
 __device__ __forceinline__ uint32_t packed_flip(float s) {
@@ -588,7 +594,7 @@ void born_packed_fwd_kernel(PackedArgs p) {
     if (!b.ok) return;
     const float s2 = s1 * s1;
     const float den = z + (p.eps == 0.f ? 0.f : p.eps / s2);
-    const float inv = den > 0.f && sc != 0.f ? 1.0f / den : 0.f;
+    const float inv = sc != 0.f ? packed_inverse(den) : 0.f;
     packed_store_row<E>((uint8_t*)p.out + ((size_t)(b.sq.q0 + b.row) * p.H + b.h) * D * kItem<E>, acc, inv, D, g);
     if (g == 0 && p.z != nullptr) p.z[(size_t)b.h * p.Nq + b.sq.q0 + b.row] = s2 * z + p.eps;
 }
@@ -630,7 +636,8 @@ void born_packed_dq_kernel(PackedArgs p) {
     delta += __shfl_xor(delta, 32);
     const size_t stat = (size_t)b.h * p.Nq + b.sq.q0 + b.row;
     const float zr = b.ok ? p.z[stat] : 1.f;
-    const float zs = zr > 0.f ? sc * fabsf(sc) / zr : 0.f;
+    float zs = zr > 0.f ? sc * fabsf(sc) / zr : 0.f;
+    if (!(fabsf(zs) <= 0x1p126f / kUp<E>)) zs = 0.f;
     if (b.ok && g == 0 && b.part == 0) {
         p.ndelta[stat] = -delta;
         p.zs[stat] = kUp<E> * zs;

@@ -103,7 +103,7 @@ __device__ __forceinline__ bool paged_row(const PagedArgs& p, ConstIntPtr table,
 // 1 / Z, without the s^2 of both; 0 for rows without weight.
 __device__ __forceinline__ float paged_inverse(const PagedArgs& p, int h, float z) {
     const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
-    return den > 0.f && s != 0.f ? 1.0f / den : 0.f;
+    return s != 0.f ? packed_inverse(den) : 0.f;
 }
 
 // A operands of V^T: 16-bit, lane's 8 keys x 8 columns (x[k][...]) -> the keys

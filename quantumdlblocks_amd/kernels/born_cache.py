@@ -196,7 +196,8 @@ def flash_born_attention_paged(
     fp32: each visible key's weight p_j / (sum p + eps), summed over the heads
     that read it, is added in place at j < L: what ``born_cache_evict`` goes by.
     Lengths past the table's pages are cut to them; a sequence without visible
-    keys gets zeros.
+    keys gets zeros, and so does a head whose (sum p + eps) / scale_h ** 2 lies
+    below fp32's normal range, 2^-126.
     """
     _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
     if q.dim() != 3:

@@ -12,7 +12,8 @@ standing at the last len_q of len_k positions,
     M_ij = [causal => j <= i + len_k - len_q]
            & [window_size > 0 => i + len_k - len_q - j < window_size]
 
-Rows that see no key are zero, and so are their gradients.
+Rows that see no key are zero, and so are their gradients; so are rows whose
+(sum_j p_ij + eps) / scale_h^2 lies below fp32's normal range, 2^-126.
 
 GPU tensors with head dim <= 256 run the HIP kernels; CPU tensors and larger
 head dims the formulation in torch operations.
