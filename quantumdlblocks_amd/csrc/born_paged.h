@@ -59,7 +59,7 @@ struct PagedArgs {
     float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
     int64_t w_sb, w_sh;    // elements
     int w_len;             // columns of weights
-    float* raw;            // (B, H, raw_ld) workspace: p without s^2, where weights are kept
+    float* raw;            // (B, H, raw_ld) workspace: p without s^2, keys from paged_base on, where weights are kept
     int64_t raw_ld;
 };
 
@@ -83,6 +83,9 @@ __device__ __forceinline__ PagedSpan paged_span(const PagedArgs& p, int b) {
     const int n = (int)min((int64_t)max(p.lens[b], 0), room);
     return {p.window > 0 ? max(0, n - p.window) : 0, n};
 }
+
+// Splits and raw weights count from here.
+__device__ __forceinline__ int paged_base(PagedSpan sp) { return sp.first & ~31; }
 
 // Page table entries and scalars that never change during a launch, read as
 // scalar loads where the index is uniform.
@@ -167,7 +170,7 @@ void born_paged_kernel(PagedArgs p) {
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, j4 = lane >> 4;
     const int heads = min(16, p.G - 16 * gb), h0 = hk * p.G + 16 * gb;
-    const int base = sp.first & ~31;  // splits count from here
+    const int base = paged_base(sp);
     const int s0 = base + split * p.chunk, s1 = min(sp.n, s0 + p.chunk);
     if (s0 >= s1 && split > 0) return;  // the join reads the filled splits only
     const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.table + (int64_t)b * p.table_ld);
@@ -327,10 +330,10 @@ void born_paged_kernel(PagedArgs p) {
             if (okh) {
 #pragma unroll
                 for (int t = 0; t < 2; ++t) {
-                    const int key = key0 + 16 * t + 4 * j4;
-                    float* to = p.raw + ((int64_t)b * p.H + h0 + m) * p.raw_ld + key;
+                    const int at = key0 - base + 16 * t + 4 * j4;
+                    float* to = p.raw + ((int64_t)b * p.H + h0 + m) * p.raw_ld + at;
                     const f32x4v y = {w[4 * t] * back, w[4 * t + 1] * back, w[4 * t + 2] * back, w[4 * t + 3] * back};
-                    if (key < p.raw_ld) *reinterpret_cast<f32x4v*>(to) = y;  // raw_ld: a multiple of 32
+                    if (at < p.raw_ld) *reinterpret_cast<f32x4v*>(to) = y;  // raw_ld: a multiple of 32
                 }
             }
         }
@@ -420,7 +423,7 @@ struct PagedParts {
     const float* at;
     int n;
     __device__ __forceinline__ PagedParts(const PagedArgs& p, const PagedSpan& sp, int64_t bh)
-        : at(p.part + bh * p.nsplit * (p.D + 4)), n(max(1, (sp.n - (sp.first & ~31) + p.chunk - 1) / p.chunk)) {}
+        : at(p.part + bh * p.nsplit * (p.D + 4)), n(max(1, (sp.n - paged_base(sp) + p.chunk - 1) / p.chunk)) {}
 };
 // Splits joined in a fixed order: one workgroup per (sequence, head), `ncol`
 // threads over the columns, 256 / ncol groups of them over the splits.
@@ -435,7 +438,7 @@ __global__ __launch_bounds__(256) void born_paged_join_kernel(PagedArgs p, int n
     if (WEIGH && (int)blockIdx.x >= p.B * p.H) {
         const int x = blockIdx.x - p.B * p.H, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
         const PagedSpan sp = paged_span(p, b);
-        const int j0 = (sp.first & ~31) + block * 256, j = j0 + threadIdx.x;
+        const int j0 = paged_base(sp) + block * 256, j = j0 + threadIdx.x;
         if (j0 >= sp.n) return;
         const bool seen = j >= sp.first && j < sp.n && j < p.w_len;
         float sum = 0.f;
@@ -450,7 +453,7 @@ __global__ __launch_bounds__(256) void born_paged_join_kernel(PagedArgs p, int n
             }
             __syncthreads();
             if (seen) {
-                const float* raw = p.raw + ((int64_t)b * p.H + h0) * p.raw_ld + j;
+                const float* raw = p.raw + ((int64_t)b * p.H + h0) * p.raw_ld + (j - paged_base(sp));
 #pragma unroll 4
                 for (int i = 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
             }
@@ -518,8 +521,7 @@ hipError_t launch_paged(const PagedArgs& a, hipStream_t st) {
     while (4 * ncol < a.D) ncol *= 2;
     const unsigned join = (unsigned)(a.B * a.H);
     if (a.raw != nullptr) {
-        const int64_t span = a.window > 0 && a.window + 32 < a.raw_ld ? a.window + 32 : a.raw_ld;
-        const unsigned weigh = (unsigned)((span + 255) / 256 * a.B * a.Hkv);
+        const unsigned weigh = (unsigned)((a.raw_ld + 255) / 256 * a.B * a.Hkv);
         hipLaunchKernelGGL((born_paged_join_kernel<E, true>), dim3(join + weigh), dim3(256), 0, st, a, ncol);
     } else {
         hipLaunchKernelGGL((born_paged_join_kernel<E, false>), dim3(join), dim3(256), 0, st, a, ncol);

@@ -152,7 +152,7 @@ PagedPlan paged_plan(int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t page
     if (chunk > 1024) chunk = 1024;
     r.chunk = chunk;
     r.nsplit = (span + chunk - 1) / chunk;
-    r.raw_ld = (room + 31) / 32 * 32;
+    r.raw_ld = (span + 31) / 32 * 32;
     if (r.nsplit > 1 || weigh) r.part_bytes = B * H * r.nsplit * (D + 4) * 4;
     if (weigh) r.raw_bytes = B * H * r.raw_ld * 4;
     return r;
