@@ -27,11 +27,10 @@ import torch
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
-from .flash_born_packed import _int32, _is_dual
+from .flash_born_packed import _LIMIT, _int32, _is_dual
 
 __all__ = ["born_cache_evict", "flash_born_attention_paged", "fused_qk_rope_l2_normalize_append"]
 
-_LIMIT = 1 << 30
 _INDEX = (torch.int32, torch.int64)
 
 

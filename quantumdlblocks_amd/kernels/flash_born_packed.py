@@ -31,6 +31,8 @@ from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _aligned, _apply, _autocast_d
 
 __all__ = ["flash_born_attention_packed"]
 
+_LIMIT = 1 << 30  # positions, windows
+
 
 def _token_rows(t: torch.Tensor, dtype: torch.dtype, dp: int):
     """``t`` (N, heads, D) in ``dtype``, zero-padded to ``dp`` columns, and its
@@ -304,7 +306,7 @@ def flash_born_attention_packed(
         cu_seqlens_k = cu_seqlens_q
     n_scale = scale.numel() if isinstance(scale, torch.Tensor) else 1
     _check(q, k, v, n_scale, cu_seqlens_q, cu_seqlens_k)
-    window = max(int(window_size), 0)
+    window = min(max(int(window_size), 0), _LIMIT)
     if not float(eps) >= 0.0:
         raise ValueError(f"eps must be at least 0, got {eps}")
     if q.is_cuda and q.shape[2] <= MAX_HEAD_DIM:

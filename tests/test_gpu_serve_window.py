@@ -3,11 +3,13 @@ the raw weights' workspace spans the window only."""
 
 from __future__ import annotations
 
+import sys
+
 import pytest
 import torch
 
 import serve_ref as ref
-from quantumdlblocks_amd import flash_born_attention_paged
+from quantumdlblocks_amd import flash_born_attention_packed, flash_born_attention_paged
 from test_cache import make_cache
 
 pytestmark = pytest.mark.gpu
@@ -32,3 +34,12 @@ def test_weights_of_a_window(cuda_device, dtype, window, page, H, Hkv):
     assert ref.worst(weight, (x, e)) <= 1.0
     for b, m in enumerate(lens):  # nothing is added outside the windows
         assert (weight[b, :, : max(0, m - window)] == 0.5).all() and (weight[b, :, m:] == 0.5).all()
+
+
+def test_packed_windows_past_every_key(cuda_device):
+    g = torch.Generator().manual_seed(27)
+    q, k, v = (torch.randn(90, h, 64, generator=g).to(device=cuda_device, dtype=torch.bfloat16) for h in (4, 2, 2))
+    cu = torch.tensor([0, 20, 90], dtype=torch.int32, device=cuda_device)
+    want = flash_born_attention_packed(q, k, v, 1.0, cu)
+    for window in (90, 1 << 30, 1 << 31, sys.maxsize):
+        assert torch.equal(flash_born_attention_packed(q, k, v, 1.0, cu, window_size=window), want)
