@@ -49,6 +49,7 @@
 
 #include "born_common.h"
 #include "born_fwd_fast.h"
+#include "packed_mask.h"
 
 namespace qdl {
 
@@ -104,7 +105,7 @@ __device__ __forceinline__ PackedSeq packed_seq(const PackedArgs& p, int x) {
     const int N = KEYS ? p.Nk : p.Nq, lane = threadIdx.x & 63;
     PackedSeq r;
     int s;
-    if (p.S < 64 && p.lower == 0 && p.upper == 1 << 30) {
+    if (p.S < 64 && p.lower == 0 && p.upper == kPackedFar) {
         const int a = lane <= p.S ? packed_start(cu, lane, N) : 0;
         const int e = lane < p.S ? max(packed_start(cu, lane + 1, N), a) : lane == p.S ? N : 0;
         const int tiles = (e - a + BM - 1) / BM;
@@ -488,10 +489,11 @@ struct PackedQueries {
     }
     // Zeroes a lane's overlaps with keys that its row does not see.
     __device__ __forceinline__ void mask(const PackedArgs& p, f32x16& s, int key0) const {
-        const int d = row + off - key0 - p.lower, span = p.upper - p.lower;
+        const int d = row + off - key0 - p.lower;
+        const uint32_t span = packed_span(p.lower, p.upper);
 #pragma unroll
         for (int r = 0; r < 16; ++r)
-            if ((uint32_t)(d - acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+            if ((uint32_t)(d - acc_row(r, g)) >= span) s[r] = 0.f;
     }
 };
 
@@ -810,7 +812,7 @@ void born_packed_dkdv_kernel(PackedArgs p) {
         if constexpr (DV) dv[db] = zero16();
     }
     float f = std::is_same<E, F16>::value ? kF16Start : 1.f;
-    const int span = p.upper - p.lower;
+    const uint32_t span = packed_span(p.lower, p.upper);
 
     // Row values r0 + 8 j + 4 g + e.
     auto values = [&](const float* x, int r0) __attribute__((always_inline)) {
@@ -830,7 +832,7 @@ void born_packed_dkdv_kernel(PackedArgs p) {
             const int d = i0 + r0 + off - key - p.lower;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if ((uint32_t)(d + acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+                if ((uint32_t)(d + acc_row(r, g)) >= span) s[r] = 0.f;
         }
         const f32x16 zi = values(stats[st][1], r0);
         float u[16];
@@ -993,7 +995,7 @@ void born_packed_dkdv8_kernel(PackedArgs p) {
 #pragma unroll
     for (int db = 0; db < DB; ++db) dk[db] = zero16(), dv[db] = zero16();
     float f = std::is_same<E, F16>::value ? kF16Start : 1.f;
-    const int span = p.upper - p.lower;
+    const uint32_t span = packed_span(p.lower, p.upper);
 
     auto tile = [&](int t, int st, auto kind) __attribute__((always_inline)) {
         const Tile q{ring + st * STAGE}, d{ring + st * STAGE + Tile::BYTES};
@@ -1013,7 +1015,7 @@ void born_packed_dkdv8_kernel(PackedArgs p) {
             const int x = (t0 + t) * BN + r0 + off - key - p.lower;
 #pragma unroll
             for (int r = 0; r < 16; ++r)
-                if ((uint32_t)(x + acc_row(r, g)) >= (uint32_t)span) s[r] = 0.f;
+                if ((uint32_t)(x + acc_row(r, g)) >= span) s[r] = 0.f;
         }
         PackedWeights<E> w, x;
         float uu[16];

@@ -79,7 +79,6 @@ int check_packed(const qdl_born_packed_call* c) {
 
 qdl::PackedArgs packed_args(const qdl_born_packed_call* c) {
     const int64_t it = item(c->dtype);
-    constexpr int kFar = 1 << 30;
     qdl::PackedArgs a = {};
     a.q = c->q;
     a.k = c->k;
@@ -102,8 +101,8 @@ qdl::PackedArgs packed_args(const qdl_born_packed_call* c) {
     a.Hkv = (int)c->h_kv;
     a.G = (int)(c->H / c->h_kv);
     a.D = (int)c->D;
-    a.lower = c->is_causal ? 0 : -kFar;
-    a.upper = c->window_size > 0 ? (int)c->window_size : kFar;
+    a.lower = qdl::packed_lower(c->is_causal != 0);
+    a.upper = qdl::packed_upper(c->window_size);
     a.head_splits = 1;
     a.eps = (float)c->eps;
     a.q_st = c->q_strides[0] * it;

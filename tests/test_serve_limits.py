@@ -2,8 +2,12 @@
 
 from __future__ import annotations
 
+import os
+import shutil
+import subprocess
 import sys
 
+import pytest
 import torch
 
 from quantumdlblocks_amd import _native, flash_born_attention_packed
@@ -26,3 +30,30 @@ def test_windows_past_every_key_are_cut(monkeypatch):
     for window in (sys.maxsize, 1 << 31, (1 << 30) + 1, 1 << 30, 5, -1):
         flash_born_attention_packed(x, x, x, 1.0, torch.tensor([0, 3]), window_size=window)
     assert seen == [1 << 30] * 4 + [5, 0]
+
+
+MASK = """
+#include <initializer_list>
+#include "%s"
+using namespace qdl;
+// In a constant expression an overflow of a signed sum is a compile error.
+constexpr bool agree(bool causal, int64_t window) {
+    const int lower = packed_lower(causal), upper = packed_upper(window);
+    const uint32_t span = packed_span(lower, upper);
+    // The farthest positions of 2^28 queries and keys, and those next to the bounds.
+    for (int lag : {-(1 << 29), -1, 0, 1, 99, 100, 101, (1 << 29)})
+        if (((uint32_t)(lag - lower) < span) != ((!causal || lag >= 0) && (window <= 0 || lag < window))) return false;
+    return true;
+}
+static_assert(agree(false, 0) && agree(true, 0) && agree(false, 100) && agree(true, 100) && agree(false, 1 << 30) && agree(true, 1 << 30), "mask");
+static_assert(packed_span(packed_lower(false), packed_upper(0)) == 0x80000000u, "both bounds far away");
+int main() {}
+""" % os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "quantumdlblocks_amd", "csrc", "packed_mask.h")
+
+
+def test_the_masks_span_does_not_overflow(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    (tmp_path / "mask.cpp").write_text(MASK)
+    subprocess.run([gxx, "-std=c++17", "-fsyntax-only", str(tmp_path / "mask.cpp")], check=True)
