@@ -29,7 +29,7 @@ int check_heads(int64_t dtype, int64_t H, int64_t h_kv, int64_t D) {
 }
 
 // Strides in elements: whole 16-byte pieces; a token's rows may not overlap.
-bool stride_ok(int64_t s, int64_t it) { return s >= 0 && s * it % 16 == 0 && s <= (int64_t)1 << 40; }
+bool stride_ok(int64_t s, int64_t it) { return s >= 0 && s <= (int64_t)1 << 40 && s * it % 16 == 0; }
 bool rows_ok(const int64_t st[2], int64_t it, int64_t D) {
     return stride_ok(st[0], it) && stride_ok(st[1], it) && st[0] >= D && st[0] * it < (int64_t)1 << 24;
 }
@@ -40,7 +40,7 @@ int check_cache(int64_t dtype, const int64_t ks[3], const int64_t vs[3], int64_t
     for (int i = 0; i < 3; ++i)
         if (!stride_ok(ks[i], it) || !stride_ok(vs[i], it)) return QDL_BORN_E_STRIDE;
     if (page < 1 || page > (int64_t)1 << 24 || cache_pages < 0 || cache_pages > INT32_MAX || pages < 0 || table_ld < pages ||
-        pages * page > (int64_t)1 << 30)
+        pages > (int64_t)1 << 30 || pages * page > (int64_t)1 << 30)
         return QDL_BORN_E_PAGE;
     if ((pages > 0 && !table) || (cache_pages > 0 && (!k || !v))) return QDL_BORN_E_NULL;
     if (!aligned16(k) || !aligned16(v)) return QDL_BORN_E_ALIGN;

@@ -12,6 +12,7 @@ import torch
 
 from quantumdlblocks_amd import _native, flash_born_attention_packed
 from quantumdlblocks_amd.kernels import flash_born_packed as packed
+from test_cache import _append_block, _evict_block, _paged_block
 
 
 def test_a_windows_workspace_does_not_grow_with_the_table():
@@ -57,3 +58,14 @@ def test_the_masks_span_does_not_overflow(tmp_path):
         pytest.skip("no host compiler")
     (tmp_path / "mask.cpp").write_text(MASK)
     subprocess.run([gxx, "-std=c++17", "-fsyntax-only", str(tmp_path / "mask.cpp")], check=True)
+
+
+@pytest.mark.parametrize("pages,page", [(1 << 40, 1 << 24), (1 << 62, 4), ((1 << 63) - 1, 2), ((1 << 30) + 1, 1)])
+def test_tables_whose_keys_leave_64_bits(pages, page):
+    # The product that is checked wraps to a small number.
+    lib = _native.load()
+    over = dict(pages=pages, page=page, ld=(1 << 63) - 1)
+    assert lib.qdl_flash_born_paged_forward_call(_paged_block(**over, ws_bytes=1 << 60), None) == -15
+    assert lib.qdl_flash_born_cache_append_call(_append_block(**over), None) == -15
+    assert lib.qdl_flash_born_cache_evict_call(_evict_block(**over), None) == -15
+    assert lib.qdl_flash_born_paged_workspace_size(2, 4, 2, 64, pages, page, 0, 1) == 0
