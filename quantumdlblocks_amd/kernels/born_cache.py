@@ -27,7 +27,7 @@ import torch
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
-from .flash_born_packed import _LIMIT, _int32, _is_dual
+from .flash_born_packed import _LIMIT, _call_uncompiled, _int32, _is_dual
 
 __all__ = ["born_cache_evict", "flash_born_attention_paged", "fused_qk_rope_l2_normalize_append"]
 
@@ -198,6 +198,9 @@ def flash_born_attention_paged(
     keys gets zeros, and so does a head whose (sum p + eps) / scale_h ** 2 lies
     below fp32's normal range, 2^-126.
     """
+    if torch.compiler.is_compiling():  # one graph break, as the other operators
+        return _call_uncompiled(flash_born_attention_paged, (q, k_cache, v_cache, block_table, cache_lens, scale, eps, window_size,
+                                                             key_weight))
     _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
     if q.dim() != 3:
         raise ValueError(f"q must be (B, heads, head_dim), got shape {tuple(q.shape)}")
@@ -350,6 +353,9 @@ def fused_qk_rope_l2_normalize_append(
     16 bits as the reference does.  Values that no sequence owns come out as
     zero queries; slots without a page are not written.
     """
+    if torch.compiler.is_compiling():  # one graph break, as the other operators
+        return _call_uncompiled(fused_qk_rope_l2_normalize_append, (q, k, v, cos, sin, k_cache, v_cache, block_table, cache_lens,
+                                                                    cu_seqlens, positions, eps))
     _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, cos, sin, k_cache, v_cache)
     kshape = k.shape
     if q.dim() != 3 or len(kshape) != 3 or kshape != v.shape or kshape[0] != q.shape[0] or kshape[2] != q.shape[2]:
@@ -473,6 +479,9 @@ def born_cache_evict(
     behind the last.  Keys stay rotated by the positions that they were appended
     at: pass ``positions`` to the next append.
     """
+    if torch.compiler.is_compiling():  # one graph break, as the other operators
+        return _call_uncompiled(born_cache_evict, (k_cache, v_cache, block_table, cache_lens, key_weight, budget, recent,
+                                                   out_block_table))
     _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
     strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
