@@ -43,6 +43,11 @@ def _no_grad(what: str, *tensors) -> None:
         raise RuntimeError(f"{what} has no forward-mode derivative: call it with the tensors' primals")
 
 
+def _written(*tensors) -> None:
+    """Counts a kernel's writes for autograd, as torch's in-place operations do."""
+    torch.autograd.graph.increment_version(tensors)
+
+
 def _bad_cache(name: str, c: torch.Tensor):
     return ValueError(f"{name} needs unit stride along head_dim, other strides that are multiples of 16 bytes and a 16-byte "
                       f"aligned base, got strides {c.stride()}")
@@ -248,6 +253,8 @@ def flash_born_attention_paged(
         _DTYPE_CODE[dt], B, H, Hkv, D, q_c.data_ptr(), sb, sh, out.data_ptr(), k_cache.data_ptr(), v_cache.data_ptr(), *strides,
         P, page, table.data_ptr(), pages, ld, lens.data_ptr(), scale_p, n_scale, scale_value, window, eps, w_ptr, w_sb, w_sh, w_len,
         0 if ws is None else ws.data_ptr(), size))
+    if key_weight is not None:
+        _written(key_weight)
     return out
 
 
@@ -411,6 +418,7 @@ def fused_qk_rope_l2_normalize_append(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
         k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(), table.shape[1], ld, lens.data_ptr(),
         0 if cu is None else cu.data_ptr(), *rot, 0 if pos is None else pos.data_ptr(), eps))
+    _written(k_cache, v_cache)
     return out
 
 
@@ -524,4 +532,5 @@ def born_cache_evict(
         table.shape[1], ld, lens.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1), wshape[2], budget, recent,
         0 if to is None else to.data_ptr(), 0 if to is None else to.shape[1], to_ld,
         weight.data_ptr(), new_lens.data_ptr(), kept.data_ptr()))
+    _written(k_cache, v_cache)
     return new_lens, weight, kept
