@@ -53,9 +53,11 @@ def _bad_cache(name: str, c: torch.Tensor):
                       f"aligned base, got strides {c.stride()}")
 
 
-def _check_cache(k_cache, v_cache, block_table, cache_lens, B, written: bool):
-    """The caches' (page, token, head) strides on the GPU.  Decoding calls this
-    for every layer and token: plain tests in a row, no loops over tensors."""
+def _check_cache(k_cache, v_cache, block_table, cache_lens, B, written: bool, apart: bool = False):
+    """The caches' (page, token, head) strides on the GPU.  ``apart``: the two
+    are written each for itself, so that one row may not be of both.  Decoding
+    calls this for every layer and token: plain tests in a row, no loops over
+    tensors."""
     shape, dt = k_cache.shape, k_cache.dtype
     if len(shape) != 4 or shape != v_cache.shape or v_cache.dtype != dt:
         raise ValueError(f"k_cache and v_cache must share one (pages, page_size, key_heads, head_dim) shape and dtype, got "
@@ -79,6 +81,8 @@ def _check_cache(k_cache, v_cache, block_table, cache_lens, B, written: bool):
         for name, st in (("k_cache", ks), ("v_cache", vs)):
             if (st[0] == 0 and P > 1) or (st[1] == 0 and page > 1) or (st[2] == 0 and Hkv > 1) or (st[3] == 0 and D > 1):
                 raise ValueError(f"{name} is written and must not overlap itself, got strides {st}")
+    if apart and P and k_cache.data_ptr() == v_cache.data_ptr():
+        raise ValueError("k_cache and v_cache are both written and must not share memory")
     if dev < 0:
         return ()
     if D % 8 or D > MAX_HEAD_DIM or dt not in _DTYPE_CODE:
@@ -370,7 +374,7 @@ def fused_qk_rope_l2_normalize_append(
                          f"{tuple(kshape)}, {tuple(v.shape)}")
     N, H, D = q.shape
     B = block_table.shape[0] if block_table.dim() == 2 else -1
-    strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
+    strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True, apart=True)
     P, page, Hkv, Dk = k_cache.shape
     if Dk != D or kshape[1] != Hkv or H < 1 or H % Hkv or D % 2:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(kshape)} do not fit caches of {Hkv} key heads of {Dk}, or "
@@ -492,7 +496,7 @@ def born_cache_evict(
                                                    out_block_table))
     _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
-    strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True)
+    strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True, apart=out_block_table is None)
     P, page, Hkv, D = k_cache.shape
     dev, at = k_cache.device, k_cache.get_device()
     budget, recent = int(budget), int(recent)

@@ -10,7 +10,13 @@ import sys
 import pytest
 import torch
 
-from quantumdlblocks_amd import _native, flash_born_attention_packed
+from quantumdlblocks_amd import (
+    _native,
+    born_cache_evict,
+    flash_born_attention_packed,
+    flash_born_attention_paged,
+    fused_qk_rope_l2_normalize_append,
+)
 from quantumdlblocks_amd.kernels import flash_born_packed as packed
 from test_cache import _append_block, _evict_block, _paged_block
 
@@ -69,3 +75,21 @@ def test_tables_whose_keys_leave_64_bits(pages, page):
     assert lib.qdl_flash_born_cache_append_call(_append_block(**over), None) == -15
     assert lib.qdl_flash_born_cache_evict_call(_evict_block(**over), None) == -15
     assert lib.qdl_flash_born_paged_workspace_size(2, 4, 2, 64, pages, page, 0, 1) == 0
+
+
+def test_one_tensor_as_both_caches():
+    # Read and moved to other pages it may be both; two writers of one row it may not.
+    c = torch.rand(6, 4, 1, 8)
+    table, lens, to = torch.tensor([[0, 1]], dtype=torch.int32), torch.tensor([6], dtype=torch.int32), torch.tensor([[3]], dtype=torch.int32)
+    x, w = torch.rand(1, 1, 8), torch.rand(1, 1, 8)
+    flash_born_attention_paged(x, c, c, table, lens, 1.0)
+    before = c.clone()
+    with pytest.raises(ValueError, match="share"):
+        fused_qk_rope_l2_normalize_append(x, x, 2 * x, None, None, c, c, table, lens)
+    with pytest.raises(ValueError, match="share"):
+        born_cache_evict(c, c, table, lens, w, 3)
+    assert torch.equal(c, before)
+    _, _, kept = born_cache_evict(c, c, table, lens, w, 3, 0, to)
+    assert torch.equal(c[3, :3], before[:2].flatten(0, 1)[kept[0, 0].long()])
+    none = torch.rand(0, 4, 1, 8)  # nothing to share
+    fused_qk_rope_l2_normalize_append(x, x, x, None, None, none, none, table, lens)
