@@ -20,9 +20,12 @@
 // leave the registers: the two 16-key products' C layout is the B operand of
 // the 32-key one in the key order that the V loads use.
 //
-// The weights are rounded once to 16 bits, as that product's operand; the
-// denominator and the raw weights for key_weight take them in fp32.  Splits are
-// written and joined in fp32.
+// No weight is rounded to 16 bits: its 16-bit form and that of what is left of it
+// are two products with the same operand of V, which costs nothing beside the
+// loads (us with one product and with two, by graph replay: bf16 64 sequences of
+// 1024 keys, 8 key heads, D128 66.2 and 66.5; 16 of 4096, D256 115.9 and 116.3;
+// 32 heads a key head, D64 35.4 and 35.7).  The denominator and the raw weights
+// for key_weight take them in fp32; splits are written and joined in fp32.
 //
 // bf16, 32 sequences of 2048 to 14622 keys, 8 key heads D128: 808 MB in 163 us
 // (5.0 TB/s) and a join of 5; one sequence of 1531 keys: 5.4 us and 3.5.
@@ -55,7 +58,7 @@ struct PagedArgs {
     int gblocks;           // 16-head blocks of a group
     float eps;
     int64_t q_sb, q_sh, kp, kt, kh, vp, vt, vh;  // bytes
-    float* part;           // (B, H, nsplit, D + 1): numerators, denominator; or nullptr (one split)
+    float* part;           // (B, H, nsplit, D + 4): denominator, three unused, numerators; or nullptr (one split)
     float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
     int64_t w_sb, w_sh;    // elements
     int w_len;             // columns of weights
@@ -348,16 +351,21 @@ void born_paged_kernel(PagedArgs p) {
                         acc[vb * VC + e] = mfma16_f32(__uint_as_float(x.v[vb][i][e]), w[i], acc[vb * VC + e]);
             }
         } else {
-            u32x4 pk;
+            // In two 16-bit parts, so that only the output is rounded.
+            u32x4 hi, lo;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                pk[i] = E::pack(w[2 * i], w[2 * i + 1]);  // the product's operand; the sum takes them as they are
+                hi[i] = E::pack(w[2 * i], w[2 * i + 1]);
+                lo[i] = E::pack(w[2 * i] - E::lo(hi[i]), w[2 * i + 1] - E::hi(hi[i]));
                 z = (z + w[2 * i]) + w[2 * i + 1];
             }
 #pragma unroll
             for (int vb = 0; vb < VB; ++vb)
 #pragma unroll
-                for (int e = 0; e < VC; ++e) acc[vb * VC + e] = mfma16<E>(paged_column(x.v[vb], e), pk, acc[vb * VC + e]);
+                for (int e = 0; e < VC; ++e) {
+                    const u32x4 a = paged_column(x.v[vb], e);
+                    acc[vb * VC + e] = mfma16<E>(a, lo, mfma16<E>(a, hi, acc[vb * VC + e]));
+                }
         }
     };
     const int step = 32 * NW, key0 = s0 + 32 * wave;
