@@ -24,6 +24,8 @@ from __future__ import annotations
 import functools
 
 import torch
+from torch.autograd import forward_ad
+from torch.autograd.graph import increment_version as _written  # counts a kernel's writes, as torch's in-place operations do
 
 from .. import _native
 from .flash_born import _DTYPE_CODE, MAX_HEAD_DIM, _parameter, _run_call
@@ -39,13 +41,8 @@ def _no_grad(what: str, *tensors) -> None:
         for t in tensors:
             if isinstance(t, torch.Tensor) and t.requires_grad:
                 raise RuntimeError(f"{what} has no backward: call it under torch.no_grad(), or with detached tensors")
-    if _is_dual(*tensors):
+    if forward_ad._current_level >= 0 and _is_dual(*tensors):
         raise RuntimeError(f"{what} has no forward-mode derivative: call it with the tensors' primals")
-
-
-def _written(*tensors) -> None:
-    """Counts a kernel's writes for autograd, as torch's in-place operations do."""
-    torch.autograd.graph.increment_version(tensors)
 
 
 def _bad_cache(name: str, c: torch.Tensor):
@@ -196,7 +193,8 @@ def flash_born_attention_paged(
 
     ``q`` (B, H, D), H a multiple of the caches' Hkv.  The token is the last of
     its sequence's ``cache_lens`` keys (its own key is in the cache already) and
-    sees all of them, or the last ``window_size``:
+    sees all of them, or the last ``window_size``, counted in slots: after an
+    eviction these reach back farther than as many positions.  The formula:
 
         p_j = max(0, scale_h q . k_j) ** 2,  out = sum_j p_j v_j / (sum_j p_j + eps)
 
@@ -210,7 +208,8 @@ def flash_born_attention_paged(
     if torch.compiler.is_compiling():  # one graph break, as the other operators
         return _call_uncompiled(flash_born_attention_paged, (q, k_cache, v_cache, block_table, cache_lens, scale, eps, window_size,
                                                              key_weight))
-    _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        _no_grad("flash_born_attention_paged", q, k_cache, v_cache, scale, key_weight)
     if q.dim() != 3:
         raise ValueError(f"q must be (B, heads, head_dim), got shape {tuple(q.shape)}")
     B, H, D = q.shape
@@ -245,7 +244,7 @@ def flash_born_attention_paged(
         return _eager_paged(q.detach(), k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight)
     lib = _native.load()
     dt = k_cache.dtype
-    out = torch.empty((B, H, D), dtype=dt, device=dev)
+    out = k_cache.new_empty((B, H, D))
     if B == 0:
         return out
     q_c, sb, sh = _heads(q, dt)
@@ -258,7 +257,7 @@ def flash_born_attention_paged(
         P, page, table.data_ptr(), pages, ld, lens.data_ptr(), scale_p, n_scale, scale_value, window, eps, w_ptr, w_sb, w_sh, w_len,
         0 if ws is None else ws.data_ptr(), size))
     if key_weight is not None:
-        _written(key_weight)
+        _written((key_weight,))
     return out
 
 
@@ -367,7 +366,8 @@ def fused_qk_rope_l2_normalize_append(
     if torch.compiler.is_compiling():  # one graph break, as the other operators
         return _call_uncompiled(fused_qk_rope_l2_normalize_append, (q, k, v, cos, sin, k_cache, v_cache, block_table, cache_lens,
                                                                     cu_seqlens, positions, eps))
-    _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, cos, sin, k_cache, v_cache)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        _no_grad("fused_qk_rope_l2_normalize_append", q, k, v, cos, sin, k_cache, v_cache)
     kshape = k.shape
     if q.dim() != 3 or len(kshape) != 3 or kshape != v.shape or kshape[0] != q.shape[0] or kshape[2] != q.shape[2]:
         raise ValueError(f"q must be (N, heads, head_dim) and k, v (N, key_heads, head_dim), got {tuple(q.shape)}, "
@@ -403,7 +403,7 @@ def fused_qk_rope_l2_normalize_append(
                              positions, eps)
     lib = _native.load()
     dt = k_cache.dtype
-    out = torch.empty((N, H, D), dtype=dt, device=dev)
+    out = k_cache.new_empty((N, H, D))
     if N == 0:
         return out
     if B == 0:
@@ -422,7 +422,7 @@ def fused_qk_rope_l2_normalize_append(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
         k_cache.data_ptr(), v_cache.data_ptr(), *strides, P, page, table.data_ptr(), table.shape[1], ld, lens.data_ptr(),
         0 if cu is None else cu.data_ptr(), *rot, 0 if pos is None else pos.data_ptr(), eps))
-    _written(k_cache, v_cache)
+    _written((k_cache, v_cache))
     return out
 
 
@@ -494,7 +494,8 @@ def born_cache_evict(
     if torch.compiler.is_compiling():  # one graph break, as the other operators
         return _call_uncompiled(born_cache_evict, (k_cache, v_cache, block_table, cache_lens, key_weight, budget, recent,
                                                    out_block_table))
-    _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
+    if torch.is_grad_enabled() or forward_ad._current_level >= 0:
+        _no_grad("born_cache_evict", k_cache, v_cache, key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
     strides = _check_cache(k_cache, v_cache, block_table, cache_lens, B, written=True, apart=out_block_table is None)
     P, page, Hkv, D = k_cache.shape
@@ -526,9 +527,8 @@ def born_cache_evict(
         w = w.contiguous()
     (table, ld), lens = _table(block_table), _index(cache_lens)
     to, to_ld = (None, 0) if out_block_table is None else _table(out_block_table)
-    weight = torch.empty(wshape, dtype=torch.float32, device=dev)
-    new_lens = torch.empty(B, dtype=torch.int32, device=dev)
-    kept = torch.empty((B, Hkv, budget), dtype=torch.int32, device=dev)
+    weight = w.new_empty(wshape)
+    new_lens, kept = lens.new_empty(B), lens.new_empty((B, Hkv, budget))
     if B == 0:
         return new_lens, weight, kept
     _run_call(lib.qdl_flash_born_cache_evict_call, "qdl_flash_born_cache_evict_call", dev, _native.evict_call(
@@ -536,5 +536,5 @@ def born_cache_evict(
         table.shape[1], ld, lens.data_ptr(), w.data_ptr(), w.stride(0), w.stride(1), wshape[2], budget, recent,
         0 if to is None else to.data_ptr(), 0 if to is None else to.shape[1], to_ld,
         weight.data_ptr(), new_lens.data_ptr(), kept.data_ptr()))
-    _written(k_cache, v_cache)
+    _written((k_cache, v_cache))
     return new_lens, weight, kept

@@ -37,8 +37,8 @@ def _inputs(strided=False):
     return [t.requires_grad_() if not strided else t.detach().requires_grad_() for t in (q, k, v)]
 
 
-def _call(q, k, v, scale, cu):
-    return packed._FlashBornPackedFn.apply(q, k, v, scale, cu, cu, True, 1e-12, 0)
+def _call(q, k, v, scale, cu, cu_k=None):
+    return packed._FlashBornPackedFn.apply(q, k, v, scale, cu, cu if cu_k is None else cu_k, True, 1e-12, 0)
 
 
 @pytest.mark.parametrize("strided", [False, True])
@@ -52,7 +52,7 @@ def test_backward_takes_what_the_hooks_return(blocks, strided):
         return given[-1]
 
     with torch.autograd.graph.saved_tensors_hooks(lambda t: t.detach().clone(), unpack):
-        out = _call(*leaves, scale, cu)
+        out = _call(*leaves, scale, cu, cu.clone())
     torch.autograd.grad(out, leaves, torch.ones_like(out))
     forward, backward = blocks
     assert forward["what"].endswith("forward_call") and backward["what"].endswith("backward_call")

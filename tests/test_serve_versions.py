@@ -66,5 +66,5 @@ def test_inference_tensors_are_written(dev):
 def test_what_the_kernels_write_is_counted():
     a, b = torch.zeros(3), torch.zeros(3)
     before = a._version, b._version
-    born_cache._written(a, b)
+    born_cache._written((a, b))
     assert (a._version, b._version) == (before[0] + 1, before[1] + 1)
