@@ -223,8 +223,11 @@ __device__ __forceinline__ uint32_t evict_key(float x) {
 }
 
 // 1024 threads with PER weights each: what the launch waits for is the
-// instructions of one wave, so the caches' capacity picks the fewest (4 rows of
-// 2048 weights 6.8 us with 2 each, 128 rows of up to 10000 18.7 us with 16).
+// instructions of one wave, so the caches' capacity picks the fewest that hold a
+// row at once (4 rows of 2048 weights 6.8 us with 2 each, 128 rows of up to
+// 10000 18.7 us with 16).  The whole call to a budget of 64, us with 2, 4, 8 and
+// 16 each, 128 rows of 2048: 17.0, 17.2, 19.8, 24.0; of 4096: 20.0, 17.9, 20.1,
+// 24.2; of 8192: 27.0, 25.3, 21.9, 26.2; of 16384: 39.6, 36.6, 36.7, 29.2.
 constexpr int kEvictThreads = 1024, kEvictMost = 16;
 
 template <int PER>
@@ -441,7 +444,10 @@ __global__ __launch_bounds__(256) void born_evict_move_kernel(EvictArgs p) {
 // The kept rows to the front of their own pages.  Rows only move down and keep
 // their order, so one workgroup per (sequence, key head, K or V) walks them
 // upwards: a batch is read whole before any of it is written, and what it
-// writes lies below every row still to be read.
+// writes lies below every row still to be read.  Bound by that walk where there
+// are few of them: the call in place and to other pages, us: one cache of 16384
+// halved, 8 key heads D128 189 and 38; 16 cut to 4096, 193 and 143; 64 of 2048
+// halved, 4 key heads D64, 50 and 49.
 template <int>
 __global__ __launch_bounds__(1024) void born_evict_compact_kernel(EvictArgs p) {
     constexpr int U = 4;
