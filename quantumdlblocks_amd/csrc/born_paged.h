@@ -27,8 +27,8 @@
 // 32 heads a key head, D64 35.4 and 35.7).  The denominator and the raw weights
 // for key_weight take them in fp32; splits are written and joined in fp32.
 //
-// bf16, 32 sequences of 2048 to 14622 keys, 8 key heads D128: 808 MB in 163 us
-// (5.0 TB/s) and a join of 5; one sequence of 1531 keys: 5.4 us and 3.5.
+// bf16, 32 sequences of 2048 to 14622 keys, 8 key heads D128: 808 MB in 162 us
+// (5.0 TB/s) and a join of 5; one sequence of 1531 keys: 5.6 us and 2.9.
 #pragma once
 
 #include <type_traits>
