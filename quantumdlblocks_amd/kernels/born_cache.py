@@ -148,8 +148,12 @@ def _paged_workspace(*sizes) -> int:
     return int(_native.load().qdl_flash_born_paged_workspace_size(*sizes))
 
 
-@torch.autocast("cpu", enabled=False)
-def _eager_paged(q, k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight):
+def _eager_paged(*args):
+    with torch.autocast("cpu", enabled=False):  # not as a decorator, which is one object for all threads
+        return _paged_formula(*args)
+
+
+def _paged_formula(q, k_cache, v_cache, block_table, cache_lens, scale_t, eps, window, key_weight):
     B, H, D = q.shape
     P, page, Hkv, _ = k_cache.shape
     G, L = H // Hkv, block_table.shape[1] * page

@@ -243,11 +243,14 @@ def _on_gpu(q, k, v, scale, *rest):
     return _uncompiled(_forward, q, k, v, scale, *rest, False)[0]
 
 
-@torch.autocast("cpu", enabled=False)
-@torch.autocast("cuda", enabled=False)
 def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window, target):
     """The formulas in torch operations, in fp32 (fp64 for fp64 values) under
     autocast too, one sequence at a time; the output in ``target``."""
+    with torch.autocast(q.device.type, enabled=False):  # not as a decorator, which is one object for all threads
+        return _packed_formula(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window).to(target)
+
+
+def _packed_formula(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window):
     cq, ck = cu_q.tolist(), cu_k.tolist()
     for name, c, n in (("cu_seqlens_q", cq, q.shape[0]), ("cu_seqlens_k", ck, k.shape[0])):
         if c[0] != 0 or c[-1] > n or any(a > b for a, b in zip(c, c[1:])):
@@ -276,7 +279,7 @@ def _eager_packed(q, k, v, scale_t, cu_q, cu_k, is_causal, eps, window, target):
         w = p / torch.where(den > 0, den, torch.ones_like(den))
         outs.append(torch.matmul(w, vs).permute(2, 0, 1, 3).reshape(nq, H, q.shape[2]))
     outs.append(torch.zeros((q.shape[0] - cq[-1], H, v.shape[2]), dtype=wide, device=q.device))
-    return torch.cat(outs).to(target)
+    return torch.cat(outs)
 
 
 def flash_born_attention_packed(

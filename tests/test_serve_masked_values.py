@@ -3,10 +3,14 @@ autocast, and of batches without sequences."""
 
 from __future__ import annotations
 
+import threading
+
 import pytest
 import torch
 
 from quantumdlblocks_amd import flash_born_attention_packed, flash_born_attention_paged, fused_qk_rope_l2_normalize_append
+from quantumdlblocks_amd.kernels import born_cache
+from quantumdlblocks_amd.kernels import flash_born_packed as packed
 
 BAD = [float("nan"), float("inf"), -float("inf")]
 
@@ -89,3 +93,49 @@ def test_packed_batches_without_sequences_have_zero_gradients():
     assert not out.any()
     for x, g in zip(leaves, torch.autograd.grad(out.sum(), leaves)):
         assert g.shape == x.shape and not g.any()
+
+
+@pytest.mark.parametrize("op", ["packed", "paged"])
+def test_calls_from_two_threads_leave_each_its_autocast(op, monkeypatch):
+    # One call ends while the other, of a thread without autocast, is on its way.
+    inside, ended = threading.Event(), threading.Event()
+    state = {}
+    x = torch.rand(4, 2, 8)
+    kc, vc, table, lens = _cache((5,))
+
+    class Late(torch.Tensor):
+        """Starts, or lengths, that the call reads once it is on its way."""
+
+        @classmethod
+        def __torch_function__(cls, func, types, args=(), kwargs=None):
+            if func in (torch.Tensor.tolist, torch.Tensor.long):
+                if threading.current_thread().name == "outer":
+                    assert inside.wait(30)
+                else:
+                    inside.set()
+                    assert ended.wait(30)
+            return super().__torch_function__(func, types, args, kwargs or {})
+
+    def call():
+        if op == "packed":
+            cu = torch.tensor([0, 4]).as_subclass(Late)
+            packed._eager_packed(x, x[:, :1], x[:, :1], torch.tensor(1.0), cu, cu, True, 0.1, 0, x.dtype)
+        else:
+            born_cache._eager_paged(x[:1], kc, vc, table, lens.as_subclass(Late), torch.tensor(1.0), 0.1, 0, None)
+
+    def outer():
+        with torch.autocast("cpu", dtype=torch.bfloat16):
+            call()
+            state["outer"] = torch.is_autocast_enabled("cpu")
+        ended.set()
+
+    def inner():
+        call()
+        state["inner"] = torch.is_autocast_enabled("cpu")
+
+    threads = [threading.Thread(target=f, name=f.__name__) for f in (outer, inner)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join(60)
+    assert state == {"outer": True, "inner": False}
