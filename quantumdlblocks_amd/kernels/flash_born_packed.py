@@ -193,7 +193,9 @@ class _FlashBornPackedFn(torch.autograd.Function):
     def backward(ctx, do):
         lib = _native.load()
         q, k, v, out, z, scale_flat, cu_q, cu_k = ctx.saved_tensors
-        sizes, dt, dev = ctx.sizes, ctx.dtype, out.device
+        sizes, dt, dev = ctx.sizes, ctx.dtype, do.device
+        if q.device != dev or k.device != dev or v.device != dev or out.device != dev or z.device != dev:
+            q, k, v, out, z = (t.to(dev) for t in (q, k, v, out, z))  # a hook left them elsewhere
         _, _, N, M, H, Hkv, dp = sizes
         D = ctx.head_dim
         q, q0, q1 = _token_rows(q, dt, dp)

@@ -54,6 +54,7 @@ WAYS = {
     "checkpoint": lambda layer, leaf, s: checkpoint(layer, leaf, s, use_reentrant=False),
     "offload": _offloaded,
     "copies": _hooked(lambda t: t.detach().clone(), lambda t: t.clone()),
+    "on the host": _hooked(lambda t: t.cpu(), lambda t: t),
     "strides": _hooked(lambda t: t, lambda t: t.transpose(0, -1).contiguous().transpose(0, -1)),
 }
 

@@ -107,3 +107,15 @@ def test_without_hooks_nothing_is_copied(blocks):
     out.backward(torch.ones_like(out))
     forward, backward = blocks
     assert all(forward[n] == backward[n] for n in FIELDS[:27])
+
+
+def test_hooks_that_leave_a_tensor_elsewhere(blocks):
+    # The library takes addresses on its own device only: others are brought
+    # there, or, where there is nothing to bring, refused.
+    cu = torch.tensor([0, 7], dtype=torch.int32)
+    leaves = _inputs()
+    with torch.autograd.graph.saved_tensors_hooks(lambda t: t.to("meta"), lambda t: t):
+        out = _call(*leaves, 2.0, cu)
+    with pytest.raises((RuntimeError, NotImplementedError)):
+        torch.autograd.grad(out, leaves, torch.ones_like(out))
+    assert len(blocks) == 1
