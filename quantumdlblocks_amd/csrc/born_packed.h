@@ -16,17 +16,22 @@
 // Roundings.  Scores, sums, statistics and accumulators are fp32.  The 16-bit
 // matrix instructions take 16-bit operands, so the factor that a kernel forms
 // itself is rounded once before each second product: p (forward), p / Z (dV)
-// and u (dQ, dK), half a step each.  bf16's Z adds the rounded p, so numerator
-// and denominator carry the same error; fp16's adds them in fp32.  delta comes
-// from the output as it was rounded: O in fp32 would cost 2 N H D bytes more to
-// write and to read.  Against 64 bits the 16-bit dQ and dK are 1.8 to 2.6 times
-// as far off as gradients whose only rounding is the output's (in norm: bf16
-// 3.0e-3 to 4.2e-3 for 1.7e-3, fp16 4.0e-4 to 5.4e-4 for 2.1e-4), most in short
-// sequences, where delta's error weighs more.  A simulation in 64 bits, bf16
-// D64, sequences of 2048, 64 and 2 tokens: dQ 3.3e-3, 3.5e-3, 4.0e-3, with delta
-// from an unrounded O 3.0e-3, 3.1e-3, 3.1e-3, with exact statistics 2.6e-3,
-// 2.6e-3, 2.2e-3: what is left is u's rounding, which only a second product for
-// its remainder would take away.
+// and u (dQ, dK), half a step each.  Z adds the rounded p, so numerator and
+// denominator carry the same error: a row that one key takes whole is that key's
+// v, and its delta that key's dP.  (With fp16's p added unrounded such rows'
+// gradients were off by p's rounding over a small a: dQ of a batch of 6, 20 and 7
+// tokens 14 times as far off as its output's rounding, now 5.)  delta comes from
+// the output as it was rounded: an unrounded O would cost 2 N H D bytes more to
+// write and to read.  Against 64 bits the 16-bit dQ and dK are 1.9 and 1.5 times
+// as far off as gradients whose only rounding is the output's (in norm, medians
+// of 1228 drawn batches; bf16 3.2e-3 and 2.5e-3 for 1.7e-3), 2.1 and 1.8 times in
+// one of twenty, 5.8 and 4.4 times in the worst: short sequences, where a row
+// that one key takes nearly whole has dO . v - delta next to nothing there, and
+// delta's rounding is divided by a.  A simulation in 64 bits, bf16, with
+// everything, with delta from an unrounded O, with u in two parts, with both:
+// dQ of 1500 tokens D128 1.9, 1.7, 1.5, 1.2 times, of a batch of 33, 26, 8, 2 and
+// 4 tokens D32 2.3, 1.8, 2.0, 1.4; u in two parts would take a second product in
+// kernels that the matrix pipe bounds.
 // fp32 rounds nothing on the way (3.3e-7, plain fp32 4.8e-7).
 //
 // What bounds them: the matrix pipe.  A workgroup's four waves share the tiles
@@ -562,7 +567,11 @@ void born_packed_fwd_kernel(PackedArgs p) {
                     for (int db = 0; db < DB; ++db) acc[db] *= by;
                 }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) w.w[j] = born_weight_pair<F16>(s[2 * j], s[2 * j + 1], cf, z);
+                for (int j = 0; j < 8; ++j) {
+                    const float a0 = relu_f32(s[2 * j] * cf), a1 = relu_f32(s[2 * j + 1] * cf);
+                    w.w[j] = F16::pack(a0 * a0, a1 * a1);
+                    z = F16::sum2(w.w[j], z);
+                }
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) w.w[j] = born_weight_pair<BF16>(s[2 * j], s[2 * j + 1], 1.f, z);
