@@ -239,8 +239,9 @@ class _FlashBornPackedFn(torch.autograd.Function):
 
 def _on_gpu(q, k, v, scale, *rest):
     """Through the autograd function where a derivative is recorded; it refuses a forward-mode one."""
-    if (torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
-                                     or (isinstance(scale, torch.Tensor) and scale.requires_grad))) or (forward_ad._current_level >= 0 and _is_dual(q, k, v, scale)):
+    recorded = torch.is_grad_enabled() and (q.requires_grad or k.requires_grad or v.requires_grad
+                                            or (isinstance(scale, torch.Tensor) and scale.requires_grad))
+    if recorded or (forward_ad._current_level >= 0 and _is_dual(q, k, v, scale)):
         return _apply(_FlashBornPackedFn, q, k, v, scale, *rest)
     return _uncompiled(_forward, q, k, v, scale, *rest, False)[0]
 
