@@ -497,6 +497,111 @@ typedef struct qdl_born_evict_call {
 
 int qdl_flash_born_cache_evict_call(const qdl_born_evict_call *call, qdl_stream_t stream);
 
+/*
+ * A paged cache in 4 bits.  A row (one head of one token) holds W = 32 nb
+ * columns, D rounded up to whole blocks of 32: 16 nb bytes of codes (the lower
+ * nibble is the even column; sign, two exponent bits, one mantissa bit: 0, .5,
+ * 1, 1.5, 2, 3, 4, 6) and nb scale bytes e; a value is its code times 2^(e - 127),
+ * e = 255: not a number.  k, v: cache_pages pages of page_size tokens of h_kv
+ * heads; *_strides (page, token, head) in bytes, the codes' multiples of 16, and
+ * unit strides within a row.  Pages, tables and lengths as above.
+ */
+typedef struct qdl_born_fp4_cache {
+    void *k, *v, *k_scale, *v_scale;
+    int64_t k_strides[3], v_strides[3], k_scale_strides[3], v_scale_strides[3];
+    int64_t cache_pages, page_size;
+    const int32_t *block_table;
+    int64_t pages, table_ld;
+    const int32_t *cache_lens;
+} qdl_born_fp4_cache;
+
+/*
+ * Append, as qdl_flash_born_cache_append_call, the keys and values stored in 4
+ * bits: e is the least with max |x| <= 7 2^(e - 127) over the block, at least 1,
+ * the codes are nearest, halfway to even, at most 6; blocks with an infinity or
+ * NaN get e = 255.  Keys are rotated and normalised in 64 bits, queries in fp32.
+ */
+typedef struct qdl_born_fp4_append_call {
+    int64_t struct_bytes;
+    int64_t dtype, n, B, H, h_kv, D;
+    const void *q, *k, *v;
+    int64_t q_strides[2], k_strides[2], v_strides[2];
+    void *q_out;
+    qdl_born_fp4_cache cache;
+    const int32_t *cu_seqlens;
+    const float *cos_table, *sin_table;
+    int64_t table_rows, n_freq, freq_ld;
+    const int32_t *positions;
+    double eps;
+} qdl_born_fp4_append_call;
+
+int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call *call, qdl_stream_t stream);
+
+/*
+ * Read: the values of n rows of a packed batch, k_out and v_out (n, h_kv, D)
+ * contiguous.  Rows cu_seqlens[s] .. cu_seqlens[s+1] - 1 are the last keys of
+ * sequence s; rows of no sequence, and of missing pages, are zeros.
+ */
+typedef struct qdl_born_fp4_read_call {
+    int64_t struct_bytes;
+    int64_t dtype, n, B, h_kv, D;
+    void *k_out, *v_out;
+    qdl_born_fp4_cache cache;
+    const int32_t *cu_seqlens;
+} qdl_born_fp4_read_call;
+
+int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call *call, qdl_stream_t stream);
+
+/*
+ * Attention over the cache: q (n, H, D) with strides (token, head), out (n, H,
+ * D) contiguous, both of dtype.  cu_seqlens: B + 1 starts of the sequences'
+ * tokens, or NULL: one each (n == B).  A sequence's tokens stand at the last of
+ * its keys: its i-th of m is at position cache_lens - m + i and sees the keys up
+ * to there, or the last window_size of them.  Tokens that see no key, and those
+ * of no sequence, get zeros; a key with a block of e = 255 makes NaN of every
+ * row that sees it.  The workspace's size is the size function's for the same
+ * sizes (packed: cu_seqlens != NULL; weighed: key_weight != NULL).
+ * key_weight, only where cu_seqlens is NULL: as for qdl_flash_born_paged_forward_call.
+ */
+typedef struct qdl_born_fp4_paged_call {
+    int64_t struct_bytes;
+    int64_t dtype, n, B, H, h_kv, D;
+    const void *q;
+    int64_t q_strides[2];
+    void *out;
+    qdl_born_fp4_cache cache;
+    const int32_t *cu_seqlens;
+    const float *scale;
+    int64_t n_scale;
+    double scale_value;
+    int64_t window_size;
+    double eps;
+    float *key_weight;
+    int64_t weight_strides[2], weight_len;
+    void *workspace;
+    int64_t workspace_bytes;
+} qdl_born_fp4_paged_call;
+
+int64_t qdl_flash_born_fp4_paged_workspace_size(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages,
+                                                int64_t page_size, int64_t window_size, int packed, int weighed);
+int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call *call, qdl_stream_t stream);
+
+/* Evict, as qdl_flash_born_cache_evict_call.  A row kept from a missing page arrives as zeros. */
+typedef struct qdl_born_fp4_evict_call {
+    int64_t struct_bytes;
+    int64_t B, h_kv, D;
+    qdl_born_fp4_cache cache;
+    const float *key_weight;
+    int64_t weight_strides[2], weight_len;
+    int64_t budget, recent;
+    const int32_t *out_table;
+    int64_t out_pages, out_table_ld;
+    float *weight_out;
+    int32_t *lens_out, *kept;
+} qdl_born_fp4_evict_call;
+
+int qdl_flash_born_fp4_evict_call(const qdl_born_fp4_evict_call *call, qdl_stream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

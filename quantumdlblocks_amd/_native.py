@@ -49,6 +49,11 @@ EXPORTED_SYMBOLS = (
     "qdl_flash_born_paged_forward_call",
     "qdl_flash_born_cache_append_call",
     "qdl_flash_born_cache_evict_call",
+    "qdl_flash_born_fp4_append_call",
+    "qdl_flash_born_fp4_read_call",
+    "qdl_flash_born_fp4_paged_workspace_size",
+    "qdl_flash_born_fp4_paged_forward_call",
+    "qdl_flash_born_fp4_evict_call",
 )
 
 
@@ -86,6 +91,13 @@ packed_call = _Block("@" + "q" * 8 + "q" * 3 + "q" * 6 + "qq" + "qq" + "qqd" + "
 paged_call = _Block("@" + "q" * 6 + "q" * 4 + "q" * 8 + "qq" + "qqq" + "q" + "qqd" + "qd" + "q" * 4 + "qq")
 append_call = _Block("@" + "q" * 7 + "q" * 3 + "q" * 6 + "q" + "q" * 8 + "qq" + "qqq" + "qq" + "q" * 5 + "qd")
 evict_call = _Block("@" + "q" * 5 + "q" * 8 + "qq" + "qqq" + "q" + "q" * 4 + "qq" + "qqq" + "qqq")
+
+# The fields of qdl_born_fp4_cache, in its place.
+_FP4 = "q" * 4 + "q" * 12 + "qq" + "qqq" + "q"
+fp4_append_call = _Block("@" + "q" * 7 + "q" * 3 + "q" * 6 + "q" + _FP4 + "q" + "qq" + "qqq" + "qd")
+fp4_read_call = _Block("@" + "q" * 6 + "qq" + _FP4 + "q")
+fp4_paged_call = _Block("@" + "q" * 7 + "q" * 4 + _FP4 + "q" + "qqd" + "qd" + "q" * 4 + "qq")
+fp4_evict_call = _Block("@" + "q" * 4 + _FP4 + "q" * 4 + "qq" + "qqq" + "qqq")
 
 
 _lock = threading.Lock()
@@ -136,13 +148,16 @@ def _bind(lib: ctypes.CDLL) -> None:
         call.argtypes = [ctypes.c_char_p, _ptr]  # the packed qdl_born_call, stream
     for call in (lib.qdl_flash_born_packed_forward_call, lib.qdl_flash_born_packed_backward_call,
                  lib.qdl_flash_born_paged_forward_call, lib.qdl_flash_born_cache_append_call,
-                 lib.qdl_flash_born_cache_evict_call):
+                 lib.qdl_flash_born_cache_evict_call, lib.qdl_flash_born_fp4_append_call, lib.qdl_flash_born_fp4_read_call,
+                 lib.qdl_flash_born_fp4_paged_forward_call, lib.qdl_flash_born_fp4_evict_call):
         call.restype = _int
         call.argtypes = [ctypes.c_char_p, _ptr]  # the packed argument block, stream
     lib.qdl_flash_born_packed_workspace_size.restype = _i64
     lib.qdl_flash_born_packed_workspace_size.argtypes = [ctypes.c_char_p]
     lib.qdl_flash_born_paged_workspace_size.restype = _i64
     lib.qdl_flash_born_paged_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _int]
+    lib.qdl_flash_born_fp4_paged_workspace_size.restype = _i64
+    lib.qdl_flash_born_fp4_paged_workspace_size.argtypes = [_i64, _i64, _i64, _i64, _i64, _i64, _i64, _i64, _int, _int]
     lib.qdl_flash_purified_born_fwd.restype = _int
     lib.qdl_flash_purified_born_fwd.argtypes = [
         _int, _i64, _i64, _i64, _i64,      # dtype, B, H, T, D

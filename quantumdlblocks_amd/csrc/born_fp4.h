@@ -1,0 +1,124 @@
+// A paged key-value cache in 4 bits: its rows and how they are read.
+//
+// A row (one head of one token) is W = 32 nb columns, the head dim rounded up to
+// whole blocks of 32 (zeros behind it).  A block is 16 bytes of 4-bit codes, the
+// lower nibble first, and one scale byte e: value = code 2^(e - 127), the codes
+// being sign, two exponent bits and one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6.
+// e = 255: not a number.
+//
+// Two significant bits and a power of two are exact in bf16, so every product
+// here runs on the bf16 matrix pipe whatever the type of the queries: these are
+// taken apart into bf16 parts that sum to them exactly (one for bf16, two for
+// fp16, three for fp32), and so are the fp32 weights where they are not rounded.
+//
+// A token that cannot be held (an infinity or NaN in it) has a block of scale
+// 255: every query that sees it, and no other, gets NaN.  A weight of 0 times a
+// NaN would reach the queries that do not see it, so V's bad blocks are read as
+// zeros and K's block as NaN in their place.
+#pragma once
+
+#include <type_traits>
+
+#include "born_common.h"
+#include "born_packed.h"
+#include "born_paged.h"
+
+namespace qdl {
+
+constexpr int kFp4Block = 32;
+constexpr uint32_t kFp4Bad = 255;
+
+// Strides in bytes: page, token, head.
+struct Fp4Cache {
+    uint8_t *k, *v, *ks, *vs;
+    int64_t kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh;
+    int64_t cache_pages;
+    int page, page_shift, nb;  // tokens per page, its logarithm or -1; blocks of a row
+};
+
+struct Fp4Pages {
+    const int32_t* table;  // (B, pages)
+    const int32_t* lens;   // (B)
+    int64_t table_ld;
+    int pages;
+};
+
+// Keys of sequence b, cut to its table.
+__device__ __forceinline__ int fp4_len(const Fp4Cache& c, const Fp4Pages& t, int b) {
+    return (int)min((int64_t)max(t.lens[b], 0), (int64_t)t.pages * c.page);
+}
+
+// Page index and row of key j >= 0.
+__device__ __forceinline__ int fp4_page(const Fp4Cache& c, int j) { return c.page_shift >= 0 ? j >> c.page_shift : j / c.page; }
+
+// The scale of a block as the conversions take it: fp32's exponent field.
+__device__ __forceinline__ float fp4_scale(uint32_t e) { return __uint_as_float(e << 23); }
+
+// Values 2 i and 2 i + 1 of a dword of codes, as a bf16 pair.
+template <int I>
+__device__ __forceinline__ uint32_t fp4_pair(uint32_t codes, float scale) {
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp4(codes, scale, I));
+}
+// All eight: the operand of a product over them.
+__device__ __forceinline__ u32x4 fp4_eight(uint32_t codes, float scale) {
+    return u32x4{fp4_pair<0>(codes, scale), fp4_pair<1>(codes, scale), fp4_pair<2>(codes, scale), fp4_pair<3>(codes, scale)};
+}
+
+// fp32 pairs as PARTS bf16 pairs whose sum they are (three: exactly).
+template <int PARTS>
+__device__ __forceinline__ void fp4_parts(float x, float y, uint32_t (&u)[PARTS]) {
+#pragma unroll
+    for (int i = 0; i < PARTS; ++i) {
+        u[i] = BF16::pack(x, y);
+        x -= BF16::lo(u[i]);
+        y -= BF16::hi(u[i]);
+    }
+}
+
+// bf16 parts of queries in E, and of the weights for outputs in E: with two the
+// output's rounding is the only one of 16 bits, with three fp32 has none.
+template <class E>
+constexpr int kQParts = std::is_same<E, F32>::value ? 3 : std::is_same<E, F16>::value ? 2 : 1;
+template <class E>
+constexpr int kPParts = std::is_same<E, F32>::value ? 3 : 2;
+
+// Eight values of a query from column `at` on (D - at of them, 0 behind), as operands.
+template <class E>
+__device__ __forceinline__ void fp4_query(const uint8_t* row, int at, int D, bool ok, bool neg, u32x4 (&q)[kQParts<E>]) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = 0.f;
+    if (ok && at < D) {  // D: a multiple of 8
+        if constexpr (std::is_same<E, F32>::value) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 y = ldg16(row + 4 * at + 16 * h);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * h + i] = __uint_as_float(y[i]);
+            }
+        } else {
+            const u32x4 y = ldg16(row + 2 * at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(y[i]), x[2 * i + 1] = E::hi(y[i]);
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t u[kQParts<E>];
+        fp4_parts<kQParts<E>>(neg ? -x[2 * i] : x[2 * i], neg ? -x[2 * i + 1] : x[2 * i + 1], u);
+#pragma unroll
+        for (int k = 0; k < kQParts<E>; ++k) q[k][i] = u[k];
+    }
+}
+
+template <class E>
+__device__ __forceinline__ void fp4_store4(uint8_t* row, int col, f32x4v x) {
+    if constexpr (std::is_same<E, F32>::value) {
+        *reinterpret_cast<f32x4v*>(row + 4 * col) = x;
+    } else {
+        const u32x2 y = {E::pack(x[0], x[1]), E::pack(x[2], x[3])};
+        *reinterpret_cast<u32x2*>(row + 2 * col) = y;
+    }
+}
+
+}  // namespace qdl

@@ -1,0 +1,428 @@
+// The 4-bit paged cache: appending a step's keys and values with the rotation
+// and normalisation of its queries and keys, reading rows back, and evicting.
+#pragma once
+
+#include "born_cache.h"
+#include "born_fp4.h"
+
+namespace qdl {
+
+// ---------------------------------------------------------------------------
+// Append.  Queries as in the 16-bit cache's append: fp32, rounded once.  A key
+// or value row is stored by eight columns a lane, four lanes a block:
+//   e: the least with max |x| <= 7 2^e, at least -126; codes of x / 2^e to
+//   nearest, halfway to even, at most 6.
+// (Root mean square error on Gaussian rows .112; with e = floor(log2 max) - 2
+// .115, without values past 6 .116, the better of two neighbours each time .112.)
+//
+// A key's rotation and normalisation are in 64 bits: a code is a step function
+// of its value, so that its nearest value is found whatever the order of the sums.
+// ---------------------------------------------------------------------------
+struct Fp4AppendArgs {
+    const void *q, *k, *v;
+    void* q_out;
+    Fp4Cache c;
+    Fp4Pages t;
+    const float *cos, *sin;
+    const int32_t* positions;  // (N) rows of the tables, or nullptr: the slot
+    const int32_t* cu;         // B + 1 starts, or nullptr: one token per sequence
+    int N, B, H, Hkv, D;
+    int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // bytes
+    int table_rows, n_freq;
+    int64_t freq_ld;
+    double eps;
+    int lpr, lpw;      // lanes of a query row, of a stored row
+    int q_blocks;      // workgroups of queries, those of stored rows behind them
+};
+
+// Token t's slot: its sequence and its key there; in: it belongs to one.
+struct Fp4Slot {
+    int s;
+    int64_t slot;
+    bool in;
+    __device__ __forceinline__ Fp4Slot(const int32_t* cu, const int32_t* lens, int B, int t) {
+        int first = t, last = t + 1;
+        s = t;
+        in = t < B;
+        if (cu != nullptr) {
+            int lo = 0, hi = B;  // the last start at or before t
+            while (hi - lo > 1) {
+                const int mid = (lo + hi) / 2;
+                if (cu[mid] <= t) lo = mid;
+                else hi = mid;
+            }
+            s = lo;
+            in = B > 0;
+            if (in) {
+                first = max(cu[s], 0);
+                last = cu[s + 1];
+                in = t >= first && t < last;
+            }
+        }
+        slot = in ? (int64_t)lens[s] - ((int64_t)last - t) : -1;
+    }
+    // Page (-1: none) and row in it.
+    __device__ __forceinline__ int64_t page(const Fp4Cache& c, const Fp4Pages& t, int& row) const {
+        row = 0;
+        if (slot < 0 || slot >= (int64_t)t.pages * c.page) return -1;
+        const int i = fp4_page(c, (int)slot);
+        row = (int)slot - i * c.page;
+        const int32_t p = t.table[(int64_t)s * t.table_ld + i];
+        return p >= 0 && p < c.cache_pages ? p : -1;
+    }
+};
+
+// Row of the rotary tables, as an offset.
+__device__ __forceinline__ int64_t fp4_angles(const Fp4AppendArgs& p, int t, int64_t slot) {
+    const int64_t at = p.positions != nullptr ? p.positions[t] : slot;
+    return min(max(at, (int64_t)0), (int64_t)p.table_rows - 1) * p.freq_ld;  // rows past the tables: their last
+}
+
+template <class E>
+__device__ __forceinline__ float fp4_element(const uint8_t* row, int col) {
+    if constexpr (std::is_same<E, F32>::value) {
+        return *reinterpret_cast<const float*>(row + 4 * col);
+    } else {
+        return E::lo(*reinterpret_cast<const uint16_t*>(row + 2 * col));
+    }
+}
+// Columns at .. at + 7, zeros past D or before 0.
+template <class E>
+__device__ __forceinline__ void fp4_columns(const uint8_t* row, int at, int D, float (&x)[8]) {
+    if (at >= 0 && at + 8 <= D && (at * kItem<E>) % 16 == 0) {
+        if constexpr (std::is_same<E, F32>::value) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                const u32x4 y = ldg16(row + 4 * at + 16 * h);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[4 * h + i] = __uint_as_float(y[i]);
+            }
+        } else {
+            const u32x4 y = ldg16(row + 2 * at);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(y[i]), x[2 * i + 1] = E::hi(y[i]);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = at + i >= 0 && at + i < D ? fp4_element<E>(row, at + i) : 0.f;
+    }
+}
+
+// The block's scale byte from its largest magnitude, kept as the upper 31 bits
+// of a double's magnitude with the lower ones as a sticky bit, and the exponent
+// that brings values to their codes'.
+__device__ __forceinline__ int fp4_exponent(uint32_t top) {
+    if (top >= 0x7ff00000u) return (int)kFp4Bad - 127;
+    return max((int)(top >> 20) - 1023 - 2 + ((top & 0xfffffu) > 0xc0000u ? 1 : 0), -126);
+}
+__device__ __forceinline__ uint32_t fp4_sticky(double x) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, x);
+    return ((uint32_t)(u >> 32) & 0x7fffffffu) | ((uint32_t)u != 0 ? 1u : 0u);
+}
+// x / 2^e as fp32 from its magnitude's form, sticky bit and all: halfway cases stay apart.
+__device__ __forceinline__ float fp4_scaled(uint32_t h, int e, double x) {
+    const int u = max((int)(h - ((uint32_t)(e + 896) << 20)), 0);
+    return __uint_as_float(((uint32_t)u << 3) | ((uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32) & 0x80000000u));
+}
+
+template <class E>
+__device__ __forceinline__ void fp4_append_row(const Fp4AppendArgs& p, int64_t item, int lane) {
+    const bool value = item >= (int64_t)p.N * p.Hkv;
+    if (value) item -= (int64_t)p.N * p.Hkv;
+    const int t = (int)(item / p.Hkv), h = (int)(item % p.Hkv);
+    const int c0 = 8 * lane, half = p.D >> 1;
+    const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
+    int row;
+    const int64_t page = slot.page(p.c, p.t, row);
+    if (page < 0) return;  // uniform in the row's lanes
+    const uint8_t* src = value ? (const uint8_t*)p.v + (int64_t)t * p.v_st + (int64_t)h * p.v_sh
+                               : (const uint8_t*)p.k + (int64_t)t * p.k_st + (int64_t)h * p.k_sh;
+    float x[8];
+    fp4_columns<E>(src, c0, p.D, x);
+    double y[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) y[i] = x[i];
+    if (!value) {
+        double ss = 0.0;
+        if (c0 < p.D) {
+            // Columns c and c + D / 2 are a pair.  Eight from c0 on: all in one
+            // half where D is a multiple of 16.
+            float up[8], down[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) up[i] = down[i] = 0.f;
+            if (c0 < half) fp4_columns<E>(src, c0 + half, p.D, up);
+            if (c0 + 8 > half) fp4_columns<E>(src, c0 - half, p.D, down);
+            const int64_t at = p.cos != nullptr ? fp4_angles(p, t, slot.slot) : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const bool low = c0 + i < half;
+                const int f = low ? c0 + i : c0 + i - half;
+                double c = 1.0, s = 0.0;
+                if (p.cos != nullptr && f < p.n_freq) c = p.cos[at + f], s = p.sin[at + f];
+                y[i] = low ? y[i] * c - (double)up[i] * s : (double)down[i] * s + y[i] * c;
+                ss += y[i] * y[i];
+            }
+        }
+        for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
+        const double f = 1.0 / sqrt(ss + p.eps);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) y[i] *= f;
+        if (c0 >= p.D) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[i] = 0.0;  // the padding of the last block, whatever the row
+        }
+    }
+    uint32_t u[8], top = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        u[i] = fp4_sticky(y[i]);
+        top = max(top, u[i]);
+    }
+    top = max(top, (uint32_t)__shfl_xor((int)top, 1));
+    top = max(top, (uint32_t)__shfl_xor((int)top, 2));
+    const int e = fp4_exponent(top);
+    uint32_t codes = 0;
+    if (e != (int)kFp4Bad - 127) {
+#define QDL_FP4_PACK(I)                                                                                                   \
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, fp4_scaled(u[2 * I], e, y[2 * I]),                              \
+                                                     fp4_scaled(u[2 * I + 1], e, y[2 * I + 1]), 1.0f, I)
+        QDL_FP4_PACK(0);
+        QDL_FP4_PACK(1);
+        QDL_FP4_PACK(2);
+        QDL_FP4_PACK(3);
+#undef QDL_FP4_PACK
+    }
+    if (lane >= 4 * p.c.nb) return;
+    const Fp4Cache& c = p.c;
+    uint8_t* to = value ? c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)h * c.vh : c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)h * c.kh;
+    *reinterpret_cast<uint32_t*>(to + 4 * lane) = codes;
+    if ((lane & 3) == 0) {
+        uint8_t* s = value ? c.vs + page * c.vsp + (int64_t)row * c.vst + (int64_t)h * c.vsh
+                           : c.ks + page * c.ksp + (int64_t)row * c.kst + (int64_t)h * c.ksh;
+        s[lane >> 2] = (uint8_t)(e + 127);
+    }
+}
+
+// Query rows: a group of `lpr` lanes each, lane i with VEC columns of the first
+// half and the matching ones of the second; ROWS heads of a token a group.
+template <class E, int VEC, int ROWS>
+__device__ __forceinline__ void fp4_append_queries(const Fp4AppendArgs& p, int64_t item, int lane) {
+    const int groups = (p.H + ROWS - 1) / ROWS;
+    if (item >= (int64_t)p.N * groups) return;
+    const int t = (int)(item / groups), r0 = (int)(item % groups) * ROWS, half = p.D >> 1;
+    const bool own = lane * VEC < half;  // lanes of a group past the row's chunks
+    const int o1 = lane * VEC * kItem<E>, o2 = o1 + half * kItem<E>;
+    const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
+    float c[VEC], sn[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) c[i] = 1.f, sn[i] = 0.f;
+    if (p.cos != nullptr && own) {
+        const int64_t at = fp4_angles(p, t, slot.slot);
+#pragma unroll
+        for (int i = 0; i < VEC; ++i) {
+            const int f = lane * VEC + i;
+            if (f < p.n_freq) c[i] = p.cos[at + f], sn[i] = p.sin[at + f];
+        }
+    }
+    RowVec<E, VEC> x1[ROWS], x2[ROWS];
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (r0 + i >= p.H || !own) continue;
+        const uint8_t* src = (const uint8_t*)p.q + (int64_t)t * p.q_st + (int64_t)(r0 + i) * p.q_sh;
+        x1[i].load(src + o1);
+        x2[i].load(src + o2);
+    }
+#pragma unroll
+    for (int i = 0; i < ROWS; ++i) {
+        if (r0 + i >= p.H) continue;  // uniform in the group
+        float y1[VEC], y2[VEC], ss = 0.f;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            const float a = own ? x1[i].get(e) : 0.f, b = own ? x2[i].get(e) : 0.f;
+            y1[e] = a * c[e] - b * sn[e];
+            y2[e] = a * sn[e] + b * c[e];
+            ss = fmaf(y1[e], y1[e], fmaf(y2[e], y2[e], ss));
+        }
+        for (int o = 1; o < p.lpr; o <<= 1) ss += __shfl_xor(ss, o);
+        const float f = 1.0f / sqrtf(ss + (float)p.eps);
+        if (!own) continue;
+#pragma unroll
+        for (int e = 0; e < VEC; ++e) {
+            // A token of no sequence has a zero query.
+            y1[e] = slot.in ? y1[e] * f : 0.f;
+            y2[e] = slot.in ? y2[e] * f : 0.f;
+        }
+        x1[i].set(y1);
+        x2[i].set(y2);
+        uint8_t* to = (uint8_t*)p.q_out + ((int64_t)t * p.H + r0 + i) * p.D * kItem<E>;
+        x1[i].store(to + o1);
+        x2[i].store(to + o2);
+    }
+}
+
+template <class E, int VEC, int ROWS>
+__global__ __launch_bounds__(256) void born_fp4_append_kernel(Fp4AppendArgs p) {
+    if ((int)blockIdx.x < p.q_blocks) {
+        fp4_append_queries<E, VEC, ROWS>(p, (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr, threadIdx.x & (p.lpr - 1));
+        return;
+    }
+    const int64_t item = (int64_t)(blockIdx.x - p.q_blocks) * (256 / p.lpw) + threadIdx.x / p.lpw;
+    if (item < 2 * (int64_t)p.N * p.Hkv) fp4_append_row<E>(p, item, threadIdx.x & (p.lpw - 1));
+}
+
+// ---------------------------------------------------------------------------
+// Read.  Rows (token, head) of a packed batch, each sequence's last keys, as
+// values: eight columns of K and of V a lane.
+// ---------------------------------------------------------------------------
+struct Fp4ReadArgs {
+    Fp4Cache c;
+    Fp4Pages t;
+    const int32_t* cu;
+    void *k, *v;  // (N, Hkv, D)
+    int N, B, Hkv, D;
+};
+
+template <class E>
+__device__ __forceinline__ void fp4_put8(uint8_t* to, uint32_t codes, float scale) {
+    const u32x4 y = fp4_eight(codes, scale);  // exact in bf16
+    if constexpr (std::is_same<E, BF16>::value) {
+        *reinterpret_cast<u32x4*>(to) = y;
+    } else if constexpr (std::is_same<E, F16>::value) {
+        u32x4 z;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) z[i] = F16::pack(BF16::lo(y[i]), BF16::hi(y[i]));
+        *reinterpret_cast<u32x4*>(to) = z;
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+            *reinterpret_cast<u32x4*>(to + 16 * i) = u32x4{y[2 * i] << 16, y[2 * i] & 0xffff0000u, y[2 * i + 1] << 16, y[2 * i + 1] & 0xffff0000u};
+    }
+}
+
+template <class E>
+__global__ __launch_bounds__(256) void born_fp4_read_kernel(Fp4ReadArgs p) {
+    const int per = p.D / 8;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)p.N * p.Hkv * per) return;
+    const int piece = (int)(i % per), h = (int)(i / per % p.Hkv), t = (int)(i / per / p.Hkv);
+    const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
+    int row;
+    const int64_t page = slot.page(p.c, p.t, row);
+    uint32_t k = 0, v = 0;
+    float ks = 0.f, vs = 0.f;
+    if (page >= 0) {
+        const Fp4Cache& c = p.c;
+        k = *reinterpret_cast<const uint32_t*>(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)h * c.kh + 4 * piece);
+        v = *reinterpret_cast<const uint32_t*>(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)h * c.vh + 4 * piece);
+        ks = fp4_scale(c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)h * c.ksh + (piece >> 2)]);
+        vs = fp4_scale(c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)h * c.vsh + (piece >> 2)]);
+    }
+    fp4_put8<E>((uint8_t*)p.k + i * 8 * kItem<E>, k, ks);
+    fp4_put8<E>((uint8_t*)p.v + i * 8 * kItem<E>, v, vs);
+}
+
+// ---------------------------------------------------------------------------
+// Evict: the 16-bit cache's selection, then the move of the kept rows: a lane
+// has a block of K and of V, 16 bytes of codes and a scale byte each.
+// ---------------------------------------------------------------------------
+struct Fp4EvictArgs {
+    EvictArgs s;  // the selection's, and the tables
+    Fp4Cache c;
+};
+
+struct Fp4Row {
+    u32x4 k, v;
+    uint8_t ks, vs;
+    __device__ __forceinline__ void load(const Fp4Cache& c, int64_t page, int row, int hk, int piece, bool ok) {
+        k = v = u32x4{0u, 0u, 0u, 0u};  // a missing page's rows are zeros
+        ks = vs = 0;
+        if (!ok) return;
+        k = ldg16(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)hk * c.kh + 16 * piece);
+        v = ldg16(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)hk * c.vh + 16 * piece);
+        ks = c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)hk * c.ksh + piece];
+        vs = c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)hk * c.vsh + piece];
+    }
+    __device__ __forceinline__ void store(const Fp4Cache& c, int64_t page, int row, int hk, int piece) const {
+        *reinterpret_cast<u32x4*>(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)hk * c.kh + 16 * piece) = k;
+        *reinterpret_cast<u32x4*>(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)hk * c.vh + 16 * piece) = v;
+        c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)hk * c.ksh + piece] = ks;
+        c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)hk * c.vsh + piece] = vs;
+    }
+};
+
+// Page (-1: none) and row of slot j in a table.
+__device__ __forceinline__ int fp4_slot(const Fp4Cache& c, const int32_t* table, int pages, int j, int& row) {
+    const int i = fp4_page(c, j);
+    row = j - i * c.page;
+    const int32_t p = i < pages ? table[i] : -1;
+    return p >= 0 && p < c.cache_pages ? p : -1;
+}
+
+constexpr int kFp4EvictUnroll = 4;
+inline __host__ __device__ int fp4_evict_rows(int nb) { return 256 / nb * kFp4EvictUnroll; }  // per workgroup
+
+// To other pages.
+template <int>
+__global__ __launch_bounds__(256) void born_fp4_evict_move_kernel(Fp4EvictArgs a) {
+    const EvictArgs& p = a.s;
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv, b = rest % p.B, tile = rest / p.B;
+    const int m = min(evict_len(p, b), p.budget), rows = 256 / a.c.nb;
+    const int mine = threadIdx.x / a.c.nb, piece = threadIdx.x % a.c.nb;
+    const int i0 = tile * fp4_evict_rows(a.c.nb) + mine;
+    if (mine >= rows || i0 >= m) return;
+    const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
+    const int32_t *from = p.table + (int64_t)b * p.table_ld, *to = p.to + (int64_t)b * p.to_ld;
+    Fp4Row x[kFp4EvictUnroll];
+#pragma unroll
+    for (int u = 0; u < kFp4EvictUnroll; ++u) {
+        const int i = i0 + u * rows;
+        int row = 0;
+        const int page = i < m ? fp4_slot(a.c, from, p.pages, kept[i], row) : -1;
+        x[u].load(a.c, page, row, hk, piece, page >= 0);
+    }
+#pragma unroll
+    for (int u = 0; u < kFp4EvictUnroll; ++u) {
+        const int i = i0 + u * rows;
+        int row = 0;
+        const int page = i < m ? fp4_slot(a.c, to, p.to_pages, i, row) : -1;
+        if (page >= 0) x[u].store(a.c, page, row, hk, piece);
+    }
+}
+
+// To the front of their own pages: rows only move down and keep their order, so
+// one workgroup per (sequence, key head) walks them upwards: a batch is read
+// whole before any of it is written, and what it writes lies below every row
+// still to be read.
+template <int>
+__global__ __launch_bounds__(1024) void born_fp4_evict_compact_kernel(Fp4EvictArgs a) {
+    constexpr int U = 4;
+    const EvictArgs& p = a.s;
+    const int hk = blockIdx.x % p.Hkv, b = blockIdx.x / p.Hkv;
+    const int m = min(evict_len(p, b), p.budget), rows = 1024 / a.c.nb;
+    const int mine = threadIdx.x / a.c.nb, piece = threadIdx.x % a.c.nb;
+    const int32_t* kept = p.kept + ((int64_t)b * p.Hkv + hk) * p.budget;
+    const int32_t* table = p.table + (int64_t)b * p.table_ld;
+    for (int i0 = 0; i0 < m; i0 += U * rows) {
+        Fp4Row x[U];
+        int page[U], row[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int i = i0 + u * rows + mine;
+            page[u] = -1;
+            row[u] = 0;
+            if (mine < rows && i < m && kept[i] != i) {
+                page[u] = fp4_slot(a.c, table, p.pages, i, row[u]);
+                int r;
+                const int src = fp4_slot(a.c, table, p.pages, kept[i], r);
+                x[u].load(a.c, src, r, hk, piece, src >= 0);
+            }
+        }
+        __syncthreads();
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+            if (page[u] >= 0) x[u].store(a.c, page[u], row[u], hk, piece);
+        __syncthreads();
+    }
+}
+
+}  // namespace qdl

@@ -1,0 +1,579 @@
+// Born attention over a paged cache in 4 bits, for one new token per sequence
+// or for several:
+//
+//   p_ij = (s relu(sign(s) q_i.k_j))^2 over the keys j that token i sees,
+//   O_i = sum_j p_ij v_j / (sum_j p_ij + eps).
+// Sequence b's tokens stand at the last of its n keys; token at position i sees
+// keys max(0, i - window + 1) .. i.  G = H / Hkv query heads read one key head,
+// so a sequence has new G rows for each key head: row r is head r % G of token
+// r / G.
+//
+// Narrow kernel: 16 NC rows are the columns of S^T = K Q^T (16-key products),
+// the keys split over workgroups and a workgroup's four waves, every fourth 32
+// keys each.  K's codes go from memory into the A operand by conversions alone:
+// a lane's 16 bytes are one block, and the order of the head dim's columns
+// within a product is free, so a dword of codes is an operand.  V's rows come as
+// DP / 16 columns a lane and 8 keys, are converted and paired by byte permutes.
+// The 16-key products' C layout is the next product's B operand.
+//
+// The keys are shared out on the device, which knows the lengths: chunk = the
+// keys of all sequences over the workgroups wanted, in steps of 128, and each
+// sequence takes as many chunks as it needs.  Partial sums are joined in order.
+#pragma once
+
+#include "born_fp4.h"
+
+namespace qdl {
+
+struct Fp4PagedArgs {
+    const void* q;  // rows (token, head)
+    void* out;
+    Fp4Cache c;
+    Fp4Pages t;
+    const int32_t* cu;  // B + 1 starts, or nullptr: one token per sequence
+    const float* scale;
+    float scale_value;
+    int per_head_scale;
+    int B, N, H, Hkv, G, D;
+    int window;
+    int items;             // chunks wanted; 0: one per sequence
+    int cblocks;           // column blocks of a sequence
+    float eps;
+    int64_t q_st, q_sh;    // bytes
+    int2* plan;            // (B): a sequence's first chunk and how many
+    float* part;           // (chunks, Hkv, cblocks, 16 NC, D + 4): denominator, three unused, numerators
+    float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
+    int64_t w_sb, w_sh;    // elements
+    int w_len;
+    float* raw;            // (B, H, raw_ld): p without s^2, keys from the span's first 32 on
+    int64_t raw_ld;
+};
+
+// A sequence: its tokens (rows of q), keys, and the first key that any token sees.
+struct Fp4Seq {
+    int q0, nq, n, first;
+    __device__ __forceinline__ Fp4Seq(const Fp4PagedArgs& p, int b) {
+        q0 = b;
+        nq = 1;
+        if (p.cu != nullptr) {
+            q0 = b == 0 ? 0 : min(max(p.cu[b], 0), p.N);
+            nq = max(min(p.cu[b + 1], p.N) - q0, 0);
+        }
+        n = p.c.cache_pages > 0 ? fp4_len(p.c, p.t, b) : 0;
+        first = p.window > 0 ? max(0, n - nq + 1 - p.window) : 0;
+        first = min(first, n);
+    }
+    __device__ __forceinline__ int base() const { return first & ~31; }
+    // Chunks are counted in steps of 128 keys.
+    __device__ __forceinline__ int steps() const { return max((n - base() + 127) >> 7, 1); }
+};
+
+struct Fp4Item {
+    int b, split, nsplit, chunk;  // b < 0: none
+};
+
+// Chunk `item` of the launch, found by every wave for itself.
+__device__ __forceinline__ Fp4Item fp4_item(const Fp4PagedArgs& p, int item) {
+    if (p.items == 0) return {item < p.B ? item : -1, 0, 1, 1 << 30};
+    const int lane = threadIdx.x & 63;
+    int64_t total = 0;
+    int mine = 0;  // of the first 64 sequences
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        const int s = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps() : 0;
+        if (b0 == 0) mine = s;
+        total += s;
+    }
+    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
+    const int step = (int)max((total + p.items - 1) / p.items, (int64_t)1);
+    int before = 0;
+    for (int b0 = 0; b0 < p.B; b0 += 64) {
+        if (b0 > 0) mine = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps() : 0;
+        const int k = (mine + step - 1) / step;
+        int run = k;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int y = __shfl_up(run, o);
+            if (lane >= o) run += y;
+        }
+        const int at = before + run - k;
+        const uint64_t here = __ballot(at <= item && item < at + k);
+        if (here != 0) {
+            const int l = __ffsll((long long)here) - 1;
+            return {b0 + l, item - __builtin_amdgcn_readlane(at, l), __builtin_amdgcn_readlane(k, l), step << 7};
+        }
+        before += __builtin_amdgcn_readlane(run, 63);
+    }
+    return {-1, 0, 1, 0};
+}
+
+__device__ __forceinline__ float fp4_inverse(const Fp4PagedArgs& p, int h, float z) {
+    const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
+    // A denominator that is not a number stays one.
+    return s != 0.f ? (den < 0x1p-126f ? 0.f : 1.0f / den) : 0.f;
+}
+
+template <class E, int DP>
+struct Fp4Cfg {
+    static constexpr int KB = DP == 256 ? 2 : 1;       // K: pieces of a lane's key, j4 + 4 i
+    static constexpr int KW = DP == 64 ? 2 : 4;        // dwords of a piece
+    static constexpr int KS = KB * KW;                 // 32-column products
+    static constexpr int VC = DP / 16, VD = (VC + 7) / 8;  // columns of a lane's key, dwords of codes
+};
+
+// A wave's 32 keys, as stored.
+template <class E, int DP>
+struct Fp4Keys {
+    using C = Fp4Cfg<E, DP>;
+    uint32_t k[2][C::KB][C::KW];
+    uint32_t ks[2][C::KB], kvs[2][C::KB];  // the scales of K's blocks, and of V's same ones
+    uint32_t v[8][C::VD], vs[8];
+    bool there[2];  // pages of 16 keys from a multiple of 16 (P16)
+    uint32_t seen;  // of the keys that the lane's V rows are, else
+};
+
+template <int DW>
+__device__ __forceinline__ void fp4_load(uint32_t (&to)[DW], const uint8_t* p) {
+    if constexpr (DW == 4) {
+        const u32x4 x = ldg16(p);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = x[i];
+    } else {
+        const u32x2 x = *reinterpret_cast<const u32x2*>(p);
+        to[0] = x[0];
+        to[1] = x[1];
+    }
+}
+
+// DP: 64, 128 or 256 columns; NC: 16-row column sets; WEIGH: the raw weights are
+// written too (one token per sequence); P16: pages of a multiple of 16 tokens.
+template <class E, int DP, int NC, bool WEIGH, bool P16>
+__global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
+    using C = Fp4Cfg<E, DP>;
+    constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
+    constexpr int IT = kItem<E>;
+    __shared__ float red[NW][16][DP + 4];
+    __shared__ float zred[NW][16];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int m = lane & 15, j4 = lane >> 4;
+    if (p.cu != nullptr) {
+        // Rows behind the last sequence.
+        const int last = min(max(p.cu[p.B], 0), p.N);
+        for (int r = last + blockIdx.x; r < p.N; r += gridDim.x)
+            for (int i = threadIdx.x; i < p.H * p.D * IT / 16; i += 256)
+                *reinterpret_cast<u32x4*>((uint8_t*)p.out + (int64_t)r * p.H * p.D * IT + 16 * i) = u32x4{0u, 0u, 0u, 0u};
+    }
+    const int cb = blockIdx.x % p.cblocks, rest = blockIdx.x / p.cblocks;
+    const int hk = rest % p.Hkv, item = rest / p.Hkv;
+    const Fp4Item it = fp4_item(p, item);
+    if (it.b < 0) return;
+    const int b = __builtin_amdgcn_readfirstlane(it.b);
+    const Fp4Seq sq(p, b);
+    if (it.split == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.nsplit};
+    const int rows = sq.nq * p.G, c0 = 16 * NC * cb;
+    if (c0 >= rows) return;
+    const int s0 = sq.base() + it.split * it.chunk, s1 = min(sq.n, s0 + it.chunk);
+
+    // This lane's rows and the keys that each sees: [lo, hi].
+    int tok[NC], head[NC], lo[NC], hi[NC];
+    u32x4 qr[NC][KS][QP];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int r = c0 + 16 * i + m;
+        const bool ok = r < rows;
+        tok[i] = ok ? r / p.G : 0;
+        head[i] = hk * p.G + (ok ? r - tok[i] * p.G : 0);
+        hi[i] = ok ? sq.n - sq.nq + tok[i] : -1;
+        lo[i] = p.window > 0 ? max(0, hi[i] - p.window + 1) : 0;
+        const bool neg = arg_scale(p, head[i]) < 0.f;
+        const uint8_t* row = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok[i]) * p.q_st + (int64_t)head[i] * p.q_sh;
+#pragma unroll
+        for (int a = 0; a < KB; ++a)
+#pragma unroll
+            for (int w = 0; w < KW; ++w)
+                fp4_query<E>(row, 8 * KW * (j4 + 4 * a) + 8 * w, p.D, ok, neg, qr[i][a * KW + w]);
+    }
+    // The keys that every row of the block sees.
+    const int t0 = c0 / p.G, t1 = min(c0 + 16 * NC, rows) - 1;
+    const int all_hi = sq.n - sq.nq + t0, all_lo = p.window > 0 ? sq.n - sq.nq + t1 / p.G - p.window + 1 : 0;
+
+    f32x4v acc[NC][VC];
+    float z[NC];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        z[i] = 0.f;
+#pragma unroll
+        for (int e = 0; e < VC; ++e) acc[i][e] = f32x4v{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // A lane's pieces of K and columns of V; those past the row are read from
+    // its start and taken as zeros (K) or never stored (V).
+    int ko[KB], kb[KB], vo, vb;
+    uint32_t kmask[KB];
+#pragma unroll
+    for (int a = 0; a < KB; ++a) {
+        const int at = 4 * KW * (j4 + 4 * a), blk = at / 16;
+        const bool in = blk < p.c.nb;
+        ko[a] = in ? at : 0;
+        kb[a] = in ? blk : 0;
+        kmask[a] = in ? ~0u : 0u;
+    }
+    {
+        const bool in = VC * m < kFp4Block * p.c.nb;
+        vo = in ? VC * m / 2 : 0;
+        vb = in ? VC * m / kFp4Block : 0;
+    }
+    const uint8_t *const kc = p.c.k + (int64_t)hk * p.c.kh, *const vc = p.c.v + (int64_t)hk * p.c.vh;
+    const uint8_t *const ksc = p.c.ks + (int64_t)hk * p.c.ksh, *const vsc = p.c.vs + (int64_t)hk * p.c.vsh;
+    const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.t.table + (int64_t)b * p.t.table_ld);
+
+    auto load_k = [&](Fp4Keys<E, DP>& x, int t, const uint8_t* kp, const uint8_t* ksp, const uint8_t* vsp) __attribute__((always_inline)) {
+#pragma unroll
+        for (int a = 0; a < KB; ++a) {
+            fp4_load<KW>(x.k[t][a], kp + ko[a]);
+            x.ks[t][a] = ksp[kb[a]];
+            x.kvs[t][a] = vsp[kb[a]];
+        }
+    };
+    auto load_v = [&](Fp4Keys<E, DP>& x, int i, const uint8_t* vp, const uint8_t* vsp) __attribute__((always_inline)) {
+        if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp + vo);
+        else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp + vo);
+        else fp4_load<2>(x.v[i], vp + vo);
+        x.vs[i] = vsp[vb];
+    };
+    // Keys key0 + 16 t + m for K, key0 + 16 t + 4 j4 + i for V.
+    auto load = [&](Fp4Keys<E, DP>& x, int key0) __attribute__((always_inline)) {
+        if constexpr (P16) {
+            // Keys outside [first, n) and missing pages: the loads go to the
+            // nearest key of the span, or to page 0, and use() drops what they bring.
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                const int j = min(max(key0 + 16 * t, sq.first), sq.n - 1);
+                const int i = __builtin_amdgcn_readfirstlane(fp4_page(p.c, j));
+                const int32_t page = table[i];
+                x.there[t] = page >= 0 && page < p.c.cache_pages;
+                const int64_t at = x.there[t] ? page : 0;
+                const uint8_t *kp = kc + at * p.c.kp, *ksp = ksc + at * p.c.ksp, *vp = vc + at * p.c.vp, *vsp = vsc + at * p.c.vsp;
+                auto row = [&](int r) { return (uint32_t)(min(max(key0 + 16 * t + r, sq.first), sq.n - 1) - i * p.c.page); };
+                const uint32_t rk = row(m);
+                load_k(x, t, kp + rk * (uint32_t)p.c.kt, ksp + rk * (uint32_t)p.c.kst, vsp + rk * (uint32_t)p.c.vst);
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const uint32_t rv = row(4 * j4 + r);
+                    load_v(x, 4 * t + r, vp + rv * (uint32_t)p.c.vt, vsp + rv * (uint32_t)p.c.vst);
+                }
+            }
+        } else {
+            auto find = [&](int j, int64_t& page, int& row) {
+                const bool in = j >= sq.first && j < sq.n;
+                const int i = fp4_page(p.c, in ? j : 0);
+                row = (in ? j : 0) - i * p.c.page;
+                const int32_t y = in ? table[i] : -1;
+                const bool ok = y >= 0 && y < p.c.cache_pages;
+                page = ok ? y : 0;
+                row = ok ? row : 0;
+                return ok;
+            };
+            x.there[0] = x.there[1] = true;
+            x.seen = 0;
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                int64_t page;
+                int row;
+                find(key0 + 16 * t + m, page, row);
+                load_k(x, t, kc + page * p.c.kp + (int64_t)row * p.c.kt, ksc + page * p.c.ksp + (int64_t)row * p.c.kst,
+                       vsc + page * p.c.vsp + (int64_t)row * p.c.vst);
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                int64_t page;
+                int row;
+                if (find(key0 + 16 * (i >> 2) + 4 * j4 + (i & 3), page, row)) x.seen |= 1u << i;
+                load_v(x, i, vc + page * p.c.vp + (int64_t)row * p.c.vt, vsc + page * p.c.vsp + (int64_t)row * p.c.vst);
+            }
+        }
+    };
+    auto use = [&](Fp4Keys<E, DP>& x, int key0) __attribute__((always_inline)) {
+        // K, with NaN for the blocks of tokens that are not numbers in K or V.
+        f32x4v s[NC][2];
+        bool bad = false;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int a = 0; a < KB; ++a) bad = bad || x.ks[t][a] == kFp4Bad || x.kvs[t][a] == kFp4Bad;
+        const bool any_bad = __ballot(bad) != 0;
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+#pragma unroll
+            for (int i = 0; i < NC; ++i) s[i][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int a = 0; a < KB; ++a) {
+                uint32_t e = x.ks[t][a];
+                if (any_bad && x.kvs[t][a] == kFp4Bad) e = kFp4Bad;
+                const float sc = kmask[a] ? fp4_scale(e) : 0.f;
+#pragma unroll
+                for (int w = 0; w < KW; ++w) {
+                    const u32x4 k = fp4_eight(x.k[t][a][w] & kmask[a], sc);
+#pragma unroll
+                    for (int i = 0; i < NC; ++i)
+#pragma unroll
+                        for (int u = 0; u < QP; ++u) s[i][t] = mfma16<BF16>(k, qr[i][a * KW + w][u], s[i][t]);
+                }
+            }
+        }
+        // Which of the lane's 8 keys (16 t + 4 j4 + r) are there at all.
+        const bool inside = key0 >= sq.first && key0 + 32 <= sq.n;
+        uint32_t seen = 255;
+        if constexpr (P16) {
+            if (!(inside && x.there[0] && x.there[1])) {
+                seen = 0;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const int key = key0 + 16 * (i >> 2) + 4 * j4 + (i & 3);
+                    if (x.there[i >> 2] && key >= sq.first && key < sq.n) seen |= 1u << i;
+                }
+            }
+        } else {
+            seen = x.seen;
+        }
+        const bool cut = __ballot(seen != 255) != 0 || key0 + 31 > all_hi || key0 < all_lo;
+        if (cut) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const int key = key0 + 16 * (n >> 2) + 4 * j4 + (n & 3);
+#pragma unroll
+                for (int i = 0; i < NC; ++i)
+                    if (!((seen >> n) & 1) || key > hi[i] || key < lo[i]) s[i][n >> 2][n & 3] = 0.f;
+            }
+        }
+        // V: bf16, 8 keys of a lane's columns.
+        uint32_t vv[8][VC / 2];
+#pragma unroll
+        for (int n = 0; n < 8; ++n) {
+            const bool drop = (cut && !((seen >> n) & 1)) || (any_bad && x.vs[n] == kFp4Bad);
+            const float sc = drop ? 0.f : fp4_scale(x.vs[n]);
+            uint32_t code[VD];
+#pragma unroll
+            for (int d = 0; d < VD; ++d) code[d] = drop ? 0u : x.v[n][d];
+#pragma unroll
+            for (int d = 0; d < VC / 2; d += 4) {
+                const u32x4 y = fp4_eight(code[d / 4], sc);
+#pragma unroll
+                for (int w = 0; w < 4; ++w)
+                    if (d + w < VC / 2) vv[n][d + w] = y[w];
+            }
+        }
+        u32x4 wt[NC][PP];
+#pragma unroll
+        for (int i = 0; i < NC; ++i) {
+            float w[8];
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const float r = s[i][n >> 2][n & 3], a = r < 0.f ? 0.f : r;  // NaN stays
+                w[n] = a * a;
+                z[i] += w[n];
+            }
+            if constexpr (WEIGH) {
+                if (c0 + 16 * i + m < rows) {
+#pragma unroll
+                    for (int t = 0; t < 2; ++t) {
+                        const int at = key0 - sq.base() + 16 * t + 4 * j4;
+                        const f32x4v y = {w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]};
+                        if (at < p.raw_ld)  // raw_ld: a multiple of 32
+                            *reinterpret_cast<f32x4v*>(p.raw + ((int64_t)b * p.H + head[i]) * p.raw_ld + at) = y;
+                    }
+                }
+            }
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                uint32_t u[PP];
+                fp4_parts<PP>(w[2 * n], w[2 * n + 1], u);
+#pragma unroll
+                for (int k = 0; k < PP; ++k) wt[i][k][n] = u[k];
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < VC; ++e) {
+            u32x4 a;
+#pragma unroll
+            for (int n = 0; n < 4; ++n)
+                a[n] = __builtin_amdgcn_perm(vv[2 * n + 1][e >> 1], vv[2 * n][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+#pragma unroll
+            for (int i = 0; i < NC; ++i)
+#pragma unroll
+                for (int k = 0; k < PP; ++k) acc[i][e] = mfma16<BF16>(a, wt[i][k], acc[i][e]);
+        }
+    };
+    const int step = 32 * NW;
+    {
+        Fp4Keys<E, DP> x, y;
+        int key = s0 + 32 * wave;
+        if (key < s1) load(x, key);
+        for (; key < s1; key += 2 * step) {
+            if (key + step < s1) load(y, key + step);
+            use(x, key);
+            if (key + step >= s1) break;
+            if (key + 2 * step < s1) load(x, key + 2 * step);
+            use(y, key + step);
+        }
+    }
+    // The waves' sums, in order.
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        float zz = z[i];
+        zz += __shfl_xor(zz, 16);
+        zz += __shfl_xor(zz, 32);
+        if (i > 0) __syncthreads();
+        if (j4 == 0) zred[wave][m] = zz;
+#pragma unroll
+        for (int e = 0; e < VC; ++e)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) red[wave][m][VC * (4 * j4 + r) + e] = acc[i][e][r];
+        __syncthreads();
+        const int here = min(16, rows - c0 - 16 * i);
+        for (int x = threadIdx.x; x < here * (DP / 4); x += 64 * NW) {
+            const int cc = x / (DP / 4), col = 4 * (x % (DP / 4));
+            if (col >= p.D) continue;
+            f32x4v y = *reinterpret_cast<const f32x4v*>(&red[0][cc][col]);
+            float sum = zred[0][cc];
+#pragma unroll
+            for (int w = 1; w < NW; ++w) {
+                y += *reinterpret_cast<const f32x4v*>(&red[w][cc][col]);
+                sum += zred[w][cc];
+            }
+            const int r = c0 + 16 * i + cc, t = r / p.G, h = hk * p.G + r - t * p.G;
+            if (it.nsplit > 1 || WEIGH) {
+                float* to = p.part + ((((int64_t)item * p.Hkv + hk) * p.cblocks + cb) * (16 * NC) + 16 * i + cc) * (p.D + 4);
+                *reinterpret_cast<f32x4v*>(to + 4 + col) = y;
+                if (col == 0) to[0] = sum;
+            }
+            if (it.nsplit == 1) {
+                y *= fp4_inverse(p, h, sum);
+                fp4_store4<E>((uint8_t*)p.out + ((int64_t)(sq.q0 + t) * p.H + h) * p.D * IT, col, y);
+            }
+        }
+    }
+}
+
+// A row's partial sums.
+struct Fp4Parts {
+    const float* at;
+    int64_t ld;
+    int n;
+    __device__ __forceinline__ Fp4Parts(const Fp4PagedArgs& p, int b, int hk, int r, int cols) {
+        const int2 plan = p.plan[b];
+        n = plan.y;
+        ld = (int64_t)p.Hkv * p.cblocks * cols * (p.D + 4);
+        at = p.part + plan.x * ld + (((int64_t)hk * p.cblocks + r / cols) * cols + r % cols) * (p.D + 4);
+    }
+};
+
+// Splits joined in order: one workgroup per row of a (sequence, key head),
+// `ncol` threads over the columns, 256 / ncol groups of them over the splits.
+// WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the sum
+// over the group of p_j / Z, the heads in order, is added to its weights.
+template <class E, bool WEIGH>
+__global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int ncol, int cols, int most) {
+    __shared__ f32x4v red[256];
+    __shared__ float zred[256];
+    if (WEIGH && (int)blockIdx.x >= p.B * p.Hkv * most) {
+        const int x = blockIdx.x - p.B * p.Hkv * most, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
+        const Fp4Seq sq(p, b);
+        const int j0 = sq.base() + block * 256, j = j0 + threadIdx.x;
+        if (j0 >= sq.n) return;
+        const bool seen = j >= sq.first && j < sq.n && j < p.w_len;
+        float sum = 0.f;
+        for (int g0 = 0; g0 < p.G; g0 += 256) {
+            const int gn = min(256, p.G - g0);
+            if ((int)threadIdx.x < gn) {
+                const Fp4Parts part(p, b, hk, g0 + threadIdx.x, cols);
+                float z = 0.f;
+#pragma unroll 8
+                for (int i = 0; i < part.n; ++i) z += part.at[i * part.ld];
+                zred[threadIdx.x] = fp4_inverse(p, hk * p.G + g0 + threadIdx.x, z);
+            }
+            __syncthreads();
+            if (seen) {
+                const float* raw = p.raw + ((int64_t)b * p.H + hk * p.G + g0) * p.raw_ld + (j - sq.base());
+#pragma unroll 4
+                for (int i = 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
+            }
+            __syncthreads();
+        }
+        if (seen) p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
+        return;
+    }
+    const int r = blockIdx.x % most, rest = blockIdx.x / most, hk = rest % p.Hkv, b = rest / p.Hkv;
+    const Fp4Seq sq(p, b);
+    if (r >= sq.nq * p.G) return;
+    const Fp4Parts part(p, b, hk, r, cols);
+    if (part.n == 1) return;  // written already
+    const int col = threadIdx.x % ncol, group = threadIdx.x / ncol, groups = 256 / ncol;
+    const bool ok = 4 * col < p.D;
+    f32x4v x = {0.f, 0.f, 0.f, 0.f};
+    float z = 0.f;
+#pragma unroll 4
+    for (int i = group; i < part.n; i += groups) {
+        const float* at = part.at + i * part.ld;
+        z += at[0];
+        if (ok) x += *reinterpret_cast<const f32x4v*>(at + 4 + 4 * col);
+    }
+    red[threadIdx.x] = x;
+    zred[threadIdx.x] = z;
+    __syncthreads();
+    if (group != 0 || !ok) return;
+    for (int i = 1; i < groups; ++i) {
+        x += red[i * ncol + col];
+        z += zred[i * ncol + col];
+    }
+    const int t = r / p.G, h = hk * p.G + r - t * p.G;
+    x *= fp4_inverse(p, h, z);
+    fp4_store4<E>((uint8_t*)p.out + ((int64_t)(sq.q0 + t) * p.H + h) * p.D * kItem<E>, 4 * col, x);
+}
+
+// Rows of a launch's (sequence, key head): `most` at most; chunks: workgroups of each (key head, column block).
+struct Fp4Plan {
+    int nc, cblocks, items, chunks, most;
+    int64_t plan_bytes, part_bytes, raw_bytes, raw_ld;
+    int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes; }
+};
+
+template <class E>
+hipError_t fp4_paged_fwd(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st);
+
+template <class E, int NC, bool WEIGH, bool P16>
+void launch_fp4_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    const dim3 grid((unsigned)((int64_t)plan.chunks * a.Hkv * plan.cblocks));
+    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 64, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 128, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((born_fp4_paged_kernel<E, 256, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
+}
+template <class E, bool P16>
+void launch_fp4_nc(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    if (a.raw != nullptr) launch_fp4_dp<E, 1, true, P16>(a, plan, st);
+    else if (plan.nc == 1) launch_fp4_dp<E, 1, false, P16>(a, plan, st);
+    else launch_fp4_dp<E, 2, false, P16>(a, plan, st);
+}
+
+template <class E>
+hipError_t launch_fp4_paged(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    // Offsets within a page in 32 bits; a page 0 to send masked loads to.
+    const int64_t far = (int64_t)1 << 31, page = a.c.page;
+    const bool p16 = a.c.page % 16 == 0 && page * a.c.kt < far && page * a.c.vt < far && page * a.c.kst < far && page * a.c.vst < far;
+    if (p16) launch_fp4_nc<E, true>(a, plan, st);
+    else launch_fp4_nc<E, false>(a, plan, st);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess || (a.items == 0 && a.raw == nullptr)) return e;
+    int ncol = 2;
+    while (4 * ncol < a.D) ncol *= 2;
+    const unsigned join = (unsigned)((int64_t)a.B * a.Hkv * plan.most);
+    const int cols = 16 * plan.nc;
+    if (a.raw != nullptr) {
+        const unsigned weigh = (unsigned)((a.raw_ld + 255) / 256 * a.B * a.Hkv);
+        hipLaunchKernelGGL((born_fp4_join_kernel<E, true>), dim3(join + weigh), dim3(256), 0, st, a, ncol, cols, plan.most);
+    } else {
+        hipLaunchKernelGGL((born_fp4_join_kernel<E, false>), dim3(join), dim3(256), 0, st, a, ncol, cols, plan.most);
+    }
+    return hipGetLastError();
+}
+
+}  // namespace qdl

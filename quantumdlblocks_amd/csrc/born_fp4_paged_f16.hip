@@ -1,0 +1,11 @@
+// Born attention over a 4-bit paged cache, F16 queries.
+#include "born_fp4_paged.h"
+
+namespace qdl {
+
+template <>
+hipError_t fp4_paged_fwd<F16>(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    return launch_fp4_paged<F16>(a, plan, st);
+}
+
+}  // namespace qdl
