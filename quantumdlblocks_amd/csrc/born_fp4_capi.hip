@@ -6,6 +6,7 @@
 #include "../../include/qdl_flash_born.h"
 #include "born_fp4_cache.h"
 #include "born_fp4_paged.h"
+#include "born_fp4_tiled.h"
 
 namespace {
 
@@ -68,13 +69,31 @@ void set_cache(qdl::Fp4Cache& a, qdl::Fp4Pages& t, const qdl_born_fp4_cache& c, 
     t.pages = (int)c.pages;
 }
 
+// Rows (new tokens x heads of a group) of a sequence up to which the narrow
+// kernel takes it.
+constexpr int64_t kNarrowRows = 64;
+
 // Chunks of the keys: four workgroups a compute unit.  Where a launch has more
 // sequences than a workgroup should look through, or nothing to split, one each.
 qdl::Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window, bool packed,
                       bool weighed) {
     qdl::Fp4Plan r = {};
-    const int64_t G = H / h_kv, most = (packed ? n : 1) * G, room = pages * page;
-    r.most = (int)(most < ((int64_t)1 << 30) ? most : (int64_t)1 << 30);
+    const int64_t G = H / h_kv, room = pages * page;
+    int64_t most = G;
+    if (packed) {
+        r.limit = kNarrowRows;
+        most = n * G < r.limit ? n * G : r.limit;
+        if (n * G > r.limit) {
+            const int64_t blocks = (n * G + qdl::kFp4Rows - 1) / qdl::kFp4Rows;
+            r.slots = n * G / qdl::kFp4Rows + B + 1;
+            // Two workgroups a compute unit, none under four tiles of 64 keys.
+            int64_t splits = 512 / (blocks * h_kv);
+            if (splits > room / 256) splits = room / 256;
+            r.splits = (int)(splits < 1 ? 1 : splits);
+            if (r.splits > 1) r.wide_bytes = n * H * r.splits * (D + 4) * 4;
+        }
+    }
+    r.most = (int)most;
     r.nc = !weighed && most > 16 && (!packed || n * G > 16 * B) ? 2 : 1;
     r.cblocks = (r.most + 16 * r.nc - 1) / (16 * r.nc);
     int64_t items = 0;
@@ -94,7 +113,7 @@ qdl::Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, 
 }
 bool fp4_plan_ok(const qdl::Fp4Plan& r, int64_t B, int64_t H, int64_t h_kv, bool weighed) {
     const int64_t join = B * h_kv * r.most + (weighed ? B * h_kv * (r.raw_ld / 256 + 1) : 0);
-    return r.chunks * h_kv * r.cblocks <= kMostBlocks && join <= kMostBlocks;
+    return r.chunks * h_kv * r.cblocks <= kMostBlocks && join <= kMostBlocks && r.slots * r.splits * h_kv <= kMostBlocks;
 }
 
 int64_t append_blocks(int64_t n, int64_t rows, int lanes) {
@@ -258,12 +277,15 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     a.window = (int)c->window_size;
     a.items = r.items;
     a.cblocks = r.cblocks;
+    a.limit = r.limit;
+    a.splits = r.splits;
     a.eps = (float)c->eps;
     a.q_st = c->q_strides[0] * it;
     a.q_sh = c->q_strides[1] * it;
     uint8_t* ws = static_cast<uint8_t*>(c->workspace);
     a.plan = reinterpret_cast<int2*>(ws);
     a.part = reinterpret_cast<float*>(ws + r.plan_bytes);
+    a.wide_part = reinterpret_cast<float*>(ws + r.plan_bytes + r.part_bytes + r.raw_bytes);
     if (weighed) {
         a.raw = reinterpret_cast<float*>(ws + r.plan_bytes + r.part_bytes);
         a.raw_ld = r.raw_ld;

@@ -38,6 +38,9 @@ struct Fp4PagedArgs {
     int window;
     int items;             // chunks wanted; 0: one per sequence
     int cblocks;           // column blocks of a sequence
+    int limit;             // rows of a (sequence, key head) that the narrow kernel takes
+    int splits;            // of the tiled kernel's keys
+    float* wide_part;      // (N, H, splits, D + 4), where there are several
     float eps;
     int64_t q_st, q_sh;    // bytes
     int2* plan;            // (B): a sequence's first chunk and how many
@@ -64,8 +67,9 @@ struct Fp4Seq {
         first = min(first, n);
     }
     __device__ __forceinline__ int base() const { return first & ~31; }
-    // Chunks are counted in steps of 128 keys.
-    __device__ __forceinline__ int steps() const { return max((n - base() + 127) >> 7, 1); }
+    __device__ __forceinline__ bool wide(const Fp4PagedArgs& p) const { return p.cu != nullptr && (int64_t)nq * p.G > p.limit; }
+    // The narrow kernel's chunks are counted in steps of 128 keys.
+    __device__ __forceinline__ int steps(const Fp4PagedArgs& p) const { return wide(p) ? 0 : max((n - base() + 127) >> 7, 1); }
 };
 
 struct Fp4Item {
@@ -79,15 +83,15 @@ __device__ __forceinline__ Fp4Item fp4_item(const Fp4PagedArgs& p, int item) {
     int64_t total = 0;
     int mine = 0;  // of the first 64 sequences
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int s = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps() : 0;
+        const int s = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps(p) : 0;
         if (b0 == 0) mine = s;
         total += s;
     }
     for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-    const int step = (int)max((total + p.items - 1) / p.items, (int64_t)1);
+    const int step = (int)min(max((total + p.items - 1) / p.items, (int64_t)1), (int64_t)1 << 23);  // 2^30 keys: all
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        if (b0 > 0) mine = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps() : 0;
+        if (b0 > 0) mine = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps(p) : 0;
         const int k = (mine + step - 1) / step;
         int run = k;
         for (int o = 1; o < 64; o <<= 1) {
@@ -168,6 +172,7 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
     if (it.b < 0) return;
     const int b = __builtin_amdgcn_readfirstlane(it.b);
     const Fp4Seq sq(p, b);
+    if (sq.wide(p)) return;
     if (it.split == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.nsplit};
     const int rows = sq.nq * p.G, c0 = 16 * NC * cb;
     if (c0 >= rows) return;
@@ -222,45 +227,57 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
         vo = in ? VC * m / 2 : 0;
         vb = in ? VC * m / kFp4Block : 0;
     }
+    const bool whole = kFp4Block * p.c.nb == DP;
     const uint8_t *const kc = p.c.k + (int64_t)hk * p.c.kh, *const vc = p.c.v + (int64_t)hk * p.c.vh;
     const uint8_t *const ksc = p.c.ks + (int64_t)hk * p.c.ksh, *const vsc = p.c.vs + (int64_t)hk * p.c.vsh;
     const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.t.table + (int64_t)b * p.t.table_ld);
 
-    auto load_k = [&](Fp4Keys<E, DP>& x, int t, const uint8_t* kp, const uint8_t* ksp, const uint8_t* vsp) __attribute__((always_inline)) {
+    // Offsets of the lane's K rows (m) and V rows (4 j4 + r) within 16 keys of a
+    // page: added to scalar bases they cost nothing per load.
+    uint32_t ok_[KB], oks[KB], okv[KB], ov[4], ovs[4];
+    if constexpr (P16) {
 #pragma unroll
         for (int a = 0; a < KB; ++a) {
-            fp4_load<KW>(x.k[t][a], kp + ko[a]);
-            x.ks[t][a] = ksp[kb[a]];
-            x.kvs[t][a] = vsp[kb[a]];
+            ok_[a] = m * (uint32_t)p.c.kt + ko[a];
+            oks[a] = m * (uint32_t)p.c.kst + kb[a];
+            okv[a] = m * (uint32_t)p.c.vst + kb[a];
         }
-    };
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            ov[r] = (4 * j4 + r) * (uint32_t)p.c.vt + vo;
+            ovs[r] = (4 * j4 + r) * (uint32_t)p.c.vst + vb;
+        }
+    }
     auto load_v = [&](Fp4Keys<E, DP>& x, int i, const uint8_t* vp, const uint8_t* vsp) __attribute__((always_inline)) {
-        if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp + vo);
-        else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp + vo);
-        else fp4_load<2>(x.v[i], vp + vo);
-        x.vs[i] = vsp[vb];
+        if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
+        else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp);
+        else fp4_load<2>(x.v[i], vp);
+        x.vs[i] = *vsp;
     };
     // Keys key0 + 16 t + m for K, key0 + 16 t + 4 j4 + i for V.
     auto load = [&](Fp4Keys<E, DP>& x, int key0) __attribute__((always_inline)) {
         if constexpr (P16) {
-            // Keys outside [first, n) and missing pages: the loads go to the
-            // nearest key of the span, or to page 0, and use() drops what they bring.
+            // Sixteen keys are rows of one page, all of them memory of the cache's;
+            // without a page, or behind the last key, they are read from page 0,
+            // and use() drops what no row of the block sees.
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                const int j = min(max(key0 + 16 * t, sq.first), sq.n - 1);
-                const int i = __builtin_amdgcn_readfirstlane(fp4_page(p.c, j));
+                const int j = key0 + 16 * t;
+                const int i = __builtin_amdgcn_readfirstlane(fp4_page(p.c, min(j, sq.n - 1)));
                 const int32_t page = table[i];
-                x.there[t] = page >= 0 && page < p.c.cache_pages;
+                x.there[t] = j < sq.n && page >= 0 && page < p.c.cache_pages;
                 const int64_t at = x.there[t] ? page : 0;
-                const uint8_t *kp = kc + at * p.c.kp, *ksp = ksc + at * p.c.ksp, *vp = vc + at * p.c.vp, *vsp = vsc + at * p.c.vsp;
-                auto row = [&](int r) { return (uint32_t)(min(max(key0 + 16 * t + r, sq.first), sq.n - 1) - i * p.c.page); };
-                const uint32_t rk = row(m);
-                load_k(x, t, kp + rk * (uint32_t)p.c.kt, ksp + rk * (uint32_t)p.c.kst, vsp + rk * (uint32_t)p.c.vst);
+                const int64_t row = x.there[t] ? j - i * p.c.page : 0;
+                const uint8_t *kp = kc + at * p.c.kp + row * p.c.kt, *ksp = ksc + at * p.c.ksp + row * p.c.kst;
+                const uint8_t *vp = vc + at * p.c.vp + row * p.c.vt, *vsp = vsc + at * p.c.vsp + row * p.c.vst;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const uint32_t rv = row(4 * j4 + r);
-                    load_v(x, 4 * t + r, vp + rv * (uint32_t)p.c.vt, vsp + rv * (uint32_t)p.c.vst);
+                for (int a = 0; a < KB; ++a) {
+                    fp4_load<KW>(x.k[t][a], kp + ok_[a]);
+                    x.ks[t][a] = ksp[oks[a]];
+                    x.kvs[t][a] = vsp[okv[a]];
                 }
+#pragma unroll
+                for (int r = 0; r < 4; ++r) load_v(x, 4 * t + r, vp + ov[r], vsp + ovs[r]);
             }
         } else {
             auto find = [&](int j, int64_t& page, int& row) {
@@ -280,15 +297,21 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
                 int64_t page;
                 int row;
                 find(key0 + 16 * t + m, page, row);
-                load_k(x, t, kc + page * p.c.kp + (int64_t)row * p.c.kt, ksc + page * p.c.ksp + (int64_t)row * p.c.kst,
-                       vsc + page * p.c.vsp + (int64_t)row * p.c.vst);
+                const uint8_t *kp = kc + page * p.c.kp + (int64_t)row * p.c.kt, *ksp = ksc + page * p.c.ksp + (int64_t)row * p.c.kst;
+                const uint8_t* vsp = vsc + page * p.c.vsp + (int64_t)row * p.c.vst;
+#pragma unroll
+                for (int a = 0; a < KB; ++a) {
+                    fp4_load<KW>(x.k[t][a], kp + ko[a]);
+                    x.ks[t][a] = ksp[kb[a]];
+                    x.kvs[t][a] = vsp[kb[a]];
+                }
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 int64_t page;
                 int row;
                 if (find(key0 + 16 * (i >> 2) + 4 * j4 + (i & 3), page, row)) x.seen |= 1u << i;
-                load_v(x, i, vc + page * p.c.vp + (int64_t)row * p.c.vt, vsc + page * p.c.vsp + (int64_t)row * p.c.vst);
+                load_v(x, i, vc + page * p.c.vp + (int64_t)row * p.c.vt + vo, vsc + page * p.c.vsp + (int64_t)row * p.c.vst + vb);
             }
         }
     };
@@ -301,18 +324,33 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
 #pragma unroll
             for (int a = 0; a < KB; ++a) bad = bad || x.ks[t][a] == kFp4Bad || x.kvs[t][a] == kFp4Bad;
         const bool any_bad = __ballot(bad) != 0;
+        if (any_bad) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int a = 0; a < KB; ++a)
+                    if (x.kvs[t][a] == kFp4Bad) x.ks[t][a] = kFp4Bad;
+        }
+        if (!whole) {
+#pragma unroll
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int a = 0; a < KB; ++a) {
+                    x.ks[t][a] &= kmask[a];
+#pragma unroll
+                    for (int w = 0; w < KW; ++w) x.k[t][a][w] &= kmask[a];
+                }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
 #pragma unroll
             for (int i = 0; i < NC; ++i) s[i][t] = f32x4v{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int a = 0; a < KB; ++a) {
-                uint32_t e = x.ks[t][a];
-                if (any_bad && x.kvs[t][a] == kFp4Bad) e = kFp4Bad;
-                const float sc = kmask[a] ? fp4_scale(e) : 0.f;
+                const float sc = fp4_scale(x.ks[t][a]);
 #pragma unroll
                 for (int w = 0; w < KW; ++w) {
-                    const u32x4 k = fp4_eight(x.k[t][a][w] & kmask[a], sc);
+                    const u32x4 k = fp4_eight(x.k[t][a][w], sc);
 #pragma unroll
                     for (int i = 0; i < NC; ++i)
 #pragma unroll
@@ -345,18 +383,23 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
                     if (!((seen >> n) & 1) || key > hi[i] || key < lo[i]) s[i][n >> 2][n & 3] = 0.f;
             }
         }
+        if (cut || any_bad) {
+#pragma unroll
+            for (int n = 0; n < 8; ++n)
+                if (!((seen >> n) & 1) || x.vs[n] == kFp4Bad) {
+                    x.vs[n] = 0;
+#pragma unroll
+                    for (int d = 0; d < VD; ++d) x.v[n][d] = 0;
+                }
+        }
         // V: bf16, 8 keys of a lane's columns.
         uint32_t vv[8][VC / 2];
 #pragma unroll
         for (int n = 0; n < 8; ++n) {
-            const bool drop = (cut && !((seen >> n) & 1)) || (any_bad && x.vs[n] == kFp4Bad);
-            const float sc = drop ? 0.f : fp4_scale(x.vs[n]);
-            uint32_t code[VD];
-#pragma unroll
-            for (int d = 0; d < VD; ++d) code[d] = drop ? 0u : x.v[n][d];
+            const float sc = fp4_scale(x.vs[n]);
 #pragma unroll
             for (int d = 0; d < VC / 2; d += 4) {
-                const u32x4 y = fp4_eight(code[d / 4], sc);
+                const u32x4 y = fp4_eight(x.v[n][d / 4], sc);
 #pragma unroll
                 for (int w = 0; w < 4; ++w)
                     if (d + w < VC / 2) vv[n][d + w] = y[w];
@@ -504,7 +547,7 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int 
     }
     const int r = blockIdx.x % most, rest = blockIdx.x / most, hk = rest % p.Hkv, b = rest / p.Hkv;
     const Fp4Seq sq(p, b);
-    if (r >= sq.nq * p.G) return;
+    if (sq.wide(p) || r >= sq.nq * p.G) return;
     const Fp4Parts part(p, b, hk, r, cols);
     if (part.n == 1) return;  // written already
     const int col = threadIdx.x % ncol, group = threadIdx.x / ncol, groups = 256 / ncol;
@@ -532,9 +575,11 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int 
 
 // Rows of a launch's (sequence, key head): `most` at most; chunks: workgroups of each (key head, column block).
 struct Fp4Plan {
-    int nc, cblocks, items, chunks, most;
-    int64_t plan_bytes, part_bytes, raw_bytes, raw_ld;
-    int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes; }
+    int nc, cblocks, items, chunks, most, limit;
+    int splits;     // of the tiled kernel
+    int64_t slots;  // its blocks of rows; 0: no sequence is wide
+    int64_t plan_bytes, part_bytes, raw_bytes, wide_bytes, raw_ld;
+    int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes + wide_bytes; }
 };
 
 template <class E>

@@ -1,0 +1,307 @@
+// Born attention of many new tokens per sequence over a paged cache in 4 bits:
+// the kernel for sequences with more rows (new tokens x heads of a group) than
+// the narrow one takes.
+//
+// 128 rows a workgroup, 32 a wave: S^T = K Q^T per 32 keys, the weights in
+// place, O^T += V^T P^T, as the packed forward does it from 16 bits.  Tiles of
+// keys are converted to bf16 once for the four waves: each thread has a block of
+// 32 columns of K and of V, its codes loaded two tiles ahead into registers,
+// converted one tile ahead into the other half of LDS, one barrier a tile.
+// Sixteen lanes that write LDS together have one block of 16 keys, which the
+// rows' swizzle spreads over all banks.
+//
+// Keys without a page, or past the sequence, are zeros: overlaps of 0, weights
+// of 0.  Few blocks of rows split their keys; the partial sums are joined in order.
+#pragma once
+
+#include "born_fp4_paged.h"
+
+namespace qdl {
+
+constexpr int kFp4Rows = 128;
+
+// bf16 parts of the weights.  bf16 outputs take one, rounded as the output is,
+// and Z adds the rounded weights, as in the packed forward: the matrix pipe
+// bounds this kernel, and the keys' own 4 bits are off by 60 times as much (8
+// second turns, 4583 tokens over 27 thousand keys, 32 heads over 8, D128: 327 us,
+// with two parts 420; error in norm 2.2e-3, 1.7e-3).
+template <class E>
+constexpr int kTileParts = std::is_same<E, BF16>::value ? 1 : kPParts<E>;
+
+template <class E, int DP>
+struct Fp4TileCfg {
+    static constexpr int BN = DP == 256 ? 32 : 64, SUB = BN / 32, NB = DP / 32;
+    static constexpr int BYTES = BN * DP * 2, STAGE = 2 * BYTES;
+    static constexpr int UNITS = BN * NB / 256;  // blocks of K (and of V) of a thread; 0: K or V
+    static constexpr int WPE = DP == 256 ? 1 : 2;
+};
+
+// Rows of a workgroup: rows m0 .. of sequence b's new tokens x G.
+struct Fp4Block {
+    int b, m0;  // b < 0: none
+};
+__device__ __forceinline__ Fp4Block fp4_block(const Fp4PagedArgs& p, int x) {
+    // Sequence s has the slots from cu[s] G / 128 + s on: never fewer than it has blocks.
+    const int lane = threadIdx.x & 63;
+    auto slot = [&](int s) { return (int)((int64_t)(s == 0 ? 0 : min(max(p.cu[s], 0), p.N)) * p.G / kFp4Rows) + s; };
+    int lo = 0, hi = p.B + 1;
+    while (hi - lo > 1) {
+        const int step = (hi - lo + 63) / 64, i = lo + (lane + 1) * step;
+        const bool below = i < hi && slot(i) <= x;
+        lo += (int)__popcll(__ballot(below)) * step;
+        hi = min(hi, lo + step);
+    }
+    const int s = __builtin_amdgcn_readfirstlane(lo);
+    if (s >= p.B) return {-1, 0};
+    return {s, (x - slot(s)) * kFp4Rows};
+}
+
+template <class E, int DP, bool P16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Fp4TileCfg<E, DP>::WPE)))
+void born_fp4_tiled_kernel(Fp4PagedArgs p) {
+    using C = Fp4TileCfg<E, DP>;
+    using Tile = PackedTile<BF16, DP, C::BN>;
+    constexpr int BN = C::BN, SUB = C::SUB, NB = C::NB, KS = DP / 16, DB = DP / 32, QP = kQParts<E>, IT = kItem<E>;
+    constexpr int PP = kTileParts<E>;
+    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * C::STAGE];
+    __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
+
+    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
+    const int split = rest % p.splits;
+    const Fp4Block blk = fp4_block(p, rest / p.splits);
+    if (blk.b < 0) return;
+    const Fp4Seq sq(p, blk.b);
+    const int rows = sq.nq * p.G, m0 = blk.m0;
+    if (!sq.wide(p) || m0 >= rows) return;
+
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int c = lane & 31, g = lane >> 5;
+    const int past = sq.n - sq.nq;  // keys before the first new token
+    const int m1 = min(rows, m0 + kFp4Rows) - 1;
+    // Keys that any row of the block sees, in tiles; this split's.
+    const int jlo = p.window > 0 ? max(0, past + m0 / p.G - p.window + 1) : 0, jhi = min(sq.n - 1, past + m1 / p.G);
+    const int first = jlo / BN, all = jhi >= jlo ? jhi / BN - first + 1 : 0;
+    const int per = (all + p.splits - 1) / p.splits, t0 = first + split * per, n = max(0, min(all - split * per, per));
+
+    // The wave's rows, the lane's.
+    const int rw = m0 + 32 * wave, row = rw + c;
+    const bool ok = row < rows;
+    const int tok = ok ? row / p.G : 0, head = hk * p.G + (ok ? row - tok * p.G : 0);
+    const int pos = past + tok;
+    const float sc = arg_scale(p, head);
+    u32x4 qr[KS][QP];
+    {
+        const uint8_t* at = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok) * p.q_st + (int64_t)head * p.q_sh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) fp4_query<E>(at, 16 * ks + 8 * g, p.D, ok, sc < 0.f, qr[ks]);
+    }
+    f32x16 acc[DB];
+#pragma unroll
+    for (int db = 0; db < DB; ++db) acc[db] = zero16();
+    float z = 0.f;
+
+    // A thread's key of each tile and its block; K and V of it, or one of them.
+    constexpr bool kOne = C::UNITS == 0;
+    const int key_in = DP == 256 ? 16 * (tid >> 7) + (tid & 15) : 16 * (tid >> 6) + (tid & 15);
+    const int bi = DP == 256 ? (tid >> 4) & 7 : DP == 128 ? (tid >> 4) & 3 : (tid >> 4) & 1;
+    const bool is_v = kOne && ((tid >> 5) & 1) != 0;
+    const bool in_row = bi < p.c.nb;
+    const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.t.table + (int64_t)blk.b * p.t.table_ld);
+    const uint8_t* const kc = p.c.k + (int64_t)hk * p.c.kh + 16 * bi;
+    const uint8_t* const vc = p.c.v + (int64_t)hk * p.c.vh + 16 * bi;
+    const uint8_t* const ksc = p.c.ks + (int64_t)hk * p.c.ksh + bi;
+    const uint8_t* const vsc = p.c.vs + (int64_t)hk * p.c.vsh + bi;
+
+    struct Codes {
+        u32x4 x[kOne ? 1 : 2];
+        uint32_t ks, vs;
+    };
+    Codes next;
+    // Page of the thread's key in tile t0 + u, -1: none.
+    auto page_of = [&](int u) __attribute__((always_inline)) {
+        int j = (t0 + u) * BN + key_in;
+        if constexpr (P16) {  // sixteen keys of a wave, one page: a scalar load
+            const int k0 = (t0 + u) * BN + (DP == 256 ? 16 * (wave >> 1) : 16 * wave);
+            const int i = __builtin_amdgcn_readfirstlane(fp4_page(p.c, min(k0, sq.n - 1)));
+            return (int)table[i];
+        } else {
+            return (int)table[fp4_page(p.c, min(j, sq.n - 1))];
+        }
+    };
+    auto fetch = [&](Codes& y, int u, int page) __attribute__((always_inline)) {
+        const int j = (t0 + u) * BN + key_in;
+        y.ks = y.vs = 0;
+#pragma unroll
+        for (int i = 0; i < (kOne ? 1 : 2); ++i) y.x[i] = u32x4{0u, 0u, 0u, 0u};
+        if (!(in_row && j < sq.n && page >= 0 && page < p.c.cache_pages)) return;
+        const int r = j - fp4_page(p.c, j) * p.c.page;
+        y.ks = ksc[page * p.c.ksp + (int64_t)r * p.c.kst];
+        y.vs = vsc[page * p.c.vsp + (int64_t)r * p.c.vst];
+        const uint8_t *ka = kc + page * p.c.kp + (int64_t)r * p.c.kt, *va = vc + page * p.c.vp + (int64_t)r * p.c.vt;
+        if constexpr (kOne) {
+            y.x[0] = ldg16(is_v ? va : ka);
+        } else {
+            y.x[0] = ldg16(ka);
+            y.x[1] = ldg16(va);
+        }
+    };
+    auto kt = [&](int st) { return Tile{ring + st * C::STAGE}; };
+    auto vt = [&](int st) { return Tile{ring + st * C::STAGE + C::BYTES}; };
+    auto put = [&](const Codes& y, int u) __attribute__((always_inline)) {
+        const int st = u & 1;
+        const bool bad = y.ks == kFp4Bad || y.vs == kFp4Bad;
+        const bool any_bad = __ballot(bad) != 0;
+        if (any_bad && lane == 0) bad_tile[st] = u;
+#pragma unroll
+        for (int i = 0; i < (kOne ? 1 : 2); ++i) {
+            const bool v = kOne ? is_v : i == 1;
+            const float s = fp4_scale(v ? y.vs : y.ks);
+            uint8_t* const to = ring + st * C::STAGE + (v ? C::BYTES : 0) + key_in * Tile::RB;
+#pragma unroll
+            for (int w = 0; w < 4; ++w) {
+                u32x4 x = fp4_eight(y.x[i][w], s);
+                if (any_bad && bad) x = v ? u32x4{0u, 0u, 0u, 0u} : u32x4{0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u, 0x7fc07fc0u};
+                *reinterpret_cast<u32x4*>(to + (((4 * bi + w) ^ Tile::swz(key_in)) << 4)) = x;
+            }
+        }
+    };
+
+    auto tile = [&](int u, int st, auto kind) __attribute__((always_inline)) {
+        const int key0 = (t0 + u) * BN;
+        const Tile k = kt(st), v = vt(st);
+        const bool bad_here = __builtin_amdgcn_readfirstlane(bad_tile[st]) == u;
+#pragma unroll
+        for (int nb = 0; nb < SUB; ++nb) {
+            f32x16 s = zero16();
+#pragma unroll
+            for (int ks = 0; ks < KS; ++ks) {
+                const u32x4 a = k.row(32 * nb + c, ks, g);
+#pragma unroll
+                for (int u2 = 0; u2 < QP; ++u2) s = BF16::mfma(a, qr[ks][u2], s);
+            }
+            if (bad_here) {  // the sum's NaN may have either sign, the weights take a positive one
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s[r] = s[r] == s[r] ? s[r] : __uint_as_float(0x7fc00000u);
+            }
+            if constexpr (kind.value == 2) {
+                const uint32_t span = p.window > 0 ? (uint32_t)p.window : 0x80000000u;
+                const int d = pos - key0 - 32 * nb;
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if ((uint32_t)(d - acc_row(r, g)) >= span) s[r] = 0.f;
+            }
+            uint32_t wt[8][PP];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if constexpr (PP == 1) {
+                    wt[j][0] = born_weight_pair<BF16>(s[2 * j], s[2 * j + 1], 1.f, z);
+                } else {
+                    const float a0 = relu_f32(s[2 * j]), a1 = relu_f32(s[2 * j + 1]);
+                    z = (z + a0 * a0) + a1 * a1;
+                    fp4_parts<PP>(a0 * a0, a1 * a1, wt[j]);
+                }
+            }
+#pragma unroll
+            for (int hh = 0; hh < 2; ++hh)
+#pragma unroll
+                for (int db = 0; db < DB; ++db) {
+                    const u32x4 a = v.transposed(32 * nb + 16 * hh, db, lane);
+#pragma unroll
+                    for (int k2 = 0; k2 < PP; ++k2) {
+                        const u32x4 w = {wt[4 * hh][k2], wt[4 * hh + 1][k2], wt[4 * hh + 2][k2], wt[4 * hh + 3][k2]};
+                        acc[db] = BF16::mfma(a, w, acc[db]);
+                    }
+                }
+        }
+    };
+
+    // Runs of tiles that the wave's rows see not at all, in part, whole: each
+    // a loop of its own.
+    const int a0 = p.window > 0 ? past + rw / p.G - p.window + 1 : 0, a1 = past + min(rw + 31, rows - 1) / p.G;
+    const int b0 = p.window > 0 ? past + min(rw + 31, rows - 1) / p.G - p.window + 1 : 0, b1 = past + rw / p.G;
+    const bool idle = rw >= rows;
+    const PackedRuns runs(n, t0 * BN, BN, BN, idle ? 1 << 30 : a0, idle ? 1 << 30 : a1, b0, b1);
+    if (n > 0) {
+        if (tid < 2) bad_tile[tid] = -1;
+        __syncthreads();
+        int page = page_of(0);
+        fetch(next, 0, page);
+        page = n > 1 ? page_of(1) : -1;
+        put(next, 0);
+        fetch(next, 1, page);
+        page = n > 2 ? page_of(2) : -1;
+        int u = 0;
+        auto run = [&](int end, auto kind) __attribute__((always_inline)) {
+            for (; u < end; ++u) {
+                __syncthreads();
+                if (u + 1 < n) {
+                    put(next, u + 1);
+                    if (u + 2 < n) fetch(next, u + 2, page);
+                    if (u + 3 < n) page = page_of(u + 3);
+                }
+                if constexpr (kind.value != 0) tile(u, u & 1, kind);
+            }
+        };
+        run(runs.ta, PackedIdle{});
+        run(runs.tf, PackedCut{});
+        run(runs.tg, PackedFull{});
+        run(runs.tv, PackedCut{});
+        run(n, PackedIdle{});
+    }
+    z += __shfl_xor(z, 32);
+    if (!ok) return;
+    const int64_t at = (int64_t)(sq.q0 + tok) * p.H + head;
+    if (p.splits > 1) {
+        float* to = p.wide_part + (at * p.splits + split) * (p.D + 4);
+        packed_store_row<F32>((uint8_t*)(to + 4), acc, 1.f, p.D, g);
+        if (g == 0) to[0] = z;
+    } else {
+        packed_store_row<E>((uint8_t*)p.out + at * p.D * IT, acc, fp4_inverse(p, head, z), p.D, g);
+    }
+}
+
+// The splits of the tiled kernel's rows, four columns a thread.
+template <class E>
+__global__ __launch_bounds__(256) void born_fp4_tiled_join_kernel(Fp4PagedArgs p) {
+    const int per = p.D / 4;
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= (int64_t)p.N * p.H * per) return;
+    const int col = 4 * (int)(i % per), head = (int)(i / per % p.H), t = (int)(i / per / p.H);
+    int lo = 0, hi = p.B;  // the last start at or before t
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) / 2;
+        if (p.cu[mid] <= t) lo = mid;
+        else hi = mid;
+    }
+    const Fp4Seq sq(p, lo);
+    if (t < sq.q0 || t >= sq.q0 + sq.nq || !sq.wide(p)) return;
+    const float* from = p.wide_part + ((int64_t)t * p.H + head) * p.splits * (p.D + 4);
+    f32x4v x = {0.f, 0.f, 0.f, 0.f};
+    float z = 0.f;
+    for (int k = 0; k < p.splits; ++k) {
+        z += from[(int64_t)k * (p.D + 4)];
+        x += *reinterpret_cast<const f32x4v*>(from + (int64_t)k * (p.D + 4) + 4 + col);
+    }
+    x *= fp4_inverse(p, head, z);
+    fp4_store4<E>((uint8_t*)p.out + ((int64_t)t * p.H + head) * p.D * kItem<E>, col, x);
+}
+
+template <class E, bool P16>
+void launch_fp4_tiled_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    const dim3 grid((unsigned)(plan.slots * plan.splits * a.Hkv));
+    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 64, P16>), grid, dim3(256), 0, st, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 128, P16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 256, P16>), grid, dim3(256), 0, st, a);
+}
+template <class E>
+hipError_t launch_fp4_tiled(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    if (a.c.page % 16 == 0) launch_fp4_tiled_dp<E, true>(a, plan, st);
+    else launch_fp4_tiled_dp<E, false>(a, plan, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || plan.splits == 1) return e;
+    const unsigned join = (unsigned)(((int64_t)a.N * a.H * (a.D / 4) + 255) / 256);
+    hipLaunchKernelGGL((born_fp4_tiled_join_kernel<E>), dim3(join), dim3(256), 0, st, a);
+    return hipGetLastError();
+}
+
+}  // namespace qdl

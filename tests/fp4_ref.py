@@ -5,7 +5,8 @@ Stored values are exact in bf16, so an overlap is an fp32 sum of exact products
 (the query's bf16 parts times the key): |dr| <= parts D 2^-24 sum |q k|.  The
 weights go into their product in two bf16 parts, what is left of them below
 2^-17 relative (each part takes half a step of 2^-8), fp32's in three, below two
-roundings of the square.  Sums of n terms are fp32 sums, the output is rounded
+roundings of the square; bf16's in one, half a step of 2^-8, where a sequence
+has more than 64 rows (new tokens x heads of a group).  Sums of n terms are fp32 sums, the output is rounded
 once."""
 
 from __future__ import annotations
@@ -77,13 +78,14 @@ def attend(q, cache, table, lens, scale, cu=None, eps=1e-12, window=0):
     s = s if s.numel() == H else s.repeat(H)
     o, eo = torch.zeros(N, H, D, dtype=torch.float64), torch.full((N, H, D), 1e-30, dtype=torch.float64)
     w_all, ew_all = torch.zeros(B, Hkv, room, dtype=torch.float64), torch.full((B, Hkv, room), 1e-30, dtype=torch.float64)
-    parts, up, u = PARTS[dt], WEIGHT[dt], HALF_STEP[dt]
+    parts, u = PARTS[dt], HALF_STEP[dt]
     for b in range(B):
         n, new = min(max(int(lens[b]), 0), room), cu[b + 1] - cu[b]
         k, v, ok, bad = rows(cache, table[b], n, D)
         if n == 0 or new == 0:
             continue
         i, j = n - new + torch.arange(new).view(-1, 1), torch.arange(n).view(1, -1)
+        up = HALF_STEP[dt] + 3 * U32 if dt is torch.bfloat16 and new * (H // Hkv) > 64 else WEIGHT[dt]
         keep = ok.view(1, -1) & (j <= i)
         if window > 0:
             keep = keep & (i - j < window)

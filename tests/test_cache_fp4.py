@@ -332,7 +332,7 @@ def test_argument_blocks_are_checked():
     assert rc("append", cos=P, rows=0) == -10 and rc("append", cos=P, rows=4, freqs=33, freq_ld=33) == -10
     assert rc("read", cu=0) == -5
     assert rc("paged", scale=P, n_scale=3) == -6 and rc("paged", window=-1) == -7 and rc("paged", ws=0) == -8 and rc("paged", ws_bytes=8) == -8
-    assert rc("paged", weight=P, cu=P) == -2 and rc("paged", n=1 << 27, B=1, cu=P) == -2
+    assert rc("paged", weight=P, cu=P) == -2 and rc("paged", n=1 << 28, H=256, B=1, cu=P, qs=(1 << 14, 64)) == -2
     assert rc("evict", budget=-1) == -16 and rc("evict", lens_out=P) == -2 and rc("evict", to=P) == -15 and rc("evict", kept=0) == -5
     assert rc("evict", weight=P, w_len=4, weight_out=P) == -2 and rc("evict", to=2 * P, to_pages=3, to_ld=2) == -15
     assert lib.qdl_flash_born_fp4_paged_workspace_size(2, 2, 4, 2, 64, 1 << 40, 1 << 24, 0, 0, 1) == 0
