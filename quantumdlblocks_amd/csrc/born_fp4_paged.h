@@ -66,47 +66,68 @@ struct Fp4Seq {
         first = p.window > 0 ? max(0, n - nq + 1 - p.window) : 0;
         first = min(first, n);
     }
+    __device__ __forceinline__ Fp4Seq of_lane(int l) const {
+        Fp4Seq r = *this;
+        r.q0 = __builtin_amdgcn_readlane(q0, l);
+        r.nq = __builtin_amdgcn_readlane(nq, l);
+        r.n = __builtin_amdgcn_readlane(n, l);
+        r.first = __builtin_amdgcn_readlane(first, l);
+        return r;
+    }
     __device__ __forceinline__ int base() const { return first & ~31; }
     __device__ __forceinline__ bool wide(const Fp4PagedArgs& p) const { return p.cu != nullptr && (int64_t)nq * p.G > p.limit; }
     // The narrow kernel's chunks are counted in steps of 128 keys.
     __device__ __forceinline__ int steps(const Fp4PagedArgs& p) const { return wide(p) ? 0 : max((n - base() + 127) >> 7, 1); }
 };
 
+// Inclusive sums over the lanes of a wave: lane 63 has the total.
+__device__ __forceinline__ int fp4_scan(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xf, 0xf, true);   // row_shr 1, 2, 4, 8
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xf, 0xf, true);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xa, 0xf, false);  // row_bcast 15 to rows 1 and 3
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xc, 0xf, false);  // row_bcast 31 to rows 2 and 3
+    return x;
+}
+
 struct Fp4Item {
     int b, split, nsplit, chunk;  // b < 0: none
+    Fp4Seq sq;
+    // In scalar registers: every wave has found one.
+    __device__ __forceinline__ Fp4Item uniform() const {
+        return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(split), __builtin_amdgcn_readfirstlane(nsplit),
+                __builtin_amdgcn_readfirstlane(chunk), sq.of_lane(0)};
+    }
 };
 
 // Chunk `item` of the launch, found by every wave for itself.
 __device__ __forceinline__ Fp4Item fp4_item(const Fp4PagedArgs& p, int item) {
-    if (p.items == 0) return {item < p.B ? item : -1, 0, 1, 1 << 30};
+    if (p.items == 0) return {item < p.B ? item : -1, 0, 1, 1 << 30, Fp4Seq(p, min(item, p.B - 1))};
     const int lane = threadIdx.x & 63;
-    int64_t total = 0;
-    int mine = 0;  // of the first 64 sequences
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        const int s = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps(p) : 0;
-        if (b0 == 0) mine = s;
-        total += s;
-    }
-    for (int o = 1; o < 64; o <<= 1) total += __shfl_xor(total, o);
-    const int step = (int)min(max((total + p.items - 1) / p.items, (int64_t)1), (int64_t)1 << 23);  // 2^30 keys: all
+    Fp4Seq mine(p, min(lane, p.B - 1));
+    int steps = lane < p.B ? mine.steps(p) : 0;
+    // 1024 sequences of 2^21 steps (2^28 keys; longer ones count as these) at most.
+    uint32_t total = (uint32_t)__builtin_amdgcn_readlane(fp4_scan(min(steps, 1 << 21)), 63);
+    for (int b0 = 64; b0 < p.B; b0 += 64)
+        total += (uint32_t)__builtin_amdgcn_readlane(fp4_scan(b0 + lane < p.B ? min(Fp4Seq(p, b0 + lane).steps(p), 1 << 21) : 0), 63);
+    int step = max((int)((total + (uint32_t)p.items - 1) / (uint32_t)p.items), 1);
+    if (step >= 1 << 21) step = 1 << 23;  // 2^30 keys: all of them
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
-        if (b0 > 0) mine = b0 + lane < p.B ? Fp4Seq(p, b0 + lane).steps(p) : 0;
-        const int k = (mine + step - 1) / step;
-        int run = k;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int y = __shfl_up(run, o);
-            if (lane >= o) run += y;
+        if (b0 > 0) {
+            mine = Fp4Seq(p, min(b0 + lane, p.B - 1));
+            steps = b0 + lane < p.B ? mine.steps(p) : 0;
         }
-        const int at = before + run - k;
+        const int k = (steps + step - 1) / step, run = fp4_scan(k), at = before + run - k;
         const uint64_t here = __ballot(at <= item && item < at + k);
         if (here != 0) {
-            const int l = __ffsll((long long)here) - 1;
-            return {b0 + l, item - __builtin_amdgcn_readlane(at, l), __builtin_amdgcn_readlane(k, l), step << 7};
+            const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)here) - 1);
+            return {b0 + l, item - __builtin_amdgcn_readlane(at, l), __builtin_amdgcn_readlane(k, l), step << 7, mine.of_lane(l)};
         }
         before += __builtin_amdgcn_readlane(run, 63);
     }
-    return {-1, 0, 1, 0};
+    return {-1, 0, 1, 0, mine};
 }
 
 __device__ __forceinline__ float fp4_inverse(const Fp4PagedArgs& p, int h, float z) {
@@ -122,6 +143,13 @@ struct Fp4Cfg {
     static constexpr int KS = KB * KW;                 // 32-column products
     static constexpr int VC = DP / 16, VD = (VC + 7) / 8;  // columns of a lane's key, dwords of codes
 };
+
+// Waves a SIMD should hold: of a column set's registers, and where the keys are
+// waited for.
+template <class E>
+constexpr int fp4_wpe(int DP, int NC) {
+    return DP == 256 ? 1 : NC == 2 ? (kQParts<E> < 3 || DP == 64 ? 2 : 1) : kQParts<E> == 1 || DP == 64 ? 3 : 2;
+}
 
 // A wave's 32 keys, as stored.
 template <class E, int DP>
@@ -147,10 +175,29 @@ __device__ __forceinline__ void fp4_load(uint32_t (&to)[DW], const uint8_t* p) {
     }
 }
 
+// The same by a buffer's scalar base and a lane's 32-bit offset.
+typedef __amdgpu_buffer_rsrc_t Fp4Rsrc;
+__device__ __forceinline__ Fp4Rsrc fp4_rsrc(const uint8_t* base) {
+    return __builtin_amdgcn_make_buffer_rsrc(const_cast<uint8_t*>(base), 0, 0x7fffffff, 0x00020000);
+}
+template <int DW>
+__device__ __forceinline__ void fp4_fetch(uint32_t (&to)[DW], Fp4Rsrc p, uint32_t offset) {
+    if constexpr (DW == 4) {
+        const u32x4 x = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(p, offset, 0, 0));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) to[i] = x[i];
+    } else {
+        const u32x2 x = __builtin_bit_cast(u32x2, __builtin_amdgcn_raw_buffer_load_b64(p, offset, 0, 0));
+        to[0] = x[0];
+        to[1] = x[1];
+    }
+}
+
 // DP: 64, 128 or 256 columns; NC: 16-row column sets; WEIGH: the raw weights are
 // written too (one token per sequence); P16: pages of a multiple of 16 tokens.
 template <class E, int DP, int NC, bool WEIGH, bool P16>
-__global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
+void born_fp4_paged_kernel(Fp4PagedArgs p) {
     using C = Fp4Cfg<E, DP>;
     constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
     constexpr int IT = kItem<E>;
@@ -168,10 +215,10 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
     }
     const int cb = blockIdx.x % p.cblocks, rest = blockIdx.x / p.cblocks;
     const int hk = rest % p.Hkv, item = rest / p.Hkv;
-    const Fp4Item it = fp4_item(p, item);
+    const Fp4Item it = fp4_item(p, item).uniform();
     if (it.b < 0) return;
-    const int b = __builtin_amdgcn_readfirstlane(it.b);
-    const Fp4Seq sq(p, b);
+    const int b = it.b;
+    const Fp4Seq& sq = it.sq;
     if (sq.wide(p)) return;
     if (it.split == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.nsplit};
     const int rows = sq.nq * p.G, c0 = 16 * NC * cb;
@@ -248,12 +295,6 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
             ovs[r] = (4 * j4 + r) * (uint32_t)p.c.vst + vb;
         }
     }
-    auto load_v = [&](Fp4Keys<E, DP>& x, int i, const uint8_t* vp, const uint8_t* vsp) __attribute__((always_inline)) {
-        if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
-        else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp);
-        else fp4_load<2>(x.v[i], vp);
-        x.vs[i] = *vsp;
-    };
     // Keys key0 + 16 t + m for K, key0 + 16 t + 4 j4 + i for V.
     auto load = [&](Fp4Keys<E, DP>& x, int key0) __attribute__((always_inline)) {
         if constexpr (P16) {
@@ -263,21 +304,28 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
                 const int j = key0 + 16 * t;
-                const int i = __builtin_amdgcn_readfirstlane(fp4_page(p.c, min(j, sq.n - 1)));
+                const int i = fp4_page(p.c, min(j, sq.n - 1));
                 const int32_t page = table[i];
                 x.there[t] = j < sq.n && page >= 0 && page < p.c.cache_pages;
-                const int64_t at = x.there[t] ? page : 0;
-                const int64_t row = x.there[t] ? j - i * p.c.page : 0;
-                const uint8_t *kp = kc + at * p.c.kp + row * p.c.kt, *ksp = ksc + at * p.c.ksp + row * p.c.kst;
-                const uint8_t *vp = vc + at * p.c.vp + row * p.c.vt, *vsp = vsc + at * p.c.vsp + row * p.c.vst;
+                const uint32_t at = x.there[t] ? page : 0, row = x.there[t] ? j - i * p.c.page : 0;
+                auto base = [&](const uint8_t* c, int64_t sp, int64_t st) __attribute__((always_inline)) {
+                    return fp4_rsrc(c + (uint64_t)at * (uint32_t)sp + row * (uint32_t)st);
+                };
+                const Fp4Rsrc kp = base(kc, p.c.kp, p.c.kt), ksp = base(ksc, p.c.ksp, p.c.kst);
+                const Fp4Rsrc vp = base(vc, p.c.vp, p.c.vt), vsp = base(vsc, p.c.vsp, p.c.vst);
 #pragma unroll
                 for (int a = 0; a < KB; ++a) {
-                    fp4_load<KW>(x.k[t][a], kp + ok_[a]);
-                    x.ks[t][a] = ksp[oks[a]];
-                    x.kvs[t][a] = vsp[okv[a]];
+                    fp4_fetch<KW>(x.k[t][a], kp, ok_[a]);
+                    x.ks[t][a] = __builtin_amdgcn_raw_buffer_load_b8(ksp, oks[a], 0, 0);
+                    x.kvs[t][a] = __builtin_amdgcn_raw_buffer_load_b8(vsp, okv[a], 0, 0);
                 }
 #pragma unroll
-                for (int r = 0; r < 4; ++r) load_v(x, 4 * t + r, vp + ov[r], vsp + ovs[r]);
+                for (int r = 0; r < 4; ++r) {
+                    if constexpr (VC == 4) x.v[4 * t + r][0] = __builtin_amdgcn_raw_buffer_load_b16(vp, ov[r], 0, 0);
+                    else if constexpr (VC == 8) x.v[4 * t + r][0] = __builtin_amdgcn_raw_buffer_load_b32(vp, ov[r], 0, 0);
+                    else fp4_fetch<2>(x.v[4 * t + r], vp, ov[r]);
+                    x.vs[4 * t + r] = __builtin_amdgcn_raw_buffer_load_b8(vsp, ovs[r], 0, 0);
+                }
             }
         } else {
             auto find = [&](int j, int64_t& page, int& row) {
@@ -311,7 +359,11 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
                 int64_t page;
                 int row;
                 if (find(key0 + 16 * (i >> 2) + 4 * j4 + (i & 3), page, row)) x.seen |= 1u << i;
-                load_v(x, i, vc + page * p.c.vp + (int64_t)row * p.c.vt + vo, vsc + page * p.c.vsp + (int64_t)row * p.c.vst + vb);
+                const uint8_t* vp = vc + page * p.c.vp + (int64_t)row * p.c.vt + vo;
+                if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
+                else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp);
+                else fp4_load<2>(x.v[i], vp);
+                x.vs[i] = vsc[page * p.c.vsp + (int64_t)row * p.c.vst + vb];
             }
         }
     };
@@ -392,19 +444,6 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
                     for (int d = 0; d < VD; ++d) x.v[n][d] = 0;
                 }
         }
-        // V: bf16, 8 keys of a lane's columns.
-        uint32_t vv[8][VC / 2];
-#pragma unroll
-        for (int n = 0; n < 8; ++n) {
-            const float sc = fp4_scale(x.vs[n]);
-#pragma unroll
-            for (int d = 0; d < VC / 2; d += 4) {
-                const u32x4 y = fp4_eight(x.v[n][d / 4], sc);
-#pragma unroll
-                for (int w = 0; w < 4; ++w)
-                    if (d + w < VC / 2) vv[n][d + w] = y[w];
-            }
-        }
         u32x4 wt[NC][PP];
 #pragma unroll
         for (int i = 0; i < NC; ++i) {
@@ -434,16 +473,35 @@ __global__ __launch_bounds__(256) void born_fp4_paged_kernel(Fp4PagedArgs p) {
                 for (int k = 0; k < PP; ++k) wt[i][k][n] = u[k];
             }
         }
+        // V two columns at a time: the keys' pairs of columns in bf16, regrouped
+        // to pairs of keys.
+        auto columns = [&](auto pair) __attribute__((always_inline)) {
+            constexpr int d = decltype(pair)::value;
+            uint32_t y[8];
 #pragma unroll
-        for (int e = 0; e < VC; ++e) {
-            u32x4 a;
+            for (int n = 0; n < 8; ++n) y[n] = fp4_pair<d & 3>(x.v[n][d / 4], fp4_scale(x.vs[n]));
 #pragma unroll
-            for (int n = 0; n < 4; ++n)
-                a[n] = __builtin_amdgcn_perm(vv[2 * n + 1][e >> 1], vv[2 * n][e >> 1], (e & 1) ? 0x07060302u : 0x05040100u);
+            for (int h = 0; h < 2; ++h) {
+                u32x4 a;
 #pragma unroll
-            for (int i = 0; i < NC; ++i)
+                for (int n = 0; n < 4; ++n) a[n] = __builtin_amdgcn_perm(y[2 * n + 1], y[2 * n], h ? 0x07060302u : 0x05040100u);
 #pragma unroll
-                for (int k = 0; k < PP; ++k) acc[i][e] = mfma16<BF16>(a, wt[i][k], acc[i][e]);
+                for (int i = 0; i < NC; ++i)
+#pragma unroll
+                    for (int k = 0; k < PP; ++k) acc[i][2 * d + h] = mfma16<BF16>(a, wt[i][k], acc[i][2 * d + h]);
+            }
+        };
+        columns(std::integral_constant<int, 0>{});
+        columns(std::integral_constant<int, 1>{});
+        if constexpr (VC >= 8) {
+            columns(std::integral_constant<int, 2>{});
+            columns(std::integral_constant<int, 3>{});
+        }
+        if constexpr (VC >= 16) {
+            columns(std::integral_constant<int, 4>{});
+            columns(std::integral_constant<int, 5>{});
+            columns(std::integral_constant<int, 6>{});
+            columns(std::integral_constant<int, 7>{});
         }
     };
     const int step = 32 * NW;
@@ -601,9 +659,10 @@ void launch_fp4_nc(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
 
 template <class E>
 hipError_t launch_fp4_paged(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    // Offsets within a page in 32 bits; a page 0 to send masked loads to.
+    // Pages' strides in 32 bits, rows' offsets within a page in 31.
     const int64_t far = (int64_t)1 << 31, page = a.c.page;
-    const bool p16 = a.c.page % 16 == 0 && page * a.c.kt < far && page * a.c.vt < far && page * a.c.kst < far && page * a.c.vst < far;
+    const bool p16 = a.c.page % 16 == 0 && page * a.c.kt < far && page * a.c.vt < far && page * a.c.kst < far && page * a.c.vst < far &&
+                     a.c.kp < 2 * far && a.c.vp < 2 * far && a.c.ksp < 2 * far && a.c.vsp < 2 * far;
     if (p16) launch_fp4_nc<E, true>(a, plan, st);
     else launch_fp4_nc<E, false>(a, plan, st);
     hipError_t e = hipGetLastError();
