@@ -111,7 +111,9 @@ __device__ __forceinline__ Fp4Item fp4_item(const Fp4PagedArgs& p, int item) {
     uint32_t total = (uint32_t)__builtin_amdgcn_readlane(fp4_scan(min(steps, 1 << 21)), 63);
     for (int b0 = 64; b0 < p.B; b0 += 64)
         total += (uint32_t)__builtin_amdgcn_readlane(fp4_scan(b0 + lane < p.B ? min(Fp4Seq(p, b0 + lane).steps(p), 1 << 21) : 0), 63);
-    int step = max((int)((total + (uint32_t)p.items - 1) / (uint32_t)p.items), 1);
+    // As many chunks as wanted, but no more than a third of them below 512 keys.
+    const uint32_t items = p.items, few = max(items / 3, 1u);
+    int step = max((int)max((total + items - 1) / items, min((total + few - 1) / few, 4u)), 1);
     if (step >= 1 << 21) step = 1 << 23;  // 2^30 keys: all of them
     int before = 0;
     for (int b0 = 0; b0 < p.B; b0 += 64) {
@@ -193,27 +195,31 @@ __device__ __forceinline__ void fp4_fetch(uint32_t (&to)[DW], Fp4Rsrc p, uint32_
     }
 }
 
-// DP: 64, 128 or 256 columns; NC: 16-row column sets; WEIGH: the raw weights are
-// written too (one token per sequence); P16: pages of a multiple of 16 tokens.
+// LDS of the narrow kernel: the waves' sums of 16 rows.
+template <int DP>
+constexpr int kFp4NarrowLds = 4 * 16 * (DP + 4 + 1) * 4;
+
+// Workgroup `block` of `blocks`.  DP: 64, 128 or 256 columns; NC: 16-row column
+// sets; WEIGH: the raw weights are written too (one token per sequence); P16:
+// pages of a multiple of 16 tokens.
 template <class E, int DP, int NC, bool WEIGH, bool P16>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
-void born_fp4_paged_kernel(Fp4PagedArgs p) {
+__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, uint8_t* smem, int block, int blocks) {
     using C = Fp4Cfg<E, DP>;
     constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
     constexpr int IT = kItem<E>;
-    __shared__ float red[NW][16][DP + 4];
-    __shared__ float zred[NW][16];
+    auto& red = *reinterpret_cast<float(*)[NW][16][DP + 4]>(smem);
+    auto& zred = *reinterpret_cast<float(*)[NW][16]>(smem + NW * 16 * (DP + 4) * 4);
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, j4 = lane >> 4;
     if (p.cu != nullptr) {
         // Rows behind the last sequence.
         const int last = min(max(p.cu[p.B], 0), p.N);
-        for (int r = last + blockIdx.x; r < p.N; r += gridDim.x)
+        for (int r = last + block; r < p.N; r += blocks)
             for (int i = threadIdx.x; i < p.H * p.D * IT / 16; i += 256)
                 *reinterpret_cast<u32x4*>((uint8_t*)p.out + (int64_t)r * p.H * p.D * IT + 16 * i) = u32x4{0u, 0u, 0u, 0u};
     }
-    const int cb = blockIdx.x % p.cblocks, rest = blockIdx.x / p.cblocks;
+    const int cb = block % p.cblocks, rest = block / p.cblocks;
     const int hk = rest % p.Hkv, item = rest / p.Hkv;
     const Fp4Item it = fp4_item(p, item).uniform();
     if (it.b < 0) return;
@@ -555,7 +561,14 @@ void born_fp4_paged_kernel(Fp4PagedArgs p) {
     }
 }
 
-// A row's partial sums.
+template <class E, int DP, int NC, bool WEIGH, bool P16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
+void born_fp4_paged_kernel(Fp4PagedArgs p) {
+    __shared__ __attribute__((aligned(16))) uint8_t smem[kFp4NarrowLds<DP>];
+    fp4_narrow<E, DP, NC, WEIGH, P16>(p, smem, blockIdx.x, gridDim.x);
+}
+
+// A narrow row's partial sums.
 struct Fp4Parts {
     const float* at;
     int64_t ld;
@@ -568,16 +581,22 @@ struct Fp4Parts {
     }
 };
 
-// Splits joined in order: one workgroup per row of a (sequence, key head),
-// `ncol` threads over the columns, 256 / ncol groups of them over the splits.
+// Splits joined in order.  A row's columns take `ncol` threads, its splits
+// `groups` of them, 256 / (ncol groups) rows a workgroup: first the narrow
+// kernel's rows (sequence, key head, row), then the tiled kernel's (token, head).
 // WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the sum
 // over the group of p_j / Z, the heads in order, is added to its weights.
+struct Fp4Join {
+    int ncol, groups, cols, most;
+    int64_t narrow, wide;  // rows
+    int blocks;            // workgroups of them
+};
 template <class E, bool WEIGH>
-__global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int ncol, int cols, int most) {
+__global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4Join q) {
     __shared__ f32x4v red[256];
     __shared__ float zred[256];
-    if (WEIGH && (int)blockIdx.x >= p.B * p.Hkv * most) {
-        const int x = blockIdx.x - p.B * p.Hkv * most, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
+    if (WEIGH && (int)blockIdx.x >= q.blocks) {
+        const int x = blockIdx.x - q.blocks, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
         const Fp4Seq sq(p, b);
         const int j0 = sq.base() + block * 256, j = j0 + threadIdx.x;
         if (j0 >= sq.n) return;
@@ -586,7 +605,7 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int 
         for (int g0 = 0; g0 < p.G; g0 += 256) {
             const int gn = min(256, p.G - g0);
             if ((int)threadIdx.x < gn) {
-                const Fp4Parts part(p, b, hk, g0 + threadIdx.x, cols);
+                const Fp4Parts part(p, b, hk, g0 + threadIdx.x, q.cols);
                 float z = 0.f;
 #pragma unroll 8
                 for (int i = 0; i < part.n; ++i) z += part.at[i * part.ld];
@@ -603,39 +622,63 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, int 
         if (seen) p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
         return;
     }
-    const int r = blockIdx.x % most, rest = blockIdx.x / most, hk = rest % p.Hkv, b = rest / p.Hkv;
-    const Fp4Seq sq(p, b);
-    if (sq.wide(p) || r >= sq.nq * p.G) return;
-    const Fp4Parts part(p, b, hk, r, cols);
-    if (part.n == 1) return;  // written already
-    const int col = threadIdx.x % ncol, group = threadIdx.x / ncol, groups = 256 / ncol;
-    const bool ok = 4 * col < p.D;
+    const int per = q.ncol * q.groups, mine = threadIdx.x / per, col = 4 * (threadIdx.x % q.ncol), group = threadIdx.x % per / q.ncol;
+    const int64_t unit = (int64_t)blockIdx.x * (256 / per) + mine;
+    const float* from = nullptr;
+    int64_t ld = 0, row = 0;  // row: token and head
+    int n = 0, head = 0;
+    if (unit < q.narrow) {
+        const int r = (int)(unit % q.most), hk = (int)(unit / q.most % p.Hkv), b = (int)(unit / q.most / p.Hkv);
+        const Fp4Seq sq(p, b);
+        if (!sq.wide(p) && r < sq.nq * p.G) {
+            const Fp4Parts part(p, b, hk, r, q.cols);
+            const int t = r / p.G;
+            head = hk * p.G + r - t * p.G;
+            row = (int64_t)(sq.q0 + t) * p.H + head;
+            if (part.n > 1) from = part.at, ld = part.ld, n = part.n;  // one: written already
+        }
+    } else if (unit < q.narrow + q.wide) {
+        row = unit - q.narrow;
+        head = (int)(row % p.H);
+        const int t = (int)(row / p.H);
+        int lo = 0, hi = p.B;  // the last start at or before t
+        while (hi - lo > 1) {
+            const int mid = (lo + hi) / 2;
+            if (p.cu[mid] <= t) lo = mid;
+            else hi = mid;
+        }
+        const Fp4Seq sq(p, lo);
+        if (t >= sq.q0 && t < sq.q0 + sq.nq && sq.wide(p)) from = p.wide_part + row * p.splits * (p.D + 4), ld = p.D + 4, n = p.splits;
+    }
+    const bool ok = col < p.D;
     f32x4v x = {0.f, 0.f, 0.f, 0.f};
     float z = 0.f;
 #pragma unroll 4
-    for (int i = group; i < part.n; i += groups) {
-        const float* at = part.at + i * part.ld;
+    for (int i = group; i < n; i += q.groups) {
+        const float* at = from + i * ld;
         z += at[0];
-        if (ok) x += *reinterpret_cast<const f32x4v*>(at + 4 + 4 * col);
+        if (ok) x += *reinterpret_cast<const f32x4v*>(at + 4 + col);
     }
-    red[threadIdx.x] = x;
-    zred[threadIdx.x] = z;
-    __syncthreads();
-    if (group != 0 || !ok) return;
-    for (int i = 1; i < groups; ++i) {
-        x += red[i * ncol + col];
-        z += zred[i * ncol + col];
+    if (q.groups > 1) {
+        red[threadIdx.x] = x;
+        zred[threadIdx.x] = z;
+        __syncthreads();
+        if (group != 0) return;
+        for (int i = 1; i < q.groups; ++i) {
+            x += red[threadIdx.x + i * q.ncol];
+            z += zred[threadIdx.x + i * q.ncol];
+        }
     }
-    const int t = r / p.G, h = hk * p.G + r - t * p.G;
-    x *= fp4_inverse(p, h, z);
-    fp4_store4<E>((uint8_t*)p.out + ((int64_t)(sq.q0 + t) * p.H + h) * p.D * kItem<E>, 4 * col, x);
+    if (n == 0 || !ok) return;
+    x *= fp4_inverse(p, head, z);
+    fp4_store4<E>((uint8_t*)p.out + row * p.D * kItem<E>, col, x);
 }
 
-// Rows of a launch's (sequence, key head): `most` at most; chunks: workgroups of each (key head, column block).
 struct Fp4Plan {
     int nc, cblocks, items, chunks, most, limit;
     int splits;     // of the tiled kernel
     int64_t slots;  // its blocks of rows; 0: no sequence is wide
+    Fp4Join join;
     int64_t plan_bytes, part_bytes, raw_bytes, wide_bytes, raw_ld;
     int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes + wide_bytes; }
 };
@@ -657,25 +700,21 @@ void launch_fp4_nc(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
     else launch_fp4_dp<E, 2, false, P16>(a, plan, st);
 }
 
+// Pages' strides in 32 bits, rows' offsets within a page in 31.
+inline bool fp4_p16(const Fp4Cache& c) {
+    const int64_t far = (int64_t)1 << 31, page = c.page;
+    return c.page % 16 == 0 && page * c.kt < far && page * c.vt < far && page * c.kst < far && page * c.vst < far && c.kp < 2 * far &&
+           c.vp < 2 * far && c.ksp < 2 * far && c.vsp < 2 * far;
+}
+
 template <class E>
-hipError_t launch_fp4_paged(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    // Pages' strides in 32 bits, rows' offsets within a page in 31.
-    const int64_t far = (int64_t)1 << 31, page = a.c.page;
-    const bool p16 = a.c.page % 16 == 0 && page * a.c.kt < far && page * a.c.vt < far && page * a.c.kst < far && page * a.c.vst < far &&
-                     a.c.kp < 2 * far && a.c.vp < 2 * far && a.c.ksp < 2 * far && a.c.vsp < 2 * far;
-    if (p16) launch_fp4_nc<E, true>(a, plan, st);
-    else launch_fp4_nc<E, false>(a, plan, st);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || (a.items == 0 && a.raw == nullptr)) return e;
-    int ncol = 2;
-    while (4 * ncol < a.D) ncol *= 2;
-    const unsigned join = (unsigned)((int64_t)a.B * a.Hkv * plan.most);
-    const int cols = 16 * plan.nc;
+hipError_t launch_fp4_join(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    const Fp4Join& q = plan.join;
     if (a.raw != nullptr) {
         const unsigned weigh = (unsigned)((a.raw_ld + 255) / 256 * a.B * a.Hkv);
-        hipLaunchKernelGGL((born_fp4_join_kernel<E, true>), dim3(join + weigh), dim3(256), 0, st, a, ncol, cols, plan.most);
-    } else {
-        hipLaunchKernelGGL((born_fp4_join_kernel<E, false>), dim3(join), dim3(256), 0, st, a, ncol, cols, plan.most);
+        hipLaunchKernelGGL((born_fp4_join_kernel<E, true>), dim3(q.blocks + weigh), dim3(256), 0, st, a, q);
+    } else if (q.blocks > 0) {
+        hipLaunchKernelGGL((born_fp4_join_kernel<E, false>), dim3(q.blocks), dim3(256), 0, st, a, q);
     }
     return hipGetLastError();
 }

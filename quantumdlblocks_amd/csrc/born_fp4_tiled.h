@@ -57,16 +57,12 @@ __device__ __forceinline__ Fp4Block fp4_block(const Fp4PagedArgs& p, int x) {
 }
 
 template <class E, int DP, bool P16>
-__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Fp4TileCfg<E, DP>::WPE)))
-void born_fp4_tiled_kernel(Fp4PagedArgs p) {
+__device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, uint8_t* ring, int* bad_tile, int block) {
     using C = Fp4TileCfg<E, DP>;
     using Tile = PackedTile<BF16, DP, C::BN>;
     constexpr int BN = C::BN, SUB = C::SUB, NB = C::NB, KS = DP / 16, DB = DP / 32, QP = kQParts<E>, IT = kItem<E>;
     constexpr int PP = kTileParts<E>;
-    __shared__ __attribute__((aligned(1024))) uint8_t ring[2 * C::STAGE];
-    __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
-
-    const int hk = blockIdx.x % p.Hkv, rest = blockIdx.x / p.Hkv;
+    const int hk = block % p.Hkv, rest = block / p.Hkv;
     const int split = rest % p.splits;
     const Fp4Block blk = fp4_block(p, rest / p.splits);
     if (blk.b < 0) return;
@@ -260,48 +256,39 @@ void born_fp4_tiled_kernel(Fp4PagedArgs p) {
     }
 }
 
-// The splits of the tiled kernel's rows, four columns a thread.
-template <class E>
-__global__ __launch_bounds__(256) void born_fp4_tiled_join_kernel(Fp4PagedArgs p) {
-    const int per = p.D / 4;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.N * p.H * per) return;
-    const int col = 4 * (int)(i % per), head = (int)(i / per % p.H), t = (int)(i / per / p.H);
-    int lo = 0, hi = p.B;  // the last start at or before t
-    while (hi - lo > 1) {
-        const int mid = (lo + hi) / 2;
-        if (p.cu[mid] <= t) lo = mid;
-        else hi = mid;
-    }
-    const Fp4Seq sq(p, lo);
-    if (t < sq.q0 || t >= sq.q0 + sq.nq || !sq.wide(p)) return;
-    const float* from = p.wide_part + ((int64_t)t * p.H + head) * p.splits * (p.D + 4);
-    f32x4v x = {0.f, 0.f, 0.f, 0.f};
-    float z = 0.f;
-    for (int k = 0; k < p.splits; ++k) {
-        z += from[(int64_t)k * (p.D + 4)];
-        x += *reinterpret_cast<const f32x4v*>(from + (int64_t)k * (p.D + 4) + 4 + col);
-    }
-    x *= fp4_inverse(p, head, z);
-    fp4_store4<E>((uint8_t*)p.out + ((int64_t)t * p.H + head) * p.D * kItem<E>, col, x);
+// Sequences of all sizes: workgroups of the tiled kernel's, then the narrow
+// one's, in one launch, so that neither waits for the other.
+template <class E, int DP, bool P16>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Fp4TileCfg<E, DP>::WPE)))
+void born_fp4_chunk_kernel(Fp4PagedArgs p, int tiled) {
+    constexpr int kTiles = 2 * Fp4TileCfg<E, DP>::STAGE, kBytes = kTiles > kFp4NarrowLds<DP> ? kTiles : kFp4NarrowLds<DP>;
+    __shared__ __attribute__((aligned(1024))) uint8_t smem[kBytes];
+    __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
+    if ((int)blockIdx.x < tiled) fp4_tiled<E, DP, P16>(p, smem, bad_tile, blockIdx.x);
+    else fp4_narrow<E, DP, 2, false, P16>(p, smem, blockIdx.x - tiled, gridDim.x - tiled);
 }
 
 template <class E, bool P16>
-void launch_fp4_tiled_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)(plan.slots * plan.splits * a.Hkv));
-    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 64, P16>), grid, dim3(256), 0, st, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 128, P16>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((born_fp4_tiled_kernel<E, 256, P16>), grid, dim3(256), 0, st, a);
+void launch_fp4_chunk(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    const int tiled = (int)(plan.slots * plan.splits * a.Hkv);
+    const dim3 grid((unsigned)(tiled + (int64_t)plan.chunks * a.Hkv * plan.cblocks));
+    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 64, P16>), grid, dim3(256), 0, st, a, tiled);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 128, P16>), grid, dim3(256), 0, st, a, tiled);
+    else hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 256, P16>), grid, dim3(256), 0, st, a, tiled);
 }
+
 template <class E>
-hipError_t launch_fp4_tiled(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    if (a.c.page % 16 == 0) launch_fp4_tiled_dp<E, true>(a, plan, st);
-    else launch_fp4_tiled_dp<E, false>(a, plan, st);
+hipError_t launch_fp4(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    const bool p16 = fp4_p16(a.c);
+    if (plan.slots > 0) {
+        if (p16) launch_fp4_chunk<E, true>(a, plan, st);
+        else launch_fp4_chunk<E, false>(a, plan, st);
+    } else {
+        if (p16) launch_fp4_nc<E, true>(a, plan, st);
+        else launch_fp4_nc<E, false>(a, plan, st);
+    }
     const hipError_t e = hipGetLastError();
-    if (e != hipSuccess || plan.splits == 1) return e;
-    const unsigned join = (unsigned)(((int64_t)a.N * a.H * (a.D / 4) + 255) / 256);
-    hipLaunchKernelGGL((born_fp4_tiled_join_kernel<E>), dim3(join), dim3(256), 0, st, a);
-    return hipGetLastError();
+    return e != hipSuccess ? e : launch_fp4_join<E>(a, plan, st);
 }
 
 }  // namespace qdl
