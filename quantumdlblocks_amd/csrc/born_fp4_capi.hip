@@ -69,70 +69,6 @@ void set_cache(qdl::Fp4Cache& a, qdl::Fp4Pages& t, const qdl_born_fp4_cache& c, 
     t.pages = (int)c.pages;
 }
 
-// Rows (new tokens x heads of a group) of a sequence up to which the narrow
-// kernel takes it.
-constexpr int64_t kNarrowRows = 64;
-constexpr int64_t kChunkBlocks = 1536;
-
-// How a call is shared out.  Chunks of the keys: at most two rounds of three
-// workgroups a compute unit; where a launch has more sequences than a workgroup
-// should look through, or nothing to split, one each.
-qdl::Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window, bool packed,
-                      bool weighed) {
-    qdl::Fp4Plan r = {};
-    const int64_t G = H / h_kv, room = pages * page;
-    int64_t most = G;
-    r.splits = 1;
-    if (packed) {
-        r.limit = kNarrowRows;
-        most = n * G < r.limit ? n * G : r.limit;
-        if (n * G > r.limit) {
-            const int64_t blocks = (n * G + qdl::kFp4Rows - 1) / qdl::kFp4Rows;
-            r.slots = n * G / qdl::kFp4Rows + B + 1;
-            // Two workgroups a compute unit, none under four tiles of 64 keys.
-            const int64_t span = window > 0 && window + qdl::kFp4Rows < room ? window + qdl::kFp4Rows : room;
-            int64_t splits = 512 / (blocks * h_kv);
-            if (splits > span / 256) splits = span / 256;
-            r.splits = (int)(splits < 1 ? 1 : splits);
-            if (r.splits > 1) r.wide_bytes = n * H * r.splits * (D + 4) * 4;
-        }
-    }
-    r.most = (int)most;
-    r.nc = !weighed && most > 16 && (!packed || r.slots > 0 || n * G > 16 * B) ? 2 : 1;
-    r.cblocks = (r.most + 16 * r.nc - 1) / (16 * r.nc);
-    int64_t items = 0;
-    if (B <= 1024 && room > 128) {
-        items = kChunkBlocks / (h_kv * r.cblocks);
-        if (items < 1) items = 1;
-    }
-    r.items = (int)items;
-    r.chunks = (int)(items + B);
-    r.plan_bytes = (B * 8 + 15) / 16 * 16;
-    int64_t span = window > 0 && window + 31 < room ? window + 31 : room;
-    if (span < 1) span = 1;
-    r.raw_ld = (span + 31) / 32 * 32;
-    if (items > 0 || weighed) r.part_bytes = (int64_t)r.chunks * h_kv * r.cblocks * 16 * r.nc * (D + 4) * 4;
-    if (weighed) r.raw_bytes = B * H * r.raw_ld * 4;
-
-    r.join.cols = 16 * r.nc;
-    r.join.most = r.most;
-    r.join.ncol = 2;
-    while (4 * r.join.ncol < D) r.join.ncol *= 2;
-    // Threads that share a row's splits: one for every eight that there may be.
-    const int64_t per = items / (B > 0 ? B : 1) + 1, longest = (span + 127) / 128, each = per < longest ? per : longest;
-    r.join.groups = 1;
-    while (r.join.groups * r.join.ncol < 256 && r.join.groups * 8 < each) r.join.groups *= 2;
-    if (items > 0) r.join.narrow = B * h_kv * r.most;
-    if (r.splits > 1) r.join.wide = n * H;
-    const int64_t rows = 256 / (r.join.ncol * r.join.groups), blocks = (r.join.narrow + r.join.wide + rows - 1) / rows;
-    r.join.blocks = (int)(blocks <= kMostBlocks ? blocks : kMostBlocks + 1);
-    return r;
-}
-bool fp4_plan_ok(const qdl::Fp4Plan& r, int64_t B, int64_t h_kv, bool weighed) {
-    const int64_t join = r.join.blocks + (weighed ? B * h_kv * (r.raw_ld / 256 + 1) : 0);
-    return r.slots * r.splits * h_kv + r.chunks * h_kv * r.cblocks <= kMostBlocks && join <= kMostBlocks;
-}
-
 int64_t append_blocks(int64_t n, int64_t rows, int lanes) {
     const int64_t per = 256 / lanes;
     return (n * rows + per - 1) / per;
@@ -253,7 +189,7 @@ int64_t qdl_flash_born_fp4_paged_workspace_size(int64_t n, int64_t B, int64_t H,
         pages < 0 || page_size < 1 || page_size > (int64_t)1 << 24 || pages > (int64_t)1 << 30 ||
         pages * page_size > (int64_t)1 << 30 || window_size < 0)
         return 0;
-    return fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0).bytes();
+    return qdl::fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0, kMostBlocks).bytes();
 }
 
 int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_stream_t stream) {
@@ -273,9 +209,9 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     const int64_t it = item(c->dtype);
     if (!rows_ok(c->q_strides, it)) return QDL_BORN_E_STRIDE;
     const bool weighed = c->key_weight != nullptr;
-    const qdl::Fp4Plan r = fp4_plan(c->n, c->B, c->H, c->h_kv, c->D, c->cache.pages, c->cache.page_size, c->window_size,
-                                    c->cu_seqlens != nullptr, weighed);
-    if (!fp4_plan_ok(r, c->B, c->h_kv, weighed)) return QDL_BORN_E_SHAPE;
+    const qdl::Fp4Plan r = qdl::fp4_plan(c->n, c->B, c->H, c->h_kv, c->D, c->cache.pages, c->cache.page_size, c->window_size,
+                                         c->cu_seqlens != nullptr, weighed, kMostBlocks);
+    if (!r.fits) return QDL_BORN_E_SHAPE;
     if (!c->workspace || !aligned16(c->workspace) || c->workspace_bytes < r.bytes()) return QDL_BORN_E_WORKSPACE;
     qdl::Fp4PagedArgs a = {};
     set_cache(a.c, a.t, c->cache, c->D);
@@ -296,6 +232,7 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     a.cblocks = r.cblocks;
     a.limit = r.limit;
     a.splits = r.splits;
+    a.slots = r.slots;
     a.eps = (float)c->eps;
     a.q_st = c->q_strides[0] * it;
     a.q_sh = c->q_strides[1] * it;

@@ -22,6 +22,7 @@
 #pragma once
 
 #include "born_fp4.h"
+#include "fp4_plan.h"
 
 namespace qdl {
 
@@ -40,6 +41,7 @@ struct Fp4PagedArgs {
     int cblocks;           // column blocks of a sequence
     int limit;             // rows of a (sequence, key head) that the narrow kernel takes
     int splits;            // of the tiled kernel's keys
+    int64_t slots;         // blocks of rows at most; 0: no sequence is wide
     float* wide_part;      // (N, H, splits, D + 4), where there are several
     float eps;
     int64_t q_st, q_sh;    // bytes
@@ -63,8 +65,7 @@ struct Fp4Seq {
             nq = max(min(p.cu[b + 1], p.N) - q0, 0);
         }
         n = p.c.cache_pages > 0 ? fp4_len(p.c, p.t, b) : 0;
-        first = p.window > 0 ? max(0, n - nq + 1 - p.window) : 0;
-        first = min(first, n);
+        first = fp4_first(n, nq, p.window);
     }
     __device__ __forceinline__ Fp4Seq of_lane(int l) const {
         Fp4Seq r = *this;
@@ -77,7 +78,9 @@ struct Fp4Seq {
     __device__ __forceinline__ int base() const { return first & ~31; }
     __device__ __forceinline__ bool wide(const Fp4PagedArgs& p) const { return p.cu != nullptr && (int64_t)nq * p.G > p.limit; }
     // The narrow kernel's chunks are counted in steps of 128 keys.
-    __device__ __forceinline__ int steps(const Fp4PagedArgs& p) const { return wide(p) ? 0 : max((n - base() + 127) >> 7, 1); }
+    __device__ __forceinline__ int steps(const Fp4PagedArgs& p) const { return wide(p) ? 0 : fp4_steps(n, first); }
+    // The tiled kernel's blocks of rows.
+    __device__ __forceinline__ int blocks(const Fp4PagedArgs& p) const { return wide(p) ? (nq * p.G + kFp4Rows - 1) / kFp4Rows : 0; }
 };
 
 // Inclusive sums over the lanes of a wave: lane 63 has the total.
@@ -91,51 +94,88 @@ __device__ __forceinline__ int fp4_scan(int x) {
     return x;
 }
 
-struct Fp4Item {
-    int b, split, nsplit, chunk;  // b < 0: none
-    Fp4Seq sq;
-    // In scalar registers: every wave has found one.
-    __device__ __forceinline__ Fp4Item uniform() const {
-        return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(split), __builtin_amdgcn_readfirstlane(nsplit),
-                __builtin_amdgcn_readfirstlane(chunk), sq.of_lane(0)};
+// How the device shares out a call, found by every wave for itself: chunks of
+// the narrow sequences' keys, blocks of the wide ones' rows.
+struct Fp4Share {
+    int step;          // steps of 128 keys in a chunk
+    int chunks, wide;  // how many there are
+    Fp4Seq mine;       // sequence `lane`
+
+    __device__ __forceinline__ Fp4Share(const Fp4PagedArgs& p) : step(1 << 23), chunks(p.B), wide((int)p.slots), mine(p, min(lane(), p.B - 1)) {
+        if (p.items == 0) return;  // too many sequences to look through: one chunk each, slots for blocks
+        uint64_t total = 0;  // 1024 sequences of 2^23 steps at most, 64 of them a scan
+        wide = 0;
+        each(p, [&](const Fp4Seq& s, int b0) {
+            const bool in = b0 + lane() < p.B;
+            total += (uint32_t)last(fp4_scan(in ? s.steps(p) : 0));
+            if (p.slots > 0) wide += last(fp4_scan(in ? s.blocks(p) : 0));
+            return false;
+        });
+        step = fp4_step(total, p.items);
+        chunks = 0;
+        each(p, [&](const Fp4Seq& s, int b0) {
+            chunks += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
+            return false;
+        });
+    }
+    __device__ __forceinline__ static int lane() { return threadIdx.x & 63; }
+    __device__ __forceinline__ static int last(int scan) { return __builtin_amdgcn_readlane(scan, 63); }
+    __device__ __forceinline__ int count(const Fp4PagedArgs& p, const Fp4Seq& s) const { return (s.steps(p) + step - 1) / step; }
+    // Every 64 sequences, until f is done.
+    template <class F>
+    __device__ __forceinline__ void each(const Fp4PagedArgs& p, F&& f) const {
+        if (f(mine, 0)) return;
+        for (int b0 = 64; b0 < p.B; b0 += 64)
+            if (f(Fp4Seq(p, min(b0 + lane(), p.B - 1)), b0)) return;
     }
 };
 
-// Chunk `item` of the launch, found by every wave for itself.
-__device__ __forceinline__ Fp4Item fp4_item(const Fp4PagedArgs& p, int item) {
-    if (p.items == 0) return {item < p.B ? item : -1, 0, 1, 1 << 30, Fp4Seq(p, min(item, p.B - 1))};
-    const int lane = threadIdx.x & 63;
-    Fp4Seq mine(p, min(lane, p.B - 1));
-    int steps = lane < p.B ? mine.steps(p) : 0;
-    // 1024 sequences of 2^21 steps (2^28 keys; longer ones count as these) at most.
-    uint32_t total = (uint32_t)__builtin_amdgcn_readlane(fp4_scan(min(steps, 1 << 21)), 63);
-    for (int b0 = 64; b0 < p.B; b0 += 64)
-        total += (uint32_t)__builtin_amdgcn_readlane(fp4_scan(b0 + lane < p.B ? min(Fp4Seq(p, b0 + lane).steps(p), 1 << 21) : 0), 63);
-    // As many chunks as wanted, but no more than a third of them below 512 keys.
-    const uint32_t items = p.items, few = max(items / 3, 1u);
-    int step = max((int)max((total + items - 1) / items, min((total + few - 1) / few, 4u)), 1);
-    if (step >= 1 << 21) step = 1 << 23;  // 2^30 keys: all of them
+// A sequence and which of its parts: scalars.
+struct Fp4Part {
+    int b, i, n;  // b < 0: none; part i of n
+    Fp4Seq sq;
+    __device__ __forceinline__ Fp4Part uniform() const {
+        return {__builtin_amdgcn_readfirstlane(b), __builtin_amdgcn_readfirstlane(i), __builtin_amdgcn_readfirstlane(n), sq.of_lane(0)};
+    }
+};
+// Part x of all, where sequence s has parts(s) of them.
+template <class F>
+__device__ __forceinline__ Fp4Part fp4_part(const Fp4PagedArgs& p, const Fp4Share& share, int x, F&& parts) {
+    Fp4Part r = {-1, 0, 1, share.mine};
     int before = 0;
-    for (int b0 = 0; b0 < p.B; b0 += 64) {
-        if (b0 > 0) {
-            mine = Fp4Seq(p, min(b0 + lane, p.B - 1));
-            steps = b0 + lane < p.B ? mine.steps(p) : 0;
-        }
-        const int k = (steps + step - 1) / step, run = fp4_scan(k), at = before + run - k;
-        const uint64_t here = __ballot(at <= item && item < at + k);
+    share.each(p, [&](const Fp4Seq& s, int b0) {
+        const int k = b0 + share.lane() < p.B ? parts(s) : 0, run = fp4_scan(k), at = before + run - k;
+        const uint64_t here = __ballot(at <= x && x < at + k);
         if (here != 0) {
             const int l = __builtin_amdgcn_readfirstlane(__ffsll((long long)here) - 1);
-            return {b0 + l, item - __builtin_amdgcn_readlane(at, l), __builtin_amdgcn_readlane(k, l), step << 7, mine.of_lane(l)};
+            r = {b0 + l, x - __builtin_amdgcn_readlane(at, l), __builtin_amdgcn_readlane(k, l), s.of_lane(l)};
+            return true;
         }
-        before += __builtin_amdgcn_readlane(run, 63);
-    }
-    return {-1, 0, 1, 0, mine};
+        before += share.last(run);
+        return false;
+    });
+    return r.uniform();
+}
+// Chunk `item`.
+__device__ __forceinline__ Fp4Part fp4_chunk(const Fp4PagedArgs& p, const Fp4Share& share, int item) {
+    if (p.items == 0) return {item, 0, 1, Fp4Seq(p, item)};
+    return fp4_part(p, share, item, [&](const Fp4Seq& s) { return share.count(p, s); });
 }
 
 __device__ __forceinline__ float fp4_inverse(const Fp4PagedArgs& p, int h, float z) {
     const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
     // A denominator that is not a number stays one.
     return s != 0.f ? (den < 0x1p-126f ? 0.f : 1.0f / den) : 0.f;
+}
+
+// Rows behind the last sequence: zeros, shared out over `blocks` workgroups.
+template <class E>
+__device__ __forceinline__ void fp4_behind(const Fp4PagedArgs& p, int block, int blocks) {
+    if (p.cu == nullptr) return;
+    const int last = min(max(p.cu[p.B], 0), p.N), pieces = p.H * p.D * kItem<E> / 16;
+    for (int r = last + block; r < p.N; r += blocks)
+        for (int i = threadIdx.x; i < pieces; i += 256)
+            *reinterpret_cast<u32x4*>((uint8_t*)p.out + ((int64_t)r * pieces + i) * 16) = u32x4{0u, 0u, 0u, 0u};
 }
 
 template <class E, int DP>
@@ -199,11 +239,11 @@ __device__ __forceinline__ void fp4_fetch(uint32_t (&to)[DW], Fp4Rsrc p, uint32_
 template <int DP>
 constexpr int kFp4NarrowLds = 4 * 16 * (DP + 4 + 1) * 4;
 
-// Workgroup `block` of `blocks`.  DP: 64, 128 or 256 columns; NC: 16-row column
+// Chunk and head `block` of its column block.  DP: 64, 128 or 256 columns; NC: 16-row column
 // sets; WEIGH: the raw weights are written too (one token per sequence); P16:
 // pages of a multiple of 16 tokens.
 template <class E, int DP, int NC, bool WEIGH, bool P16>
-__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, uint8_t* smem, int block, int blocks) {
+__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* smem, int block) {
     using C = Fp4Cfg<E, DP>;
     constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
     constexpr int IT = kItem<E>;
@@ -212,24 +252,17 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, uint8_t* smem,
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, j4 = lane >> 4;
-    if (p.cu != nullptr) {
-        // Rows behind the last sequence.
-        const int last = min(max(p.cu[p.B], 0), p.N);
-        for (int r = last + block; r < p.N; r += blocks)
-            for (int i = threadIdx.x; i < p.H * p.D * IT / 16; i += 256)
-                *reinterpret_cast<u32x4*>((uint8_t*)p.out + (int64_t)r * p.H * p.D * IT + 16 * i) = u32x4{0u, 0u, 0u, 0u};
-    }
-    const int cb = block % p.cblocks, rest = block / p.cblocks;
-    const int hk = rest % p.Hkv, item = rest / p.Hkv;
-    const Fp4Item it = fp4_item(p, item).uniform();
-    if (it.b < 0) return;
-    const int b = it.b;
+    // Column blocks in turn: few sequences have more than the first.
+    const int cb = block / (share.chunks * p.Hkv), rest = block - cb * share.chunks * p.Hkv;
+    const int item = rest / p.Hkv, hk = rest - item * p.Hkv;
+    const Fp4Part it = fp4_chunk(p, share, item);
+    const int b = it.b, chunk = share.step << 7;
     const Fp4Seq& sq = it.sq;
-    if (sq.wide(p)) return;
-    if (it.split == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.nsplit};
+    if (b < 0 || sq.wide(p)) return;
+    if (it.i == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.n};
     const int rows = sq.nq * p.G, c0 = 16 * NC * cb;
     if (c0 >= rows) return;
-    const int s0 = sq.base() + it.split * it.chunk, s1 = min(sq.n, s0 + it.chunk);
+    const int s0 = sq.base() + it.i * chunk, s1 = min(sq.n, s0 + chunk);
 
     // This lane's rows and the keys that each sees: [lo, hi].
     int tok[NC], head[NC], lo[NC], hi[NC];
@@ -548,12 +581,12 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, uint8_t* smem,
                 sum += zred[w][cc];
             }
             const int r = c0 + 16 * i + cc, t = r / p.G, h = hk * p.G + r - t * p.G;
-            if (it.nsplit > 1 || WEIGH) {
+            if (it.n > 1 || WEIGH) {
                 float* to = p.part + ((((int64_t)item * p.Hkv + hk) * p.cblocks + cb) * (16 * NC) + 16 * i + cc) * (p.D + 4);
                 *reinterpret_cast<f32x4v*>(to + 4 + col) = y;
                 if (col == 0) to[0] = sum;
             }
-            if (it.nsplit == 1) {
+            if (it.n == 1) {
                 y *= fp4_inverse(p, h, sum);
                 fp4_store4<E>((uint8_t*)p.out + ((int64_t)(sq.q0 + t) * p.H + h) * p.D * IT, col, y);
             }
@@ -565,7 +598,9 @@ template <class E, int DP, int NC, bool WEIGH, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
 void born_fp4_paged_kernel(Fp4PagedArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[kFp4NarrowLds<DP>];
-    fp4_narrow<E, DP, NC, WEIGH, P16>(p, smem, blockIdx.x, gridDim.x);
+    fp4_behind<E>(p, blockIdx.x, gridDim.x);
+    const Fp4Share share(p);
+    if ((int)blockIdx.x < share.chunks * p.Hkv * p.cblocks) fp4_narrow<E, DP, NC, WEIGH, P16>(p, share, smem, blockIdx.x);
 }
 
 // A narrow row's partial sums.
@@ -586,11 +621,6 @@ struct Fp4Parts {
 // kernel's rows (sequence, key head, row), then the tiled kernel's (token, head).
 // WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the sum
 // over the group of p_j / Z, the heads in order, is added to its weights.
-struct Fp4Join {
-    int ncol, groups, cols, most;
-    int64_t narrow, wide;  // rows
-    int blocks;            // workgroups of them
-};
 template <class E, bool WEIGH>
 __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4Join q) {
     __shared__ f32x4v red[256];
@@ -623,12 +653,12 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
         return;
     }
     const int per = q.ncol * q.groups, mine = threadIdx.x / per, col = 4 * (threadIdx.x % q.ncol), group = threadIdx.x % per / q.ncol;
-    const int64_t unit = (int64_t)blockIdx.x * (256 / per) + mine;
+    const int unit = blockIdx.x * (256 / per) + mine;
     const float* from = nullptr;
     int64_t ld = 0, row = 0;  // row: token and head
     int n = 0, head = 0;
     if (unit < q.narrow) {
-        const int r = (int)(unit % q.most), hk = (int)(unit / q.most % p.Hkv), b = (int)(unit / q.most / p.Hkv);
+        const int rest = unit / q.most, r = unit - rest * q.most, b = rest / p.Hkv, hk = rest - b * p.Hkv;
         const Fp4Seq sq(p, b);
         if (!sq.wide(p) && r < sq.nq * p.G) {
             const Fp4Parts part(p, b, hk, r, q.cols);
@@ -638,9 +668,9 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
             if (part.n > 1) from = part.at, ld = part.ld, n = part.n;  // one: written already
         }
     } else if (unit < q.narrow + q.wide) {
-        row = unit - q.narrow;
-        head = (int)(row % p.H);
-        const int t = (int)(row / p.H);
+        const int at = unit - q.narrow, t = at / p.H;
+        row = at;
+        head = at - t * p.H;
         int lo = 0, hi = p.B;  // the last start at or before t
         while (hi - lo > 1) {
             const int mid = (lo + hi) / 2;
@@ -653,7 +683,7 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
     const bool ok = col < p.D;
     f32x4v x = {0.f, 0.f, 0.f, 0.f};
     float z = 0.f;
-#pragma unroll 4
+#pragma unroll 8
     for (int i = group; i < n; i += q.groups) {
         const float* at = from + i * ld;
         z += at[0];
@@ -674,21 +704,12 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
     fp4_store4<E>((uint8_t*)p.out + row * p.D * kItem<E>, col, x);
 }
 
-struct Fp4Plan {
-    int nc, cblocks, items, chunks, most, limit;
-    int splits;     // of the tiled kernel
-    int64_t slots;  // its blocks of rows; 0: no sequence is wide
-    Fp4Join join;
-    int64_t plan_bytes, part_bytes, raw_bytes, wide_bytes, raw_ld;
-    int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes + wide_bytes; }
-};
-
 template <class E>
 hipError_t fp4_paged_fwd(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st);
 
 template <class E, int NC, bool WEIGH, bool P16>
 void launch_fp4_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)((int64_t)plan.chunks * a.Hkv * plan.cblocks));
+    const dim3 grid((unsigned)plan.grid);
     if (a.D <= 64) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 64, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 128, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((born_fp4_paged_kernel<E, 256, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);

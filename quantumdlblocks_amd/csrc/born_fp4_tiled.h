@@ -18,8 +18,6 @@
 
 namespace qdl {
 
-constexpr int kFp4Rows = 128;
-
 // bf16 parts of the weights.  bf16 outputs take one, rounded as the output is,
 // and Z adds the rounded weights, as in the packed forward: the matrix pipe
 // bounds this kernel, and the keys' own 4 bits are off by 60 times as much (8
@@ -36,11 +34,9 @@ struct Fp4TileCfg {
     static constexpr int WPE = DP == 256 ? 1 : 2;
 };
 
-// Rows of a workgroup: rows m0 .. of sequence b's new tokens x G.
-struct Fp4Block {
-    int b, m0;  // b < 0: none
-};
-__device__ __forceinline__ Fp4Block fp4_block(const Fp4PagedArgs& p, int x) {
+// Block x of rows: part i of a sequence's.
+__device__ __forceinline__ Fp4Part fp4_block(const Fp4PagedArgs& p, const Fp4Share& share, int x) {
+    if (p.items > 0) return fp4_part(p, share, x, [&](const Fp4Seq& s) { return s.blocks(p); });
     // Sequence s has the slots from cu[s] G / 128 + s on: never fewer than it has blocks.
     const int lane = threadIdx.x & 63;
     auto slot = [&](int s) { return (int)((int64_t)(s == 0 ? 0 : min(max(p.cu[s], 0), p.N)) * p.G / kFp4Rows) + s; };
@@ -52,23 +48,21 @@ __device__ __forceinline__ Fp4Block fp4_block(const Fp4PagedArgs& p, int x) {
         hi = min(hi, lo + step);
     }
     const int s = __builtin_amdgcn_readfirstlane(lo);
-    if (s >= p.B) return {-1, 0};
-    return {s, (x - slot(s)) * kFp4Rows};
+    const Fp4Seq sq(p, min(s, p.B - 1));
+    return Fp4Part{s < p.B ? s : -1, x - slot(s), 0, sq}.uniform();
 }
 
 template <class E, int DP, bool P16>
-__device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, uint8_t* ring, int* bad_tile, int block) {
+__device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* ring, int* bad_tile, int block) {
     using C = Fp4TileCfg<E, DP>;
     using Tile = PackedTile<BF16, DP, C::BN>;
     constexpr int BN = C::BN, SUB = C::SUB, NB = C::NB, KS = DP / 16, DB = DP / 32, QP = kQParts<E>, IT = kItem<E>;
     constexpr int PP = kTileParts<E>;
-    const int hk = block % p.Hkv, rest = block / p.Hkv;
-    const int split = rest % p.splits;
-    const Fp4Block blk = fp4_block(p, rest / p.splits);
-    if (blk.b < 0) return;
-    const Fp4Seq sq(p, blk.b);
-    const int rows = sq.nq * p.G, m0 = blk.m0;
-    if (!sq.wide(p) || m0 >= rows) return;
+    const int idx = block / p.Hkv, hk = block - idx * p.Hkv, split = idx / share.wide;
+    const Fp4Part blk = fp4_block(p, share, idx - split * share.wide);
+    const Fp4Seq& sq = blk.sq;
+    const int rows = sq.nq * p.G, m0 = blk.i * kFp4Rows;
+    if (blk.b < 0 || !sq.wide(p) || m0 >= rows) return;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
@@ -256,25 +250,29 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, uint8_t* ring, 
     }
 }
 
-// Sequences of all sizes: workgroups of the tiled kernel's, then the narrow
-// one's, in one launch, so that neither waits for the other.
+// Sequences of all sizes in one launch, so that neither kernel waits for the
+// other: the tiled one's workgroups, the narrow one's, and those of the grid
+// that the host could not know to be none.
 template <class E, int DP, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Fp4TileCfg<E, DP>::WPE)))
-void born_fp4_chunk_kernel(Fp4PagedArgs p, int tiled) {
+void born_fp4_chunk_kernel(Fp4PagedArgs p) {
     constexpr int kTiles = 2 * Fp4TileCfg<E, DP>::STAGE, kBytes = kTiles > kFp4NarrowLds<DP> ? kTiles : kFp4NarrowLds<DP>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kBytes];
     __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
-    if ((int)blockIdx.x < tiled) fp4_tiled<E, DP, P16>(p, smem, bad_tile, blockIdx.x);
-    else fp4_narrow<E, DP, 2, false, P16>(p, smem, blockIdx.x - tiled, gridDim.x - tiled);
+    fp4_behind<E>(p, blockIdx.x, gridDim.x);
+    const Fp4Share share(p);
+    const int tiled = share.wide * p.splits * p.Hkv, narrow = share.chunks * p.Hkv * p.cblocks;
+    const int x = blockIdx.x;
+    if (x < tiled) fp4_tiled<E, DP, P16>(p, share, smem, bad_tile, x);
+    else if (x < tiled + narrow) fp4_narrow<E, DP, 2, false, P16>(p, share, smem, x - tiled);
 }
 
 template <class E, bool P16>
 void launch_fp4_chunk(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const int tiled = (int)(plan.slots * plan.splits * a.Hkv);
-    const dim3 grid((unsigned)(tiled + (int64_t)plan.chunks * a.Hkv * plan.cblocks));
-    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 64, P16>), grid, dim3(256), 0, st, a, tiled);
-    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 128, P16>), grid, dim3(256), 0, st, a, tiled);
-    else hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 256, P16>), grid, dim3(256), 0, st, a, tiled);
+    const dim3 grid((unsigned)plan.grid);
+    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 64, P16>), grid, dim3(256), 0, st, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 128, P16>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 256, P16>), grid, dim3(256), 0, st, a);
 }
 
 template <class E>

@@ -1,0 +1,126 @@
+// How attention over the 4-bit cache is shared out: the host sizes launches and
+// workspaces from what it knows, the device shares out what is there by the same
+// rules.  Apart from the kernels, so that a host compiler takes it.
+#pragma once
+
+#include <cstdint>
+
+namespace qdl {
+
+constexpr int kFp4Rows = 128;  // rows (new tokens x heads of a group) of the tiled kernel's workgroups
+// Rows of a (sequence, key head) up to which the narrow kernel takes it.
+constexpr int kFp4Narrow = 64;
+// Workgroups of the narrow kernel that a launch's chunks of keys are made for:
+// two rounds of three a compute unit.
+constexpr int kFp4Wanted = 1536;
+// Sequences that a workgroup looks through to share out the keys.
+constexpr int kFp4Shared = 1024;
+
+// The first key that any of a sequence's nq new tokens sees, of n keys.
+constexpr int fp4_first(int n, int nq, int window) {
+    const int first = window > 0 && n - nq + 1 - window > 0 ? n - nq + 1 - window : 0;
+    return first < n ? first : n;
+}
+// Chunks are counted in steps of 128 keys, from a multiple of 32 on.
+constexpr int fp4_steps(int n, int first) {
+    const int steps = (n - (first & ~31) + 127) >> 7;
+    return steps > 1 ? steps : 1;
+}
+// Steps in a chunk, of `total` (up to 2^33) in a launch: as many chunks as
+// wanted, but no more than a third of them below 512 keys.
+constexpr int fp4_step(uint64_t total, uint32_t items) {
+    if (total >= (uint64_t)1 << 31) {  // in eights, rounded up
+        const uint64_t step = 8 * ((uint64_t)((uint32_t)(total >> 3) / items) + 2);
+        return (int)(step < (uint64_t)1 << 23 ? step : (uint64_t)1 << 23);  // 2^30 keys: all of a sequence
+    }
+    const uint32_t t = (uint32_t)total, few = items / 3 > 1 ? items / 3 : 1;
+    const uint32_t even = (t + items - 1) / items, some = (t + few - 1) / few;
+    const uint32_t step = even > (some < 4u ? some : 4u) ? even : (some < 4u ? some : 4u);
+    return (int)(step < 1u ? 1u : step < 1u << 23 ? step : 1u << 23);
+}
+
+struct Fp4Join {
+    int ncol, groups, cols, most;
+    int narrow, wide;  // rows
+    int blocks;        // workgroups of them
+};
+
+struct Fp4Plan {
+    int nc, cblocks;    // 16-row column sets of a narrow workgroup; column blocks of a sequence
+    int items, chunks;  // chunks wanted (0: one per sequence), and at most
+    int most, limit;    // rows of a narrow sequence
+    int splits;         // of a wide sequence's keys
+    int64_t slots;      // blocks of wide rows at most; 0: no sequence is wide
+    int64_t grid;       // workgroups
+    Fp4Join join;
+    int64_t plan_bytes, part_bytes, raw_bytes, wide_bytes, raw_ld;
+    bool fits;  // the launches, in what they are counted in
+    constexpr int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes + wide_bytes; }
+};
+
+// packed: several tokens a sequence; weighed: the keys' weights are kept.
+// kMost: workgroups of a launch at most.
+constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window,
+                           bool packed, bool weighed, int64_t kMost) {
+    Fp4Plan r = {};
+    const int64_t G = H / h_kv, room = pages * page;
+    auto seen = [=](int64_t tokens) {  // keys that a sequence's tokens see
+        const int64_t x = window > 0 && window + tokens - 1 < room ? window + tokens - 1 : room;
+        return x > 1 ? x : 1;
+    };
+    // Else every sequence is one chunk, and blocks of wide rows have slots by their starts.
+    const bool shared = B <= kFp4Shared && room > 128;
+    int64_t most = G;
+    r.splits = 1;
+    if (packed) {
+        r.limit = kFp4Narrow;
+        most = n * G < r.limit ? n * G : r.limit;
+        if (n * G > r.limit) {
+            const int64_t blocks = (n * G + kFp4Rows - 1) / kFp4Rows, some = n * G / (r.limit + 1);
+            r.slots = n * G / kFp4Rows + (!shared ? B + 1 : B < some ? B : some);
+            // Two workgroups a compute unit, none under two tiles of 64 keys.
+            int64_t splits = 512 / (blocks * h_kv);
+            if (splits > seen(kFp4Rows) / 128) splits = seen(kFp4Rows) / 128;
+            r.splits = (int)(splits < 1 ? 1 : splits);
+            if (r.splits > 1) r.wide_bytes = n * H * r.splits * (D + 4) * 4;
+        }
+    }
+    r.most = (int)most;
+    r.nc = !weighed && most > 16 && (!packed || r.slots > 0 || n * G > 16 * B) ? 2 : 1;
+    r.cblocks = (r.most + 16 * r.nc - 1) / (16 * r.nc);
+    int64_t items = 0;
+    if (shared) {
+        items = kFp4Wanted / (h_kv * r.cblocks);
+        if (items < 1) items = 1;
+    }
+    r.items = (int)items;
+    // No narrow sequence has more tokens than rows.
+    const int64_t longest = (seen(packed ? kFp4Narrow : 1) + 31 + 127) / 128;
+    r.chunks = (int)(items == 0 ? B : items + B < B * longest ? items + B : B * longest);
+    r.grid = r.slots * r.splits * h_kv + (int64_t)r.chunks * h_kv * r.cblocks;
+    r.plan_bytes = (B * 8 + 15) / 16 * 16;
+    if (items > 0 || weighed) r.part_bytes = (int64_t)r.chunks * h_kv * r.cblocks * 16 * r.nc * (D + 4) * 4;
+    r.raw_ld = (seen(1) + 31 + 31) / 32 * 32;
+    if (weighed) r.raw_bytes = B * H * r.raw_ld * 4;
+
+    r.join.cols = 16 * r.nc;
+    r.join.most = r.most;
+    r.join.ncol = 2;
+    while (4 * r.join.ncol < D) r.join.ncol *= 2;
+    // Threads that share a row's splits: one for every three that there may be.
+    const int64_t per = items / (B > 0 ? B : 1) + 1, each = per < longest ? per : longest;
+    r.join.groups = 1;
+    while (r.join.groups * r.join.ncol < 256 && r.join.groups * 3 < each) r.join.groups *= 2;
+    const int64_t narrow = items > 0 ? B * h_kv * r.most : 0, wide = r.splits > 1 ? n * H : 0;
+    const int64_t rows = 256 / (r.join.ncol * r.join.groups), blocks = (narrow + wide + rows - 1) / rows;
+    const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
+    r.fits = r.grid <= kMost && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    if (r.fits) {
+        r.join.narrow = (int)narrow;
+        r.join.wide = (int)wide;
+        r.join.blocks = (int)blocks;
+    }
+    return r;
+}
+
+}  // namespace qdl

@@ -4,6 +4,9 @@ one and of several tokens, evicting, refusals, and the C ABI's checks."""
 from __future__ import annotations
 
 import math
+import os
+import shutil
+import subprocess
 
 import pytest
 import torch
@@ -336,3 +339,73 @@ def test_argument_blocks_are_checked():
     assert rc("evict", budget=-1) == -16 and rc("evict", lens_out=P) == -2 and rc("evict", to=P) == -15 and rc("evict", kept=0) == -5
     assert rc("evict", weight=P, w_len=4, weight_out=P) == -2 and rc("evict", to=2 * P, to_pages=3, to_ld=2) == -15
     assert lib.qdl_flash_born_fp4_paged_workspace_size(2, 2, 4, 2, 64, 1 << 40, 1 << 24, 0, 0, 1) == 0
+
+
+SHARES = r"""
+#include <algorithm>
+#include <cstdio>
+#include <random>
+#include <vector>
+#include "%s"
+using namespace qdl;
+int main() {
+    std::mt19937_64 g(1);
+    auto upto = [&](int64_t most) { return (int64_t)(g() %% (uint64_t)(most + 1)); };
+    auto log_upto = [&](int bits) { return upto((int64_t)1 << upto(bits)); };
+    for (int round = 0; round < 200000; ++round) {
+        const int64_t B = 1 + upto(round %% 50 == 0 ? 3000 : 20), h_kv = 1 + upto(8), G = 1 + log_upto(6), H = h_kv * G, D = 64;
+        const int64_t page = 1 + log_upto(8), pages = log_upto(round %% 7 ? 10 : 22), room = pages * page;
+        const int64_t window = upto(2) ? 0 : 1 + log_upto(12);
+        const bool packed = upto(3) != 0, weighed = !packed && upto(1);
+        std::vector<int64_t> nq(B, 1), n(B);
+        int64_t N = 0;
+        for (int64_t b = 0; b < B; ++b) {
+            if (packed) nq[b] = upto(3) ? upto(8) : log_upto(10);
+            N += nq[b];
+            n[b] = upto(3) ? std::min(room, log_upto(30)) : room;
+        }
+        if (packed) N += upto(2);
+        if (!N || room > (int64_t)1 << 30) continue;
+        const Fp4Plan r = fp4_plan(N, B, H, h_kv, D, pages, page, window, packed, weighed, (1 << 24) - 1);
+        uint64_t total = 0;
+        int64_t wide = 0, chunks = 0;
+        auto is_wide = [&](int64_t b) { return packed && nq[b] * G > r.limit; };
+        auto steps = [&](int64_t b) { return is_wide(b) ? 0 : fp4_steps((int)n[b], fp4_first((int)n[b], (int)nq[b], (int)window)); };
+        for (int64_t b = 0; b < B; ++b) {
+            total += steps(b);
+            if (is_wide(b)) wide += (nq[b] * G + kFp4Rows - 1) / kFp4Rows;
+            if (!is_wide(b) && nq[b] * G > (int64_t)r.cblocks * 16 * r.nc) return printf("rows %%d\n", round), 1;
+            const int64_t base = fp4_first((int)n[b], (int)nq[b], (int)window) & ~31;
+            if (weighed && (n[b] - base + 31) / 32 * 32 > r.raw_ld) return printf("raw %%d\n", round), 1;
+        }
+        if (wide && !r.slots) return printf("no slots %%d\n", round), 1;
+        if (r.items > 0) {
+            const int64_t step = fp4_step(total, r.items);
+            for (int64_t b = 0; b < B; ++b) chunks += (steps(b) + step - 1) / step;
+            if (wide > r.slots) return printf("slots %%d\n", round), 1;
+        } else {
+            chunks = B;
+            for (int64_t b = 0; b < B; ++b)  // one chunk has to reach the end
+                if (n[b] > (int64_t)1 << 30) return 1;
+            if (r.slots && r.slots < N * G / kFp4Rows + B + 1) return printf("slots by starts %%d\n", round), 1;
+        }
+        if (chunks > r.chunks) return printf("chunks %%d: %%ld of %%d\n", round, (long)chunks, r.chunks), 1;
+        const int64_t parts = r.items > 0 || weighed ? (int64_t)r.chunks * h_kv * r.cblocks * 16 * r.nc * (D + 4) * 4 : 0;
+        if (r.part_bytes != parts || r.grid < (int64_t)r.chunks * h_kv * r.cblocks + (r.slots * r.splits) * h_kv) return 1;
+        if (r.fits && r.items > 0 && (int64_t)r.join.narrow != B * h_kv * r.most) return 1;
+    }
+    return 0;
+}
+"""
+
+
+def test_what_the_device_shares_out_fits_what_the_host_made_room_for(tmp_path):
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    header = os.path.join(os.path.dirname(born_fp4.__file__), "..", "csrc", "fp4_plan.h")
+    (tmp_path / "shares.cpp").write_text(SHARES % os.path.abspath(header))
+    subprocess.run([gxx, "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", str(tmp_path / "shares.cpp"), "-o",
+                    str(tmp_path / "shares")], check=True)
+    got = subprocess.run([str(tmp_path / "shares")], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr

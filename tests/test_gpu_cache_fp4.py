@@ -178,6 +178,13 @@ def test_several_tokens_long_and_mixed(cuda_device, dtype, D):
     _attend(cuda_device, [900], 32, 4, 4, D, DT[dtype], new=[1], scale=scale, eps=0.3, seed=10)
 
 
+@pytest.mark.parametrize("dtype", list(DT))
+def test_several_tokens_over_tables_of_one_step(cuda_device, dtype):
+    """No more than 128 keys a sequence: nothing to share out."""
+    _attend(cuda_device, [112, 90, 0, 7, 100], 16, 4, 2, 64, DT[dtype], new=[112, 50, 0, 7, 33], seed=11)
+    _attend(cuda_device, [100, 90, 3], 5, 6, 1, 128, DT[dtype], new=[1, 80, 3], window=40, seed=12)
+
+
 @pytest.mark.parametrize("several", [False, True])
 def test_missing_pages_lengths_and_bytes_of_nobody(cuda_device, several):
     new = [40, 60, 3] if several else None
@@ -434,6 +441,9 @@ def test_many_sequences(cuda_device):
     _attend(cuda_device, lens, 4, 2, 1, 32, torch.bfloat16, seed=30)
     _attend(cuda_device, lens, 4, 2, 1, 32, torch.bfloat16, new=[(i // 3) % 3 for i in range(1100)], seed=31)
     _attend(cuda_device, [40 * (i % 9) for i in range(130)], 16, 2, 1, 32, torch.bfloat16, seed=32)
+    _attend(cuda_device, [40 * (i % 9) for i in range(130)], 16, 2, 1, 32, torch.bfloat16, new=[(i % 5) * (i % 9) for i in range(130)], seed=33)
+    new = [70 if i in (3, 500, 1099) else i % 2 for i in range(1100)]
+    _attend(cuda_device, [2 * x + i % 5 for i, x in enumerate(new)], 16, 2, 1, 32, torch.bfloat16, new=new, seed=34)
 
 
 def test_empty_calls(cuda_device):
