@@ -503,8 +503,8 @@ int qdl_flash_born_cache_evict_call(const qdl_born_evict_call *call, qdl_stream_
  * nibble is the even column; sign, two exponent bits, one mantissa bit: 0, .5,
  * 1, 1.5, 2, 3, 4, 6) and nb scale bytes e; a value is its code times 2^(e - 127),
  * e = 255: not a number.  k, v: cache_pages pages of page_size tokens of h_kv
- * heads; *_strides (page, token, head) in bytes, the codes' multiples of 16, and
- * unit strides within a row.  Pages, tables and lengths as above.
+ * heads; *_strides (page, token, head) in bytes, under 2^32, the codes' multiples
+ * of 16, and unit strides within a row.  Pages, tables and lengths as above.
  */
 typedef struct qdl_born_fp4_cache {
     void *k, *v, *k_scale, *v_scale;

@@ -28,13 +28,19 @@ namespace qdl {
 constexpr int kFp4Block = 32;
 constexpr uint32_t kFp4Bad = 255;
 
-// Strides in bytes: page, token, head.
+// Strides in bytes: page, token, head; in 32 bits, so that an address takes one
+// multiplication a stride.
 struct Fp4Cache {
     uint8_t *k, *v, *ks, *vs;
-    int64_t kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh;
-    int64_t cache_pages;
+    uint32_t kp, kt, kh, vp, vt, vh, ksp, kst, ksh, vsp, vst, vsh;
+    int cache_pages;
     int page, page_shift, nb;  // tokens per page, its logarithm or -1; blocks of a row
 };
+
+// Row (page, token, head) of one of the tensors.
+__device__ __forceinline__ uint64_t fp4_at(uint32_t page, uint32_t sp, uint32_t row, uint32_t st, uint32_t head, uint32_t sh) {
+    return (uint64_t)page * sp + (uint64_t)row * st + (uint64_t)head * sh;
+}
 
 struct Fp4Pages {
     const int32_t* table;  // (B, pages)

@@ -31,8 +31,9 @@ struct Fp4AppendArgs {
     int table_rows, n_freq;
     int64_t freq_ld;
     double eps;
-    int lpr, lpw;      // lanes of a query row, of a stored row
-    int q_blocks;      // workgroups of queries, those of stored rows behind them
+    int lpr, lpw;       // lanes of a query row, of a stored row
+    int q_blocks;       // workgroups of queries; those of stored rows behind them:
+    int heads, tokens;  // groups of heads, of tokens
 };
 
 // Token t's slot: its sequence and its key there; in: it belongs to one.
@@ -62,7 +63,7 @@ struct Fp4Slot {
         slot = in ? (int64_t)lens[s] - ((int64_t)last - t) : -1;
     }
     // Page (-1: none) and row in it.
-    __device__ __forceinline__ int64_t page(const Fp4Cache& c, const Fp4Pages& t, int& row) const {
+    __device__ __forceinline__ int page(const Fp4Cache& c, const Fp4Pages& t, int& row) const {
         row = 0;
         if (slot < 0 || slot >= (int64_t)t.pages * c.page) return -1;
         const int i = fp4_page(c, (int)slot);
@@ -86,27 +87,31 @@ __device__ __forceinline__ float fp4_element(const uint8_t* row, int col) {
         return E::lo(*reinterpret_cast<const uint16_t*>(row + 2 * col));
     }
 }
-// Columns at .. at + 7, zeros past D or before 0.
+// Columns at .. at + 7 of a row as they are, zeros past D or before 0.
 template <class E>
-__device__ __forceinline__ void fp4_columns(const uint8_t* row, int at, int D, float (&x)[8]) {
-    if (at >= 0 && at + 8 <= D && (at * kItem<E>) % 16 == 0) {
-        if constexpr (std::is_same<E, F32>::value) {
+struct Fp4Eight {
+    static constexpr int W = kItem<E> / 2;
+    u32x4 u[W];
+    __device__ __forceinline__ void load(const uint8_t* row, int at, int D) {
+        if (at >= 0 && at + 8 <= D && (at * kItem<E>) % 16 == 0) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 y = ldg16(row + 4 * at + 16 * h);
-#pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * h + i] = __uint_as_float(y[i]);
-            }
+            for (int i = 0; i < W; ++i) u[i] = ldg16(row + kItem<E> * at + 16 * i);
         } else {
-            const u32x4 y = ldg16(row + 2 * at);
+            float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(y[i]), x[2 * i + 1] = E::hi(y[i]);
+            for (int i = 0; i < 8; ++i) x[i] = at + i >= 0 && at + i < D ? fp4_element<E>(row, at + i) : 0.f;
+#pragma unroll
+            for (int i = 0; i < 4 * W; ++i) {
+                if constexpr (std::is_same<E, F32>::value) u[i >> 2][i & 3] = __float_as_uint(x[i]);
+                else u[0][i] = E::pack(x[2 * i], x[2 * i + 1]);  // exact: they are E's
+            }
         }
-    } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = at + i >= 0 && at + i < D ? fp4_element<E>(row, at + i) : 0.f;
     }
-}
+    __device__ __forceinline__ float get(int i) const {
+        if constexpr (std::is_same<E, F32>::value) return __uint_as_float(u[i >> 2][i & 3]);
+        else return (i & 1) ? E::hi(u[0][i >> 1]) : E::lo(u[0][i >> 1]);
+    }
+};
 
 // The block's scale byte from its largest magnitude, kept as the upper 31 bits
 // of a double's magnitude with the lower ones as a sticky bit, and the exponent
@@ -125,53 +130,8 @@ __device__ __forceinline__ float fp4_scaled(uint32_t h, int e, double x) {
     return __uint_as_float(((uint32_t)u << 3) | ((uint32_t)(__builtin_bit_cast(uint64_t, x) >> 32) & 0x80000000u));
 }
 
-template <class E>
-__device__ __forceinline__ void fp4_append_row(const Fp4AppendArgs& p, int64_t item, int lane) {
-    const bool value = item >= (int64_t)p.N * p.Hkv;
-    if (value) item -= (int64_t)p.N * p.Hkv;
-    const int t = (int)(item / p.Hkv), h = (int)(item % p.Hkv);
-    const int c0 = 8 * lane, half = p.D >> 1;
-    const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
-    int row;
-    const int64_t page = slot.page(p.c, p.t, row);
-    if (page < 0) return;  // uniform in the row's lanes
-    const uint8_t* src = value ? (const uint8_t*)p.v + (int64_t)t * p.v_st + (int64_t)h * p.v_sh
-                               : (const uint8_t*)p.k + (int64_t)t * p.k_st + (int64_t)h * p.k_sh;
-    float x[8];
-    fp4_columns<E>(src, c0, p.D, x);
-    double y[8];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = x[i];
-    if (!value) {
-        double ss = 0.0;
-        if (c0 < p.D) {
-            // Columns c and c + D / 2 are a pair.  Eight from c0 on: all in one
-            // half where D is a multiple of 16.
-            float up[8], down[8];
-#pragma unroll
-            for (int i = 0; i < 8; ++i) up[i] = down[i] = 0.f;
-            if (c0 < half) fp4_columns<E>(src, c0 + half, p.D, up);
-            if (c0 + 8 > half) fp4_columns<E>(src, c0 - half, p.D, down);
-            const int64_t at = p.cos != nullptr ? fp4_angles(p, t, slot.slot) : 0;
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const bool low = c0 + i < half;
-                const int f = low ? c0 + i : c0 + i - half;
-                double c = 1.0, s = 0.0;
-                if (p.cos != nullptr && f < p.n_freq) c = p.cos[at + f], s = p.sin[at + f];
-                y[i] = low ? y[i] * c - (double)up[i] * s : (double)down[i] * s + y[i] * c;
-                ss += y[i] * y[i];
-            }
-        }
-        for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
-        const double f = 1.0 / sqrt(ss + p.eps);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) y[i] *= f;
-        if (c0 >= p.D) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) y[i] = 0.0;  // the padding of the last block, whatever the row
-        }
-    }
+// Eight columns of a stored row: codes and, from a block's first lane, its scale.
+__device__ __forceinline__ void fp4_store_row(const double (&y)[8], uint8_t* to, uint8_t* scale, int lane, bool in) {
     uint32_t u[8], top = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
@@ -183,8 +143,8 @@ __device__ __forceinline__ void fp4_append_row(const Fp4AppendArgs& p, int64_t i
     const int e = fp4_exponent(top);
     uint32_t codes = 0;
     if (e != (int)kFp4Bad - 127) {
-#define QDL_FP4_PACK(I)                                                                                                   \
-    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, fp4_scaled(u[2 * I], e, y[2 * I]),                              \
+#define QDL_FP4_PACK(I)                                                                                            \
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, fp4_scaled(u[2 * I], e, y[2 * I]),                       \
                                                      fp4_scaled(u[2 * I + 1], e, y[2 * I + 1]), 1.0f, I)
         QDL_FP4_PACK(0);
         QDL_FP4_PACK(1);
@@ -192,14 +152,77 @@ __device__ __forceinline__ void fp4_append_row(const Fp4AppendArgs& p, int64_t i
         QDL_FP4_PACK(3);
 #undef QDL_FP4_PACK
     }
-    if (lane >= 4 * p.c.nb) return;
-    const Fp4Cache& c = p.c;
-    uint8_t* to = value ? c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)h * c.vh : c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)h * c.kh;
+    if (!in) return;
     *reinterpret_cast<uint32_t*>(to + 4 * lane) = codes;
-    if ((lane & 3) == 0) {
-        uint8_t* s = value ? c.vs + page * c.vsp + (int64_t)row * c.vst + (int64_t)h * c.vsh
-                           : c.ks + page * c.ksp + (int64_t)row * c.kst + (int64_t)h * c.ksh;
-        s[lane >> 2] = (uint8_t)(e + 127);
+    if ((lane & 3) == 0) scale[lane >> 2] = (uint8_t)(e + 127);
+}
+
+// Keys or values of a token: `lpw` lanes, HEADS heads from h0 on, the token's
+// slot and angles found once.
+template <class E, int HEADS>
+__device__ __forceinline__ void fp4_append_rows(const Fp4AppendArgs& p, bool value, int t, int h0, int lane) {
+    const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
+    int row;
+    const int page = slot.page(p.c, p.t, row);
+    if (page < 0) return;  // uniform in the token's lanes
+    const int c0 = 8 * lane, half = p.D >> 1;
+    const bool in = lane < 4 * p.c.nb;
+    const Fp4Cache& c = p.c;
+    uint8_t* const to = value ? c.v + fp4_at(page, c.vp, row, c.vt, h0, c.vh) : c.k + fp4_at(page, c.kp, row, c.kt, h0, c.kh);
+    uint8_t* const scale = value ? c.vs + fp4_at(page, c.vsp, row, c.vst, h0, c.vsh) : c.ks + fp4_at(page, c.ksp, row, c.kst, h0, c.ksh);
+    const uint32_t th = value ? c.vh : c.kh, sh = value ? c.vsh : c.ksh;
+    const uint8_t* const src = value ? (const uint8_t*)p.v + (int64_t)t * p.v_st + (int64_t)h0 * p.v_sh
+                                     : (const uint8_t*)p.k + (int64_t)t * p.k_st + (int64_t)h0 * p.k_sh;
+    const int64_t hs = value ? p.v_sh : p.k_sh;
+    // Columns c and c + D / 2 are a pair.  Eight from c0 on: all in one half where
+    // D is a multiple of 16; `down` holds partners of the upper half's.
+    const bool both = c0 < half && c0 + 8 > half;
+    Fp4Eight<E> x[HEADS], up[HEADS], down[HEADS];
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        if (h0 + i >= p.Hkv) break;
+        x[i].load(src + i * hs, c0, p.D);
+        if (!value) {
+            up[i].load(src + i * hs, c0 < half ? c0 + half : c0 - half, p.D);
+            if (both) down[i].load(src + i * hs, c0 - half, p.D);
+        }
+    }
+    if (value) {
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            if (h0 + i >= p.Hkv) break;
+            double y[8];
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = x[i].get(e);
+            fp4_store_row(y, to + (uint64_t)i * th, scale + (uint64_t)i * sh, lane, in);
+        }
+        return;
+    }
+    float cs[8], sn[8];
+    const int64_t at = p.cos != nullptr ? fp4_angles(p, t, slot.slot) : 0;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+        const int f = c0 + e < half ? c0 + e : c0 + e - half;
+        cs[e] = 1.f, sn[e] = 0.f;
+        if (p.cos != nullptr && c0 < p.D && f < p.n_freq) cs[e] = p.cos[at + f], sn[e] = p.sin[at + f];
+    }
+#pragma unroll
+    for (int i = 0; i < HEADS; ++i) {
+        if (h0 + i >= p.Hkv) break;
+        double y[8], ss = 0.0;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const bool low = c0 + e < half;
+            const float other = both && !low ? down[i].get(e) : up[i].get(e);
+            y[e] = low ? (double)x[i].get(e) * cs[e] - (double)other * sn[e] : (double)other * sn[e] + (double)x[i].get(e) * cs[e];
+            ss += y[e] * y[e];
+        }
+        if (c0 >= p.D) ss = 0.0;
+        for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
+        const double f = 1.0 / sqrt(ss + p.eps);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) y[e] = c0 < p.D ? y[e] * f : 0.0;  // the padding of the last block, whatever the row
+        fp4_store_row(y, to + (uint64_t)i * th, scale + (uint64_t)i * sh, lane, in);
     }
 }
 
@@ -266,20 +289,26 @@ __global__ __launch_bounds__(256) void born_fp4_append_kernel(Fp4AppendArgs p) {
         fp4_append_queries<E, VEC, ROWS>(p, (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr, threadIdx.x & (p.lpr - 1));
         return;
     }
-    const int64_t item = (int64_t)(blockIdx.x - p.q_blocks) * (256 / p.lpw) + threadIdx.x / p.lpw;
-    if (item < 2 * (int64_t)p.N * p.Hkv) fp4_append_row<E>(p, item, threadIdx.x & (p.lpw - 1));
+    const int x = blockIdx.x - p.q_blocks, which = x / p.tokens, per = 256 / p.lpw;  // keys' groups of heads, then values'
+    const int t = (x - which * p.tokens) * per + threadIdx.x / p.lpw;
+    const bool value = which >= p.heads;
+    if (t < p.N) fp4_append_rows<E, ROWS>(p, value, t, ROWS * (value ? which - p.heads : which), threadIdx.x & (p.lpw - 1));
 }
 
 // ---------------------------------------------------------------------------
 // Read.  Rows (token, head) of a packed batch, each sequence's last keys, as
-// values: eight columns of K and of V a lane.
+// values: eight columns of K and of V a lane, `lpr` lanes a token, its slot found
+// once for four heads; the lanes' tokens follow each other, as a head's rows do in
+// the cache.
 // ---------------------------------------------------------------------------
+constexpr int kFp4ReadHeads = 4;
 struct Fp4ReadArgs {
     Fp4Cache c;
     Fp4Pages t;
     const int32_t* cu;
-    void *k, *v;  // (N, Hkv, D)
+    void *k, *v;     // (N, Hkv, D)
     int N, B, Hkv, D;
+    int lpr, heads;  // lanes of a row, groups of heads
 };
 
 template <class E>
@@ -301,24 +330,30 @@ __device__ __forceinline__ void fp4_put8(uint8_t* to, uint32_t codes, float scal
 
 template <class E>
 __global__ __launch_bounds__(256) void born_fp4_read_kernel(Fp4ReadArgs p) {
-    const int per = p.D / 8;
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= (int64_t)p.N * p.Hkv * per) return;
-    const int piece = (int)(i % per), h = (int)(i / per % p.Hkv), t = (int)(i / per / p.Hkv);
+    const int group = blockIdx.x % p.heads, h0 = kFp4ReadHeads * group, piece = threadIdx.x & (p.lpr - 1);
+    const int t = blockIdx.x / p.heads * (256 / p.lpr) + threadIdx.x / p.lpr;
+    if (t >= p.N || 8 * piece >= p.D) return;
     const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
     int row;
-    const int64_t page = slot.page(p.c, p.t, row);
-    uint32_t k = 0, v = 0;
-    float ks = 0.f, vs = 0.f;
-    if (page >= 0) {
-        const Fp4Cache& c = p.c;
-        k = *reinterpret_cast<const uint32_t*>(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)h * c.kh + 4 * piece);
-        v = *reinterpret_cast<const uint32_t*>(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)h * c.vh + 4 * piece);
-        ks = fp4_scale(c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)h * c.ksh + (piece >> 2)]);
-        vs = fp4_scale(c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)h * c.vsh + (piece >> 2)]);
+    const int page = slot.page(p.c, p.t, row);
+    const Fp4Cache& c = p.c;
+    uint32_t k[kFp4ReadHeads], v[kFp4ReadHeads], ks[kFp4ReadHeads], vs[kFp4ReadHeads];
+#pragma unroll
+    for (int i = 0; i < kFp4ReadHeads; ++i) {
+        k[i] = v[i] = ks[i] = vs[i] = 0;
+        if (page < 0 || h0 + i >= p.Hkv) continue;
+        k[i] = *reinterpret_cast<const uint32_t*>(c.k + fp4_at(page, c.kp, row, c.kt, h0 + i, c.kh) + 4 * piece);
+        v[i] = *reinterpret_cast<const uint32_t*>(c.v + fp4_at(page, c.vp, row, c.vt, h0 + i, c.vh) + 4 * piece);
+        ks[i] = c.ks[fp4_at(page, c.ksp, row, c.kst, h0 + i, c.ksh) + (piece >> 2)];
+        vs[i] = c.vs[fp4_at(page, c.vsp, row, c.vst, h0 + i, c.vsh) + (piece >> 2)];
     }
-    fp4_put8<E>((uint8_t*)p.k + i * 8 * kItem<E>, k, ks);
-    fp4_put8<E>((uint8_t*)p.v + i * 8 * kItem<E>, v, vs);
+    const int64_t at = (((int64_t)t * p.Hkv + h0) * p.D + 8 * piece) * kItem<E>;
+#pragma unroll
+    for (int i = 0; i < kFp4ReadHeads; ++i) {
+        if (h0 + i >= p.Hkv) break;
+        fp4_put8<E>((uint8_t*)p.k + at + (int64_t)i * p.D * kItem<E>, k[i], fp4_scale(ks[i]));
+        fp4_put8<E>((uint8_t*)p.v + at + (int64_t)i * p.D * kItem<E>, v[i], fp4_scale(vs[i]));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -333,20 +368,20 @@ struct Fp4EvictArgs {
 struct Fp4Row {
     u32x4 k, v;
     uint8_t ks, vs;
-    __device__ __forceinline__ void load(const Fp4Cache& c, int64_t page, int row, int hk, int piece, bool ok) {
+    __device__ __forceinline__ void load(const Fp4Cache& c, int page, int row, int hk, int piece, bool ok) {
         k = v = u32x4{0u, 0u, 0u, 0u};  // a missing page's rows are zeros
         ks = vs = 0;
         if (!ok) return;
-        k = ldg16(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)hk * c.kh + 16 * piece);
-        v = ldg16(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)hk * c.vh + 16 * piece);
-        ks = c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)hk * c.ksh + piece];
-        vs = c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)hk * c.vsh + piece];
+        k = ldg16(c.k + fp4_at(page, c.kp, row, c.kt, hk, c.kh) + 16 * piece);
+        v = ldg16(c.v + fp4_at(page, c.vp, row, c.vt, hk, c.vh) + 16 * piece);
+        ks = c.ks[fp4_at(page, c.ksp, row, c.kst, hk, c.ksh) + piece];
+        vs = c.vs[fp4_at(page, c.vsp, row, c.vst, hk, c.vsh) + piece];
     }
-    __device__ __forceinline__ void store(const Fp4Cache& c, int64_t page, int row, int hk, int piece) const {
-        *reinterpret_cast<u32x4*>(c.k + page * c.kp + (int64_t)row * c.kt + (int64_t)hk * c.kh + 16 * piece) = k;
-        *reinterpret_cast<u32x4*>(c.v + page * c.vp + (int64_t)row * c.vt + (int64_t)hk * c.vh + 16 * piece) = v;
-        c.ks[page * c.ksp + (int64_t)row * c.kst + (int64_t)hk * c.ksh + piece] = ks;
-        c.vs[page * c.vsp + (int64_t)row * c.vst + (int64_t)hk * c.vsh + piece] = vs;
+    __device__ __forceinline__ void store(const Fp4Cache& c, int page, int row, int hk, int piece) const {
+        *reinterpret_cast<u32x4*>(c.k + fp4_at(page, c.kp, row, c.kt, hk, c.kh) + 16 * piece) = k;
+        *reinterpret_cast<u32x4*>(c.v + fp4_at(page, c.vp, row, c.vt, hk, c.vh) + 16 * piece) = v;
+        c.ks[fp4_at(page, c.ksp, row, c.kst, hk, c.ksh) + piece] = ks;
+        c.vs[fp4_at(page, c.vsp, row, c.vst, hk, c.vsh) + piece] = vs;
     }
 };
 

@@ -28,12 +28,13 @@ int check_heads(int64_t dtype, int64_t H, int64_t h_kv, int64_t D) {
 }
 
 bool stride_ok(int64_t s, int64_t unit) { return s >= 0 && s <= (int64_t)1 << 40 && s % unit == 0; }
+bool cache_stride_ok(int64_t s, int64_t unit) { return stride_ok(s, unit) && s < (int64_t)1 << 32; }
 bool rows_ok(const int64_t st[2], int64_t it) { return stride_ok(st[0] * it, 16) && stride_ok(st[1] * it, 16); }
 
 int check_cache(const qdl_born_fp4_cache& c, int64_t B) {
     for (int i = 0; i < 3; ++i)
-        if (!stride_ok(c.k_strides[i], 16) || !stride_ok(c.v_strides[i], 16) || !stride_ok(c.k_scale_strides[i], 1) ||
-            !stride_ok(c.v_scale_strides[i], 1))
+        if (!cache_stride_ok(c.k_strides[i], 16) || !cache_stride_ok(c.v_strides[i], 16) || !cache_stride_ok(c.k_scale_strides[i], 1) ||
+            !cache_stride_ok(c.v_scale_strides[i], 1))
             return QDL_BORN_E_STRIDE;
     if (c.page_size < 1 || c.page_size > (int64_t)1 << 24 || c.cache_pages < 0 || c.cache_pages > INT32_MAX || c.pages < 0 ||
         c.table_ld < c.pages || c.pages > (int64_t)1 << 30 || c.pages * c.page_size > (int64_t)1 << 30)
@@ -55,11 +56,11 @@ void set_cache(qdl::Fp4Cache& a, qdl::Fp4Pages& t, const qdl_born_fp4_cache& c, 
     a.v = static_cast<uint8_t*>(c.v);
     a.ks = static_cast<uint8_t*>(c.k_scale);
     a.vs = static_cast<uint8_t*>(c.v_scale);
-    a.kp = c.k_strides[0], a.kt = c.k_strides[1], a.kh = c.k_strides[2];
-    a.vp = c.v_strides[0], a.vt = c.v_strides[1], a.vh = c.v_strides[2];
-    a.ksp = c.k_scale_strides[0], a.kst = c.k_scale_strides[1], a.ksh = c.k_scale_strides[2];
-    a.vsp = c.v_scale_strides[0], a.vst = c.v_scale_strides[1], a.vsh = c.v_scale_strides[2];
-    a.cache_pages = c.cache_pages;
+    a.kp = (uint32_t)c.k_strides[0], a.kt = (uint32_t)c.k_strides[1], a.kh = (uint32_t)c.k_strides[2];
+    a.vp = (uint32_t)c.v_strides[0], a.vt = (uint32_t)c.v_strides[1], a.vh = (uint32_t)c.v_strides[2];
+    a.ksp = (uint32_t)c.k_scale_strides[0], a.kst = (uint32_t)c.k_scale_strides[1], a.ksh = (uint32_t)c.k_scale_strides[2];
+    a.vsp = (uint32_t)c.v_scale_strides[0], a.vst = (uint32_t)c.v_scale_strides[1], a.vsh = (uint32_t)c.v_scale_strides[2];
+    a.cache_pages = (int)c.cache_pages;
     a.page = (int)c.page_size;
     a.page_shift = shift_of(c.page_size);
     a.nb = (int)((D + qdl::kFp4Block - 1) / qdl::kFp4Block);
@@ -132,9 +133,12 @@ int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call* c, qdl_stream
     while (a.lpr * vec < c->D / 2) a.lpr *= 2;
     a.lpw = 4;
     while (a.lpw < 4 * a.c.nb) a.lpw *= 2;
+    // Groups of four heads where single ones would fill the chip twice over.
     const bool many = c->n * c->H * a.lpr >= (int64_t)1 << 20;
     const int64_t queries = append_blocks(c->n, many ? (c->H + 3) / 4 : c->H, a.lpr);
-    const int64_t blocks = queries + (c->cache.cache_pages > 0 ? append_blocks(c->n, 2 * c->h_kv, a.lpw) : 0);
+    a.heads = many ? (int)((c->h_kv + 3) / 4) : (int)c->h_kv;
+    a.tokens = (int)append_blocks(c->n, 1, a.lpw);
+    const int64_t blocks = queries + (c->cache.cache_pages > 0 ? 2 * (int64_t)a.heads * a.tokens : 0);
     if (blocks > kMostBlocks) return QDL_BORN_E_SHAPE;
     a.q_blocks = (int)queries;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
@@ -163,8 +167,6 @@ int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call* c, qdl_stream_t s
     if (c->n == 0) return QDL_BORN_OK;
     if (!c->k_out || !c->v_out || !c->cu_seqlens) return QDL_BORN_E_NULL;
     if (!aligned16(c->k_out) || !aligned16(c->v_out)) return QDL_BORN_E_ALIGN;
-    const int64_t blocks = (c->n * c->h_kv * (c->D / 8) + 255) / 256;
-    if (blocks > kMostBlocks) return QDL_BORN_E_SHAPE;
     qdl::Fp4ReadArgs a = {};
     set_cache(a.c, a.t, c->cache, c->D);
     a.cu = c->cu_seqlens;
@@ -174,6 +176,11 @@ int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call* c, qdl_stream_t s
     a.B = (int)c->B;
     a.Hkv = (int)c->h_kv;
     a.D = (int)c->D;
+    a.lpr = 1;
+    while (a.lpr * 8 < c->D) a.lpr *= 2;
+    a.heads = (int)((c->h_kv + qdl::kFp4ReadHeads - 1) / qdl::kFp4ReadHeads);
+    const int64_t blocks = append_blocks(c->n, 1, a.lpr) * a.heads;
+    if (blocks > kMostBlocks) return QDL_BORN_E_SHAPE;
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (c->dtype) {
         case QDL_BORN_DTYPE_BF16: hipLaunchKernelGGL((qdl::born_fp4_read_kernel<qdl::BF16>), dim3((unsigned)blocks), dim3(256), 0, s, a); break;

@@ -314,8 +314,8 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
         vb = in ? VC * m / kFp4Block : 0;
     }
     const bool whole = kFp4Block * p.c.nb == DP;
-    const uint8_t *const kc = p.c.k + (int64_t)hk * p.c.kh, *const vc = p.c.v + (int64_t)hk * p.c.vh;
-    const uint8_t *const ksc = p.c.ks + (int64_t)hk * p.c.ksh, *const vsc = p.c.vs + (int64_t)hk * p.c.vsh;
+    const uint8_t *const kc = p.c.k + (uint64_t)hk * p.c.kh, *const vc = p.c.v + (uint64_t)hk * p.c.vh;
+    const uint8_t *const ksc = p.c.ks + (uint64_t)hk * p.c.ksh, *const vsc = p.c.vs + (uint64_t)hk * p.c.vsh;
     const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.t.table + (int64_t)b * p.t.table_ld);
 
     // Offsets of the lane's K rows (m) and V rows (4 j4 + r) within 16 keys of a
@@ -324,14 +324,14 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
     if constexpr (P16) {
 #pragma unroll
         for (int a = 0; a < KB; ++a) {
-            ok_[a] = m * (uint32_t)p.c.kt + ko[a];
-            oks[a] = m * (uint32_t)p.c.kst + kb[a];
-            okv[a] = m * (uint32_t)p.c.vst + kb[a];
+            ok_[a] = m * p.c.kt + ko[a];
+            oks[a] = m * p.c.kst + kb[a];
+            okv[a] = m * p.c.vst + kb[a];
         }
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            ov[r] = (4 * j4 + r) * (uint32_t)p.c.vt + vo;
-            ovs[r] = (4 * j4 + r) * (uint32_t)p.c.vst + vb;
+            ov[r] = (4 * j4 + r) * p.c.vt + vo;
+            ovs[r] = (4 * j4 + r) * p.c.vst + vb;
         }
     }
     // Keys key0 + 16 t + m for K, key0 + 16 t + 4 j4 + i for V.
@@ -347,8 +347,8 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
                 const int32_t page = table[i];
                 x.there[t] = j < sq.n && page >= 0 && page < p.c.cache_pages;
                 const uint32_t at = x.there[t] ? page : 0, row = x.there[t] ? j - i * p.c.page : 0;
-                auto base = [&](const uint8_t* c, int64_t sp, int64_t st) __attribute__((always_inline)) {
-                    return fp4_rsrc(c + (uint64_t)at * (uint32_t)sp + row * (uint32_t)st);
+                auto base = [&](const uint8_t* c, uint32_t sp, uint32_t st) __attribute__((always_inline)) {
+                    return fp4_rsrc(c + (uint64_t)at * sp + row * st);
                 };
                 const Fp4Rsrc kp = base(kc, p.c.kp, p.c.kt), ksp = base(ksc, p.c.ksp, p.c.kst);
                 const Fp4Rsrc vp = base(vc, p.c.vp, p.c.vt), vsp = base(vsc, p.c.vsp, p.c.vst);
@@ -367,25 +367,23 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
                 }
             }
         } else {
-            auto find = [&](int j, int64_t& page, int& row) {
+            auto find = [&](int j, uint32_t& page, uint32_t& row) {
                 const bool in = j >= sq.first && j < sq.n;
                 const int i = fp4_page(p.c, in ? j : 0);
-                row = (in ? j : 0) - i * p.c.page;
                 const int32_t y = in ? table[i] : -1;
                 const bool ok = y >= 0 && y < p.c.cache_pages;
                 page = ok ? y : 0;
-                row = ok ? row : 0;
+                row = ok ? j - i * p.c.page : 0;
                 return ok;
             };
             x.there[0] = x.there[1] = true;
             x.seen = 0;
 #pragma unroll
             for (int t = 0; t < 2; ++t) {
-                int64_t page;
-                int row;
+                uint32_t page, row;
                 find(key0 + 16 * t + m, page, row);
-                const uint8_t *kp = kc + page * p.c.kp + (int64_t)row * p.c.kt, *ksp = ksc + page * p.c.ksp + (int64_t)row * p.c.kst;
-                const uint8_t* vsp = vsc + page * p.c.vsp + (int64_t)row * p.c.vst;
+                const uint8_t *kp = kc + fp4_at(page, p.c.kp, row, p.c.kt, 0, 0), *ksp = ksc + fp4_at(page, p.c.ksp, row, p.c.kst, 0, 0);
+                const uint8_t* vsp = vsc + fp4_at(page, p.c.vsp, row, p.c.vst, 0, 0);
 #pragma unroll
                 for (int a = 0; a < KB; ++a) {
                     fp4_load<KW>(x.k[t][a], kp + ko[a]);
@@ -395,14 +393,13 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
             }
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                int64_t page;
-                int row;
+                uint32_t page, row;
                 if (find(key0 + 16 * (i >> 2) + 4 * j4 + (i & 3), page, row)) x.seen |= 1u << i;
-                const uint8_t* vp = vc + page * p.c.vp + (int64_t)row * p.c.vt + vo;
+                const uint8_t* vp = vc + fp4_at(page, p.c.vp, row, p.c.vt, 0, 0) + vo;
                 if constexpr (VC == 4) x.v[i][0] = *reinterpret_cast<const uint16_t*>(vp);
                 else if constexpr (VC == 8) x.v[i][0] = *reinterpret_cast<const uint32_t*>(vp);
                 else fp4_load<2>(x.v[i], vp);
-                x.vs[i] = vsc[page * p.c.vsp + (int64_t)row * p.c.vst + vb];
+                x.vs[i] = vsc[fp4_at(page, p.c.vsp, row, p.c.vst, 0, 0) + vb];
             }
         }
     };
@@ -721,11 +718,10 @@ void launch_fp4_nc(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
     else launch_fp4_dp<E, 2, false, P16>(a, plan, st);
 }
 
-// Pages' strides in 32 bits, rows' offsets within a page in 31.
+// Rows' offsets within a page in 31 bits.
 inline bool fp4_p16(const Fp4Cache& c) {
     const int64_t far = (int64_t)1 << 31, page = c.page;
-    return c.page % 16 == 0 && page * c.kt < far && page * c.vt < far && page * c.kst < far && page * c.vst < far && c.kp < 2 * far &&
-           c.vp < 2 * far && c.ksp < 2 * far && c.vsp < 2 * far;
+    return c.page % 16 == 0 && page * c.kt < far && page * c.vt < far && page * c.kst < far && page * c.vst < far;
 }
 
 template <class E>

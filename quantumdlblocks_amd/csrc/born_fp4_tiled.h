@@ -97,10 +97,10 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     const bool is_v = kOne && ((tid >> 5) & 1) != 0;
     const bool in_row = bi < p.c.nb;
     const ConstIntPtr table = (ConstIntPtr)(uintptr_t)(p.t.table + (int64_t)blk.b * p.t.table_ld);
-    const uint8_t* const kc = p.c.k + (int64_t)hk * p.c.kh + 16 * bi;
-    const uint8_t* const vc = p.c.v + (int64_t)hk * p.c.vh + 16 * bi;
-    const uint8_t* const ksc = p.c.ks + (int64_t)hk * p.c.ksh + bi;
-    const uint8_t* const vsc = p.c.vs + (int64_t)hk * p.c.vsh + bi;
+    const uint8_t* const kc = p.c.k + (uint64_t)hk * p.c.kh + 16 * bi;
+    const uint8_t* const vc = p.c.v + (uint64_t)hk * p.c.vh + 16 * bi;
+    const uint8_t* const ksc = p.c.ks + (uint64_t)hk * p.c.ksh + bi;
+    const uint8_t* const vsc = p.c.vs + (uint64_t)hk * p.c.vsh + bi;
 
     struct Codes {
         u32x4 x[kOne ? 1 : 2];
@@ -125,9 +125,9 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
         for (int i = 0; i < (kOne ? 1 : 2); ++i) y.x[i] = u32x4{0u, 0u, 0u, 0u};
         if (!(in_row && j < sq.n && page >= 0 && page < p.c.cache_pages)) return;
         const int r = j - fp4_page(p.c, j) * p.c.page;
-        y.ks = ksc[page * p.c.ksp + (int64_t)r * p.c.kst];
-        y.vs = vsc[page * p.c.vsp + (int64_t)r * p.c.vst];
-        const uint8_t *ka = kc + page * p.c.kp + (int64_t)r * p.c.kt, *va = vc + page * p.c.vp + (int64_t)r * p.c.vt;
+        y.ks = ksc[fp4_at(page, p.c.ksp, r, p.c.kst, 0, 0)];
+        y.vs = vsc[fp4_at(page, p.c.vsp, r, p.c.vst, 0, 0)];
+        const uint8_t *ka = kc + fp4_at(page, p.c.kp, r, p.c.kt, 0, 0), *va = vc + fp4_at(page, p.c.vp, r, p.c.vt, 0, 0);
         if constexpr (kOne) {
             y.x[0] = ldg16(is_v ? va : ka);
         } else {

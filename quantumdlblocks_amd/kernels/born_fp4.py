@@ -124,6 +124,8 @@ def _check_fp4(cache, block_table, cache_lens, B, head_dim, written: bool, apart
     if sk[3] != 1 or (k0 | k1 | k2 | pk) % 16 or sv[3] != 1 or (v0 | v1 | v2 | pv) % 16:
         raise ValueError(f"codes need unit stride along a row, other strides that are multiples of 16 and a 16-byte aligned base, "
                          f"got strides {sk} and {sv}")
+    if max(k0, k1, k2, v0, v1, v2) >> 32:
+        raise ValueError(f"a cache's strides lie under 2^32, got {sk} and {sv}")
     if nb > 1 and (sks[3] != 1 or svs[3] != 1):
         raise ValueError(f"scales need unit stride along a row, got strides {sks} and {svs}")
     return pk, pv, pks, pvs, k0, k1, k2, v0, v1, v2, *three(sks), *three(svs), P, page
