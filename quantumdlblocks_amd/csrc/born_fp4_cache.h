@@ -30,6 +30,7 @@ struct Fp4AppendArgs {
     int64_t q_st, q_sh, k_st, k_sh, v_st, v_sh;  // bytes
     int table_rows, n_freq;
     int64_t freq_ld;
+    int wide_tables;           // rows of whole, aligned 16-byte pieces
     double eps;
     int lpr, lpw;       // lanes of a query row, of a stored row
     int q_blocks;       // workgroups of queries; those of stored rows behind them:
@@ -74,7 +75,7 @@ struct Fp4Slot {
 };
 
 // Row of the rotary tables, as an offset.
-__device__ __forceinline__ int64_t fp4_angles(const Fp4AppendArgs& p, int t, int64_t slot) {
+__device__ __forceinline__ int64_t fp4_angle_row(const Fp4AppendArgs& p, int t, int64_t slot) {
     const int64_t at = p.positions != nullptr ? p.positions[t] : slot;
     return min(max(at, (int64_t)0), (int64_t)p.table_rows - 1) * p.freq_ld;  // rows past the tables: their last
 }
@@ -87,15 +88,17 @@ __device__ __forceinline__ float fp4_element(const uint8_t* row, int col) {
         return E::lo(*reinterpret_cast<const uint16_t*>(row + 2 * col));
     }
 }
-// Columns at .. at + 7 of a row as they are, zeros past D or before 0.
-template <class E>
+// Columns at .. at + 7 of a row as they are, zeros past D or before 0.  WHOLE: D
+// is a multiple of 16, so that eight columns from a multiple of eight are one
+// aligned piece, in one half of the row, or past it.
+template <class E, bool WHOLE>
 struct Fp4Eight {
     static constexpr int W = kItem<E> / 2;
     u32x4 u[W];
     __device__ __forceinline__ void load(const uint8_t* row, int at, int D) {
-        if (at >= 0 && at + 8 <= D && (at * kItem<E>) % 16 == 0) {
+        if constexpr (WHOLE) {
 #pragma unroll
-            for (int i = 0; i < W; ++i) u[i] = ldg16(row + kItem<E> * at + 16 * i);
+            for (int i = 0; i < W; ++i) u[i] = at < D ? ldg16(row + kItem<E> * at + 16 * i) : u32x4{0u, 0u, 0u, 0u};
         } else {
             float x[8];
 #pragma unroll
@@ -157,9 +160,33 @@ __device__ __forceinline__ void fp4_store_row(const double (&y)[8], uint8_t* to,
     if ((lane & 3) == 0) scale[lane >> 2] = (uint8_t)(e + 127);
 }
 
-// Keys or values of a token: `lpw` lanes, HEADS heads from h0 on, the token's
-// slot and angles found once.
-template <class E, int HEADS>
+// Heads of stored rows that a token's lanes go through, ROWS at a time.
+template <int ROWS>
+constexpr int kFp4AppendHeads = ROWS > 1 ? 8 : 1;
+
+// Angles f0 .. f0 + VEC - 1 of a row of the tables; 1 and 0 past their columns.
+template <int VEC>
+__device__ __forceinline__ void fp4_angles(const Fp4AppendArgs& p, int64_t row, int f0, float (&c)[VEC], float (&s)[VEC]) {
+    if (p.wide_tables && f0 + VEC <= p.n_freq) {  // f0: a multiple of 4
+#pragma unroll
+        for (int i = 0; i < VEC; i += 4) {
+            const f32x4v x = *reinterpret_cast<const f32x4v*>(p.cos + row + f0 + i), y = *reinterpret_cast<const f32x4v*>(p.sin + row + f0 + i);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) c[i + e] = x[e], s[i + e] = y[e];
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < VEC; ++i) {
+        const bool in = p.cos != nullptr && f0 + i < p.n_freq;
+        c[i] = in ? p.cos[row + f0 + i] : 1.f;
+        s[i] = in ? p.sin[row + f0 + i] : 0.f;
+    }
+}
+
+// Keys or values of a token: `lpw` lanes, heads from h0 on, HEADS at a time, the
+// token's slot and angles found once.
+template <class E, int HEADS, bool WHOLE>
 __device__ __forceinline__ void fp4_append_rows(const Fp4AppendArgs& p, bool value, int t, int h0, int lane) {
     const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
     int row;
@@ -168,61 +195,77 @@ __device__ __forceinline__ void fp4_append_rows(const Fp4AppendArgs& p, bool val
     const int c0 = 8 * lane, half = p.D >> 1;
     const bool in = lane < 4 * p.c.nb;
     const Fp4Cache& c = p.c;
-    uint8_t* const to = value ? c.v + fp4_at(page, c.vp, row, c.vt, h0, c.vh) : c.k + fp4_at(page, c.kp, row, c.kt, h0, c.kh);
-    uint8_t* const scale = value ? c.vs + fp4_at(page, c.vsp, row, c.vst, h0, c.vsh) : c.ks + fp4_at(page, c.ksp, row, c.kst, h0, c.ksh);
+    const int h1 = min(h0 + kFp4AppendHeads<HEADS>, p.Hkv);
+    uint8_t* const to = value ? c.v + fp4_at(page, c.vp, row, c.vt, 0, 0) : c.k + fp4_at(page, c.kp, row, c.kt, 0, 0);
+    uint8_t* const scale = value ? c.vs + fp4_at(page, c.vsp, row, c.vst, 0, 0) : c.ks + fp4_at(page, c.ksp, row, c.kst, 0, 0);
     const uint32_t th = value ? c.vh : c.kh, sh = value ? c.vsh : c.ksh;
-    const uint8_t* const src = value ? (const uint8_t*)p.v + (int64_t)t * p.v_st + (int64_t)h0 * p.v_sh
-                                     : (const uint8_t*)p.k + (int64_t)t * p.k_st + (int64_t)h0 * p.k_sh;
+    const uint8_t* const src = value ? (const uint8_t*)p.v + (int64_t)t * p.v_st : (const uint8_t*)p.k + (int64_t)t * p.k_st;
     const int64_t hs = value ? p.v_sh : p.k_sh;
-    // Columns c and c + D / 2 are a pair.  Eight from c0 on: all in one half where
-    // D is a multiple of 16; `down` holds partners of the upper half's.
-    const bool both = c0 < half && c0 + 8 > half;
-    Fp4Eight<E> x[HEADS], up[HEADS], down[HEADS];
-#pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
-        if (h0 + i >= p.Hkv) break;
-        x[i].load(src + i * hs, c0, p.D);
-        if (!value) {
-            up[i].load(src + i * hs, c0 < half ? c0 + half : c0 - half, p.D);
-            if (both) down[i].load(src + i * hs, c0 - half, p.D);
-        }
-    }
     if (value) {
+        for (int h = h0; h < h1; h += HEADS) {
+            Fp4Eight<E, WHOLE> x[HEADS];
 #pragma unroll
-        for (int i = 0; i < HEADS; ++i) {
-            if (h0 + i >= p.Hkv) break;
-            double y[8];
+            for (int i = 0; i < HEADS; ++i)
+                if (h + i < h1) x[i].load(src + (h + i) * hs, c0, p.D);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = x[i].get(e);
-            fp4_store_row(y, to + (uint64_t)i * th, scale + (uint64_t)i * sh, lane, in);
+            for (int i = 0; i < HEADS; ++i) {
+                if (h + i >= h1) break;
+                double y[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) y[e] = x[i].get(e);
+                fp4_store_row(y, to + (uint64_t)(h + i) * th, scale + (uint64_t)(h + i) * sh, lane, in);
+            }
         }
         return;
     }
+    // Columns c and c + D / 2 are a pair; where eight are of both halves, `down`
+    // holds the partners of the upper half's.
+    const bool both = !WHOLE && c0 < half && c0 + 8 > half;
     float cs[8], sn[8];
-    const int64_t at = p.cos != nullptr ? fp4_angles(p, t, slot.slot) : 0;
-#pragma unroll
-    for (int e = 0; e < 8; ++e) {
-        const int f = c0 + e < half ? c0 + e : c0 + e - half;
-        cs[e] = 1.f, sn[e] = 0.f;
-        if (p.cos != nullptr && c0 < p.D && f < p.n_freq) cs[e] = p.cos[at + f], sn[e] = p.sin[at + f];
-    }
-#pragma unroll
-    for (int i = 0; i < HEADS; ++i) {
-        if (h0 + i >= p.Hkv) break;
-        double y[8], ss = 0.0;
+    const int64_t at = p.cos != nullptr ? fp4_angle_row(p, t, slot.slot) : 0;
+    if (both) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
-            const bool low = c0 + e < half;
-            const float other = both && !low ? down[i].get(e) : up[i].get(e);
-            y[e] = low ? (double)x[i].get(e) * cs[e] - (double)other * sn[e] : (double)other * sn[e] + (double)x[i].get(e) * cs[e];
-            ss += y[e] * y[e];
+            const int f = c0 + e < half ? c0 + e : c0 + e - half;
+            const bool there = p.cos != nullptr && f < p.n_freq;
+            cs[e] = there ? p.cos[at + f] : 1.f;
+            sn[e] = there ? p.sin[at + f] : 0.f;
         }
-        if (c0 >= p.D) ss = 0.0;
-        for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
-        const double f = 1.0 / sqrt(ss + p.eps);
+    } else if (c0 < p.D) {
+        fp4_angles(p, at, c0 < half ? c0 : c0 - half, cs, sn);
+    } else {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) y[e] = c0 < p.D ? y[e] * f : 0.0;  // the padding of the last block, whatever the row
-        fp4_store_row(y, to + (uint64_t)i * th, scale + (uint64_t)i * sh, lane, in);
+        for (int e = 0; e < 8; ++e) cs[e] = 1.f, sn[e] = 0.f;
+    }
+    for (int h = h0; h < h1; h += HEADS) {
+        Fp4Eight<E, WHOLE> x[HEADS], up[HEADS], down[WHOLE ? 1 : HEADS];
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            if (h + i >= h1) break;
+            const uint8_t* from = src + (h + i) * hs;
+            x[i].load(from, c0, p.D);
+            up[i].load(from, c0 < half ? c0 + half : c0 < p.D ? c0 - half : p.D, p.D);
+            if constexpr (!WHOLE) down[i].load(from, both ? c0 - half : p.D, p.D);
+        }
+#pragma unroll
+        for (int i = 0; i < HEADS; ++i) {
+            if (h + i >= h1) break;
+            double y[8], ss = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const bool low = (WHOLE ? c0 : c0 + e) < half;
+                float other = up[i].get(e);
+                if constexpr (!WHOLE) other = both && !low ? down[i].get(e) : other;
+                y[e] = low ? (double)x[i].get(e) * cs[e] - (double)other * sn[e] : (double)other * sn[e] + (double)x[i].get(e) * cs[e];
+                ss += y[e] * y[e];
+            }
+            if (c0 >= p.D) ss = 0.0;
+            for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
+            const double f = 1.0 / sqrt(ss + p.eps);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) y[e] = c0 < p.D ? y[e] * f : 0.0;  // the padding of the last block, whatever the row
+            fp4_store_row(y, to + (uint64_t)(h + i) * th, scale + (uint64_t)(h + i) * sh, lane, in);
+        }
     }
 }
 
@@ -237,16 +280,7 @@ __device__ __forceinline__ void fp4_append_queries(const Fp4AppendArgs& p, int64
     const int o1 = lane * VEC * kItem<E>, o2 = o1 + half * kItem<E>;
     const Fp4Slot slot(p.cu, p.t.lens, p.B, t);
     float c[VEC], sn[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; ++i) c[i] = 1.f, sn[i] = 0.f;
-    if (p.cos != nullptr && own) {
-        const int64_t at = fp4_angles(p, t, slot.slot);
-#pragma unroll
-        for (int i = 0; i < VEC; ++i) {
-            const int f = lane * VEC + i;
-            if (f < p.n_freq) c[i] = p.cos[at + f], sn[i] = p.sin[at + f];
-        }
-    }
+    fp4_angles(p, p.cos != nullptr ? fp4_angle_row(p, t, slot.slot) : 0, own ? lane * VEC : 0, c, sn);
     RowVec<E, VEC> x1[ROWS], x2[ROWS];
 #pragma unroll
     for (int i = 0; i < ROWS; ++i) {
@@ -283,16 +317,17 @@ __device__ __forceinline__ void fp4_append_queries(const Fp4AppendArgs& p, int64
     }
 }
 
-template <class E, int VEC, int ROWS>
+template <class E, int VEC, int ROWS, bool WHOLE>
 __global__ __launch_bounds__(256) void born_fp4_append_kernel(Fp4AppendArgs p) {
     if ((int)blockIdx.x < p.q_blocks) {
         fp4_append_queries<E, VEC, ROWS>(p, (int64_t)blockIdx.x * (256 / p.lpr) + threadIdx.x / p.lpr, threadIdx.x & (p.lpr - 1));
         return;
     }
-    const int x = blockIdx.x - p.q_blocks, which = x / p.tokens, per = 256 / p.lpw;  // keys' groups of heads, then values'
+    const int x = blockIdx.x - p.q_blocks;
+    const int which = x / p.tokens, per = 256 / p.lpw;  // keys' groups of heads, then values'
     const int t = (x - which * p.tokens) * per + threadIdx.x / p.lpw;
     const bool value = which >= p.heads;
-    if (t < p.N) fp4_append_rows<E, ROWS>(p, value, t, ROWS * (value ? which - p.heads : which), threadIdx.x & (p.lpw - 1));
+    if (t < p.N) fp4_append_rows<E, ROWS, WHOLE>(p, value, t, kFp4AppendHeads<ROWS> * (value ? which - p.heads : which), threadIdx.x & (p.lpw - 1));
 }
 
 // ---------------------------------------------------------------------------

@@ -75,10 +75,10 @@ int64_t append_blocks(int64_t n, int64_t rows, int lanes) {
     return (n * rows + per - 1) / per;
 }
 
-template <class E, int VEC>
+template <class E, int VEC, bool WHOLE>
 void launch_append(const qdl::Fp4AppendArgs& a, bool many, int64_t blocks, hipStream_t st) {
-    if (many) hipLaunchKernelGGL((qdl::born_fp4_append_kernel<E, VEC, 4>), dim3((unsigned)blocks), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((qdl::born_fp4_append_kernel<E, VEC, 1>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    if (many) hipLaunchKernelGGL((qdl::born_fp4_append_kernel<E, VEC, 4, WHOLE>), dim3((unsigned)blocks), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((qdl::born_fp4_append_kernel<E, VEC, 1, WHOLE>), dim3((unsigned)blocks), dim3(256), 0, st, a);
 }
 
 }  // namespace
@@ -126,9 +126,11 @@ int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call* c, qdl_stream
     a.table_rows = (int)c->table_rows;
     a.n_freq = (int)c->n_freq;
     a.freq_ld = c->freq_ld;
+    a.wide_tables = c->cos_table && c->freq_ld % 4 == 0 && aligned16(c->cos_table) && aligned16(c->sin_table) ? 1 : 0;
     a.eps = c->eps;
     // 16-byte pieces where half a row holds whole ones, else 8-byte pieces.
-    const int vec = c->dtype != QDL_BORN_DTYPE_F32 && c->D % 16 == 0 ? 8 : 4;
+    const bool whole = c->D % 16 == 0;
+    const int vec = c->dtype != QDL_BORN_DTYPE_F32 && whole ? 8 : 4;
     a.lpr = 1;
     while (a.lpr * vec < c->D / 2) a.lpr *= 2;
     a.lpw = 4;
@@ -136,7 +138,8 @@ int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call* c, qdl_stream
     // Groups of four heads where single ones would fill the chip twice over.
     const bool many = c->n * c->H * a.lpr >= (int64_t)1 << 20;
     const int64_t queries = append_blocks(c->n, many ? (c->H + 3) / 4 : c->H, a.lpr);
-    a.heads = many ? (int)((c->h_kv + 3) / 4) : (int)c->h_kv;
+    const int each = many ? qdl::kFp4AppendHeads<4> : qdl::kFp4AppendHeads<1>;
+    a.heads = (int)((c->h_kv + each - 1) / each);
     a.tokens = (int)append_blocks(c->n, 1, a.lpw);
     const int64_t blocks = queries + (c->cache.cache_pages > 0 ? 2 * (int64_t)a.heads * a.tokens : 0);
     if (blocks > kMostBlocks) return QDL_BORN_E_SHAPE;
@@ -144,14 +147,17 @@ int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call* c, qdl_stream
     hipStream_t s = reinterpret_cast<hipStream_t>(stream);
     switch (c->dtype) {
         case QDL_BORN_DTYPE_BF16:
-            if (vec == 8) launch_append<qdl::BF16, 8>(a, many, blocks, s);
-            else launch_append<qdl::BF16, 4>(a, many, blocks, s);
+            if (whole) launch_append<qdl::BF16, 8, true>(a, many, blocks, s);
+            else launch_append<qdl::BF16, 4, false>(a, many, blocks, s);
             break;
         case QDL_BORN_DTYPE_F16:
-            if (vec == 8) launch_append<qdl::F16, 8>(a, many, blocks, s);
-            else launch_append<qdl::F16, 4>(a, many, blocks, s);
+            if (whole) launch_append<qdl::F16, 8, true>(a, many, blocks, s);
+            else launch_append<qdl::F16, 4, false>(a, many, blocks, s);
             break;
-        default: launch_append<qdl::F32, 4>(a, many, blocks, s); break;
+        default:
+            if (whole) launch_append<qdl::F32, 4, true>(a, many, blocks, s);
+            else launch_append<qdl::F32, 4, false>(a, many, blocks, s);
+            break;
     }
     return hip_status(hipGetLastError());
 }
