@@ -264,25 +264,6 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
     if (c0 >= rows) return;
     const int s0 = sq.base() + it.i * chunk, s1 = min(sq.n, s0 + chunk);
 
-    // This lane's rows and the keys that each sees: [lo, hi].
-    int tok[NC], head[NC], lo[NC], hi[NC];
-    u32x4 qr[NC][KS][QP];
-#pragma unroll
-    for (int i = 0; i < NC; ++i) {
-        const int r = c0 + 16 * i + m;
-        const bool ok = r < rows;
-        tok[i] = ok ? r / p.G : 0;
-        head[i] = hk * p.G + (ok ? r - tok[i] * p.G : 0);
-        hi[i] = ok ? sq.n - sq.nq + tok[i] : -1;
-        lo[i] = p.window > 0 ? max(0, hi[i] - p.window + 1) : 0;
-        const bool neg = arg_scale(p, head[i]) < 0.f;
-        const uint8_t* row = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok[i]) * p.q_st + (int64_t)head[i] * p.q_sh;
-#pragma unroll
-        for (int a = 0; a < KB; ++a)
-#pragma unroll
-            for (int w = 0; w < KW; ++w)
-                fp4_query<E>(row, 8 * KW * (j4 + 4 * a) + 8 * w, p.D, ok, neg, qr[i][a * KW + w]);
-    }
     // The keys that every row of the block sees.
     const int t0 = c0 / p.G, t1 = min(c0 + 16 * NC, rows) - 1;
     const int all_hi = sq.n - sq.nq + t0, all_lo = p.window > 0 ? sq.n - sq.nq + t1 / p.G - p.window + 1 : 0;
@@ -403,6 +384,31 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
             }
         }
     };
+    // The first keys are on their way before anything waits for the queries.
+    const int step = 32 * NW;
+    Fp4Keys<E, DP> x, y;
+    const int key_first = s0 + 32 * wave;
+    if (key_first < s1) load(x, key_first);
+
+    // This lane's rows and the keys that each sees: [lo, hi].
+    int tok[NC], head[NC], lo[NC], hi[NC];
+    u32x4 qr[NC][KS][QP];
+#pragma unroll
+    for (int i = 0; i < NC; ++i) {
+        const int r = c0 + 16 * i + m;
+        const bool ok = r < rows;
+        tok[i] = ok ? r / p.G : 0;
+        head[i] = hk * p.G + (ok ? r - tok[i] * p.G : 0);
+        hi[i] = ok ? sq.n - sq.nq + tok[i] : -1;
+        lo[i] = p.window > 0 ? max(0, hi[i] - p.window + 1) : 0;
+        const bool neg = arg_scale(p, head[i]) < 0.f;
+        const uint8_t* row = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok[i]) * p.q_st + (int64_t)head[i] * p.q_sh;
+#pragma unroll
+        for (int a = 0; a < KB; ++a)
+#pragma unroll
+            for (int w = 0; w < KW; ++w)
+                fp4_query<E>(row, 8 * KW * (j4 + 4 * a) + 8 * w, p.D, ok, neg, qr[i][a * KW + w]);
+    }
     auto use = [&](Fp4Keys<E, DP>& x, int key0) __attribute__((always_inline)) {
         // K, with NaN for the blocks of tokens that are not numbers in K or V.
         f32x4v s[NC][2];
@@ -540,18 +546,12 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
             columns(std::integral_constant<int, 7>{});
         }
     };
-    const int step = 32 * NW;
-    {
-        Fp4Keys<E, DP> x, y;
-        int key = s0 + 32 * wave;
-        if (key < s1) load(x, key);
-        for (; key < s1; key += 2 * step) {
-            if (key + step < s1) load(y, key + step);
-            use(x, key);
-            if (key + step >= s1) break;
-            if (key + 2 * step < s1) load(x, key + 2 * step);
-            use(y, key + step);
-        }
+    for (int key = key_first; key < s1; key += 2 * step) {
+        if (key + step < s1) load(y, key + step);
+        use(x, key);
+        if (key + step >= s1) break;
+        if (key + 2 * step < s1) load(x, key + 2 * step);
+        use(y, key + step);
     }
     // The waves' sums, in order.
 #pragma unroll

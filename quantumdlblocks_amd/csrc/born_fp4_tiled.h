@@ -79,12 +79,6 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     const int tok = ok ? row / p.G : 0, head = hk * p.G + (ok ? row - tok * p.G : 0);
     const int pos = past + tok;
     const float sc = arg_scale(p, head);
-    u32x4 qr[KS][QP];
-    {
-        const uint8_t* at = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok) * p.q_st + (int64_t)head * p.q_sh;
-#pragma unroll
-        for (int ks = 0; ks < KS; ++ks) fp4_query<E>(at, 16 * ks + 8 * g, p.D, ok, sc < 0.f, qr[ks]);
-    }
     f32x16 acc[DB];
 #pragma unroll
     for (int db = 0; db < DB; ++db) acc[db] = zero16();
@@ -156,6 +150,22 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
         }
     };
 
+    // The first tiles' codes are on their way before anything waits for the queries.
+    int page = -1;
+    Codes first_codes;
+    if (n > 0) {
+        page = page_of(0);
+        const int page1 = n > 1 ? page_of(1) : -1;
+        fetch(first_codes, 0, page);
+        fetch(next, 1, page1);
+        page = n > 2 ? page_of(2) : -1;
+    }
+    u32x4 qr[KS][QP];
+    {
+        const uint8_t* at = (const uint8_t*)p.q + (int64_t)(sq.q0 + tok) * p.q_st + (int64_t)head * p.q_sh;
+#pragma unroll
+        for (int ks = 0; ks < KS; ++ks) fp4_query<E>(at, 16 * ks + 8 * g, p.D, ok, sc < 0.f, qr[ks]);
+    }
     auto tile = [&](int u, int st, auto kind) __attribute__((always_inline)) {
         const int key0 = (t0 + u) * BN;
         const Tile k = kt(st), v = vt(st);
@@ -214,12 +224,7 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     if (n > 0) {
         if (tid < 2) bad_tile[tid] = -1;
         __syncthreads();
-        int page = page_of(0);
-        fetch(next, 0, page);
-        page = n > 1 ? page_of(1) : -1;
-        put(next, 0);
-        fetch(next, 1, page);
-        page = n > 2 ? page_of(2) : -1;
+        put(first_codes, 0);
         int u = 0;
         auto run = [&](int end, auto kind) __attribute__((always_inline)) {
             for (; u < end; ++u) {

@@ -107,12 +107,16 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     r.join.most = r.most;
     r.join.ncol = 2;
     while (4 * r.join.ncol < D) r.join.ncol *= 2;
-    // Threads that share a row's splits: one for every three that there may be.
+    // Threads that share a row's splits: as many as there may be, until the launch
+    // fills the chip.
     const int64_t per = items / (B > 0 ? B : 1) + 1, each = per < longest ? per : longest;
-    r.join.groups = 1;
-    while (r.join.groups * r.join.ncol < 256 && r.join.groups * 3 < each) r.join.groups *= 2;
     const int64_t narrow = items > 0 ? B * h_kv * r.most : 0, wide = r.splits > 1 ? n * H : 0;
-    const int64_t rows = 256 / (r.join.ncol * r.join.groups), blocks = (narrow + wide + rows - 1) / rows;
+    int64_t blocks = 0;
+    for (r.join.groups = 1;; r.join.groups *= 2) {
+        const int64_t rows = 256 / (r.join.ncol * r.join.groups);
+        blocks = (narrow + wide + rows - 1) / rows;
+        if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
+    }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
     r.fits = r.grid <= kMost && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {

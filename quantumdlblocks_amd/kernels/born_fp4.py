@@ -47,6 +47,7 @@ __all__ = [
 
 _BLOCK = 32
 _BAD = 255
+_U8 = torch.uint8
 
 
 class BornCacheFp4(NamedTuple):
@@ -72,63 +73,66 @@ def born_cache_fp4(pages: int, page_size: int, key_heads: int, head_dim: int, de
     return BornCacheFp4(*made)
 
 
-def _check_fp4(cache, block_table, cache_lens, B, head_dim, written: bool, apart: bool = False):
-    """(k, v, k_scale, v_scale), and the cache's fields of the argument blocks up
-    to page_size, on the GPU.  ``head_dim`` None: any.  Plain tests in a row, as
-    for the 16-bit cache: decoding calls this for every layer and token."""
+def _check_fp4(cache, block_table, cache_lens, B, head_dim, written: bool):
+    """The cache's fields of the argument blocks up to page_size, on the GPU.
+    ``head_dim`` None: any.  ``written``: the tensors are, so none may overlap
+    itself or be another.  Plain tests in a row, as for the 16-bit cache: decoding
+    calls this for every layer and token."""
     if len(cache) != 4:
         raise ValueError(f"a 4-bit cache is its codes and scales (k, v, k_scale, v_scale), got {len(cache)} tensors")
     k, v, ks, vs = cache
-    shape, sshape = k.shape, ks.shape
+    shape, sshape, tshape = k.shape, ks.shape, block_table.shape
     if len(shape) != 4 or v.shape != shape or len(sshape) != 4 or vs.shape != sshape or sshape[:3] != shape[:3] or shape[3] != 16 * sshape[3]:
         raise ValueError(f"a 4-bit cache is codes (pages, page_size, key_heads, 16 n) and scales (pages, page_size, key_heads, n), "
                          f"got {[tuple(t.shape) for t in cache]}")
-    u8 = torch.uint8
-    if k.dtype is not u8 or v.dtype is not u8 or ks.dtype is not u8 or vs.dtype is not u8:
+    if k.dtype is not _U8 or v.dtype is not _U8 or ks.dtype is not _U8 or vs.dtype is not _U8:
         raise ValueError(f"a 4-bit cache is held in uint8, got {[t.dtype for t in cache]}")
     P, page, Hkv, nb = sshape
     if page < 1 or Hkv < 1 or nb < 1:
         raise ValueError(f"page_size, key_heads and head_dim must be positive, got {tuple(shape)}")
     if head_dim is not None and not _BLOCK * (nb - 1) < head_dim <= _BLOCK * nb:
         raise ValueError(f"head_dim {head_dim} does not fit a cache of {nb} blocks of {_BLOCK} columns")
-    tshape, lshape = block_table.shape, cache_lens.shape
     if len(tshape) != 2 or tshape[0] != B or block_table.dtype not in _INDEX:
         raise ValueError(f"block_table must be (B={B}, pages) int32, got {block_table.dtype} {tuple(tshape)}")
-    if len(lshape) != 1 or lshape[0] != B or cache_lens.dtype not in _INDEX:
-        raise ValueError(f"cache_lens must be (B={B},) int32, got {cache_lens.dtype} {tuple(lshape)}")
+    if cache_lens.shape != (B,) or cache_lens.dtype not in _INDEX:
+        raise ValueError(f"cache_lens must be (B={B},) int32, got {cache_lens.dtype} {tuple(cache_lens.shape)}")
     if tshape[1] * page > _LIMIT:
         raise ValueError(f"block_table holds {tshape[1]} pages of {page}: more than 2^30 keys a sequence")
     dev = k.get_device()
-    if (v.get_device() != dev or ks.get_device() != dev or vs.get_device() != dev or block_table.get_device() != dev
-            or cache_lens.get_device() != dev):
+    if not (v.get_device() == ks.get_device() == vs.get_device() == block_table.get_device() == cache_lens.get_device() == dev):
         raise ValueError(f"the cache, block_table and cache_lens must be on one device, got {[t.device for t in cache]}, "
                          f"{block_table.device}, {cache_lens.device}")
-    sk, sv, sks, svs = k.stride(), v.stride(), ks.stride(), vs.stride()
+    k0, k1, k2, k3 = k.stride()
+    v0, v1, v2, v3 = v.stride()
+    s0, s1, s2, s3 = ks.stride()
+    u0, u1, u2, u3 = vs.stride()
+    pk, pv, ps, pu = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
     if written:
-        for name, t, st in (("k", k, sk), ("v", v, sv), ("k_scale", ks, sks), ("v_scale", vs, svs)):
-            if any(s == 0 and n > 1 for n, s in zip(t.shape, st)):
-                raise ValueError(f"{name} is written and must not overlap itself, got strides {st}")
-    pk, pv, pks, pvs = k.data_ptr(), v.data_ptr(), ks.data_ptr(), vs.data_ptr()
-    if apart and P and len({pk, pv, pks, pvs}) != 4:
-        raise ValueError("the cache's four tensors are all written and must not share memory")
+        if not (k0 and k1 and k2 and k3 and v0 and v1 and v2 and v3 and s0 and s1 and s2 and s3 and u0 and u1 and u2 and u3):
+            for name, t in zip(("k", "v", "k_scale", "v_scale"), cache):
+                if any(s == 0 and n > 1 for n, s in zip(t.shape, t.stride())):
+                    raise ValueError(f"{name} is written and must not overlap itself, got strides {t.stride()}")
+        if P and (pk == pv or ps == pu or pk == ps or pk == pu or pv == ps or pv == pu):
+            raise ValueError("the cache's four tensors are all written and must not share memory")
     if dev < 0:
         return ()
     if nb * _BLOCK > MAX_HEAD_DIM:
         raise NotImplementedError(f"paged caches take head dims up to {MAX_HEAD_DIM}, got {nb} blocks of {_BLOCK}")
-
-    def three(st):
-        return st[0] if P > 1 else 0, st[1] if page > 1 else 0, st[2] if Hkv > 1 else 0
-
-    k0, k1, k2 = three(sk)
-    v0, v1, v2 = three(sv)
-    if sk[3] != 1 or (k0 | k1 | k2 | pk) % 16 or sv[3] != 1 or (v0 | v1 | v2 | pv) % 16:
+    if P <= 1:
+        k0 = v0 = s0 = u0 = 0
+    if page == 1:
+        k1 = v1 = s1 = u1 = 0
+    if Hkv == 1:
+        k2 = v2 = s2 = u2 = 0
+    any_stride = k0 | k1 | k2 | v0 | v1 | v2
+    if k3 != 1 or v3 != 1 or (any_stride | pk | pv) & 15:
         raise ValueError(f"codes need unit stride along a row, other strides that are multiples of 16 and a 16-byte aligned base, "
-                         f"got strides {sk} and {sv}")
-    if max(k0, k1, k2, v0, v1, v2) >> 32:
-        raise ValueError(f"a cache's strides lie under 2^32, got {sk} and {sv}")
-    if nb > 1 and (sks[3] != 1 or svs[3] != 1):
-        raise ValueError(f"scales need unit stride along a row, got strides {sks} and {svs}")
-    return pk, pv, pks, pvs, k0, k1, k2, v0, v1, v2, *three(sks), *three(svs), P, page
+                         f"got strides {k.stride()} and {v.stride()}")
+    if (any_stride | s0 | s1 | s2 | u0 | u1 | u2) >> 32:
+        raise ValueError(f"a cache's strides lie under 2^32, got {[t.stride() for t in cache]}")
+    if nb > 1 and (s3 != 1 or u3 != 1):
+        raise ValueError(f"scales need unit stride along a row, got strides {ks.stride()} and {vs.stride()}")
+    return pk, pv, ps, pu, k0, k1, k2, v0, v1, v2, s0, s1, s2, u0, u1, u2, P, page
 
 
 def _check_type(D: int, dtype: torch.dtype) -> None:
@@ -137,7 +141,7 @@ def _check_type(D: int, dtype: torch.dtype) -> None:
 
 
 def _check_starts(cu_seqlens, B, dev, at) -> None:
-    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] != B + 1 or cu_seqlens.dtype not in _INDEX or cu_seqlens.get_device() != at:
+    if cu_seqlens.shape != (B + 1,) or cu_seqlens.dtype not in _INDEX or cu_seqlens.get_device() != at:
         raise ValueError(f"cu_seqlens must be (B + 1 = {B + 1},) int32 on {dev}, got {cu_seqlens.dtype} {tuple(cu_seqlens.shape)} "
                          f"on {cu_seqlens.device}")
 
@@ -266,7 +270,7 @@ def fused_qk_rope_l2_normalize_append_fp4(
                          f"{tuple(kshape)}, {tuple(v.shape)}")
     N, H, D = q.shape
     B = block_table.shape[0] if block_table.dim() == 2 else -1
-    fields = _check_fp4(cache, block_table, cache_lens, B, D, written=True, apart=True)
+    fields = _check_fp4(cache, block_table, cache_lens, B, D, written=True)
     Hkv = cache[0].shape[2]
     if kshape[1] != Hkv or H < 1 or H % Hkv or D % 2:
         raise ValueError(f"q {tuple(q.shape)} and k {tuple(kshape)} do not fit a cache of {Hkv} key heads, or head_dim is odd")
@@ -278,7 +282,7 @@ def fused_qk_rope_l2_normalize_append_fp4(
             raise ValueError(f"without cu_seqlens there is one token per sequence, got {N} tokens and {B} sequences")
     else:
         _check_starts(cu_seqlens, B, dev, at)
-    if positions is not None and (positions.dim() != 1 or positions.shape[0] != N or positions.dtype not in _INDEX
+    if positions is not None and (positions.shape != (N,) or positions.dtype not in _INDEX
                                   or positions.get_device() != at):
         raise ValueError(f"positions must be (N={N},) int32 on {dev}, got {positions.dtype} {tuple(positions.shape)} on "
                          f"{positions.device}")
@@ -294,7 +298,7 @@ def fused_qk_rope_l2_normalize_append_fp4(
                              positions, eps)
     _check_type(D, dt)
     lib = _native.load()
-    out = torch.empty((N, H, D), dtype=dt, device=dev)
+    out = q.new_empty((N, H, D))
     if N == 0:
         return out
     if B == 0:
@@ -310,7 +314,7 @@ def fused_qk_rope_l2_normalize_append_fp4(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), k_c.data_ptr(), v_c.data_ptr(), q0, q1, k0, k1, v0, v1, out.data_ptr(),
         *fields, table.data_ptr(), table.shape[1], ld, lens.data_ptr(), 0 if cu is None else cu.data_ptr(), *rot,
         0 if pos is None else pos.data_ptr(), eps))
-    _written(tuple(cache))
+    _written(cache)
     return out
 
 
@@ -357,7 +361,8 @@ def born_cache_read_fp4(
         return tuple(out)
     _check_type(D, dtype)
     lib = _native.load()
-    k, v = (torch.empty((N, Hkv, D), dtype=dtype, device=dev) for _ in range(2))
+    k = torch.empty((N, Hkv, D), dtype=dtype, device=dev)
+    v = torch.empty_like(k)
     if N == 0:
         return k, v
     if B == 0:
@@ -503,7 +508,7 @@ def flash_born_attention_paged_fp4(
     dt = q.dtype
     _check_type(D, dt)
     lib = _native.load()
-    out = torch.empty((N, H, D), dtype=dt, device=dev)
+    out = q.new_empty((N, H, D))
     if N == 0:
         return out
     if B == 0:
@@ -513,7 +518,7 @@ def flash_born_attention_paged_fp4(
     cu = None if cu_seqlens is None else _index(cu_seqlens)
     pages = table.shape[1]
     size = _paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, w_ptr != 0)
-    ws = torch.empty(size, dtype=torch.uint8, device=dev)
+    ws = lens.new_empty((size + 3) // 4)
     _run_call(lib.qdl_flash_born_fp4_paged_forward_call, "qdl_flash_born_fp4_paged_forward_call", dev, _native.fp4_paged_call(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), st, sh, out.data_ptr(), *fields, table.data_ptr(), pages, ld,
         lens.data_ptr(), 0 if cu is None else cu.data_ptr(), scale_p, n_scale, scale_value, window, eps, w_ptr, w_sb, w_sh, w_len,
@@ -543,7 +548,7 @@ def born_cache_evict_fp4(
     if torch.is_grad_enabled() or forward_ad._current_level >= 0:
         _no_grad("born_cache_evict_fp4", key_weight)
     B = block_table.shape[0] if block_table.dim() == 2 else -1
-    fields = _check_fp4(cache, block_table, cache_lens, B, None, written=True, apart=True)
+    fields = _check_fp4(cache, block_table, cache_lens, B, None, written=True)
     page, Hkv, nb = cache[2].shape[1:]
     dev, at = cache[0].device, cache[0].get_device()
     budget, recent = int(budget), int(recent)
