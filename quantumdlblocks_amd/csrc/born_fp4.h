@@ -91,6 +91,12 @@ constexpr int kPParts = std::is_same<E, F32>::value ? 3 : 2;
 // Eight values of a query from column `at` on (D - at of them, 0 behind), as operands.
 template <class E>
 __device__ __forceinline__ void fp4_query(const uint8_t* row, int at, int D, bool ok, bool neg, u32x4 (&q)[kQParts<E>]) {
+    if constexpr (std::is_same<E, BF16>::value) {
+        u32x4 y = {0u, 0u, 0u, 0u};
+        if (ok && at < D) y = ldg16(row + 2 * at) ^ (neg ? 0x80008000u : 0u);
+        q[0] = y;
+        return;
+    }
     float x[8];
 #pragma unroll
     for (int i = 0; i < 8; ++i) x[i] = 0.f;

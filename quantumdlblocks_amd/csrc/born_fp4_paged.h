@@ -101,17 +101,19 @@ struct Fp4Share {
     int chunks, wide;  // how many there are
     Fp4Seq mine;       // sequence `lane`
 
-    __device__ __forceinline__ Fp4Share(const Fp4PagedArgs& p) : step(1 << 23), chunks(p.B), wide((int)p.slots), mine(p, min(lane(), p.B - 1)) {
+    // totals: chunks and wide are wanted.
+    __device__ __forceinline__ Fp4Share(const Fp4PagedArgs& p, bool totals) : step(1 << 23), chunks(p.B), wide((int)p.slots), mine(p, min(lane(), p.B - 1)) {
         if (p.items == 0) return;  // too many sequences to look through: one chunk each, slots for blocks
         uint64_t total = 0;  // 1024 sequences of 2^23 steps at most, 64 of them a scan
         wide = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
             const bool in = b0 + lane() < p.B;
             total += (uint32_t)last(fp4_scan(in ? s.steps(p) : 0));
-            if (p.slots > 0) wide += last(fp4_scan(in ? s.blocks(p) : 0));
+            if (totals) wide += last(fp4_scan(in ? s.blocks(p) : 0));
             return false;
         });
         step = fp4_step(total, p.items);
+        if (!totals) return;
         chunks = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
             chunks += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
@@ -239,11 +241,11 @@ __device__ __forceinline__ void fp4_fetch(uint32_t (&to)[DW], Fp4Rsrc p, uint32_
 template <int DP>
 constexpr int kFp4NarrowLds = 4 * 16 * (DP + 4 + 1) * 4;
 
-// Chunk and head `block` of its column block.  DP: 64, 128 or 256 columns; NC: 16-row column
+// Chunk `item` of the keys, key head hk, column block cb.  DP: 64, 128 or 256 columns; NC: 16-row column
 // sets; WEIGH: the raw weights are written too (one token per sequence); P16:
 // pages of a multiple of 16 tokens.
 template <class E, int DP, int NC, bool WEIGH, bool P16>
-__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* smem, int block) {
+__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* smem, int item, int hk, int cb) {
     using C = Fp4Cfg<E, DP>;
     constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
     constexpr int IT = kItem<E>;
@@ -252,9 +254,6 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, j4 = lane >> 4;
-    // Column blocks in turn: few sequences have more than the first.
-    const int cb = block / (share.chunks * p.Hkv), rest = block - cb * share.chunks * p.Hkv;
-    const int item = rest / p.Hkv, hk = rest - item * p.Hkv;
     const Fp4Part it = fp4_chunk(p, share, item);
     const int b = it.b, chunk = share.step << 7;
     const Fp4Seq& sq = it.sq;
@@ -265,8 +264,11 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
     const int s0 = sq.base() + it.i * chunk, s1 = min(sq.n, s0 + chunk);
 
     // The keys that every row of the block sees.
-    const int t0 = c0 / p.G, t1 = min(c0 + 16 * NC, rows) - 1;
-    const int all_hi = sq.n - sq.nq + t0, all_lo = p.window > 0 ? sq.n - sq.nq + t1 / p.G - p.window + 1 : 0;
+    int all_hi = sq.n - 1, all_lo = sq.first;
+    if (p.cu != nullptr) {
+        all_hi = sq.n - sq.nq + c0 / p.G;
+        if (p.window > 0) all_lo = sq.n - sq.nq + (min(c0 + 16 * NC, rows) - 1) / p.G - p.window + 1;
+    }
 
     f32x4v acc[NC][VC];
     float z[NC];
@@ -397,7 +399,7 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
     for (int i = 0; i < NC; ++i) {
         const int r = c0 + 16 * i + m;
         const bool ok = r < rows;
-        tok[i] = ok ? r / p.G : 0;
+        tok[i] = ok && p.cu != nullptr ? r / p.G : 0;
         head[i] = hk * p.G + (ok ? r - tok[i] * p.G : 0);
         hi[i] = ok ? sq.n - sq.nq + tok[i] : -1;
         lo[i] = p.window > 0 ? max(0, hi[i] - p.window + 1) : 0;
@@ -577,7 +579,7 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
                 y += *reinterpret_cast<const f32x4v*>(&red[w][cc][col]);
                 sum += zred[w][cc];
             }
-            const int r = c0 + 16 * i + cc, t = r / p.G, h = hk * p.G + r - t * p.G;
+            const int r = c0 + 16 * i + cc, t = p.cu != nullptr ? r / p.G : 0, h = hk * p.G + r - t * p.G;
             if (it.n > 1 || WEIGH) {
                 float* to = p.part + ((((int64_t)item * p.Hkv + hk) * p.cblocks + cb) * (16 * NC) + 16 * i + cc) * (p.D + 4);
                 *reinterpret_cast<f32x4v*>(to + 4 + col) = y;
@@ -595,9 +597,8 @@ template <class E, int DP, int NC, bool WEIGH, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
 void born_fp4_paged_kernel(Fp4PagedArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[kFp4NarrowLds<DP>];
-    fp4_behind<E>(p, blockIdx.x, gridDim.x);
-    const Fp4Share share(p);
-    if ((int)blockIdx.x < share.chunks * p.Hkv * p.cblocks) fp4_narrow<E, DP, NC, WEIGH, P16>(p, share, smem, blockIdx.x);
+    if (blockIdx.x == 0 && blockIdx.z == 0) fp4_behind<E>(p, blockIdx.y, gridDim.y);
+    fp4_narrow<E, DP, NC, WEIGH, P16>(p, Fp4Share(p, false), smem, blockIdx.y, blockIdx.x, blockIdx.z);
 }
 
 // A narrow row's partial sums.
@@ -706,7 +707,7 @@ hipError_t fp4_paged_fwd(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t
 
 template <class E, int NC, bool WEIGH, bool P16>
 void launch_fp4_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)plan.grid);
+    const dim3 grid((unsigned)a.Hkv, (unsigned)plan.chunks, (unsigned)plan.cblocks);
     if (a.D <= 64) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 64, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 128, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((born_fp4_paged_kernel<E, 256, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);

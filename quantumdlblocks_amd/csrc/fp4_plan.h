@@ -118,7 +118,8 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
     }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
-    r.fits = r.grid <= kMost && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    // The narrow kernel's own grid has heads, chunks and column blocks as dimensions.
+    r.fits = r.grid <= kMost && h_kv < 65536 && r.chunks < 65536 && r.cblocks < 65536 && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.wide = (int)wide;
