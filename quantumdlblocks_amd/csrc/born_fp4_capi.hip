@@ -243,6 +243,7 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     a.window = (int)c->window_size;
     a.items = r.items;
     a.cblocks = r.cblocks;
+    a.cols = 16 * r.nc;
     a.limit = r.limit;
     a.splits = r.splits;
     a.slots = r.slots;

@@ -37,16 +37,17 @@ struct Fp4PagedArgs {
     int per_head_scale;
     int B, N, H, Hkv, G, D;
     int window;
-    int items;             // chunks wanted; 0: one per sequence
-    int cblocks;           // column blocks of a sequence
+    int items;             // units (a chunk of keys and a column block) wanted; 0: cblocks for each sequence
+    int cblocks;           // column blocks of a sequence at most
+    int cols;              // rows of one
     int limit;             // rows of a (sequence, key head) that the narrow kernel takes
     int splits;            // of the tiled kernel's keys
     int64_t slots;         // blocks of rows at most; 0: no sequence is wide
     float* wide_part;      // (N, H, splits, D + 4), where there are several
     float eps;
     int64_t q_st, q_sh;    // bytes
-    int2* plan;            // (B): a sequence's first chunk and how many
-    float* part;           // (chunks, Hkv, cblocks, 16 NC, D + 4): denominator, three unused, numerators
+    int2* plan;            // (B): a sequence's first unit and its chunks
+    float* part;           // (units, Hkv, cols, D + 4): denominator, three unused, numerators
     float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
     int64_t w_sb, w_sh;    // elements
     int w_len;
@@ -79,6 +80,8 @@ struct Fp4Seq {
     __device__ __forceinline__ bool wide(const Fp4PagedArgs& p) const { return p.cu != nullptr && (int64_t)nq * p.G > p.limit; }
     // The narrow kernel's chunks are counted in steps of 128 keys.
     __device__ __forceinline__ int steps(const Fp4PagedArgs& p) const { return wide(p) ? 0 : fp4_steps(n, first); }
+    // The narrow kernel's column blocks.
+    __device__ __forceinline__ int columns(const Fp4PagedArgs& p) const { return wide(p) ? 0 : fp4_blocks(nq * p.G, p.cols); }
     // The tiled kernel's blocks of rows.
     __device__ __forceinline__ int blocks(const Fp4PagedArgs& p) const { return wide(p) ? (nq * p.G + kFp4Rows - 1) / kFp4Rows : 0; }
 };
@@ -94,35 +97,40 @@ __device__ __forceinline__ int fp4_scan(int x) {
     return x;
 }
 
-// How the device shares out a call, found by every wave for itself: chunks of
-// the narrow sequences' keys, blocks of the wide ones' rows.
+// How the device shares out a call, found by every wave for itself: units (a
+// chunk of the keys and a column block) of the narrow sequences, blocks of the
+// wide ones' rows.
 struct Fp4Share {
-    int step;          // steps of 128 keys in a chunk
-    int chunks, wide;  // how many there are
-    Fp4Seq mine;       // sequence `lane`
+    int step;         // steps of 128 keys in a chunk
+    int units, wide;  // how many there are
+    Fp4Seq mine;      // sequence `lane`
 
-    // totals: chunks and wide are wanted.
-    __device__ __forceinline__ Fp4Share(const Fp4PagedArgs& p, bool totals) : step(1 << 23), chunks(p.B), wide((int)p.slots), mine(p, min(lane(), p.B - 1)) {
+    // totals: units and wide are wanted.
+    __device__ __forceinline__ Fp4Share(const Fp4PagedArgs& p, bool totals) : step(1 << 23), units(p.B * p.cblocks), wide((int)p.slots), mine(p, min(lane(), p.B - 1)) {
         if (p.items == 0) return;  // too many sequences to look through: one chunk each, slots for blocks
-        uint64_t total = 0;  // 1024 sequences of 2^23 steps at most, 64 of them a scan
+        uint64_t total = 0;
         wide = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
             const bool in = b0 + lane() < p.B;
-            total += (uint32_t)last(fp4_scan(in ? s.steps(p) : 0));
+            const uint64_t mine = in ? (uint64_t)(uint32_t)s.steps(p) * (uint32_t)s.columns(p) : 0;
+            // Sums of 64 in 32 bits, the upper ones where there are any.
+            total += (uint32_t)last(fp4_scan((int)(mine & 0xffffffu)));
+            if (__ballot(mine >> 24 != 0) != 0) total += (uint64_t)(uint32_t)last(fp4_scan((int)(mine >> 24))) << 24;
             if (totals) wide += last(fp4_scan(in ? s.blocks(p) : 0));
             return false;
         });
         step = fp4_step(total, p.items);
         if (!totals) return;
-        chunks = 0;
+        units = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
-            chunks += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
+            units += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
             return false;
         });
     }
     __device__ __forceinline__ static int lane() { return threadIdx.x & 63; }
     __device__ __forceinline__ static int last(int scan) { return __builtin_amdgcn_readlane(scan, 63); }
-    __device__ __forceinline__ int count(const Fp4PagedArgs& p, const Fp4Seq& s) const { return (s.steps(p) + step - 1) / step; }
+    __device__ __forceinline__ int chunks(const Fp4PagedArgs& p, const Fp4Seq& s) const { return (s.steps(p) + step - 1) / step; }
+    __device__ __forceinline__ int count(const Fp4PagedArgs& p, const Fp4Seq& s) const { return chunks(p, s) * s.columns(p); }
     // Every 64 sequences, until f is done.
     template <class F>
     __device__ __forceinline__ void each(const Fp4PagedArgs& p, F&& f) const {
@@ -158,10 +166,13 @@ __device__ __forceinline__ Fp4Part fp4_part(const Fp4PagedArgs& p, const Fp4Shar
     });
     return r.uniform();
 }
-// Chunk `item`.
-__device__ __forceinline__ Fp4Part fp4_chunk(const Fp4PagedArgs& p, const Fp4Share& share, int item) {
-    if (p.items == 0) return {item, 0, 1, Fp4Seq(p, item)};
-    return fp4_part(p, share, item, [&](const Fp4Seq& s) { return share.count(p, s); });
+// Unit x: part i is column block i % columns of chunk i / columns.
+__device__ __forceinline__ Fp4Part fp4_unit(const Fp4PagedArgs& p, const Fp4Share& share, int x) {
+    if (p.items == 0) {
+        const int b = p.cblocks > 1 ? x / p.cblocks : x;
+        return {b, x - b * p.cblocks, p.cblocks, Fp4Seq(p, b)};
+    }
+    return fp4_part(p, share, x, [&](const Fp4Seq& s) { return share.count(p, s); });
 }
 
 __device__ __forceinline__ float fp4_inverse(const Fp4PagedArgs& p, int h, float z) {
@@ -241,11 +252,11 @@ __device__ __forceinline__ void fp4_fetch(uint32_t (&to)[DW], Fp4Rsrc p, uint32_
 template <int DP>
 constexpr int kFp4NarrowLds = 4 * 16 * (DP + 4 + 1) * 4;
 
-// Chunk `item` of the keys, key head hk, column block cb.  DP: 64, 128 or 256 columns; NC: 16-row column
+// Unit `unit` of key head hk.  DP: 64, 128 or 256 columns; NC: 16-row column
 // sets; WEIGH: the raw weights are written too (one token per sequence); P16:
 // pages of a multiple of 16 tokens.
 template <class E, int DP, int NC, bool WEIGH, bool P16>
-__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* smem, int item, int hk, int cb) {
+__device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* smem, int unit, int hk) {
     using C = Fp4Cfg<E, DP>;
     constexpr int NW = 4, QP = kQParts<E>, PP = kPParts<E>, KB = C::KB, KW = C::KW, KS = C::KS, VC = C::VC, VD = C::VD;
     constexpr int IT = kItem<E>;
@@ -254,14 +265,16 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int m = lane & 15, j4 = lane >> 4;
-    const Fp4Part it = fp4_chunk(p, share, item);
+    const Fp4Part it = fp4_unit(p, share, unit);
     const int b = it.b, chunk = share.step << 7;
     const Fp4Seq& sq = it.sq;
     if (b < 0 || sq.wide(p)) return;
-    if (it.i == 0 && hk == 0 && cb == 0 && threadIdx.x == 0) p.plan[b] = int2{item, it.n};
+    const int columns = p.items == 0 ? p.cblocks : sq.columns(p);
+    const int c = columns > 1 ? it.i / columns : it.i, cb = it.i - c * columns, nsplit = p.items == 0 ? 1 : share.chunks(p, sq);
+    if (it.i == 0 && hk == 0 && threadIdx.x == 0) p.plan[b] = int2{unit, nsplit};
     const int rows = sq.nq * p.G, c0 = 16 * NC * cb;
     if (c0 >= rows) return;
-    const int s0 = sq.base() + it.i * chunk, s1 = min(sq.n, s0 + chunk);
+    const int s0 = sq.base() + (p.items == 0 ? 0 : c) * chunk, s1 = min(sq.n, s0 + chunk);
 
     // The keys that every row of the block sees.
     int all_hi = sq.n - 1, all_lo = sq.first;
@@ -580,12 +593,12 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
                 sum += zred[w][cc];
             }
             const int r = c0 + 16 * i + cc, t = p.cu != nullptr ? r / p.G : 0, h = hk * p.G + r - t * p.G;
-            if (it.n > 1 || WEIGH) {
-                float* to = p.part + ((((int64_t)item * p.Hkv + hk) * p.cblocks + cb) * (16 * NC) + 16 * i + cc) * (p.D + 4);
+            if (nsplit > 1 || WEIGH) {
+                float* to = p.part + (((int64_t)unit * p.Hkv + hk) * (16 * NC) + 16 * i + cc) * (p.D + 4);
                 *reinterpret_cast<f32x4v*>(to + 4 + col) = y;
                 if (col == 0) to[0] = sum;
             }
-            if (it.n == 1) {
+            if (nsplit == 1) {
                 y *= fp4_inverse(p, h, sum);
                 fp4_store4<E>((uint8_t*)p.out + ((int64_t)(sq.q0 + t) * p.H + h) * p.D * IT, col, y);
             }
@@ -597,8 +610,8 @@ template <class E, int DP, int NC, bool WEIGH, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
 void born_fp4_paged_kernel(Fp4PagedArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[kFp4NarrowLds<DP>];
-    if (blockIdx.x == 0 && blockIdx.z == 0) fp4_behind<E>(p, blockIdx.y, gridDim.y);
-    fp4_narrow<E, DP, NC, WEIGH, P16>(p, Fp4Share(p, false), smem, blockIdx.y, blockIdx.x, blockIdx.z);
+    if (blockIdx.x == 0) fp4_behind<E>(p, blockIdx.y, gridDim.y);
+    fp4_narrow<E, DP, NC, WEIGH, P16>(p, Fp4Share(p, false), smem, blockIdx.y, blockIdx.x);
 }
 
 // A narrow row's partial sums.
@@ -606,11 +619,12 @@ struct Fp4Parts {
     const float* at;
     int64_t ld;
     int n;
-    __device__ __forceinline__ Fp4Parts(const Fp4PagedArgs& p, int b, int hk, int r, int cols) {
+    __device__ __forceinline__ Fp4Parts(const Fp4PagedArgs& p, const Fp4Seq& sq, int b, int hk, int r) {
         const int2 plan = p.plan[b];
+        const int cb = r / p.cols;
         n = plan.y;
-        ld = (int64_t)p.Hkv * p.cblocks * cols * (p.D + 4);
-        at = p.part + plan.x * ld + (((int64_t)hk * p.cblocks + r / cols) * cols + r % cols) * (p.D + 4);
+        ld = (int64_t)sq.columns(p) * p.Hkv * p.cols * (p.D + 4);
+        at = p.part + (((int64_t)(plan.x + cb) * p.Hkv + hk) * p.cols + r - cb * p.cols) * (p.D + 4);
     }
 };
 
@@ -633,7 +647,7 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
         for (int g0 = 0; g0 < p.G; g0 += 256) {
             const int gn = min(256, p.G - g0);
             if ((int)threadIdx.x < gn) {
-                const Fp4Parts part(p, b, hk, g0 + threadIdx.x, q.cols);
+                const Fp4Parts part(p, sq, b, hk, g0 + threadIdx.x);
                 float z = 0.f;
 #pragma unroll 8
                 for (int i = 0; i < part.n; ++i) z += part.at[i * part.ld];
@@ -659,7 +673,7 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
         const int rest = unit / q.most, r = unit - rest * q.most, b = rest / p.Hkv, hk = rest - b * p.Hkv;
         const Fp4Seq sq(p, b);
         if (!sq.wide(p) && r < sq.nq * p.G) {
-            const Fp4Parts part(p, b, hk, r, q.cols);
+            const Fp4Parts part(p, sq, b, hk, r);
             const int t = r / p.G;
             head = hk * p.G + r - t * p.G;
             row = (int64_t)(sq.q0 + t) * p.H + head;
@@ -707,7 +721,7 @@ hipError_t fp4_paged_fwd(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t
 
 template <class E, int NC, bool WEIGH, bool P16>
 void launch_fp4_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)a.Hkv, (unsigned)plan.chunks, (unsigned)plan.cblocks);
+    const dim3 grid((unsigned)a.Hkv, (unsigned)plan.units);
     if (a.D <= 64) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 64, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 128, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((born_fp4_paged_kernel<E, 256, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);

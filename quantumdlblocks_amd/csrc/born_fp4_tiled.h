@@ -266,14 +266,13 @@ void born_fp4_chunk_kernel(Fp4PagedArgs p) {
     __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
     fp4_behind<E>(p, blockIdx.x, gridDim.x);
     const Fp4Share share(p, true);
-    const int tiled = share.wide * p.splits * p.Hkv, narrow = share.chunks * p.Hkv * p.cblocks;
+    const int tiled = share.wide * p.splits * p.Hkv, narrow = share.units * p.Hkv;
     const int x = blockIdx.x;
     if (x < tiled) {
         fp4_tiled<E, DP, P16>(p, share, smem, bad_tile, x);
     } else if (x < tiled + narrow) {
-        // Column blocks in turn: few sequences have more than the first.
-        const int y = x - tiled, cb = y / (share.chunks * p.Hkv), rest = y - cb * share.chunks * p.Hkv, item = rest / p.Hkv;
-        fp4_narrow<E, DP, 2, false, P16>(p, share, smem, item, rest - item * p.Hkv, cb);
+        const int y = x - tiled, unit = y / p.Hkv;
+        fp4_narrow<E, DP, 2, false, P16>(p, share, smem, unit, y - unit * p.Hkv);
     }
 }
 

@@ -10,6 +10,7 @@ namespace qdl {
 constexpr int kFp4Rows = 128;  // rows (new tokens x heads of a group) of the tiled kernel's workgroups
 // Rows of a (sequence, key head) up to which the narrow kernel takes it.
 constexpr int kFp4Narrow = 64;
+constexpr int kFp4AllNarrow = 512;  // rows of a launch, likewise
 // Workgroups of the narrow kernel that a launch's chunks of keys are made for:
 // two rounds of three a compute unit.
 constexpr int kFp4Wanted = 1536;
@@ -26,12 +27,17 @@ constexpr int fp4_steps(int n, int first) {
     const int steps = (n - (first & ~31) + 127) >> 7;
     return steps > 1 ? steps : 1;
 }
-// Steps in a chunk, of `total` (up to 2^33) in a launch: as many chunks as
-// wanted, but no more than a third of them below 512 keys.
+// A narrow sequence's column blocks of `cols` rows each; every one of them goes
+// through every chunk of the keys.
+constexpr int fp4_blocks(int64_t rows, int cols) { return (int)((rows + cols - 1) / cols); }
+// Steps in a chunk, where the launch's sequences have `total` steps times column
+// blocks: as many units (a chunk and a column block) as wanted, but no more than
+// a third of them below 512 keys.  At least total / items, so that there are no
+// more units than items and one for each column block.
 constexpr int fp4_step(uint64_t total, uint32_t items) {
-    if (total >= (uint64_t)1 << 31) {  // in eights, rounded up
-        const uint64_t step = 8 * ((uint64_t)((uint32_t)(total >> 3) / items) + 2);
-        return (int)(step < (uint64_t)1 << 23 ? step : (uint64_t)1 << 23);  // 2^30 keys: all of a sequence
+    if (total >= (uint64_t)1 << 31) {  // a little more, in fp32
+        const float step = (float)total / (float)items * 1.001f + 1.0f;
+        return step < 8388608.0f ? (int)step + 1 : 1 << 23;  // 2^30 keys: all of a sequence
     }
     const uint32_t t = (uint32_t)total, few = items / 3 > 1 ? items / 3 : 1;
     const uint32_t even = (t + items - 1) / items, some = (t + few - 1) / few;
@@ -40,15 +46,16 @@ constexpr int fp4_step(uint64_t total, uint32_t items) {
 }
 
 struct Fp4Join {
-    int ncol, groups, cols, most;
+    int ncol, groups, most;
     int narrow, wide;  // rows
     int blocks;        // workgroups of them
 };
 
 struct Fp4Plan {
-    int nc, cblocks;    // 16-row column sets of a narrow workgroup; column blocks of a sequence
-    int items, chunks;  // chunks wanted (0: one per sequence), and at most
-    int most, limit;    // rows of a narrow sequence
+    int nc, cblocks;   // 16-row column sets of a narrow workgroup; column blocks of a sequence at most
+    int items;         // units wanted; 0: cblocks for each sequence
+    int64_t units;     // at most
+    int most, limit;   // rows of a narrow sequence
     int splits;         // of a wide sequence's keys
     int64_t slots;      // blocks of wide rows at most; 0: no sequence is wide
     int64_t grid;       // workgroups
@@ -73,7 +80,8 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     int64_t most = G;
     r.splits = 1;
     if (packed) {
-        r.limit = kFp4Narrow;
+        // Few rows in all are narrow however they are shared out.
+        r.limit = n * G <= kFp4AllNarrow ? kFp4AllNarrow : kFp4Narrow;
         most = n * G < r.limit ? n * G : r.limit;
         if (n * G > r.limit) {
             const int64_t blocks = (n * G + kFp4Rows - 1) / kFp4Rows, some = n * G / (r.limit + 1);
@@ -88,29 +96,25 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     r.most = (int)most;
     r.nc = !weighed && most > 16 && (!packed || r.slots > 0 || n * G > 16 * B) ? 2 : 1;
     r.cblocks = (r.most + 16 * r.nc - 1) / (16 * r.nc);
-    int64_t items = 0;
-    if (shared) {
-        items = kFp4Wanted / (h_kv * r.cblocks);
-        if (items < 1) items = 1;
-    }
-    r.items = (int)items;
-    // No narrow sequence has more tokens than rows.
-    const int64_t longest = (seen(packed ? kFp4Narrow : 1) + 31 + 127) / 128;
-    r.chunks = (int)(items == 0 ? B : items + B < B * longest ? items + B : B * longest);
-    r.grid = r.slots * r.splits * h_kv + (int64_t)r.chunks * h_kv * r.cblocks;
+    r.items = (int)(!shared ? 0 : kFp4Wanted / h_kv > 1 ? kFp4Wanted / h_kv : 1);
+    // Column blocks of all narrow sequences; none of these has more tokens than rows.
+    const int64_t cols = 16 * r.nc, each_has = B * r.cblocks, by_rows = n * G / cols + B;
+    const int64_t all = packed && by_rows < each_has ? by_rows : each_has;
+    const int64_t longest = (seen(packed ? r.limit : 1) + 31 + 127) / 128;
+    r.units = !shared ? each_has : r.items + all < all * longest ? r.items + all : all * longest;
+    r.grid = (r.slots * r.splits + r.units) * h_kv;
     r.plan_bytes = (B * 8 + 15) / 16 * 16;
-    if (items > 0 || weighed) r.part_bytes = (int64_t)r.chunks * h_kv * r.cblocks * 16 * r.nc * (D + 4) * 4;
+    if (shared || weighed) r.part_bytes = r.units * h_kv * cols * (D + 4) * 4;
     r.raw_ld = (seen(1) + 31 + 31) / 32 * 32;
     if (weighed) r.raw_bytes = B * H * r.raw_ld * 4;
 
-    r.join.cols = 16 * r.nc;
     r.join.most = r.most;
     r.join.ncol = 2;
     while (4 * r.join.ncol < D) r.join.ncol *= 2;
     // Threads that share a row's splits: as many as there may be, until the launch
     // fills the chip.
-    const int64_t per = items / (B > 0 ? B : 1) + 1, each = per < longest ? per : longest;
-    const int64_t narrow = items > 0 ? B * h_kv * r.most : 0, wide = r.splits > 1 ? n * H : 0;
+    const int64_t per = r.items / (B > 0 ? B : 1) + 1, each = per < longest ? per : longest;
+    const int64_t narrow = shared ? B * h_kv * r.most : 0, wide = r.splits > 1 ? n * H : 0;
     int64_t blocks = 0;
     for (r.join.groups = 1;; r.join.groups *= 2) {
         const int64_t rows = 256 / (r.join.ncol * r.join.groups);
@@ -118,8 +122,8 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
     }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
-    // The narrow kernel's own grid has heads, chunks and column blocks as dimensions.
-    r.fits = r.grid <= kMost && h_kv < 65536 && r.chunks < 65536 && r.cblocks < 65536 && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    // The narrow kernel's own grid has heads and units as dimensions.
+    r.fits = r.grid <= kMost && (r.slots > 0 || r.units < 65536) && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.wide = (int)wide;

@@ -368,30 +368,30 @@ int main() {
         if (!N || room > (int64_t)1 << 30) continue;
         const Fp4Plan r = fp4_plan(N, B, H, h_kv, D, pages, page, window, packed, weighed, (1 << 24) - 1);
         uint64_t total = 0;
-        int64_t wide = 0, chunks = 0;
+        int64_t wide = 0, units = 0, cols = 16 * r.nc;
         auto is_wide = [&](int64_t b) { return packed && nq[b] * G > r.limit; };
-        auto steps = [&](int64_t b) { return is_wide(b) ? 0 : fp4_steps((int)n[b], fp4_first((int)n[b], (int)nq[b], (int)window)); };
+        auto steps = [&](int64_t b) { return fp4_steps((int)n[b], fp4_first((int)n[b], (int)nq[b], (int)window)); };
+        auto columns = [&](int64_t b) { return is_wide(b) ? 0 : fp4_blocks(nq[b] * G, (int)cols); };
         for (int64_t b = 0; b < B; ++b) {
-            total += steps(b);
+            total += (uint64_t)steps(b) * columns(b);
             if (is_wide(b)) wide += (nq[b] * G + kFp4Rows - 1) / kFp4Rows;
-            if (!is_wide(b) && nq[b] * G > (int64_t)r.cblocks * 16 * r.nc) return printf("rows %%d\n", round), 1;
+            if (columns(b) > r.cblocks || (!is_wide(b) && nq[b] * G > r.most)) return printf("rows %%d\n", round), 1;
             const int64_t base = fp4_first((int)n[b], (int)nq[b], (int)window) & ~31;
             if (weighed && (n[b] - base + 31) / 32 * 32 > r.raw_ld) return printf("raw %%d\n", round), 1;
         }
         if (wide && !r.slots) return printf("no slots %%d\n", round), 1;
         if (r.items > 0) {
             const int64_t step = fp4_step(total, r.items);
-            for (int64_t b = 0; b < B; ++b) chunks += (steps(b) + step - 1) / step;
+            if (step < 1 || step > 1 << 23) return printf("step %%d\n", round), 1;
+            for (int64_t b = 0; b < B; ++b) units += (steps(b) + step - 1) / step * columns(b);
             if (wide > r.slots) return printf("slots %%d\n", round), 1;
         } else {
-            chunks = B;
-            for (int64_t b = 0; b < B; ++b)  // one chunk has to reach the end
-                if (n[b] > (int64_t)1 << 30) return 1;
+            units = B * r.cblocks;
             if (r.slots && r.slots < N * G / kFp4Rows + B + 1) return printf("slots by starts %%d\n", round), 1;
         }
-        if (chunks > r.chunks) return printf("chunks %%d: %%ld of %%d\n", round, (long)chunks, r.chunks), 1;
-        const int64_t parts = r.items > 0 || weighed ? (int64_t)r.chunks * h_kv * r.cblocks * 16 * r.nc * (D + 4) * 4 : 0;
-        if (r.part_bytes != parts || r.grid < (int64_t)r.chunks * h_kv * r.cblocks + (r.slots * r.splits) * h_kv) return 1;
+        if (units > r.units) return printf("units %%d: %%ld of %%ld\n", round, (long)units, (long)r.units), 1;
+        const int64_t parts = r.items > 0 || weighed ? r.units * h_kv * cols * (D + 4) * 4 : 0;
+        if (r.part_bytes != parts || r.grid != (r.units + r.slots * r.splits) * h_kv) return 1;
         if (r.fits && r.items > 0 && (int64_t)r.join.narrow != B * h_kv * r.most) return 1;
     }
     return 0;

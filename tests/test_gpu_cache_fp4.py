@@ -165,8 +165,9 @@ def test_several_tokens_head_dims_and_groups(cuda_device, dtype, D, H, Hkv):
 @pytest.mark.parametrize("dtype", list(DT))
 @pytest.mark.parametrize("page", [1, 7, 16, 24, 64])
 @pytest.mark.parametrize("window", [0, 1, 50])
-def test_several_tokens_pages_and_windows(cuda_device, dtype, page, window):
-    _attend(cuda_device, [300, 31, 2, 129, 8], page, 4, 2, 64, DT[dtype], new=[70, 31, 1, 4, 12], window=window, seed=7)  # 12 of 8
+@pytest.mark.parametrize("H", [4, 16])  # all rows narrow, some wide
+def test_several_tokens_pages_and_windows(cuda_device, dtype, page, window, H):
+    _attend(cuda_device, [300, 31, 2, 129, 8], page, H, 2, 64, DT[dtype], new=[70, 31, 1, 4, 12], window=window, seed=7)  # 12 of 8
 
 
 @pytest.mark.parametrize("dtype", list(DT))
@@ -174,6 +175,7 @@ def test_several_tokens_pages_and_windows(cuda_device, dtype, page, window):
 def test_several_tokens_long_and_mixed(cuda_device, dtype, D):
     scale = torch.tensor([1.0, -2.0, 30.0, 0.1])
     _attend(cuda_device, [1500, 700, 1, 333], 16, 4, 2, D, DT[dtype], new=[1, 300, 1, 9], scale=scale, seed=8)
+    _attend(cuda_device, [900, 2000, 333], 16, 4, 1, D, DT[dtype], new=[40, 1, 50], scale=scale, seed=13)
     _attend(cuda_device, [1200], 16, 8, 2, D, DT[dtype], new=[260], window=300, seed=9)
     _attend(cuda_device, [900], 32, 4, 4, D, DT[dtype], new=[1], scale=scale, eps=0.3, seed=10)
 
@@ -181,7 +183,8 @@ def test_several_tokens_long_and_mixed(cuda_device, dtype, D):
 @pytest.mark.parametrize("dtype", list(DT))
 def test_several_tokens_over_tables_of_one_step(cuda_device, dtype):
     """No more than 128 keys a sequence: nothing to share out."""
-    _attend(cuda_device, [112, 90, 0, 7, 100], 16, 4, 2, 64, DT[dtype], new=[112, 50, 0, 7, 33], seed=11)
+    for H in (2, 8):
+        _attend(cuda_device, [112, 90, 0, 7, 100], 16, H, 2, 64, DT[dtype], new=[112, 50, 0, 7, 33], seed=11)
     _attend(cuda_device, [100, 90, 3], 5, 6, 1, 128, DT[dtype], new=[1, 80, 3], window=40, seed=12)
 
 
@@ -209,9 +212,9 @@ def test_missing_pages_lengths_and_bytes_of_nobody(cuda_device, several):
 @pytest.mark.parametrize("D", [64, 128, 256])
 def test_tokens_that_are_no_numbers_reach_those_that_see_them_alone(cuda_device, dtype, D):
     dt = DT[dtype]
-    for n_new, page in ((9, 4), (150, 16), (150, 1)):
+    for n_new, page, G in ((9, 4, 2), (150, 16, 2), (150, 16, 8), (150, 1, 4)):
         g = torch.Generator().manual_seed(7)
-        k, v, x = (torch.rand(n_new, h, D, generator=g).to(dt) for h in (2, 2, 4))
+        k, v, x = (torch.rand(n_new, h, D, generator=g).to(dt) for h in (2, 2, 2 * G))
         a, b = n_new // 3, 2 * n_new // 3
         k[a, 0, 5], v[b, 1, 40] = math.nan, math.inf
         cache = born_cache_fp4(-(-n_new // page), page, 2, D, device=cuda_device)
@@ -223,7 +226,7 @@ def test_tokens_that_are_no_numbers_reach_those_that_see_them_alone(cuda_device,
         nan = out.isnan()
         assert torch.equal(nan.all(-1), nan.any(-1))
         for h, at in ((0, a), (1, b)):
-            for i in (2 * h, 2 * h + 1):
+            for i in range(G * h, G * h + G):
                 assert torch.nonzero(nan[:, i].any(-1)).view(-1).tolist() == [at, at + 1]
         # One token, which sees them all.
         weight = torch.zeros(1, 2, n_new, device=cuda_device)
@@ -470,7 +473,7 @@ def test_second_turns_agree_with_the_wide_attention(cuda_device):
     lens, new = [900, 250, 411], [300, 250, 7]
     cache, table, n, _ = ref.make_cache(lens, 16, 2, 128, seed=14, device=cuda_device)
     cu, ck = (torch.tensor(serve_ref.starts(x), device=cuda_device, **INT) for x in (new, lens))
-    q = torch.nn.functional.normalize(torch.randn(sum(new), 8, 128, generator=torch.Generator().manual_seed(15)), dim=-1)
+    q = torch.nn.functional.normalize(torch.randn(sum(new), 8, 128, generator=torch.Generator().manual_seed(15)), dim=-1)  # 2228 rows
     q = q.to(cuda_device, torch.float32)
     k, v = born_cache_read_fp4(cache, table, n, ck, sum(lens), dtype=torch.float32)
     for window in (0, 100):
