@@ -629,8 +629,7 @@ struct Fp4Parts {
 };
 
 // Splits joined in order.  A row's columns take `ncol` threads, its splits
-// `groups` of them, 256 / (ncol groups) rows a workgroup: first the narrow
-// kernel's rows (sequence, key head, row), then the tiled kernel's (token, head).
+// `groups` of them, 256 / (ncol groups) rows a workgroup.
 // WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the sum
 // over the group of p_j / Z, the heads in order, is added to its weights.
 template <class E, bool WEIGH>
@@ -669,28 +668,42 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
     const float* from = nullptr;
     int64_t ld = 0, row = 0;  // row: token and head
     int n = 0, head = 0;
-    if (unit < q.narrow) {
-        const int rest = unit / q.most, r = unit - rest * q.most, b = rest / p.Hkv, hk = rest - b * p.Hkv;
-        const Fp4Seq sq(p, b);
-        if (!sq.wide(p) && r < sq.nq * p.G) {
-            const Fp4Parts part(p, sq, b, hk, r);
+    if (unit < q.narrow + q.rows) {
+        int b, hk, r;
+        Fp4Seq sq(p, 0);
+        if (unit < q.narrow) {
+            const int rest = unit / q.most;
+            r = unit - rest * q.most;
+            b = rest / p.Hkv;
+            hk = rest - b * p.Hkv;
+            sq = Fp4Seq(p, b);
+        } else {
+            const int at = unit - q.narrow, t = at / p.H, h = at - t * p.H;
+            b = t;
+            if (p.cu != nullptr) {
+                int hi = p.B;  // the last start at or before t
+                b = 0;
+                while (hi - b > 1) {
+                    const int mid = (b + hi) / 2;
+                    if (p.cu[mid] <= t) b = mid;
+                    else hi = mid;
+                }
+            }
+            sq = Fp4Seq(p, b);
+            hk = h / p.G;
+            r = t >= sq.q0 ? (t - sq.q0) * p.G + h - hk * p.G : INT_MAX;
+        }
+        if (r < sq.nq * p.G) {
             const int t = r / p.G;
             head = hk * p.G + r - t * p.G;
             row = (int64_t)(sq.q0 + t) * p.H + head;
-            if (part.n > 1) from = part.at, ld = part.ld, n = part.n;  // one: written already
+            if (sq.wide(p)) {
+                if (unit >= q.narrow) from = p.wide_part + row * p.splits * (p.D + 4), ld = p.D + 4, n = p.splits;
+            } else if (unit < q.narrow || p.slots == 0) {
+                const Fp4Parts part(p, sq, b, hk, r);
+                if (part.n > 1) from = part.at, ld = part.ld, n = part.n;  // one: written already
+            }
         }
-    } else if (unit < q.narrow + q.wide) {
-        const int at = unit - q.narrow, t = at / p.H;
-        row = at;
-        head = at - t * p.H;
-        int lo = 0, hi = p.B;  // the last start at or before t
-        while (hi - lo > 1) {
-            const int mid = (lo + hi) / 2;
-            if (p.cu[mid] <= t) lo = mid;
-            else hi = mid;
-        }
-        const Fp4Seq sq(p, lo);
-        if (t >= sq.q0 && t < sq.q0 + sq.nq && sq.wide(p)) from = p.wide_part + row * p.splits * (p.D + 4), ld = p.D + 4, n = p.splits;
     }
     const bool ok = col < p.D;
     f32x4v x = {0.f, 0.f, 0.f, 0.f};

@@ -47,8 +47,9 @@ constexpr int fp4_step(uint64_t total, uint32_t items) {
 
 struct Fp4Join {
     int ncol, groups, most;
-    int narrow, wide;  // rows
-    int blocks;        // workgroups of them
+    int narrow;  // rows as (sequence, key head, up to `most`): the narrow ones beside a tiled kernel's
+    int rows;    // rows as (token, head): all, or the wide ones
+    int blocks;  // workgroups of them
 };
 
 struct Fp4Plan {
@@ -114,19 +115,20 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     // Threads that share a row's splits: as many as there may be, until the launch
     // fills the chip.
     const int64_t per = r.items / (B > 0 ? B : 1) + 1, each = per < longest ? per : longest;
-    const int64_t narrow = shared ? B * h_kv * r.most : 0, wide = r.splits > 1 ? n * H : 0;
+    const int64_t narrow = shared && r.slots > 0 ? B * h_kv * r.most : 0;
+    const int64_t rows = (r.slots > 0 ? r.splits > 1 : shared) ? n * H : 0;
     int64_t blocks = 0;
     for (r.join.groups = 1;; r.join.groups *= 2) {
-        const int64_t rows = 256 / (r.join.ncol * r.join.groups);
-        blocks = (narrow + wide + rows - 1) / rows;
+        const int64_t each_block = 256 / (r.join.ncol * r.join.groups);
+        blocks = (narrow + rows + each_block - 1) / each_block;
         if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
     }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
     // The narrow kernel's own grid has heads and units as dimensions.
-    r.fits = r.grid <= kMost && (r.slots > 0 || r.units < 65536) && narrow + wide < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    r.fits = r.grid <= kMost && (r.slots > 0 || r.units < 65536) && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
-        r.join.wide = (int)wide;
+        r.join.rows = (int)rows;
         r.join.blocks = (int)blocks;
     }
     return r;

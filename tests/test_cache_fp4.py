@@ -392,7 +392,8 @@ int main() {
         if (units > r.units) return printf("units %%d: %%ld of %%ld\n", round, (long)units, (long)r.units), 1;
         const int64_t parts = r.items > 0 || weighed ? r.units * h_kv * cols * (D + 4) * 4 : 0;
         if (r.part_bytes != parts || r.grid != (r.units + r.slots * r.splits) * h_kv) return 1;
-        if (r.fits && r.items > 0 && (int64_t)r.join.narrow != B * h_kv * r.most) return 1;
+        if (r.fits && r.items > 0 && r.join.narrow != (r.slots ? B * h_kv * r.most : 0)) return 1;
+        if (r.fits && r.join.rows != ((r.slots ? r.splits > 1 : r.items > 0) ? N * H : 0)) return 1;
     }
     return 0;
 }
