@@ -34,8 +34,20 @@ struct Fp4TileCfg {
     static constexpr int WPE = DP == 256 ? 1 : 2;
 };
 
-// Block x of rows: part i of a sequence's.
+// Block x of rows: part i of a sequence's.  With a lane for each sequence those
+// of the longest come first, so that a launch ends with short ones.
 __device__ __forceinline__ Fp4Part fp4_block(const Fp4PagedArgs& p, const Fp4Share& share, int x) {
+    if (p.items > 0 && p.B <= 64) {
+        const int k = share.lane() < p.B ? share.mine.blocks(p) : 0;
+        int before = 0;
+        for (int j = 0; j < p.B; ++j) {
+            const int n = __builtin_amdgcn_readlane(share.mine.n, j);
+            if (n > share.mine.n || (n == share.mine.n && j < share.lane())) before += __builtin_amdgcn_readlane(k, j);
+        }
+        const uint64_t here = __ballot(before <= x && x < before + k);
+        const int l = __builtin_amdgcn_readfirstlane(here != 0 ? __ffsll((long long)here) - 1 : 0);
+        return Fp4Part{here != 0 ? l : -1, x - __builtin_amdgcn_readlane(before, l), 0, share.mine.of_lane(l)}.uniform();
+    }
     if (p.items > 0) return fp4_part(p, share, x, [&](const Fp4Seq& s) { return s.blocks(p); });
     // Sequence s has the slots from cu[s] G / 128 + s on: never fewer than it has blocks.
     const int lane = threadIdx.x & 63;
