@@ -185,12 +185,14 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
 #pragma unroll
         for (int nb = 0; nb < SUB; ++nb) {
             f32x16 s = zero16();
+            __builtin_amdgcn_s_setprio(1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
                 const u32x4 a = k.row(32 * nb + c, ks, g);
 #pragma unroll
                 for (int u2 = 0; u2 < QP; ++u2) s = BF16::mfma(a, qr[ks][u2], s);
             }
+            __builtin_amdgcn_s_setprio(0);
             if (bad_here) {  // the sum's NaN may have either sign, the weights take a positive one
 #pragma unroll
                 for (int r = 0; r < 16; ++r) s[r] = s[r] == s[r] ? s[r] : __uint_as_float(0x7fc00000u);
@@ -267,46 +269,49 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     }
 }
 
-// Sequences of all sizes in one launch, so that neither kernel waits for the
-// other: the tiled one's workgroups, the narrow one's, and those of the grid
-// that the host could not know to be none.
-template <class E, int DP, bool P16>
+// Wide sequences alone, or sequences of all sizes in one launch (NARROW), so that
+// neither kernel waits for the other: the tiled one's workgroups, the narrow one's,
+// and those of the grid that the host could not know to be none.
+template <class E, int DP, bool P16, bool NARROW>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(Fp4TileCfg<E, DP>::WPE)))
 void born_fp4_chunk_kernel(Fp4PagedArgs p) {
-    constexpr int kTiles = 2 * Fp4TileCfg<E, DP>::STAGE, kBytes = kTiles > kFp4NarrowLds<DP> ? kTiles : kFp4NarrowLds<DP>;
+    constexpr int kTiles = 2 * Fp4TileCfg<E, DP>::STAGE, kBytes = kTiles > kFp4NarrowLds<DP> || !NARROW ? kTiles : kFp4NarrowLds<DP>;
     __shared__ __attribute__((aligned(1024))) uint8_t smem[kBytes];
     __shared__ int bad_tile[2];  // the last tile of each stage that holds a token that is not a number
-    fp4_behind<E>(p, blockIdx.x, gridDim.x);
+    if constexpr (NARROW) fp4_behind<E>(p, blockIdx.x, gridDim.x);
     const Fp4Share share(p, true);
-    const int tiled = share.wide * p.splits * p.Hkv, narrow = share.units * p.Hkv;
-    const int x = blockIdx.x;
+    const int tiled = share.wide * p.splits * p.Hkv, x = blockIdx.x;
     if (x < tiled) {
         fp4_tiled<E, DP, P16>(p, share, smem, bad_tile, x);
-    } else if (x < tiled + narrow) {
+    } else if (NARROW && x < tiled + share.units * p.Hkv) {
         const int y = x - tiled, unit = y / p.Hkv;
         fp4_narrow<E, DP, 2, false, P16>(p, share, smem, unit, y - unit * p.Hkv);
     }
 }
 
+template <class E, bool P16, bool NARROW>
+void launch_fp4_chunk_dp(const Fp4PagedArgs& a, int64_t grid, hipStream_t st) {
+    const dim3 g((unsigned)grid);
+    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 64, P16, NARROW>), g, dim3(256), 0, st, a);
+    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 128, P16, NARROW>), g, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 256, P16, NARROW>), g, dim3(256), 0, st, a);
+}
 template <class E, bool P16>
-void launch_fp4_chunk(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)plan.grid);
-    if (a.D <= 64) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 64, P16>), grid, dim3(256), 0, st, a);
-    else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 128, P16>), grid, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((born_fp4_chunk_kernel<E, 256, P16>), grid, dim3(256), 0, st, a);
+hipError_t launch_fp4_parts(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
+    if (plan.slots > 0 && !plan.apart) {
+        launch_fp4_chunk_dp<E, P16, true>(a, plan.grid, st);
+        return hipGetLastError();
+    }
+    launch_fp4_nc<E, P16>(a, plan, st);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess || plan.slots == 0) return e;
+    launch_fp4_chunk_dp<E, P16, false>(a, plan.slots * plan.splits * a.Hkv, st);
+    return hipGetLastError();
 }
 
 template <class E>
 hipError_t launch_fp4(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const bool p16 = fp4_p16(a.c);
-    if (plan.slots > 0) {
-        if (p16) launch_fp4_chunk<E, true>(a, plan, st);
-        else launch_fp4_chunk<E, false>(a, plan, st);
-    } else {
-        if (p16) launch_fp4_nc<E, true>(a, plan, st);
-        else launch_fp4_nc<E, false>(a, plan, st);
-    }
-    const hipError_t e = hipGetLastError();
+    const hipError_t e = fp4_p16(a.c) ? launch_fp4_parts<E, true>(a, plan, st) : launch_fp4_parts<E, false>(a, plan, st);
     return e != hipSuccess ? e : launch_fp4_join<E>(a, plan, st);
 }
 

@@ -8,12 +8,24 @@
 namespace qdl {
 
 constexpr int kFp4Rows = 128;  // rows (new tokens x heads of a group) of the tiled kernel's workgroups
-// Rows of a (sequence, key head) up to which the narrow kernel takes it.
-constexpr int kFp4Narrow = 64;
-constexpr int kFp4AllNarrow = 512;  // rows of a launch, likewise
-// Workgroups of the narrow kernel that a launch's chunks of keys are made for:
-// two rounds of three a compute unit.
-constexpr int kFp4Wanted = 1536;
+// Rows of a (sequence, key head) up to which the narrow kernel takes it.  us with
+// 32 and with 64: 32 sequences of 16 tokens over 4096 keys at most, 8 key heads
+// D128, 4 heads each, 64 and 74; 4 of 64 over 8000, 4 key heads, 45 and 47; few
+// rows the same.  A launch of few rows that are narrow in the mean goes to the
+// narrow kernel whole: 16 sequences of 5 tokens 28 and 33, 8 of 30 fp32 27 and 29;
+// not by the rows alone: one sequence of 128 tokens over 30000 keys 167 and 83.
+constexpr int kFp4Narrow = 32;
+constexpr int kFp4AllNarrow = 512, kFp4AllMean = 64;  // rows of a launch, and of its sequences in the mean, likewise
+// Workgroups of the narrow kernel that a launch's chunks of keys are made for: two
+// rounds of as many as a compute unit holds, three with one column set, two with two.
+constexpr int fp4_wanted(int nc) { return nc == 1 ? 1536 : 1024; }
+// Narrow and wide sequences have a launch each where the keys times key heads are
+// this many and the sequences' rows in the mean fit a narrow workgroup: most are
+// narrow then, and their own launch has three workgroups a compute unit for two.
+// us apart and together, 8 key heads D128, 4 heads each: 64 sequences of 4 tokens
+// over 8192 keys at most 67 and 104; where a few are wide it costs, 31 single
+// tokens beside one of 200 94 and 86, of 512 (mean 68: together) 158 and 127.
+constexpr int64_t kFp4Apart = (int64_t)1 << 20;
 // Sequences that a workgroup looks through to share out the keys.
 constexpr int kFp4Shared = 1024;
 
@@ -59,6 +71,7 @@ struct Fp4Plan {
     int most, limit;   // rows of a narrow sequence
     int splits;         // of a wide sequence's keys
     int64_t slots;      // blocks of wide rows at most; 0: no sequence is wide
+    bool apart;         // narrow and wide sequences in launches of their own
     int64_t grid;       // workgroups
     Fp4Join join;
     int64_t plan_bytes, part_bytes, raw_bytes, wide_bytes, raw_ld;
@@ -82,7 +95,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     r.splits = 1;
     if (packed) {
         // Few rows in all are narrow however they are shared out.
-        r.limit = n * G <= kFp4AllNarrow ? kFp4AllNarrow : kFp4Narrow;
+        r.limit = n * G <= kFp4AllNarrow && n * G <= kFp4AllMean * B ? kFp4AllNarrow : kFp4Narrow;
         most = n * G < r.limit ? n * G : r.limit;
         if (n * G > r.limit) {
             const int64_t blocks = (n * G + kFp4Rows - 1) / kFp4Rows, some = n * G / (r.limit + 1);
@@ -95,9 +108,10 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         }
     }
     r.most = (int)most;
-    r.nc = !weighed && most > 16 && (!packed || r.slots > 0 || n * G > 16 * B) ? 2 : 1;
+    r.apart = r.slots > 0 && n * G <= kFp4Narrow * B && B * seen(r.limit) * h_kv >= kFp4Apart;
+    r.nc = !weighed && most > 16 && (!packed || (r.slots > 0 && !r.apart) || n * G > 16 * B) ? 2 : 1;
     r.cblocks = (r.most + 16 * r.nc - 1) / (16 * r.nc);
-    r.items = (int)(!shared ? 0 : kFp4Wanted / h_kv > 1 ? kFp4Wanted / h_kv : 1);
+    r.items = (int)(!shared ? 0 : fp4_wanted(r.nc) / h_kv > 1 ? fp4_wanted(r.nc) / h_kv : 1);
     // Column blocks of all narrow sequences; none of these has more tokens than rows.
     const int64_t cols = 16 * r.nc, each_has = B * r.cblocks, by_rows = n * G / cols + B;
     const int64_t all = packed && by_rows < each_has ? by_rows : each_has;
@@ -125,7 +139,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
     // The narrow kernel's own grid has heads and units as dimensions.
-    r.fits = r.grid <= kMost && (r.slots > 0 || r.units < 65536) && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    r.fits = r.grid <= kMost && ((r.slots > 0 && !r.apart) || r.units < 65536) && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.rows = (int)rows;

@@ -6,7 +6,8 @@ Stored values are exact in bf16, so an overlap is an fp32 sum of exact products
 weights go into their product in two bf16 parts, what is left of them below
 2^-17 relative (each part takes half a step of 2^-8), fp32's in three, below two
 roundings of the square; bf16's in one, half a step of 2^-8, where a sequence
-has more than 64 rows (new tokens x heads of a group) and the call more than 512.  Sums of n terms are fp32 sums, the output is rounded
+has more than 32 rows (new tokens x heads of a group), but for calls of 512 rows
+or fewer and at most 64 a sequence in the mean.  Sums of n terms are fp32 sums, the output is rounded
 once."""
 
 from __future__ import annotations
@@ -72,7 +73,11 @@ def attend(q, cache, table, lens, scale, cu=None, eps=1e-12, window=0):
     q, table, lens = q.detach().cpu().double(), table.cpu(), lens.cpu()
     N, H, D = q.shape
     B, Hkv, page = table.shape[0], cache[0].shape[2], cache[0].shape[1]
-    room = table.shape[1] * page
+    room, G = table.shape[1] * page, H // Hkv
+
+    def wide(new):  # rows of the kernel for many new tokens
+        return new * G > 32 and not (N * G <= 512 and N * G <= 64 * B)
+
     cu = list(range(B + 1)) if cu is None else [int(x) for x in cu]
     s = torch.as_tensor(scale, dtype=torch.float64).detach().reshape(-1).cpu()
     s = s if s.numel() == H else s.repeat(H)
@@ -85,7 +90,7 @@ def attend(q, cache, table, lens, scale, cu=None, eps=1e-12, window=0):
         if n == 0 or new == 0:
             continue
         i, j = n - new + torch.arange(new).view(-1, 1), torch.arange(n).view(1, -1)
-        up = HALF_STEP[dt] + 3 * U32 if dt is torch.bfloat16 and new * (H // Hkv) > 64 and N * (H // Hkv) > 512 else WEIGHT[dt]
+        up = HALF_STEP[dt] + 3 * U32 if dt is torch.bfloat16 and wide(new) else WEIGHT[dt]
         keep = ok.view(1, -1) & (j <= i)
         if window > 0:
             keep = keep & (i - j < window)

@@ -106,8 +106,9 @@ def test_read(cuda_device, dtype, D):
 # ---------------------------------------------------------------------------
 # Attention
 # ---------------------------------------------------------------------------
-def _attend(dev, lens, page, H, Hkv, D, dtype, new=None, window=0, scale=2.0, eps=1e-12, weigh=False, seed=0, size=1.0):
+def _attend(dev, lens, page, H, Hkv, D, dtype, new=None, window=0, scale=2.0, eps=1e-12, weigh=False, seed=0, size=1.0, columns=0):
     cache, table, n, _ = ref.make_cache(lens, page, Hkv, D, seed)
+    table = torch.nn.functional.pad(table, (0, max(0, columns - table.shape[1])), value=-1)
     cu = None if new is None else serve_ref.starts(new)
     N = len(lens) if new is None else cu[-1] + 2  # two rows behind the last sequence
     q = torch.nn.functional.normalize(torch.randn(N, H, D, generator=torch.Generator().manual_seed(seed + 1)) + 0.1, dim=-1) * size
@@ -115,7 +116,7 @@ def _attend(dev, lens, page, H, Hkv, D, dtype, new=None, window=0, scale=2.0, ep
     weight = torch.full((len(lens), Hkv, max(lens + [1])), 0.5, device=dev) if weigh else None
     c, t, l, x, s, starts = _to(dev, cache, table, n, q, scale, None if cu is None else torch.tensor(cu, **INT))
     out = flash_born_attention_paged_fp4(x, c, t, l, s, starts, eps, window, weight)
-    o, w = ref.attend(q, cache, table, n, scale, cu, eps, window)
+    o, w = ref.attend(q, cache, table[:, : max(1, -(-max(lens + [1]) // page))], n, scale, cu, eps, window)
     assert out.dtype is dtype and ref.worst(out, o) <= 1.0
     if new is not None:
         assert not out[-2:].any()
@@ -186,6 +187,17 @@ def test_several_tokens_over_tables_of_one_step(cuda_device, dtype):
     for H in (2, 8):
         _attend(cuda_device, [112, 90, 0, 7, 100], 16, H, 2, 64, DT[dtype], new=[112, 50, 0, 7, 33], seed=11)
     _attend(cuda_device, [100, 90, 3], 5, 6, 1, 128, DT[dtype], new=[1, 80, 3], window=40, seed=12)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("page", [16, 10])
+def test_few_tokens_each_over_wide_tables(cuda_device, dtype, D, page):
+    """Tables of 2^17 keys: narrow and wide sequences in launches of their own."""
+    new = [60, 1, 4, 0, 9, 8, 3] + [5] * 14
+    _attend(cuda_device, [60, 300, 4, 7, 1000, 20, 33] + [40 + i for i in range(14)], page, 4, 1, D, DT[dtype], new=new, seed=16,
+            columns=(1 << 17) // page)
+    _attend(cuda_device, [60, 300, 0, 7], page, 4, 1, D, DT[dtype], seed=16, columns=(1 << 17) // page, weigh=True)
 
 
 @pytest.mark.parametrize("several", [False, True])
