@@ -4,14 +4,14 @@
 // whole blocks of 32 (zeros behind it).  A block is 16 bytes of 4-bit codes, the
 // lower nibble first, and one scale byte e: value = code 2^(e - 127), the codes
 // being sign, two exponent bits and one mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6.
-// e = 255: not a number.
+// e = 255: not a number; 253 and 254 are not written.
 //
 // Two significant bits and a power of two are exact in bf16, so every product
 // here runs on the bf16 matrix pipe whatever the type of the queries: these are
 // taken apart into bf16 parts that sum to them exactly (one for bf16, two for
 // fp16, three for fp32), and so are the fp32 weights where they are not rounded.
 //
-// A token that cannot be held (an infinity or NaN in it) has a block of scale
+// A token that cannot be held (an infinity, NaN or magnitude past 7 2^125 in it) has a block of scale
 // 255: every query that sees it, and no other, gets NaN.  A weight of 0 times a
 // NaN would reach the queries that do not see it, so V's bad blocks are read as
 // zeros and K's block as NaN in their place.

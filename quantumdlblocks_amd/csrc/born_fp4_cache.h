@@ -11,7 +11,8 @@ namespace qdl {
 // Append.  Queries as in the 16-bit cache's append: fp32, rounded once.  A key
 // or value row is stored by eight columns a lane, four lanes a block:
 //   e: the least with max |x| <= 7 2^e, at least -126; codes of x / 2^e to
-//   nearest, halfway to even, at most 6.
+//   nearest, halfway to even, at most 6.  e past 125 is not a number: a code of 4
+//   would be infinite, as its product with a weight of 0 would not be 0.
 // (Root mean square error on Gaussian rows .112; with e = floor(log2 max) - 2
 // .115, without values past 6 .116, the better of two neighbours each time .112.)
 //
@@ -120,8 +121,8 @@ struct Fp4Eight {
 // of a double's magnitude with the lower ones as a sticky bit, and the exponent
 // that brings values to their codes'.
 __device__ __forceinline__ int fp4_exponent(uint32_t top) {
-    if (top >= 0x7ff00000u) return (int)kFp4Bad - 127;
-    return max((int)(top >> 20) - 1023 - 2 + ((top & 0xfffffu) > 0xc0000u ? 1 : 0), -126);
+    const int e = (int)(top >> 20) - 1023 - 2 + ((top & 0xfffffu) > 0xc0000u ? 1 : 0);
+    return e > 125 ? (int)kFp4Bad - 127 : max(e, -126);
 }
 __device__ __forceinline__ uint32_t fp4_sticky(double x) {
     const uint64_t u = __builtin_bit_cast(uint64_t, x);

@@ -210,7 +210,8 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     if (c->struct_bytes != (int64_t)sizeof(qdl_born_fp4_paged_call)) return QDL_BORN_E_SHAPE;
     int rc = check_heads(c->dtype, c->H, c->h_kv, c->D);
     if (rc != QDL_BORN_OK) return rc;
-    if (c->n < 0 || c->n > kMostRows || c->B < 0 || c->B > kMostHeads || (!c->cu_seqlens && c->n != c->B)) return QDL_BORN_E_SHAPE;
+    if (c->n < 0 || c->n > kMostRows || c->B < 0 || c->B > kMostHeads || (c->B == 0 && c->n > 0) || (!c->cu_seqlens && c->n != c->B))
+        return QDL_BORN_E_SHAPE;
     if (c->scale && c->n_scale != 1 && c->n_scale != c->H) return QDL_BORN_E_SCALE;
     if (c->window_size < 0 || c->window_size > (int64_t)1 << 30) return QDL_BORN_E_WINDOW;
     if (!(c->eps >= 0.0) || (c->key_weight && (c->cu_seqlens || c->weight_len < 0 || c->weight_len > INT32_MAX))) return QDL_BORN_E_SHAPE;
@@ -243,6 +244,7 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     a.window = (int)c->window_size;
     a.items = r.items;
     a.cblocks = r.cblocks;
+    a.units = (int)r.units;
     a.cols = 16 * r.nc;
     a.limit = r.limit;
     a.splits = r.splits;

@@ -39,6 +39,7 @@ struct Fp4PagedArgs {
     int window;
     int items;             // units (a chunk of keys and a column block) wanted; 0: cblocks for each sequence
     int cblocks;           // column blocks of a sequence at most
+    int units;             // at most: `part` has room for no more
     int cols;              // rows of one
     int limit;             // rows of a (sequence, key head) that the narrow kernel takes
     int splits;            // of the tiled kernel's keys
@@ -121,11 +122,13 @@ struct Fp4Share {
         });
         step = fp4_step(total, p.items);
         if (!totals) return;
+        wide = min(wide, (int)p.slots);
         units = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
             units += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
             return false;
         });
+        units = min(units, p.units);  // more only where starts do not ascend
     }
     __device__ __forceinline__ static int lane() { return threadIdx.x & 63; }
     __device__ __forceinline__ static int last(int scan) { return __builtin_amdgcn_readlane(scan, 63); }
@@ -622,8 +625,10 @@ struct Fp4Parts {
     __device__ __forceinline__ Fp4Parts(const Fp4PagedArgs& p, const Fp4Seq& sq, int b, int hk, int r) {
         const int2 plan = p.plan[b];
         const int cb = r / p.cols;
-        n = plan.y;
-        ld = (int64_t)sq.columns(p) * p.Hkv * p.cols * (p.D + 4);
+        // In bounds also where starts do not ascend, and not all units had room.
+        const int columns = sq.columns(p);
+        n = plan.x >= 0 && plan.y > 0 && (int64_t)plan.x + (int64_t)plan.y * columns <= p.units ? plan.y : 0;
+        ld = (int64_t)columns * p.Hkv * p.cols * (p.D + 4);
         at = p.part + (((int64_t)(plan.x + cb) * p.Hkv + hk) * p.cols + r - cb * p.cols) * (p.D + 4);
     }
 };

@@ -74,7 +74,7 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     const Fp4Part blk = fp4_block(p, share, idx - split * share.wide);
     const Fp4Seq& sq = blk.sq;
     const int rows = sq.nq * p.G, m0 = blk.i * kFp4Rows;
-    if (blk.b < 0 || !sq.wide(p) || m0 >= rows) return;
+    if (blk.b < 0 || !sq.wide(p) || m0 < 0 || m0 >= rows) return;  // before the first: starts that do not ascend
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
@@ -178,10 +178,20 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) fp4_query<E>(at, 16 * ks + 8 * g, p.D, ok, sc < 0.f, qr[ks]);
     }
+    // Rows that are not numbers, or infinite: their sums may be NaN.
+    bool bad_row = false;
+#pragma unroll
+    for (int ks = 0; ks < KS; ++ks)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const uint32_t e = qr[ks][0][i] & 0x7f807f80u;
+            bad_row = bad_row || (e & 0xffffu) == 0x7f80u || e >= 0x7f800000u;
+        }
+    const bool bad_rows = __ballot(bad_row) != 0;
     auto tile = [&](int u, int st, auto kind) __attribute__((always_inline)) {
         const int key0 = (t0 + u) * BN;
         const Tile k = kt(st), v = vt(st);
-        const bool bad_here = __builtin_amdgcn_readfirstlane(bad_tile[st]) == u;
+        const bool bad_here = bad_rows || __builtin_amdgcn_readfirstlane(bad_tile[st]) == u;
 #pragma unroll
         for (int nb = 0; nb < SUB; ++nb) {
             f32x16 s = zero16();

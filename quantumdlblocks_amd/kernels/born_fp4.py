@@ -9,7 +9,8 @@ lower nibble the even one (sign, two exponent bits, one mantissa bit: 0, 0.5, 1,
 2 ** (e - 127).  e is the least with max |x| <= 7 * 2 ** (e - 127) over the block
 (at least 1), codes are the nearest, halfway to the even one, and at most 6.
 The values stored for a row of normal ones are off by 0.112 of it in norm.
-They are exact in bf16; a block with an infinity or NaN has e = 255.
+They are exact in bf16; a block with an infinity, a NaN or a magnitude past
+7 * 2 ** 125 has e = 255: not a number.
 
     born_cache_fp4                            an empty cache
     fused_qk_rope_l2_normalize_append_fp4     a step's new tokens, written to their slots
@@ -159,7 +160,7 @@ def _encode(x: torch.Tensor):
     D = x.shape[-1]
     x = torch.nn.functional.pad(x.double(), (0, -D % _BLOCK)).unflatten(-1, (-1, _BLOCK))
     top = x.abs().amax(-1)
-    bad = ~x.isfinite().all(-1)
+    bad = ~(top <= 7 * 2.0**125)
     m, e = torch.frexp(torch.where(bad, torch.ones_like(top), top))
     e = torch.where(top == 0, torch.full_like(e, -126), e - 3 + (m > 0.875)).clamp(min=-126)
     y = torch.where(bad.unsqueeze(-1), torch.zeros_like(x), x * _power(-e).unsqueeze(-1))
@@ -256,8 +257,8 @@ def fused_qk_rope_l2_normalize_append_fp4(
     The arguments are the same but for ``cache``; ``k`` and ``v`` have ``q``'s
     dtype or are cast to it.  Keys are rotated and normalised in 64 bits before
     their codes are chosen, so these do not depend on the order of a sum; queries
-    in fp32, rounded once.  A token with an infinity or NaN in its key or value
-    makes NaN of the rows that see it.
+    in fp32, rounded once.  A token with an infinity or NaN in its key or value,
+    or a value past 7 * 2 ** 125, makes NaN of the rows that see it.
     """
     if torch.compiler.is_compiling():  # one graph break, as the other operators
         return _call_uncompiled(fused_qk_rope_l2_normalize_append_fp4, (q, k, v, cos, sin, cache, block_table, cache_lens, cu_seqlens,

@@ -25,7 +25,7 @@ WEIGHT = {torch.bfloat16: 2.0 ** -17 + 3 * U32, torch.float16: 2.0 ** -17 + 3 * 
 
 def store_block(x):
     """32 Python floats -> (scale byte, 32 codes), by trying every code."""
-    if not all(math.isfinite(v) for v in x):
+    if not all(abs(v) <= 7.0 * 2.0 ** 125 for v in x):
         return 255, [0] * 32
     top = max(abs(v) for v in x)
     e = -126

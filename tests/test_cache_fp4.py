@@ -39,6 +39,7 @@ def test_the_stored_codes_are_the_nearest():
         blocks.append([x * size * (1 + 2.0 ** -40) for x in ties] + [0.0] * 19)
         blocks.append([x * size * (1 - 2.0 ** -40) for x in ties] + [7.0 * size] + [0.0] * 18)
     blocks += [[0.0] * 32, [2.0 ** -140] * 32, [math.inf] + [1.0] * 31, [1.0] * 31 + [math.nan]]
+    blocks += [[7 * 2.0 ** 125] * 32, [7 * 2.0 ** 125 * (1 + 2.0 ** -24)] + [1.0] * 31, [-1.99 * 2.0 ** 127] * 32]
     codes, scales = born_fp4._encode(torch.tensor(blocks, dtype=torch.float64))
     for x, c, s in zip(blocks, codes.tolist(), scales.tolist()):
         e, want = ref.store_block(x)
@@ -336,6 +337,7 @@ def test_argument_blocks_are_checked():
     assert rc("read", cu=0) == -5
     assert rc("paged", scale=P, n_scale=3) == -6 and rc("paged", window=-1) == -7 and rc("paged", ws=0) == -8 and rc("paged", ws_bytes=8) == -8
     assert rc("paged", weight=P, cu=P) == -2 and rc("paged", n=1 << 28, H=256, B=1, cu=P, qs=(1 << 14, 64)) == -2
+    assert rc("paged", n=500, B=0, cu=P) == -2  # tokens of no sequence
     assert rc("evict", budget=-1) == -16 and rc("evict", lens_out=P) == -2 and rc("evict", to=P) == -15 and rc("evict", kept=0) == -5
     assert rc("evict", weight=P, w_len=4, weight_out=P) == -2 and rc("evict", to=2 * P, to_pages=3, to_ld=2) == -15
     assert lib.qdl_flash_born_fp4_paged_workspace_size(2, 2, 4, 2, 64, 1 << 40, 1 << 24, 0, 0, 1) == 0
