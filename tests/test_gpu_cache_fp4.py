@@ -64,6 +64,31 @@ def test_append(cuda_device, dtype, D, freqs, rope):
 
 
 @pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [128, 72])
+def test_append_of_many_tokens(cuda_device, dtype, D):
+    """Enough of them that a token's lanes take several heads."""
+    dt, page, H, Hkv = DT[dtype], 16, 42 if D == 72 else 35, 7
+    half, vec = D // 2, 8 if dtype != "fp32" and D % 16 == 0 else 4
+    lanes = 1 << (-(-half // vec) - 1).bit_length()
+    N = -(-(1 << 20) // (H * lanes)) + 3
+    new, B = [N - 50, 7, 0, 40], 4
+    full = [N - 50 + 20, 7, 5, 60]
+    cache, table, n, _ = ref.make_cache(full, page, Hkv, D, seed=19)
+    g = torch.Generator().manual_seed(19)
+    q, k, v = (torch.randn(N, h, D, generator=g).to(dt) for h in (H, Hkv, Hkv))
+    cu = torch.tensor(serve_ref.starts(new), **INT)
+    ang = torch.rand(N, half - 1, generator=g) * 6
+    want = tuple(t.clone() for t in cache)
+    qd = fused_qk_rope_l2_normalize_append_fp4(q.double(), k.double(), v.double(), ang.cos(), ang.sin(), want, table, n, cu)
+    dev = _to(cuda_device, q, k, v, ang.cos(), ang.sin(), cache, table, n, cu)
+    got = fused_qk_rope_l2_normalize_append_fp4(*dev)
+    d = (got.double().cpu() - qd).abs()
+    assert (d <= serve_ref.HALF_STEP[dt] * 1.02 * qd.abs() + (D + 32) * 2.0 ** -24).all() and not got[-3:].any()
+    for a, b in zip(dev[5], want):
+        assert torch.equal(a.cpu(), b)
+
+
+@pytest.mark.parametrize("dtype", list(DT))
 def test_values_at_the_codes_borders(cuda_device, dtype):
     ties = [0.0, 0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0, 6.0, 7.0, -0.25, -0.75, -1.25, -1.75, -2.5, -3.5, -5.0, -7.0, -0.0]
     near = [x * (1 + s * torch.finfo(DT[dtype]).eps) for x in ties for s in (-1, 1)]
@@ -199,7 +224,8 @@ def test_few_tokens_each_over_wide_tables(cuda_device, dtype, D, page):
     new = [60, 1, 4, 0, 9, 8, 3] + [5] * 14
     _attend(cuda_device, [60, 300, 4, 7, 1000, 20, 33] + [40 + i for i in range(14)], page, 4, 1, D, DT[dtype], new=new, seed=16,
             columns=(1 << 17) // page)
-    _attend(cuda_device, [60, 300, 0, 7], page, 4, 1, D, DT[dtype], seed=16, columns=(1 << 17) // page, weigh=True)
+    for weigh in (False, True):
+        _attend(cuda_device, [60, 300, 0, 7], page, 4, 1, D, DT[dtype], seed=16, columns=(1 << 17) // page, weigh=weigh)
 
 
 @pytest.mark.parametrize("several", [False, True])
