@@ -39,7 +39,6 @@ struct Fp4PagedArgs {
     int window;
     int items;             // units (a chunk of keys and a column block) wanted; 0: cblocks for each sequence
     int cblocks;           // column blocks of a sequence at most
-    int units;             // at most: `part` has room for no more
     int cols;              // rows of one
     int limit;             // rows of a (sequence, key head) that the narrow kernel takes
     int splits;            // of the tiled kernel's keys
@@ -54,6 +53,7 @@ struct Fp4PagedArgs {
     int w_len;
     float* raw;            // (B, H, raw_ld): p without s^2, keys from the span's first 32 on
     int64_t raw_ld;
+    int units;             // at most: `part` has room for no more
 };
 
 // A sequence: its tokens (rows of q), keys, and the first key that any token sees.
@@ -122,13 +122,11 @@ struct Fp4Share {
         });
         step = fp4_step(total, p.items);
         if (!totals) return;
-        wide = min(wide, (int)p.slots);
         units = 0;
         each(p, [&](const Fp4Seq& s, int b0) {
             units += last(fp4_scan(b0 + lane() < p.B ? count(p, s) : 0));
             return false;
         });
-        units = min(units, p.units);  // more only where starts do not ascend
     }
     __device__ __forceinline__ static int lane() { return threadIdx.x & 63; }
     __device__ __forceinline__ static int last(int scan) { return __builtin_amdgcn_readlane(scan, 63); }
@@ -596,7 +594,7 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
                 sum += zred[w][cc];
             }
             const int r = c0 + 16 * i + cc, t = p.cu != nullptr ? r / p.G : 0, h = hk * p.G + r - t * p.G;
-            if (nsplit > 1 || WEIGH) {
+            if ((nsplit > 1 || WEIGH) && unit < p.units) {  // more only where starts do not ascend
                 float* to = p.part + (((int64_t)unit * p.Hkv + hk) * (16 * NC) + 16 * i + cc) * (p.D + 4);
                 *reinterpret_cast<f32x4v*>(to + 4 + col) = y;
                 if (col == 0) to[0] = sum;

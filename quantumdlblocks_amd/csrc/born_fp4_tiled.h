@@ -74,7 +74,8 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
     const Fp4Part blk = fp4_block(p, share, idx - split * share.wide);
     const Fp4Seq& sq = blk.sq;
     const int rows = sq.nq * p.G, m0 = blk.i * kFp4Rows;
-    if (blk.b < 0 || !sq.wide(p) || m0 < 0 || m0 >= rows) return;  // before the first: starts that do not ascend
+    // Where starts do not ascend there are more blocks than slots, or some before the first.
+    if (blk.b < 0 || !sq.wide(p) || (uint32_t)m0 >= (uint32_t)rows || (uint32_t)split >= (uint32_t)p.splits) return;
 
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int c = lane & 31, g = lane >> 5;
@@ -178,16 +179,11 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
 #pragma unroll
         for (int ks = 0; ks < KS; ++ks) fp4_query<E>(at, 16 * ks + 8 * g, p.D, ok, sc < 0.f, qr[ks]);
     }
-    // Rows that are not numbers, or infinite: their sums may be NaN.
-    bool bad_row = false;
+    // Rows that are not numbers, or infinite, whose sums may be NaN: 0 times them is.
+    f32x16 none = zero16();
 #pragma unroll
-    for (int ks = 0; ks < KS; ++ks)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const uint32_t e = qr[ks][0][i] & 0x7f807f80u;
-            bad_row = bad_row || (e & 0xffffu) == 0x7f80u || e >= 0x7f800000u;
-        }
-    const bool bad_rows = __ballot(bad_row) != 0;
+    for (int ks = 0; ks < KS; ++ks) none = BF16::mfma(u32x4{0u, 0u, 0u, 0u}, qr[ks][0], none);
+    const bool bad_rows = __ballot(none[0] != none[0]) != 0;
     auto tile = [&](int u, int st, auto kind) __attribute__((always_inline)) {
         const int key0 = (t0 + u) * BN;
         const Tile k = kt(st), v = vt(st);
