@@ -518,8 +518,9 @@ typedef struct qdl_born_fp4_cache {
 /*
  * Append, as qdl_flash_born_cache_append_call, the keys and values stored in 4
  * bits: e is the least with max |x| <= 7 2^(e - 127) over the block, at least 1,
- * the codes are nearest, halfway to even, at most 6; blocks with an infinity or
- * NaN get e = 255.  Keys are rotated and normalised in 64 bits, queries in fp32.
+ * the codes are nearest, halfway to even, at most 6; blocks with an infinity, a
+ * NaN or a magnitude past 7 2^125 get e = 255.  Keys are rotated and normalised
+ * in 64 bits, queries in fp32.
  */
 typedef struct qdl_born_fp4_append_call {
     int64_t struct_bytes;
@@ -559,7 +560,7 @@ int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call *call, qdl_stream_
  * its keys: its i-th of m is at position cache_lens - m + i and sees the keys up
  * to there, or the last window_size of them.  Tokens that see no key, and those
  * of no sequence, get zeros; a key with a block of e = 255 makes NaN of every
- * row that sees it.  The workspace's size is the size function's for the same
+ * row that sees it.  B up to 65535.  The workspace's size is the size function's for the same
  * sizes (packed: cu_seqlens != NULL; weighed: key_weight != NULL).
  * key_weight, only where cu_seqlens is NULL: as for qdl_flash_born_paged_forward_call.
  */

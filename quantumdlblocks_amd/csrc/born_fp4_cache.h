@@ -18,6 +18,9 @@ namespace qdl {
 //
 // A key's rotation and normalisation are in 64 bits: a code is a step function
 // of its value, so that its nearest value is found whatever the order of the sums.
+//
+// Bound by memory: 16384 tokens, 32 heads over 8, D128 bf16: 353 MB in 88 us (4.0
+// TB/s); 64 single tokens, 16 heads over 4: 5.5 us.
 // ---------------------------------------------------------------------------
 struct Fp4AppendArgs {
     const void *q, *k, *v;
@@ -161,7 +164,9 @@ __device__ __forceinline__ void fp4_store_row(const double (&y)[8], uint8_t* to,
     if ((lane & 3) == 0) scale[lane >> 2] = (uint8_t)(e + 127);
 }
 
-// Heads of stored rows that a token's lanes go through, ROWS at a time.
+// Heads of stored rows that a token's lanes go through, ROWS at a time: its slot
+// and angles once for them (the 16384 tokens read back too, 8 key heads: 99 us with
+// 8, 101 with 4, 115 with 2).
 template <int ROWS>
 constexpr int kFp4AppendHeads = ROWS > 1 ? 8 : 1;
 
@@ -335,7 +340,8 @@ __global__ __launch_bounds__(256) void born_fp4_append_kernel(Fp4AppendArgs p) {
 // Read.  Rows (token, head) of a packed batch, each sequence's last keys, as
 // values: eight columns of K and of V a lane, `lpr` lanes a token, its slot found
 // once for four heads; the lanes' tokens follow each other, as a head's rows do in
-// the cache.
+// the cache.  Bound by memory: 63 thousand keys of 8 heads D128 to bf16, 326 MB in
+// 66 us (4.9 TB/s); 1531 keys 4.2 us.
 // ---------------------------------------------------------------------------
 constexpr int kFp4ReadHeads = 4;
 struct Fp4ReadArgs {
@@ -394,7 +400,9 @@ __global__ __launch_bounds__(256) void born_fp4_read_kernel(Fp4ReadArgs p) {
 
 // ---------------------------------------------------------------------------
 // Evict: the 16-bit cache's selection, then the move of the kept rows: a lane
-// has a block of K and of V, 16 bytes of codes and a scale byte each.
+// has a block of K and of V, 16 bytes of codes and a scale byte each.  16 caches cut
+// from 97 thousand tokens to 4096 each, 8 key heads D128: selection 19 us, move 49
+// for 140 MB of scattered rows of 64 and 4 bytes.
 // ---------------------------------------------------------------------------
 struct Fp4EvictArgs {
     EvictArgs s;  // the selection's, and the tables

@@ -135,7 +135,8 @@ int qdl_flash_born_fp4_append_call(const qdl_born_fp4_append_call* c, qdl_stream
     while (a.lpr * vec < c->D / 2) a.lpr *= 2;
     a.lpw = 4;
     while (a.lpw < 4 * a.c.nb) a.lpw *= 2;
-    // Groups of four heads where single ones would fill the chip twice over.
+    // Groups of four heads where single ones would fill the chip twice over (16384
+    // tokens, 32 heads over 8, D128, read back too: 100 us, with single ones 144).
     const bool many = c->n * c->H * a.lpr >= (int64_t)1 << 20;
     const int64_t queries = append_blocks(c->n, many ? (c->H + 3) / 4 : c->H, a.lpr);
     const int each = many ? qdl::kFp4AppendHeads<4> : qdl::kFp4AppendHeads<1>;

@@ -19,6 +19,14 @@
 // The keys are shared out on the device, which knows the lengths: chunk = the
 // keys of all sequences over the workgroups wanted, in steps of 128, and each
 // sequence takes as many chunks as it needs.  Partial sums are joined in order.
+//
+// 32 single tokens over long caches (267 MB, 8 key heads D128, 4 heads each, bf16):
+// 57 us, 4.7 TB/s, and a join of 5: K's and V's conversions, some 340 vector and
+// 230 scalar instructions for a wave's 32 keys, take 42% of the cycles beside the
+// loads, which are two steps ahead.  16 sequences of 5 tokens over 51 thousand keys
+// (4 key heads) 20 us and 5 where the bytes take 6; one token over 1531 keys 7 and
+// 4: chains of loads, the lengths, the table's entry, the codes, the partial sums,
+// a microsecond each.  Read without a page's base in scalars, 92 us for 73.
 #pragma once
 
 #include "born_fp4.h"
@@ -200,8 +208,8 @@ struct Fp4Cfg {
     static constexpr int VC = DP / 16, VD = (VC + 7) / 8;  // columns of a lane's key, dwords of codes
 };
 
-// Waves a SIMD should hold: of a column set's registers, and where the keys are
-// waited for.
+// Waves a SIMD that the registers of a column set and of its queries' parts leave
+// without spills.
 template <class E>
 constexpr int fp4_wpe(int DP, int NC) {
     return DP == 256 ? 1 : NC == 2 ? (kQParts<E> < 3 || DP == 64 ? 2 : 1) : kQParts<E> == 1 || DP == 64 ? 3 : 2;

@@ -10,6 +10,13 @@
 // Sixteen lanes that write LDS together have one block of 16 keys, which the
 // rows' swizzle spreads over all banks.
 //
+// 8 second turns (4583 tokens over 27 thousand keys, 32 heads over 8, D128 bf16):
+// 245 us, 920 TFLOP/s, and a join of 5; a large matrix product has 1200.  The
+// vector instructions issue in 36% of the cycles and the matrix instructions in
+// 26, the rest waits: two workgroups a compute unit is what 239 registers leave,
+// and with one column block of 32 rows a wave each operand read from LDS feeds
+// one product.  A higher priority around the overlaps' products: 254 us for 258.
+//
 // Keys without a page, or past the sequence, are zeros: overlaps of 0, weights
 // of 0.  Few blocks of rows split their keys; the partial sums are joined in order.
 #pragma once
@@ -20,9 +27,8 @@ namespace qdl {
 
 // bf16 parts of the weights.  bf16 outputs take one, rounded as the output is,
 // and Z adds the rounded weights, as in the packed forward: the matrix pipe
-// bounds this kernel, and the keys' own 4 bits are off by 60 times as much (8
-// second turns, 4583 tokens over 27 thousand keys, 32 heads over 8, D128: 327 us,
-// with two parts 420; error in norm 2.2e-3, 1.7e-3).
+// bounds this kernel, and the keys' own 4 bits are off by 50 times as much (the 8
+// second turns: 264 us, with two parts 343; error in norm 2.3e-3, 1.7e-3).
 template <class E>
 constexpr int kTileParts = std::is_same<E, BF16>::value ? 1 : kPParts<E>;
 
@@ -35,7 +41,8 @@ struct Fp4TileCfg {
 };
 
 // Block x of rows: part i of a sequence's.  With a lane for each sequence those
-// of the longest come first, so that a launch ends with short ones.
+// of the longest come first, so that a launch ends with short ones (the 8 second
+// turns 264 us, in the sequences' order 327).
 __device__ __forceinline__ Fp4Part fp4_block(const Fp4PagedArgs& p, const Fp4Share& share, int x) {
     if (p.items > 0 && p.B <= 64) {
         const int k = share.lane() < p.B ? share.mine.blocks(p) : 0;

@@ -18,6 +18,9 @@ constexpr int kFp4Narrow = 32;
 constexpr int kFp4AllNarrow = 512, kFp4AllMean = 64;  // rows of a launch, and of its sequences in the mean, likewise
 // Workgroups of the narrow kernel that a launch's chunks of keys are made for: two
 // rounds of as many as a compute unit holds, three with one column set, two with two.
+// us with 512, 768, 1024, 1536, 2048: 32 single tokens over long caches 76, 72, 74,
+// 65, 67; 16 sequences of 5 tokens (two column sets, before chunks of few keys were
+// made fewer) 49, 51, 50, 55, 59.
 constexpr int fp4_wanted(int nc) { return nc == 1 ? 1536 : 1024; }
 // Narrow and wide sequences have a launch each where the keys times key heads are
 // this many and the sequences' rows in the mean fit a narrow workgroup: most are
@@ -100,7 +103,9 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         if (n * G > r.limit) {
             const int64_t blocks = (n * G + kFp4Rows - 1) / kFp4Rows, some = n * G / (r.limit + 1);
             r.slots = n * G / kFp4Rows + (!shared ? B + 1 : B < some ? B : some);
-            // Two workgroups a compute unit, none under two tiles of 64 keys.
+            // Two workgroups a compute unit, none under two tiles of 64 keys (a mixed
+            // step of 9 sequences 22.4 us, with four tiles 34.3, with one 21.4 and twice
+            // the partial sums).
             int64_t splits = 512 / (blocks * h_kv);
             if (splits > seen(kFp4Rows) / 128) splits = seen(kFp4Rows) / 128;
             r.splits = (int)(splits < 1 ? 1 : splits);
