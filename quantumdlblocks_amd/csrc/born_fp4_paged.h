@@ -653,6 +653,17 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
         const int j0 = sq.base() + block * 256, j = j0 + threadIdx.x;
         if (j0 >= sq.n) return;
         const bool seen = j >= sq.first && j < sq.n && j < p.w_len;
+        // On their way before the denominators are known (16 caches of 52 thousand
+        // keys, 4 key heads D64, 4 heads each: 22.4 us, after them 23.3).
+        constexpr int kFirst = 4;
+        float* const weight = p.weights + (int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j;
+        float first[kFirst] = {}, old = 0.f;
+        if (seen) {
+            old = *weight;
+#pragma unroll
+            for (int i = 0; i < kFirst; ++i)
+                if (i < p.G) first[i] = p.raw[((int64_t)b * p.H + hk * p.G + i) * p.raw_ld + (j - sq.base())];
+        }
         float sum = 0.f;
         for (int g0 = 0; g0 < p.G; g0 += 256) {
             const int gn = min(256, p.G - g0);
@@ -666,12 +677,17 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
             __syncthreads();
             if (seen) {
                 const float* raw = p.raw + ((int64_t)b * p.H + hk * p.G + g0) * p.raw_ld + (j - sq.base());
+                if (g0 == 0) {
+#pragma unroll
+                    for (int i = 0; i < kFirst; ++i)
+                        if (i < gn) sum = fmaf(first[i], zred[i], sum);
+                }
 #pragma unroll 4
-                for (int i = 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
+                for (int i = g0 == 0 ? kFirst : 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
             }
             __syncthreads();
         }
-        if (seen) p.weights[(int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j] += sum;
+        if (seen) *weight = old + sum;
         return;
     }
     const int per = q.ncol * q.groups, mine = threadIdx.x / per, col = 4 * (threadIdx.x % q.ncol), group = threadIdx.x % per / q.ncol;
