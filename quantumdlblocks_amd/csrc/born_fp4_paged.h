@@ -21,7 +21,7 @@
 // sequence takes as many chunks as it needs.  Partial sums are joined in order.
 //
 // 32 single tokens over long caches (267 MB, 8 key heads D128, 4 heads each, bf16):
-// 57 us, 4.7 TB/s, and a join of 5: K's and V's conversions, some 340 vector and
+// 65 us, 4.1 TB/s, and a join of 5: K's and V's conversions, some 340 vector and
 // 230 scalar instructions for a wave's 32 keys, take 42% of the cycles beside the
 // loads, which are two steps ahead.  16 sequences of 5 tokens over 51 thousand keys
 // (4 key heads) 20 us and 5 where the bytes take 6; one token over 1531 keys 7 and

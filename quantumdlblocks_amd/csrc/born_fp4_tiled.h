@@ -11,7 +11,7 @@
 // rows' swizzle spreads over all banks.
 //
 // 8 second turns (4583 tokens over 27 thousand keys, 32 heads over 8, D128 bf16):
-// 245 us, 920 TFLOP/s, and a join of 5; a large matrix product has 1200.  The
+// 248 us, 910 TFLOP/s, and a join of 5; a large matrix product has 1200.  The
 // vector instructions issue in 36% of the cycles and the matrix instructions in
 // 26, the rest waits: two workgroups a compute unit is what 239 registers leave,
 // and with one column block of 32 rows a wave each operand read from LDS feeds
