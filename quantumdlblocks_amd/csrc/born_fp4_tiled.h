@@ -11,11 +11,13 @@
 // rows' swizzle spreads over all banks.
 //
 // 8 second turns (4583 tokens over 27 thousand keys, 32 heads over 8, D128 bf16):
-// 248 us, 910 TFLOP/s, and a join of 5; a large matrix product has 1200.  The
-// vector instructions issue in 36% of the cycles and the matrix instructions in
-// 26, the rest waits: two workgroups a compute unit is what 239 registers leave,
-// and with one column block of 32 rows a wave each operand read from LDS feeds
-// one product.  A higher priority around the overlaps' products: 254 us for 258.
+// 332 us, 680 TFLOP/s of the formula's, and a join of 5; a large matrix product
+// has 1200.  The weights' two parts make three products of the formula's two: with
+// one part it was 250 us, but a row was off by 2.3e-3 in norm where the narrow
+// kernel's are by 1.7e-3, so that its precision hung on what else was in the batch.
+// Two workgroups a compute unit is what 256 registers leave, and with one column
+// block of 32 rows a wave each operand of K from LDS feeds one product.  A higher
+// priority around the overlaps' products: 254 us for 258 (with one part).
 //
 // Keys without a page, or past the sequence, are zeros: overlaps of 0, weights
 // of 0.  Few blocks of rows split their keys; the partial sums are joined in order.
@@ -24,13 +26,6 @@
 #include "born_fp4_paged.h"
 
 namespace qdl {
-
-// bf16 parts of the weights.  bf16 outputs take one, rounded as the output is,
-// and Z adds the rounded weights, as in the packed forward: the matrix pipe
-// bounds this kernel, and the keys' own 4 bits are off by 50 times as much (the 8
-// second turns: 264 us, with two parts 343; error in norm 2.3e-3, 1.7e-3).
-template <class E>
-constexpr int kTileParts = std::is_same<E, BF16>::value ? 1 : kPParts<E>;
 
 template <class E, int DP>
 struct Fp4TileCfg {
@@ -75,8 +70,7 @@ template <class E, int DP, bool P16>
 __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share& share, uint8_t* ring, int* bad_tile, int block) {
     using C = Fp4TileCfg<E, DP>;
     using Tile = PackedTile<BF16, DP, C::BN>;
-    constexpr int BN = C::BN, SUB = C::SUB, NB = C::NB, KS = DP / 16, DB = DP / 32, QP = kQParts<E>, IT = kItem<E>;
-    constexpr int PP = kTileParts<E>;
+    constexpr int BN = C::BN, SUB = C::SUB, NB = C::NB, KS = DP / 16, DB = DP / 32, QP = kQParts<E>, PP = kPParts<E>, IT = kItem<E>;
     const int idx = block / p.Hkv, hk = block - idx * p.Hkv, split = idx / share.wide;
     const Fp4Part blk = fp4_block(p, share, idx - split * share.wide);
     const Fp4Seq& sq = blk.sq;
@@ -220,13 +214,9 @@ __device__ __forceinline__ void fp4_tiled(const Fp4PagedArgs& p, const Fp4Share&
             uint32_t wt[8][PP];
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                if constexpr (PP == 1) {
-                    wt[j][0] = born_weight_pair<BF16>(s[2 * j], s[2 * j + 1], 1.f, z);
-                } else {
-                    const float a0 = relu_f32(s[2 * j]), a1 = relu_f32(s[2 * j + 1]);
-                    z = (z + a0 * a0) + a1 * a1;
-                    fp4_parts<PP>(a0 * a0, a1 * a1, wt[j]);
-                }
+                const float a0 = relu_f32(s[2 * j]), a1 = relu_f32(s[2 * j + 1]);
+                z = (z + a0 * a0) + a1 * a1;
+                fp4_parts<PP>(a0 * a0, a1 * a1, wt[j]);
             }
 #pragma unroll
             for (int hh = 0; hh < 2; ++hh)

@@ -1,0 +1,77 @@
+"""The 4-bit paged cache on the GPU where it is easiest to get wrong: precision
+whatever else is in the batch, values that are not numbers, exact ties, large
+batches, wide tables, and memory behind the tensors."""
+
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import fp4_ref as ref
+import serve_ref
+from quantumdlblocks_amd import (
+    _native,
+    born_cache_fp4,
+    flash_born_attention_paged_fp4,
+    fused_qk_rope_l2_normalize_append_fp4,
+)
+from quantumdlblocks_amd.kernels import born_fp4
+
+pytestmark = pytest.mark.gpu
+
+DT = {"bf16": torch.bfloat16, "fp16": torch.float16, "fp32": torch.float32}
+INT = dict(dtype=torch.int32)
+
+
+def _rows(cache, table, n, D):
+    """fp4_ref.rows for long caches: every key at once."""
+    kc, vc, ks, vs = (t.cpu() for t in cache)
+    page, j = kc.shape[1], torch.arange(n)
+    t = table[j // page].long()
+    ok = (t >= 0) & (t < kc.shape[0])
+    t, r = torch.where(ok, t, torch.zeros_like(t)), torch.where(ok, j % page, torch.zeros_like(j))
+    bad = (ks[t, r] == 255).any(-1) | (vs[t, r] == 255).any(-1)
+    return ref.value(kc[t, r], ks[t, r])[..., :D], ref.value(vc[t, r], vs[t, r])[..., :D], ok, bad
+
+
+@pytest.fixture(autouse=True)
+def _every_key_at_once(monkeypatch):
+    monkeypatch.setattr(ref, "rows", _rows)
+
+
+def _queries(N, H, D, dtype, seed):
+    x = torch.randn(N, H, D, generator=torch.Generator().manual_seed(seed)) + 0.1
+    return torch.nn.functional.normalize(x, dim=-1).to(dtype)
+
+
+def _tight(q, cache, table, lens, scale, cu, eps=1e-12, window=0):
+    """fp4_ref.attend a few tokens at a time: the bound of 32 rows or fewer."""
+    G, outs = q.shape[1] // cache[0].shape[2], []
+    for b in range(len(cu) - 1):
+        new, few = cu[b + 1] - cu[b], max(1, 32 // G)
+        for i in range(0, new, few):
+            m = min(few, new - i)
+            n = torch.tensor([int(lens[b]) - new + i + m])
+            outs.append(ref.attend(q[cu[b] + i : cu[b] + i + m], cache, table[b : b + 1], n, scale, [0, m], eps, window)[0])
+    return tuple(torch.cat(x) for x in zip(*outs))
+
+
+# ---------------------------------------------------------------------------
+# Precision
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_a_rows_precision_is_its_own(cuda_device, dtype, D):
+    """The same bound whether a sequence has few new tokens or many, alone, beside
+    others, or beside sequences without new tokens."""
+    scale = torch.tensor([1.0, -2.0, 30.0, 0.1, 1.0, 2.0, 3.0, 4.0])
+    for new in ([60], [60, 0, 0, 0], [60, 300], [1, 60, 9], [4, 5]):
+        lens = [x + 200 + 10 * i for i, x in enumerate(new)]
+        cache, table, n, _ = ref.make_cache(lens, 16, 2, D, seed=41)
+        cu = serve_ref.starts(new)
+        q = _queries(cu[-1], 8, D, DT[dtype], 42)
+        out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device), n.to(cuda_device),
+                                             scale.to(cuda_device), torch.tensor(cu, device=cuda_device, **INT))
+        assert ref.worst(out, _tight(q, cache, table, n, scale, cu)) <= 1.0
