@@ -11,13 +11,13 @@
 // rows' swizzle spreads over all banks.
 //
 // 8 second turns (4583 tokens over 27 thousand keys, 32 heads over 8, D128 bf16):
-// 332 us, 680 TFLOP/s of the formula's, and a join of 5; a large matrix product
+// 330 us, 685 TFLOP/s of the formula's, and a join of 5; a large matrix product
 // has 1200.  The weights' two parts make three products of the formula's two: with
 // one part it was 250 us, but a row was off by 2.3e-3 in norm where the narrow
 // kernel's are by 1.7e-3, so that its precision hung on what else was in the batch.
 // Two workgroups a compute unit is what 256 registers leave, and with one column
 // block of 32 rows a wave each operand of K from LDS feeds one product.  A higher
-// priority around the overlaps' products: 254 us for 258 (with one part).
+// priority around the overlaps' products: 328 us for 332.
 //
 // Keys without a page, or past the sequence, are zeros: overlaps of 0, weights
 // of 0.  Few blocks of rows split their keys; the partial sums are joined in order.

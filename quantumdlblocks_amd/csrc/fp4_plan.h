@@ -11,11 +11,18 @@ constexpr int kFp4Rows = 128;  // rows (new tokens x heads of a group) of the ti
 // Rows of a (sequence, key head) up to which the narrow kernel takes it.  us with
 // 32 and with 64: 32 sequences of 16 tokens over 4096 keys at most, 8 key heads
 // D128, 4 heads each, 64 and 74; 4 of 64 over 8000, 4 key heads, 45 and 47; few
-// rows the same.  A launch of few rows that are narrow in the mean goes to the
-// narrow kernel whole: 16 sequences of 5 tokens 28 and 33, 8 of 30 fp32 27 and 29;
-// not by the rows alone: one sequence of 128 tokens over 30000 keys 167 and 83.
+// rows the same.
 constexpr int kFp4Narrow = 32;
-constexpr int kFp4AllNarrow = 512, kFp4AllMean = 64;  // rows of a launch, and of its sequences in the mean, likewise
+// A launch of few rows goes to the narrow kernel whole, if it does not lose much
+// where one sequence has all of them: every 32 rows go through the keys again, so
+// rows times keys times key heads decide, whatever the number of sequences, which
+// may hold empty ones.  us narrow and tiled, one sequence with all rows, D128: 512
+// rows over 2000 keys of 8 heads (2^23.1) 31 and 36, over 8000 of 2 (2^23) 30 and
+// 40, over 30000 of one (2^23.9) 48 and 42, over 8000 of 8 (2^25) 60 and 50, over
+// 30000 of 8 161 and 105; 128 over 30000 of 8 (2^24.9) 58 and 52.  What it is for:
+// 16 sequences of 5 tokens, 4 heads over 4 key heads, 27 and 30, of 8 27 and 34.
+constexpr int kFp4AllNarrow = 512;
+constexpr int64_t kFp4AllWork = (int64_t)1 << 24;
 // Workgroups of the narrow kernel that a launch's chunks of keys are made for: two
 // rounds of as many as a compute unit holds, three with one column set, two with two.
 // us with 512, 768, 1024, 1536, 2048: 32 single tokens over long caches 76, 72, 74,
@@ -98,7 +105,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     r.splits = 1;
     if (packed) {
         // Few rows in all are narrow however they are shared out.
-        r.limit = n * G <= kFp4AllNarrow && n * G <= kFp4AllMean * B ? kFp4AllNarrow : kFp4Narrow;
+        r.limit = n * G <= kFp4AllNarrow && n * G * seen(n) * h_kv <= kFp4AllWork ? kFp4AllNarrow : kFp4Narrow;
         most = n * G < r.limit ? n * G : r.limit;
         if (n * G > r.limit) {
             const int64_t blocks = (n * G + kFp4Rows - 1) / kFp4Rows, some = n * G / (r.limit + 1);

@@ -1,0 +1,49 @@
+"""The 4-bit paged cache's launches on the CPU, and its formulas where they are
+easiest to get wrong."""
+
+from __future__ import annotations
+
+import os
+import shutil
+import subprocess
+
+import pytest
+
+from quantumdlblocks_amd.kernels import born_fp4
+
+HEADER = os.path.abspath(os.path.join(os.path.dirname(born_fp4.__file__), "..", "csrc", "fp4_plan.h"))
+
+
+def _run(tmp_path, body):
+    """A program over the launches' rules; its output's last line where it fails."""
+    gxx = shutil.which("g++")
+    if gxx is None:
+        pytest.skip("no host compiler")
+    (tmp_path / "plan.cpp").write_text('#include <cstdio>\n#include <random>\n#include "%s"\nusing namespace qdl;\n'
+                                       'const int64_t kMost = (1 << 24) - 1;\nint main() {\n%s\nreturn 0;\n}\n' % (HEADER, body))
+    subprocess.run([gxx, "-std=c++17", "-O1", "-fsanitize=undefined", "-fno-sanitize-recover", str(tmp_path / "plan.cpp"), "-o",
+                    str(tmp_path / "plan")], check=True)
+    got = subprocess.run([str(tmp_path / "plan")], capture_output=True, text=True)
+    assert got.returncode == 0, got.stdout + got.stderr
+
+
+def test_sequences_without_tokens_do_not_choose_the_kernel(tmp_path):
+    """Which sequences are narrow goes by the tokens, heads and keys: a prompt does
+    not fall to the narrow kernel for the empty sequences beside it."""
+    _run(tmp_path, r"""
+    std::mt19937_64 g(2);
+    auto upto = [&](int64_t most) { return (int64_t)(g() % (uint64_t)(most + 1)); };
+    for (int i = 0; i < 100000; ++i) {
+        const int64_t h_kv = 1 + upto(8), H = h_kv * (1 + upto(8)), n = 1 + upto(700), page = 16, pages = 1 + upto((int64_t)1 << upto(12));
+        const int64_t window = upto(1) ? 0 : 1 + upto(5000);
+        int limit = 0;
+        for (int64_t B : {1, 2, 8, 63, 500}) {
+            const Fp4Plan r = fp4_plan(n, B, H, h_kv, 64, pages, page, window, true, false, kMost);
+            if (limit && r.limit != limit) return printf("%ld rows of %ld sequences: %d and %d\n", (long)(n * H / h_kv), (long)B, limit, r.limit), 1;
+            limit = r.limit;
+        }
+    }
+    // 128 tokens behind a long conversation, beside seven empty sequences; drafts.
+    if (fp4_plan(128, 8, 32, 8, 128, 1900, 16, 0, true, false, kMost).slots == 0) return printf("a prompt\n"), 1;
+    if (fp4_plan(80, 16, 16, 4, 128, 512, 16, 0, true, false, kMost).slots != 0) return printf("drafts\n"), 1;
+    """)
