@@ -560,7 +560,7 @@ int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call *call, qdl_stream_
  * its keys: its i-th of m is at position cache_lens - m + i and sees the keys up
  * to there, or the last window_size of them.  Tokens that see no key, and those
  * of no sequence, get zeros; a key with a block of e = 255 makes NaN of every
- * row that sees it.  B up to 65535.  The workspace's size is the size function's for the same
+ * row that sees it.  B up to 65536.  The workspace's size is the size function's for the same
  * sizes (packed: cu_seqlens != NULL; weighed: key_weight != NULL).
  * key_weight, only where cu_seqlens is NULL: as for qdl_flash_born_paged_forward_call.
  */

@@ -619,8 +619,9 @@ template <class E, int DP, int NC, bool WEIGH, bool P16>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(fp4_wpe<E>(DP, NC))))
 void born_fp4_paged_kernel(Fp4PagedArgs p) {
     __shared__ __attribute__((aligned(16))) uint8_t smem[kFp4NarrowLds<DP>];
-    if (blockIdx.x == 0) fp4_behind<E>(p, blockIdx.y, gridDim.y);
-    fp4_narrow<E, DP, NC, WEIGH, P16>(p, Fp4Share(p, false), smem, blockIdx.y, blockIdx.x);
+    const int unit = blockIdx.z * gridDim.y + blockIdx.y;
+    if (blockIdx.x == 0) fp4_behind<E>(p, unit, gridDim.y * gridDim.z);
+    if (unit < p.units) fp4_narrow<E, DP, NC, WEIGH, P16>(p, Fp4Share(p, false), smem, unit, blockIdx.x);
 }
 
 // A narrow row's partial sums.
@@ -761,7 +762,9 @@ hipError_t fp4_paged_fwd(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t
 
 template <class E, int NC, bool WEIGH, bool P16>
 void launch_fp4_dp(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
-    const dim3 grid((unsigned)a.Hkv, (unsigned)plan.units);
+    // A grid's second and third dimensions hold 65535.
+    const int64_t z = (plan.units + 65534) / 65535, y = (plan.units + z - 1) / z;
+    const dim3 grid((unsigned)a.Hkv, (unsigned)y, (unsigned)z);
     if (a.D <= 64) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 64, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else if (a.D <= 128) hipLaunchKernelGGL((born_fp4_paged_kernel<E, 128, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);
     else hipLaunchKernelGGL((born_fp4_paged_kernel<E, 256, NC, WEIGH, P16>), grid, dim3(256), 0, st, a);

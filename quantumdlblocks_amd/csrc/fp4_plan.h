@@ -150,8 +150,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
     }
     const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
-    // The narrow kernel's own grid has heads and units as dimensions.
-    r.fits = r.grid <= kMost && ((r.slots > 0 && !r.apart) || r.units < 65536) && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    r.fits = r.grid <= kMost && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.rows = (int)rows;

@@ -47,3 +47,15 @@ def test_sequences_without_tokens_do_not_choose_the_kernel(tmp_path):
     if (fp4_plan(128, 8, 32, 8, 128, 1900, 16, 0, true, false, kMost).slots == 0) return printf("a prompt\n"), 1;
     if (fp4_plan(80, 16, 16, 4, 128, 512, 16, 0, true, false, kMost).slots != 0) return printf("drafts\n"), 1;
     """)
+
+
+def test_sequences_of_several_column_blocks_fit_a_launch(tmp_path):
+    """As many sequences as a call takes, whatever the heads of a group."""
+    _run(tmp_path, r"""
+    for (int64_t G : {1, 16, 17, 20, 33, 40, 64, 100})
+        for (int weighed : {0, 1})
+            for (int64_t B : {1000, 1025, 22000, 33000, 65535, 65536})
+                for (int64_t pages : {1, 8, 1000})
+                    if (!fp4_plan(B, B, G, 1, 128, pages, 16, 0, false, weighed, kMost).fits)
+                        return printf("%ld sequences of %ld heads, %ld pages, %d\n", (long)B, (long)G, (long)pages, weighed), 1;
+    """)

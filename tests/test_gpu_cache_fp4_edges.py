@@ -75,3 +75,25 @@ def test_a_rows_precision_is_its_own(cuda_device, dtype, D):
         out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device), n.to(cuda_device),
                                              scale.to(cuda_device), torch.tensor(cu, device=cuda_device, **INT))
         assert ref.worst(out, _tight(q, cache, table, n, scale, cu)) <= 1.0
+
+
+# ---------------------------------------------------------------------------
+# Large batches
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("weigh", [False, True])
+def test_sequences_of_several_column_blocks_each(cuda_device, weigh):
+    """Forty heads over one key head: two or three blocks of columns a sequence,
+    more of them than a grid's second dimension holds."""
+    B, H, D = 33000, 40, 8
+    cache, _, _, _ = ref.make_cache([16] * 64, 16, 1, D, seed=45, extra=0)
+    table, n = (torch.arange(B, **INT) % 64).view(-1, 1), torch.arange(B, **INT) % 17
+    q = _queries(B, H, D, torch.bfloat16, 46)
+    dev = tuple(t.to(cuda_device) for t in cache)
+    weight = torch.zeros(B, 1, 16, device=cuda_device) if weigh else None
+    out = flash_born_attention_paged_fp4(q.to(cuda_device), dev, table.to(cuda_device), n.to(cuda_device), 2.0, key_weight=weight)
+    # The first, the last, and those about the 65536th block.
+    some = torch.tensor([*range(70), *range(32700, 32840), *range(B - 70, B)])
+    o, w = ref.attend(q[some], cache, table[some], n[some], 2.0)
+    assert ref.worst(out[some.to(cuda_device)], o) <= 1.0
+    if weigh:
+        assert ref.worst(weight[some.to(cuda_device)], (w[0], w[1] + 2.0 ** -24 * w[0])) <= 1.0
