@@ -201,9 +201,11 @@ int64_t qdl_flash_born_fp4_paged_workspace_size(int64_t n, int64_t B, int64_t H,
                                                 int64_t page_size, int64_t window_size, int packed, int weighed) {
     if (n <= 0 || n > kMostRows || B < 0 || B > kMostHeads || H <= 0 || H > kMostHeads || h_kv <= 0 || H % h_kv != 0 || D <= 0 || D > 256 ||
         pages < 0 || page_size < 1 || page_size > (int64_t)1 << 24 || pages > (int64_t)1 << 30 ||
-        pages * page_size > (int64_t)1 << 30 || window_size < 0)
+        pages * page_size > (int64_t)1 << 30 || window_size < 0 || weighed < 0)
         return 0;
-    return qdl::fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0, kMostBlocks).bytes();
+    return qdl::fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0, kMostBlocks,
+                         weighed > 1 ? weighed : INT32_MAX)
+        .bytes();
 }
 
 int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_stream_t stream) {
@@ -223,9 +225,9 @@ int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_
     if (!aligned16(c->q) || !aligned16(c->out)) return QDL_BORN_E_ALIGN;
     const int64_t it = item(c->dtype);
     if (!rows_ok(c->q_strides, it)) return QDL_BORN_E_STRIDE;
-    const bool weighed = c->key_weight != nullptr;
+    const bool weighed = c->key_weight != nullptr && c->weight_len > 0;
     const qdl::Fp4Plan r = qdl::fp4_plan(c->n, c->B, c->H, c->h_kv, c->D, c->cache.pages, c->cache.page_size, c->window_size,
-                                         c->cu_seqlens != nullptr, weighed, kMostBlocks);
+                                         c->cu_seqlens != nullptr, weighed, kMostBlocks, weighed ? c->weight_len : 0);
     if (!r.fits) return QDL_BORN_E_SHAPE;
     if (!c->workspace || !aligned16(c->workspace) || c->workspace_bytes < r.bytes()) return QDL_BORN_E_WORKSPACE;
     qdl::Fp4PagedArgs a = {};

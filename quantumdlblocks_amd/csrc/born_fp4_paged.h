@@ -59,7 +59,7 @@ struct Fp4PagedArgs {
     float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
     int64_t w_sb, w_sh;    // elements
     int w_len;
-    float* raw;            // (B, H, raw_ld): p without s^2, keys from the span's first 32 on
+    float* raw;            // (B, H, raw_ld): p without s^2, of keys from the span's first 32 on, as far as weights are kept
     int64_t raw_ld;
     int units;             // at most: `part` has room for no more
 };
@@ -642,30 +642,34 @@ struct Fp4Parts {
 
 // Splits joined in order.  A row's columns take `ncol` threads, its splits
 // `groups` of them, 256 / (ncol groups) rows a workgroup.
-// WEIGH: in the same launch, for each (sequence, key head) and 256 keys, the sum
-// over the group of p_j / Z, the heads in order, is added to its weights.
-template <class E, bool WEIGH>
+// WEIGH: in the same launch, for each (sequence, key head), 256 keys at a time, the
+// sum over the group of p_j / Z, the heads in order, is added to its weights; by a
+// workgroup once (1), or again and again (2).
+template <class E, int WEIGH>
 __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4Join q) {
     __shared__ f32x4v red[256];
     __shared__ float zred[256];
-    if (WEIGH && (int)blockIdx.x >= q.blocks) {
-        const int x = blockIdx.x - q.blocks, hk = x % p.Hkv, b = x / p.Hkv % p.B, block = x / p.Hkv / p.B;
+    if (WEIGH != 0 && (int)blockIdx.x >= q.blocks) {
+        const int x = blockIdx.x - q.blocks, hk = x % p.Hkv, b = x / p.Hkv % p.B;
         const Fp4Seq sq(p, b);
-        const int j0 = sq.base() + block * 256, j = j0 + threadIdx.x;
-        if (j0 >= sq.n) return;
-        const bool seen = j >= sq.first && j < sq.n && j < p.w_len;
+        const int start = sq.base() + x / p.Hkv / p.B * 256, end = min(sq.n, p.w_len);
+        if (start >= end) return;
+        const bool once = WEIGH == 1;
+        float* const weight = p.weights + (int64_t)b * p.w_sb + (int64_t)hk * p.w_sh;
+        auto raw = [&](int g, int j) __attribute__((always_inline)) {
+            return p.raw[((int64_t)b * p.H + hk * p.G + g) * p.raw_ld + (j - sq.base())];
+        };
+        auto seen = [&](int j) __attribute__((always_inline)) { return j >= sq.first && j < end; };
         // On their way before the denominators are known (16 caches of 52 thousand
         // keys, 4 key heads D64, 4 heads each: 22.4 us, after them 23.3).
         constexpr int kFirst = 4;
-        float* const weight = p.weights + (int64_t)b * p.w_sb + (int64_t)hk * p.w_sh + j;
-        float first[kFirst] = {}, old = 0.f;
-        if (seen) {
-            old = *weight;
+        float first[kFirst] = {}, old = 0.f, sum = 0.f;
+        if (once && seen(start + threadIdx.x)) {
+            old = weight[start + threadIdx.x];
 #pragma unroll
             for (int i = 0; i < kFirst; ++i)
-                if (i < p.G) first[i] = p.raw[((int64_t)b * p.H + hk * p.G + i) * p.raw_ld + (j - sq.base())];
+                if (i < p.G) first[i] = raw(i, start + threadIdx.x);
         }
-        float sum = 0.f;
         for (int g0 = 0; g0 < p.G; g0 += 256) {
             const int gn = min(256, p.G - g0);
             if ((int)threadIdx.x < gn) {
@@ -676,19 +680,28 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
                 zred[threadIdx.x] = fp4_inverse(p, hk * p.G + g0 + threadIdx.x, z);
             }
             __syncthreads();
-            if (seen) {
-                const float* raw = p.raw + ((int64_t)b * p.H + hk * p.G + g0) * p.raw_ld + (j - sq.base());
-                if (g0 == 0) {
+            if (once) {
+                if (seen(start + threadIdx.x)) {
+                    if (g0 == 0) {
 #pragma unroll
-                    for (int i = 0; i < kFirst; ++i)
-                        if (i < gn) sum = fmaf(first[i], zred[i], sum);
-                }
+                        for (int i = 0; i < kFirst; ++i)
+                            if (i < gn) sum = fmaf(first[i], zred[i], sum);
+                    }
 #pragma unroll 4
-                for (int i = g0 == 0 ? kFirst : 0; i < gn; ++i) sum = fmaf(raw[(int64_t)i * p.raw_ld], zred[i], sum);
+                    for (int i = g0 == 0 ? kFirst : 0; i < gn; ++i) sum = fmaf(raw(g0 + i, start + threadIdx.x), zred[i], sum);
+                }
+            } else {
+                for (int j = start + threadIdx.x; j < end; j += q.weigh * 256) {
+                    if (!seen(j)) continue;
+                    float more = 0.f;
+#pragma unroll 4
+                    for (int i = 0; i < gn; ++i) more = fmaf(raw(g0 + i, j), zred[i], more);
+                    weight[j] += more;
+                }
             }
             __syncthreads();
         }
-        if (seen) *weight = old + sum;
+        if (once && seen(start + threadIdx.x)) weight[start + threadIdx.x] = old + sum;
         return;
     }
     const int per = q.ncol * q.groups, mine = threadIdx.x / per, col = 4 * (threadIdx.x % q.ncol), group = threadIdx.x % per / q.ncol;
@@ -786,10 +799,11 @@ template <class E>
 hipError_t launch_fp4_join(const Fp4PagedArgs& a, const Fp4Plan& plan, hipStream_t st) {
     const Fp4Join& q = plan.join;
     if (a.raw != nullptr) {
-        const unsigned weigh = (unsigned)((a.raw_ld + 255) / 256 * a.B * a.Hkv);
-        hipLaunchKernelGGL((born_fp4_join_kernel<E, true>), dim3(q.blocks + weigh), dim3(256), 0, st, a, q);
+        const dim3 grid((unsigned)(q.blocks + (int64_t)q.weigh * a.B * a.Hkv));
+        if ((int64_t)q.weigh * 256 >= a.raw_ld) hipLaunchKernelGGL((born_fp4_join_kernel<E, 1>), grid, dim3(256), 0, st, a, q);
+        else hipLaunchKernelGGL((born_fp4_join_kernel<E, 2>), grid, dim3(256), 0, st, a, q);
     } else if (q.blocks > 0) {
-        hipLaunchKernelGGL((born_fp4_join_kernel<E, false>), dim3(q.blocks), dim3(256), 0, st, a, q);
+        hipLaunchKernelGGL((born_fp4_join_kernel<E, 0>), dim3(q.blocks), dim3(256), 0, st, a, q);
     }
     return hipGetLastError();
 }

@@ -36,6 +36,11 @@ constexpr int fp4_wanted(int nc) { return nc == 1 ? 1536 : 1024; }
 // over 8192 keys at most 67 and 104; where a few are wide it costs, 31 single
 // tokens beside one of 200 94 and 86, of 512 (mean 68: together) 158 and 127.
 constexpr int64_t kFp4Apart = (int64_t)1 << 20;
+// Workgroups that add the keys' weights up, 256 keys at a time each, at most: the
+// host knows the table's room only, and more of them find no keys.  us with 2^12,
+// 2^14 and any number of them: 64 sequences of 1000 keys, 8 key heads, 32 heads,
+// tables of 131072 keys 37, 44, 191; of 16000 keys, tables of 16384, 325, 344, 351.
+constexpr int64_t kFp4Weigh = (int64_t)1 << 12;
 // Sequences that a workgroup looks through to share out the keys.
 constexpr int kFp4Shared = 1024;
 
@@ -72,6 +77,7 @@ struct Fp4Join {
     int narrow;  // rows as (sequence, key head, up to `most`): the narrow ones beside a tiled kernel's
     int rows;    // rows as (token, head): all, or the wide ones
     int blocks;  // workgroups of them
+    int weigh;   // workgroups of a (sequence, key head) behind them that add its keys' weights up
 };
 
 struct Fp4Plan {
@@ -89,10 +95,10 @@ struct Fp4Plan {
     constexpr int64_t bytes() const { return plan_bytes + part_bytes + raw_bytes + wide_bytes; }
 };
 
-// packed: several tokens a sequence; weighed: the keys' weights are kept.
-// kMost: workgroups of a launch at most.
+// packed: several tokens a sequence; weighed: the keys' weights are kept, of the
+// first weight_len keys.  kMost: workgroups of a launch at most.
 constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_t D, int64_t pages, int64_t page, int64_t window,
-                           bool packed, bool weighed, int64_t kMost) {
+                           bool packed, bool weighed, int64_t kMost, int64_t weight_len = (int64_t)1 << 31) {
     Fp4Plan r = {};
     const int64_t G = H / h_kv, room = pages * page;
     auto seen = [=](int64_t tokens) {  // keys that a sequence's tokens see
@@ -133,6 +139,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     r.plan_bytes = (B * 8 + 15) / 16 * 16;
     if (shared || weighed) r.part_bytes = r.units * h_kv * cols * (D + 4) * 4;
     r.raw_ld = (seen(1) + 31 + 31) / 32 * 32;
+    if (r.raw_ld > (weight_len + 31) / 32 * 32) r.raw_ld = (weight_len + 31) / 32 * 32;
     if (weighed) r.raw_bytes = B * H * r.raw_ld * 4;
 
     r.join.most = r.most;
@@ -149,12 +156,14 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
         blocks = (narrow + rows + each_block - 1) / each_block;
         if (2 * r.join.groups * r.join.ncol > 256 || r.join.groups >= each || blocks >= 1024) break;
     }
-    const int64_t weigh = weighed ? B * h_kv * ((r.raw_ld + 255) / 256) : 0;
-    r.fits = r.grid <= kMost && narrow + rows < (int64_t)1 << 31 && blocks + weigh <= kMost;
+    const int64_t heads = B * h_kv, share = heads < kFp4Weigh ? kFp4Weigh / (heads > 0 ? heads : 1) : 1, keys = (r.raw_ld + 255) / 256;
+    const int64_t weigh = weighed ? (keys < share ? keys : share) : 0;
+    r.fits = r.grid <= kMost && narrow + rows < (int64_t)1 << 31 && blocks + heads * weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.rows = (int)rows;
         r.join.blocks = (int)blocks;
+        r.join.weigh = (int)weigh;
     }
     return r;
 }

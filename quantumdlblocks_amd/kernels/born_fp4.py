@@ -455,7 +455,8 @@ def flash_born_attention_paged_fp4(
     ``scale``: a float or a tensor of 1 or H values.  ``key_weight`` (B, Hkv, L)
     fp32, only without ``cu_seqlens``: each visible key's weight p_j / (sum p +
     eps), summed over the heads that read it, is added in place at j < L: what
-    ``born_cache_evict_fp4`` goes by.  Lengths past the table's pages are cut to
+    ``born_cache_evict_fp4`` goes by; the call's workspace holds B H fp32 values for
+    each of these L keys, or of the table's where it has fewer.  Lengths past the table's pages are cut to
     them first.  Tokens that see no key get zeros, so do tokens of no sequence,
     and heads whose (sum p + eps) / scale_h ** 2 lies below fp32's normal range,
     2^-126; a key that is not a number makes NaN of the rows that see it.
@@ -518,7 +519,7 @@ def flash_born_attention_paged_fp4(
     (table, ld), lens = _table(block_table), _index(cache_lens)
     cu = None if cu_seqlens is None else _index(cu_seqlens)
     pages = table.shape[1]
-    size = _paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, w_ptr != 0)
+    size = _paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, w_len if w_ptr else 0)
     ws = lens.new_empty((size + 3) // 4)
     _run_call(lib.qdl_flash_born_fp4_paged_forward_call, "qdl_flash_born_fp4_paged_forward_call", dev, _native.fp4_paged_call(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), st, sh, out.data_ptr(), *fields, table.data_ptr(), pages, ld,

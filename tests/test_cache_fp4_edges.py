@@ -9,6 +9,7 @@ import subprocess
 
 import pytest
 
+from quantumdlblocks_amd import _native
 from quantumdlblocks_amd.kernels import born_fp4
 
 HEADER = os.path.abspath(os.path.join(os.path.dirname(born_fp4.__file__), "..", "csrc", "fp4_plan.h"))
@@ -59,3 +60,23 @@ def test_sequences_of_several_column_blocks_fit_a_launch(tmp_path):
                     if (!fp4_plan(B, B, G, 1, 128, pages, 16, 0, false, weighed, kMost).fits)
                         return printf("%ld sequences of %ld heads, %ld pages, %d\n", (long)B, (long)G, (long)pages, weighed), 1;
     """)
+
+
+def test_weights_of_few_keys_take_little_room(tmp_path):
+    """What is kept of the keys sizes the workspace, not the table; wide tables do
+    not make a launch too large."""
+    _run(tmp_path, r"""
+    for (int64_t B : {1, 64, 300, 4000})
+        for (int64_t pages : {1, 100, 65536}) {
+            const int64_t room = pages * 16;
+            for (int64_t keys : {1, 31, 100, 5000, 1 << 20}) {
+                const Fp4Plan r = fp4_plan(B, B, 32, 8, 128, pages, 16, 0, false, true, kMost, keys);
+                const int64_t kept = keys < room ? keys : room;
+                if (!r.fits || r.raw_bytes > B * 32 * 4 * (kept + 93) || r.raw_ld < kept) return printf("%ld %ld %ld\n", (long)B, (long)pages, (long)keys), 1;
+                if (r.join.weigh * B * 8 > kFp4Weigh && r.join.weigh > 1) return printf("launch\n"), 1;
+            }
+        }
+    """)
+    lib = _native.load()
+    size = lambda *a: lib.qdl_flash_born_fp4_paged_workspace_size(64, 64, 32, 8, 128, 8192, 16, 0, 0, *a)  # noqa: E731
+    assert size(0) < size(4096) < 64 << 20 < 1 << 30 < size(1) == size(1 << 20) and size(-1) == 0

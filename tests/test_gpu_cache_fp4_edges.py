@@ -97,3 +97,42 @@ def test_sequences_of_several_column_blocks_each(cuda_device, weigh):
     assert ref.worst(out[some.to(cuda_device)], o) <= 1.0
     if weigh:
         assert ref.worst(weight[some.to(cuda_device)], (w[0], w[1] + 2.0 ** -24 * w[0])) <= 1.0
+
+
+# ---------------------------------------------------------------------------
+# The keys' weights
+# ---------------------------------------------------------------------------
+def test_weights_of_few_keys_over_wide_tables(cuda_device):
+    """Tables of 2^20 keys a sequence for 520 sequences of 8 key heads: neither the
+    launch nor its workspace goes by them where the weights kept are few."""
+    B, Hkv = 520, 8
+    lens = [300 if i % 40 == 0 else i % 50 for i in range(B)]
+    cache, table, n, _ = ref.make_cache(lens, 256, Hkv, 32, seed=47)
+    wide = torch.full((B, 4096), -1, **INT)
+    wide[:, : table.shape[1]] = table
+    q = _queries(B, Hkv, 32, torch.bfloat16, 48)
+    weight = torch.full((B, Hkv, 280), 0.25, device=cuda_device)
+    torch.cuda.reset_peak_memory_stats()
+    before = torch.cuda.memory_allocated()
+    out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), wide.to(cuda_device), n.to(cuda_device), 2.0,
+                                         key_weight=weight)
+    assert torch.cuda.max_memory_allocated() - before < 256 << 20
+    o, w = ref.attend(q, cache, table, n, 2.0)
+    y, e = (t[..., :280] for t in w)
+    assert ref.worst(out, o) <= 1.0 and ref.worst(weight, (y + 0.25, e + 2.0 ** -24 * (y + 0.25))) <= 1.0
+
+
+@pytest.mark.parametrize("window", [0, 40])
+@pytest.mark.parametrize("kept", [1, 50, 100, 700])
+def test_weights_of_some_of_the_keys(cuda_device, window, kept):
+    lens = [690, 33, 0, 100]
+    for page in (16, 7):
+        cache, table, n, _ = ref.make_cache(lens, page, 2, 64, seed=49)
+        q = _queries(4, 8, 64, torch.float16, 50)
+        room = torch.full((4, 2, kept + 40), 0.25, device=cuda_device)  # rows with others' values behind them
+        flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device), n.to(cuda_device), 2.0,
+                                       window_size=window, key_weight=room[..., :kept])
+        y, e = ref.attend(q, cache, table, n, 2.0, None, 1e-12, window)[1]
+        m = min(kept, y.shape[2])
+        assert ref.worst(room[..., :m], (y[..., :m] + 0.25, e[..., :m] + 2.0 ** -24 * (y[..., :m] + 0.25))) <= 1.0
+        assert (room[..., m:] == 0.25).all()
