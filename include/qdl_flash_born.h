@@ -563,7 +563,8 @@ int qdl_flash_born_fp4_read_call(const qdl_born_fp4_read_call *call, qdl_stream_
  * row that sees it.  B up to 65536.  The workspace's size is the size function's for the same
  * sizes (packed: cu_seqlens != NULL; weighed: 0 without key_weight, else its
  * weight_len, where 1 stands for any: H fp32 values for each of the weight_len
- * keys a sequence, or of as many as the table has room for).
+ * keys a sequence, or of as many as the table has room for); it is 0 for sizes
+ * that the call refuses.
  * key_weight, only where cu_seqlens is NULL: as for qdl_flash_born_paged_forward_call.
  */
 typedef struct qdl_born_fp4_paged_call {

@@ -203,9 +203,9 @@ int64_t qdl_flash_born_fp4_paged_workspace_size(int64_t n, int64_t B, int64_t H,
         pages < 0 || page_size < 1 || page_size > (int64_t)1 << 24 || pages > (int64_t)1 << 30 ||
         pages * page_size > (int64_t)1 << 30 || window_size < 0 || weighed < 0)
         return 0;
-    return qdl::fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0, kMostBlocks,
-                         weighed > 1 ? weighed : INT32_MAX)
-        .bytes();
+    const qdl::Fp4Plan r = qdl::fp4_plan(n, B, H, h_kv, D, pages, page_size, window_size, packed != 0, weighed != 0, kMostBlocks,
+                                         weighed > 1 ? weighed : INT32_MAX);
+    return r.fits ? r.bytes() : 0;
 }
 
 int qdl_flash_born_fp4_paged_forward_call(const qdl_born_fp4_paged_call* c, qdl_stream_t stream) {

@@ -140,7 +140,8 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     if (shared || weighed) r.part_bytes = r.units * h_kv * cols * (D + 4) * 4;
     r.raw_ld = (seen(1) + 31 + 31) / 32 * 32;
     if (r.raw_ld > (weight_len + 31) / 32 * 32) r.raw_ld = (weight_len + 31) / 32 * 32;
-    if (weighed) r.raw_bytes = B * H * r.raw_ld * 4;
+    const bool countable = r.raw_ld < ((int64_t)1 << 60) / (B * H + 1);
+    if (weighed && countable) r.raw_bytes = B * H * r.raw_ld * 4;
 
     r.join.most = r.most;
     r.join.ncol = 2;
@@ -158,7 +159,7 @@ constexpr Fp4Plan fp4_plan(int64_t n, int64_t B, int64_t H, int64_t h_kv, int64_
     }
     const int64_t heads = B * h_kv, share = heads < kFp4Weigh ? kFp4Weigh / (heads > 0 ? heads : 1) : 1, keys = (r.raw_ld + 255) / 256;
     const int64_t weigh = weighed ? (keys < share ? keys : share) : 0;
-    r.fits = r.grid <= kMost && narrow + rows < (int64_t)1 << 31 && blocks + heads * weigh <= kMost;
+    r.fits = r.grid <= kMost && (countable || !weighed) && narrow + rows < (int64_t)1 << 31 && blocks + heads * weigh <= kMost;
     if (r.fits) {
         r.join.narrow = (int)narrow;
         r.join.rows = (int)rows;

@@ -80,3 +80,12 @@ def test_weights_of_few_keys_take_little_room(tmp_path):
     lib = _native.load()
     size = lambda *a: lib.qdl_flash_born_fp4_paged_workspace_size(64, 64, 32, 8, 128, 8192, 16, 0, 0, *a)  # noqa: E731
     assert size(0) < size(4096) < 64 << 20 < 1 << 30 < size(1) == size(1 << 20) and size(-1) == 0
+
+
+def test_workspaces_of_calls_that_are_refused_are_empty():
+    """More workgroups than a launch counts, or more bytes than 64 bits do."""
+    size = _native.load().qdl_flash_born_fp4_paged_workspace_size
+    for a in ((1 << 16, 1 << 16, 256, 256, 8, 1, 16, 0, 0, 1), (1 << 28, 5, 64, 64, 64, 4, 16, 0, 1, 0),
+              (1 << 16, 1 << 16, 1 << 16, 1, 64, 1 << 14, 1 << 16, 0, 0, 1)):
+        assert size(*a) == 0
+    assert size(1 << 16, 1 << 16, 128, 128, 8, 1, 16, 0, 0, 1) > 0
