@@ -423,7 +423,8 @@ def _paged_formula(q, cache, block_table, cache_lens, scale_t, cu, eps, window, 
         w = p / torch.where(den == 0, torch.ones_like(den), den)
         if key_weight is not None:
             m = min(L, key_weight.shape[2])
-            key_weight[b, :, :m] += w.sum((1, 2))[:, :m].to(key_weight.dtype)
+            seen = torch.where(keep, w, torch.zeros_like(w))  # a row that is not a number is NaN throughout
+            key_weight[b, :, :m] += seen.sum((1, 2))[:, :m].to(key_weight.dtype)
         o = torch.matmul(w, v.permute(1, 0, 2).unsqueeze(1))
         out[a0 : a0 + new] = o.permute(2, 0, 1, 3).reshape(new, H, D).to(q.dtype)
     return out

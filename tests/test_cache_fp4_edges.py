@@ -3,13 +3,16 @@ easiest to get wrong."""
 
 from __future__ import annotations
 
+import math
 import os
 import shutil
 import subprocess
 
 import pytest
+import torch
 
-from quantumdlblocks_amd import _native
+import fp4_ref as ref
+from quantumdlblocks_amd import _native, flash_born_attention_paged_fp4
 from quantumdlblocks_amd.kernels import born_fp4
 
 HEADER = os.path.abspath(os.path.join(os.path.dirname(born_fp4.__file__), "..", "csrc", "fp4_plan.h"))
@@ -89,3 +92,21 @@ def test_workspaces_of_calls_that_are_refused_are_empty():
               (1 << 16, 1 << 16, 1 << 16, 1, 64, 1 << 14, 1 << 16, 0, 0, 1)):
         assert size(*a) == 0
     assert size(1 << 16, 1 << 16, 128, 128, 8, 1, 16, 0, 0, 1) > 0
+
+
+@pytest.mark.parametrize("window", [0, 30])
+def test_keys_that_are_not_seen_keep_their_weights(window):
+    """A row that is not a number makes NaN of the weights that it sees, of no other."""
+    cache, table, n, _ = ref.make_cache([90, 60], 5, 2, 64, seed=51)
+    table[0, 8] = -1
+    t, r = int(table[0, 17]), 0
+    cache[2][t, r, 1, 0] = 255  # key 85
+    q = torch.randn(2, 4, 64, generator=torch.Generator().manual_seed(52))
+    q[1, 0, 7] = math.nan
+    weight = torch.full((2, 2, 120), 0.5)
+    flash_born_attention_paged_fp4(q, cache, table, n, 1.0, window_size=window, key_weight=weight)
+    j = torch.arange(120)
+    for b, h, m in ((0, 1, 90), (1, 0, 60)):
+        seen = (j < m) & (j >= (m - window if window else 0)) & ~((b == 0) & (j // 5 == 8))
+        assert torch.equal(weight[b, h].isnan(), seen) and (weight[b, h][~seen] == 0.5).all()
+    assert weight[0, 0].isfinite().all() and weight[1, 1].isfinite().all()
