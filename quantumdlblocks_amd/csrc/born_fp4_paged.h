@@ -59,7 +59,7 @@ struct Fp4PagedArgs {
     float* weights;        // (B, Hkv, L) or nullptr: += sum over the group of p / Z
     int64_t w_sb, w_sh;    // elements
     int w_len;
-    float* raw;            // (B, H, raw_ld): p without s^2, of keys from the span's first 32 on, as far as weights are kept
+    float* raw;            // (B, H, raw_ld): p without s^2, -1 without a page, of keys from the span's first 32 on, as far as weights are kept
     int64_t raw_ld;
     int units;             // at most: `part` has room for no more
 };
@@ -525,7 +525,11 @@ __device__ __forceinline__ void fp4_narrow(const Fp4PagedArgs& p, const Fp4Share
 #pragma unroll
                     for (int t = 0; t < 2; ++t) {
                         const int at = key0 - sq.base() + 16 * t + 4 * j4;
-                        const f32x4v y = {w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]};
+                        f32x4v y = {w[4 * t], w[4 * t + 1], w[4 * t + 2], w[4 * t + 3]};
+                        if (cut) {  // keys without a page are marked: a denominator that is not a number is not theirs
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) y[r] = (seen >> (4 * t + r)) & 1 ? y[r] : -1.f;
+                        }
                         if (at < p.raw_ld)  // raw_ld: a multiple of 32
                             *reinterpret_cast<f32x4v*>(p.raw + ((int64_t)b * p.H + head[i]) * p.raw_ld + at) = y;
                     }
@@ -660,6 +664,10 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
             return p.raw[((int64_t)b * p.H + hk * p.G + g) * p.raw_ld + (j - sq.base())];
         };
         auto seen = [&](int j) __attribute__((always_inline)) { return j >= sq.first && j < end; };
+        auto add = [&](float& sum, float w, float inverse) __attribute__((always_inline)) {
+            const float y = fmaf(w, inverse, sum);
+            sum = w < 0.f ? sum : y;  // no page
+        };
         // On their way before the denominators are known (16 caches of 52 thousand
         // keys, 4 key heads D64, 4 heads each: 22.4 us, after them 23.3).
         constexpr int kFirst = 4;
@@ -685,17 +693,17 @@ __global__ __launch_bounds__(256) void born_fp4_join_kernel(Fp4PagedArgs p, Fp4J
                     if (g0 == 0) {
 #pragma unroll
                         for (int i = 0; i < kFirst; ++i)
-                            if (i < gn) sum = fmaf(first[i], zred[i], sum);
+                            if (i < gn) add(sum, first[i], zred[i]);
                     }
 #pragma unroll 4
-                    for (int i = g0 == 0 ? kFirst : 0; i < gn; ++i) sum = fmaf(raw(g0 + i, start + threadIdx.x), zred[i], sum);
+                    for (int i = g0 == 0 ? kFirst : 0; i < gn; ++i) add(sum, raw(g0 + i, start + threadIdx.x), zred[i]);
                 }
             } else {
                 for (int j = start + threadIdx.x; j < end; j += q.weigh * 256) {
                     if (!seen(j)) continue;
                     float more = 0.f;
 #pragma unroll 4
-                    for (int i = 0; i < gn; ++i) more = fmaf(raw(g0 + i, j), zred[i], more);
+                    for (int i = 0; i < gn; ++i) add(more, raw(g0 + i, j), zred[i]);
                     weight[j] += more;
                 }
             }

@@ -136,3 +136,27 @@ def test_weights_of_some_of_the_keys(cuda_device, window, kept):
         m = min(kept, y.shape[2])
         assert ref.worst(room[..., :m], (y[..., :m] + 0.25, e[..., :m] + 2.0 ** -24 * (y[..., :m] + 0.25))) <= 1.0
         assert (room[..., m:] == 0.25).all()
+
+
+def test_keys_that_are_not_seen_keep_their_weights(cuda_device):
+    """A row that is not a number makes NaN of the weights that it sees, of no other."""
+    for dt in DT.values():
+        for page, window in ((16, 0), (16, 30), (5, 0), (5, 30)):
+            cache, table, n, _ = ref.make_cache([90, 60], page, 2, 64, seed=51)
+            table[0, 40 // page] = -1
+            table[0, 70 // page] = cache[0].shape[0] + 2
+            t, r = int(table[0, 85 // page]), 85 % page
+            cache[2][t, r, 1, 0] = 255
+            q = _queries(2, 4, 64, dt, 52)
+            q[1, 0, 7] = math.nan
+            weight = torch.full((2, 2, 120), 0.5, device=cuda_device)
+            flash_born_attention_paged_fp4(q.to(cuda_device), tuple(x.to(cuda_device) for x in cache), table.to(cuda_device), n.to(cuda_device),
+                                           1.0, window_size=window, key_weight=weight)
+            j = torch.arange(120)
+            for b, h in ((0, 1), (1, 0)):  # the bad key's head, the bad query's
+                m = int(n[b])
+                at = torch.div(j, page, rounding_mode="floor").clamp(max=table.shape[1] - 1)
+                seen = (j < m) & (j >= (m - window if window else 0)) & (table[b][at] >= 0) & (table[b][at] < cache[0].shape[0])
+                assert torch.equal(weight[b, h].cpu().isnan(), seen)
+                assert (weight[b, h].cpu()[~seen] == 0.5).all()
+            assert weight[0, 0].isfinite().all() and weight[1, 1].isfinite().all()
