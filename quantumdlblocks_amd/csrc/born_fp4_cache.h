@@ -267,9 +267,16 @@ __device__ __forceinline__ void fp4_append_rows(const Fp4AppendArgs& p, bool val
             }
             if (c0 >= p.D) ss = 0.0;
             for (int o = 1; o < p.lpw; o <<= 1) ss += __shfl_xor(ss, o);
-            const double f = 1.0 / sqrt(ss + p.eps);
+            // Quotients rounded once, as ties between codes have it: the product with
+            // the reciprocal, and what it leaves of y, again, if anything (a zero keeps
+            // its sign).  Denominators of 0, an infinity or NaN take the product alone.
+            const double den = sqrt(ss + p.eps), f = 1.0 / den;
+            const bool exact = f > 0.0 && f < HUGE_VAL;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) y[e] = c0 < p.D ? y[e] * f : 0.0;  // the padding of the last block, whatever the row
+            for (int e = 0; e < 8; ++e) {
+                const double g = y[e] * f, left = fma(-g, den, y[e]);
+                y[e] = c0 >= p.D ? 0.0 : exact && left != 0.0 ? fma(left, f, g) : g;  // zeros: the padding of the last block, whatever the row
+            }
             fp4_store_row(y, to + (uint64_t)(h + i) * th, scale + (uint64_t)(h + i) * sh, lane, in);
         }
     }

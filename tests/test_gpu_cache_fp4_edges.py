@@ -160,3 +160,34 @@ def test_keys_that_are_not_seen_keep_their_weights(cuda_device):
                 assert torch.equal(weight[b, h].cpu().isnan(), seen)
                 assert (weight[b, h].cpu()[~seen] == 0.5).all()
             assert weight[0, 0].isfinite().all() and weight[1, 1].isfinite().all()
+
+
+# ---------------------------------------------------------------------------
+# Ties
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", ["fp16", "fp32"])
+def test_keys_that_lie_halfway_between_two_codes(cuda_device, dtype):
+    """Keys of a whole norm whose normalised values are exact: a code that is one
+    of two as near, or the block's exponent, goes by the quotient's last bit."""
+    rows = []
+    for norm in (49, 75, 77, 91, 93, 99, 103, 105, 107, 117):
+        for t in (7, 6, 5, 3):  # eighths of the norm: 7 / 8 is the largest value of its exponent
+            rest = (8 * norm) ** 2 - (t * norm) ** 2
+            parts = []
+            for _ in range(5):  # sums of squares, the largest first
+                parts.append(math.isqrt(rest))
+                rest -= parts[-1] ** 2
+            if rest == 0 and max(parts) < t * norm:
+                rows.append([t * norm / 8] + [x / 8 for x in parts] + [0.0, -0.0] + [0.0] * 8)
+    k = torch.tensor(rows, dtype=torch.float64).to(DT[dtype]).view(-1, 1, 16)
+    assert len(rows) > 10 and torch.equal(k.double().flatten().cpu(), torch.tensor(rows, dtype=torch.float64).flatten())
+    N = k.shape[0]
+    table, n = torch.arange(N, **INT).view(-1, 1), torch.ones(N, **INT)
+    got = born_cache_fp4(N, 1, 1, 16, device=cuda_device)
+    fused_qk_rope_l2_normalize_append_fp4(*(k.to(cuda_device) for _ in range(3)), None, None, got, table.to(cuda_device), n.to(cuda_device), eps=0.0)
+    for i, row in enumerate(rows):
+        norm = math.sqrt(sum(x * x for x in row))
+        assert norm == int(norm)
+        e, codes = ref.store_block([x / norm for x in row] + [0.0] * 16)
+        c = got.k[i, 0, 0].tolist()
+        assert int(got.k_scale[i, 0, 0, 0]) == e and [c[j // 2] >> 4 * (j % 2) & 15 for j in range(32)] == codes
