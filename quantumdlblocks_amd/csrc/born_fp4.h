@@ -88,6 +88,20 @@ constexpr int kQParts = std::is_same<E, F32>::value ? 3 : std::is_same<E, F16>::
 template <class E>
 constexpr int kPParts = std::is_same<E, F32>::value ? 3 : 2;
 
+// The same of values that bf16 may round to an infinity: its largest number first
+// where they are finite, and nothing behind an infinity.
+template <int PARTS>
+__device__ __forceinline__ void fp4_large_parts(float x, float y, uint32_t (&u)[PARTS]) {
+    auto first = [](float z) __attribute__((always_inline)) {
+        return fabsf(z) >= 0x1.FFp127f && fabsf(z) < HUGE_VALF ? copysignf(0x1.FEp127f, z) : z;
+    };
+    u[0] = BF16::pack(first(x), first(y));
+    uint32_t rest[PARTS - 1];
+    fp4_parts<PARTS - 1>(fabsf(x) == HUGE_VALF ? 0.f : x - BF16::lo(u[0]), fabsf(y) == HUGE_VALF ? 0.f : y - BF16::hi(u[0]), rest);
+#pragma unroll
+    for (int i = 1; i < PARTS; ++i) u[i] = rest[i - 1];
+}
+
 // Eight values of a query from column `at` on (D - at of them, 0 behind), as operands.
 template <class E>
 __device__ __forceinline__ void fp4_query(const uint8_t* row, int at, int D, bool ok, bool neg, u32x4 (&q)[kQParts<E>]) {
@@ -95,31 +109,46 @@ __device__ __forceinline__ void fp4_query(const uint8_t* row, int at, int D, boo
         u32x4 y = {0u, 0u, 0u, 0u};
         if (ok && at < D) y = ldg16(row + 2 * at) ^ (neg ? 0x80008000u : 0u);
         q[0] = y;
-        return;
-    }
-    float x[8];
+    } else {
+        float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = 0.f;
-    if (ok && at < D) {  // D: a multiple of 8
-        if constexpr (std::is_same<E, F32>::value) {
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        if (ok && at < D) {  // D: a multiple of 8
+            if constexpr (std::is_same<E, F32>::value) {
 #pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                const u32x4 y = ldg16(row + 4 * at + 16 * h);
+                for (int h = 0; h < 2; ++h) {
+                    const u32x4 y = ldg16(row + 4 * at + 16 * h);
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[4 * h + i] = __uint_as_float(y[i]);
+                    for (int i = 0; i < 4; ++i) x[4 * h + i] = __uint_as_float(y[i]);
+                }
+            } else {
+                const u32x4 y = ldg16(row + 2 * at);
+#pragma unroll
+                for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(y[i]), x[2 * i + 1] = E::hi(y[i]);
             }
-        } else {
-            const u32x4 y = ldg16(row + 2 * at);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) x[2 * i] = E::lo(y[i]), x[2 * i + 1] = E::hi(y[i]);
         }
-    }
+        float top = 0.f;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        uint32_t u[kQParts<E>];
-        fp4_parts<kQParts<E>>(neg ? -x[2 * i] : x[2 * i], neg ? -x[2 * i + 1] : x[2 * i + 1], u);
+        for (int i = 0; i < 8; ++i) {
+            x[i] = neg ? -x[i] : x[i];
+            top = fmaxf(top, fabsf(x[i]));
+        }
+        const bool large = top >= 0x1.FFp127f;
 #pragma unroll
-        for (int k = 0; k < kQParts<E>; ++k) q[k][i] = u[k];
+        for (int i = 0; i < 4; ++i) {
+            uint32_t u[kQParts<E>];
+            fp4_parts<kQParts<E>>(x[2 * i], x[2 * i + 1], u);
+#pragma unroll
+            for (int k = 0; k < kQParts<E>; ++k) q[k][i] = u[k];
+        }
+        if (!large) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            uint32_t u[kQParts<E>];
+            fp4_large_parts<kQParts<E>>(x[2 * i], x[2 * i + 1], u);
+#pragma unroll
+            for (int k = 0; k < kQParts<E>; ++k) q[k][i] = u[k];
+        }
     }
 }
 

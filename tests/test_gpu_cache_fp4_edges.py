@@ -191,3 +191,57 @@ def test_keys_that_lie_halfway_between_two_codes(cuda_device, dtype):
         e, codes = ref.store_block([x / norm for x in row] + [0.0] * 16)
         c = got.k[i, 0, 0].tolist()
         assert int(got.k_scale[i, 0, 0, 0]) == e and [c[j // 2] >> 4 * (j % 2) & 15 for j in range(32)] == codes
+
+
+# ---------------------------------------------------------------------------
+# Queries that are infinite, or nearly so
+# ---------------------------------------------------------------------------
+@pytest.mark.parametrize("dtype", list(DT))
+@pytest.mark.parametrize("D", [64, 128, 256])
+@pytest.mark.parametrize("new", [[9, 3, 5], [200, 3, 100]])
+def test_infinite_queries_follow_the_formula(cuda_device, dtype, D, new):
+    """An overlap with an infinity is infinite, its weight too or, where it is
+    negative, none; with a value of 0 it is not a number."""
+    cache, table, n, _ = ref.make_cache([210, 40, 150], 16, 2, D, seed=53)
+    kc = cache[0]
+    # Column 4 of every key: of one sign, but for head 1's, where some are zeros.
+    byte = kc[..., 2]
+    byte[...] = (byte & 0xF0) | 0x0A
+    byte[1::3, :, 1] &= 0xF0
+    cu = serve_ref.starts(new)
+    G, dt = 4, DT[dtype]
+    for bad, scale in ((math.inf, 1.0), (-math.inf, 1.0), (math.inf, -1.0), (-math.inf, -2.0)):
+        q = _queries(cu[-1], 2 * G, D, dt, 54)
+        at = [(cu[b] + i, h) for b in range(3) for i, h in ((0, 1), (new[b] - 1, 6), (new[b] // 2, 0))]
+        for i, h in at:
+            q[i, h, 4] = bad
+        out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device),
+                                             n.to(cuda_device), scale, torch.tensor(cu, device=cuda_device, **INT)).cpu()
+        for i, h in at:
+            b = max(x for x in range(3) if cu[x] <= i)
+            m = int(n[b]) - cu[b + 1] + i + 1  # the keys that this token sees
+            k, v, _, _ = _rows(cache, table[b], m, D)
+            r = scale * (q[i, h].double() * k[:, h // G]).sum(-1)
+            p = torch.where(r < 0, torch.zeros_like(r), r * r)
+            want = ((p / (p.sum() + 1e-12)).unsqueeze(-1) * v[:, h // G]).sum(0)
+            assert want.isnan().all() or not want.any()
+            assert torch.equal(out[i, h].isnan(), want.isnan()) and not out[i, h].nan_to_num().any()
+        fine = torch.ones(cu[-1], 2 * G, dtype=torch.bool)
+        for i, h in at:
+            fine[i, h] = False
+        assert out[fine].isfinite().all()
+
+
+def test_queries_as_large_as_they_get(cuda_device):
+    """Past bf16's largest, over keys so small that the overlaps are ordinary."""
+    for new in ([1, 1], [40, 70]):
+        cache, table, n, _ = ref.make_cache([100, 80], 16, 2, 64, seed=55)
+        cache[2].fill_(127 - 120)
+        cu = serve_ref.starts(new)
+        q = _queries(cu[-1], 8, 64, torch.float32, 56)
+        big = torch.finfo(torch.float32).max
+        q = q / q.abs().amax(-1, keepdim=True) * big
+        q[:, :, 3], q[:, :, 5] = big, -big * (1 - 2.0 ** -20)
+        out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device), n.to(cuda_device),
+                                             1.0, torch.tensor(cu, device=cuda_device, **INT))
+        assert ref.worst(out, ref.attend(q, cache, table, n, 1.0, cu)[0]) <= 1.0
