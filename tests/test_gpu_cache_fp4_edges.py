@@ -99,6 +99,28 @@ def test_sequences_of_several_column_blocks_each(cuda_device, weigh):
         assert ref.worst(weight[some.to(cuda_device)], (w[0], w[1] + 2.0 ** -24 * w[0])) <= 1.0
 
 
+def test_many_long_sequences_share_the_keys(cuda_device):
+    """More than two rounds of 64 sequences, with keys enough to be split."""
+    g = torch.Generator().manual_seed(43)
+    lens = [int(x) for x in torch.randint(150, 900, (200,), generator=g)]
+    lens[7], lens[70], lens[199] = 6000, 0, 5000
+    some = [int(x) for x in torch.randint(0, 6, (200,), generator=g)]
+    wide = [90 if i in (3, 68, 199) else x for i, x in enumerate(some)]
+    cache, table, n, _ = ref.make_cache(lens, 16, 1, 64, seed=43)
+    dev = tuple(t.to(cuda_device) for t in cache)
+    for new, window in ((None, 0), (None, 300), (some, 0), (wide, 0), (wide, 100)):
+        cu = list(range(201)) if new is None else serve_ref.starts(new)
+        q = _queries(cu[-1], 2, 64, torch.bfloat16, 44)
+        weight = torch.zeros(200, 1, 6000, device=cuda_device) if new is None else None
+        out = flash_born_attention_paged_fp4(q.to(cuda_device), dev, table.to(cuda_device), n.to(cuda_device), 2.0,
+                                             None if new is None else torch.tensor(cu, device=cuda_device, **INT), 1e-12, window, weight)
+        o, w = ref.attend(q, cache, table, n, 2.0, None if new is None else cu, 1e-12, window)
+        assert ref.worst(out, o) <= 1.0
+        if new is None:
+            y, e = (t[..., :6000] for t in w)
+            assert ref.worst(weight, (y, e + 2.0 ** -24 * y)) <= 1.0
+
+
 # ---------------------------------------------------------------------------
 # The keys' weights
 # ---------------------------------------------------------------------------
@@ -245,3 +267,61 @@ def test_queries_as_large_as_they_get(cuda_device):
         out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(t.to(cuda_device) for t in cache), table.to(cuda_device), n.to(cuda_device),
                                              1.0, torch.tensor(cu, device=cuda_device, **INT))
         assert ref.worst(out, ref.attend(q, cache, table, n, 1.0, cu)[0]) <= 1.0
+
+
+# ---------------------------------------------------------------------------
+# Memory behind the tensors
+# ---------------------------------------------------------------------------
+def _guarded(dev, size):
+    """size bytes with a pattern on both sides, and what is left of the pattern."""
+    pad = 1 << 16
+    room = torch.full((pad + size + pad,), 0xA5, dtype=torch.uint8, device=dev)
+    return room[pad : pad + size], lambda: bool((room[:pad] == 0xA5).all() and (room[pad + size :] == 0xA5).all())
+
+
+def _attend_guarded(q, cache, table, n, cu, window=0, weight=None):
+    """The library's call with guards about its output and its workspace."""
+    N, H, D = q.shape
+    B, pages = table.shape
+    page, Hkv = cache[0].shape[1:3]
+    fields = born_fp4._check_fp4(cache, table, n, B, D, written=False)
+    size = born_fp4._paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, 0 if weight is None else weight.shape[2])
+    size = -(-size // 4) * 4
+    out, out_ok = _guarded(q.device, q.numel() * q.element_size())
+    ws, ws_ok = _guarded(q.device, size)
+    w = (0, 0, 0, 0) if weight is None else (weight.data_ptr(), weight.stride(0), weight.stride(1), weight.shape[2])
+    block = _native.fp4_paged_call(born_fp4._DTYPE_CODE[q.dtype], N, B, H, Hkv, D, q.data_ptr(), q.stride(0), q.stride(1), out.data_ptr(),
+                                   *fields, table.data_ptr(), pages, table.stride(0), n.data_ptr(), 0 if cu is None else cu.data_ptr(), 0, 1, 1.0,
+                                   window, 1e-12, *w, ws.data_ptr(), size)
+    assert _native.load().qdl_flash_born_fp4_paged_forward_call(block, torch.cuda.current_stream().cuda_stream) == 0
+    torch.cuda.synchronize()
+    assert out_ok() and ws_ok()
+    return out.view(q.dtype).view(N, H, D)
+
+
+@pytest.mark.parametrize("B,room,N,H", [(100, 2000, 64, 16), (100, 100, 64, 16), (1100, 400, 96, 8), (6, 4000, 600, 8), (6, 100, 600, 8),
+                                        (80, 3000, 700, 4), (3, 5000, 40, 4)])
+def test_starts_of_any_order_write_nothing_else(cuda_device, B, room, N, H):
+    cache, table, n, _ = ref.make_cache([room, room - 90], 16, 2, 64, seed=57, device=cuda_device)
+    table, n = table.repeat(-(-B // 2), 1)[:B].contiguous(), n.repeat(-(-B // 2))[:B].contiguous()
+    q = _queries(N, H, 64, torch.bfloat16, 58).to(cuda_device)
+    even = torch.tensor([i * N // B for i in range(B + 1)], device=cuda_device, **INT)
+    for window in (0, 70):
+        want = _attend_guarded(q, cache, table, n, even, window)
+        assert torch.equal(want, flash_born_attention_paged_fp4(q, cache, table, n, 1.0, even, window_size=window))
+        for starts in (([0, N] * B)[:B] + [N], [0] + [N - i % 7 * 5 for i in range(B)], [N] * B + [0], ([-5, N + 9] * B)[:B] + [N],
+                       [0] + [N // 2] * (B - 1) + [N // 3], [0, N] + [N // 3] * (B - 1)):
+            _attend_guarded(q, cache, table, n, torch.tensor(starts, device=cuda_device, **INT), window)
+        assert torch.equal(_attend_guarded(q, cache, table, n, even, window), want)
+
+
+@pytest.mark.parametrize("lens,H,page", [([3000, 1, 700], 4, 16), ([3000, 1, 700], 40, 16), ([100] * 80, 2, 7), ([60000], 4, 64)])
+def test_one_token_writes_nothing_else(cuda_device, lens, H, page):
+    cache, table, n, _ = ref.make_cache(lens, page, 2, 64, seed=59, device=cuda_device)
+    q = _queries(len(lens), H, 64, torch.float16, 60).to(cuda_device)
+    for window in (0, 1, 333):
+        for keys in (0, 1, 50, max(lens)):
+            room, ok = _guarded(cuda_device, len(lens) * 2 * keys * 4)
+            weight = room.view(torch.float32).view(len(lens), 2, keys) if keys else None
+            _attend_guarded(q, cache, table, n, None, window, weight)
+            assert ok()
