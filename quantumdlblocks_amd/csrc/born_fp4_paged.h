@@ -187,7 +187,7 @@ __device__ __forceinline__ Fp4Part fp4_unit(const Fp4PagedArgs& p, const Fp4Shar
 __device__ __forceinline__ float fp4_inverse(const Fp4PagedArgs& p, int h, float z) {
     const float s = arg_scale(p, h), den = z + (p.eps == 0.f ? 0.f : p.eps / (s * s));
     // A denominator that is not a number stays one.
-    return s != 0.f ? (den < 0x1p-126f ? 0.f : 1.0f / den) : 0.f;
+    return s != 0.f ? (den < 0x1p-126f ? 0.f : 1.0f / den) : z == z ? 0.f : z;
 }
 
 // Rows behind the last sequence: zeros, shared out over `blocks` workgroups.

@@ -184,6 +184,18 @@ def test_keys_that_are_not_seen_keep_their_weights(cuda_device):
             assert weight[0, 0].isfinite().all() and weight[1, 1].isfinite().all()
 
 
+def test_weights_of_heads_without_a_scale(cuda_device):
+    """0 times a key that is not a number is none either, for all that the row sees."""
+    cache, table, n, _ = ref.make_cache([90, 60], 16, 2, 64, seed=61)
+    cache[3][int(table[0, 2]), 7, 1, 1] = 255
+    q = _queries(2, 4, 64, torch.bfloat16, 62)
+    weight = torch.full((2, 2, 90), 0.5, device=cuda_device)
+    out = flash_born_attention_paged_fp4(q.to(cuda_device), tuple(x.to(cuda_device) for x in cache), table.to(cuda_device), n.to(cuda_device),
+                                         0.0, key_weight=weight)
+    assert out[0, 2:].isnan().all() and not out[0, :2].any() and not out[1].any()
+    assert weight[0, 1].isnan().all() and (weight[0, 0] == 0.5).all() and (weight[1] == 0.5).all()
+
+
 # ---------------------------------------------------------------------------
 # Ties
 # ---------------------------------------------------------------------------
