@@ -21,12 +21,15 @@
 // sequence takes as many chunks as it needs.  Partial sums are joined in order.
 //
 // 32 single tokens over long caches (267 MB, 8 key heads D128, 4 heads each, bf16):
-// 65 us, 4.1 TB/s, and a join of 5: K's and V's conversions, some 340 vector and
-// 230 scalar instructions for a wave's 32 keys, take 42% of the cycles beside the
-// loads, which are two steps ahead.  16 sequences of 5 tokens over 51 thousand keys
-// (4 key heads) 20 us and 5 where the bytes take 6; one token over 1531 keys 7 and
-// 4: chains of loads, the lengths, the table's entry, the codes, the partial sums,
-// a microsecond each.  Read without a page's base in scalars, 92 us for 73.
+// 65 us, 4.1 TB/s, and a join of 5: K's and V's conversions make most of some 195
+// vector instructions for a wave's 32 keys, beside 24 matrix and 140 scalar ones,
+// and the vector instructions take half of the SIMDs' cycles beside the loads, which
+// are two steps ahead.  16 sequences of 5 tokens over 51 thousand keys (4 key heads)
+// 20 us and 6 where the bytes take 6: with two column sets the loads' descriptors do
+// not fit the scalar registers, and each 32 keys read some 60 back; one token over
+// 1531 keys 7 and 4: chains of loads, the lengths, the table's entry, the codes, the
+// partial sums, a microsecond each.  Read without a page's base in scalars, 92 us
+// for 73.
 #pragma once
 
 #include "born_fp4.h"
@@ -208,8 +211,9 @@ struct Fp4Cfg {
     static constexpr int VC = DP / 16, VD = (VC + 7) / 8;  // columns of a lane's key, dwords of codes
 };
 
-// Waves a SIMD that the registers of a column set and of its queries' parts leave
-// without spills.
+// Waves a SIMD that the kernel's registers are held to.  One column set keeps all of
+// them, and so does bf16; with two at D256 fp16 spills some 55 vector registers and
+// fp32 some 145, in the loop.
 template <class E>
 constexpr int fp4_wpe(int DP, int NC) {
     return DP == 256 ? 1 : NC == 2 ? (kQParts<E> < 3 || DP == 64 ? 2 : 1) : kQParts<E> == 1 || DP == 64 ? 3 : 2;

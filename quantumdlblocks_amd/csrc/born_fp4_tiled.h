@@ -15,7 +15,8 @@
 // has 1200.  The weights' two parts make three products of the formula's two: with
 // one part it was 250 us, but a row was off by 2.3e-3 in norm where the narrow
 // kernel's are by 1.7e-3, so that its precision hung on what else was in the batch.
-// Two workgroups a compute unit is what 256 registers leave, and with one column
+// The matrix pipe is busy in 50% of the cycles, vector instructions issue in 55:
+// two workgroups a compute unit is what 256 registers leave, and with one column
 // block of 32 rows a wave each operand of K from LDS feeds one product.  A higher
 // priority around the overlaps' products: 328 us for 332.
 //
@@ -32,12 +33,14 @@ struct Fp4TileCfg {
     static constexpr int BN = DP == 256 ? 32 : 64, SUB = BN / 32, NB = DP / 32;
     static constexpr int BYTES = BN * DP * 2, STAGE = 2 * BYTES;
     static constexpr int UNITS = BN * NB / 256;  // blocks of K (and of V) of a thread; 0: K or V
+    // Waves a SIMD.  fp32 at D128 spills some 65 vector registers, 115 with the narrow
+    // part, fp16 up to 5; at D256 the narrow part makes fp16 spill some 55, fp32 150.
     static constexpr int WPE = DP == 256 ? 1 : 2;
 };
 
 // Block x of rows: part i of a sequence's.  With a lane for each sequence those
 // of the longest come first, so that a launch ends with short ones (the 8 second
-// turns 264 us, in the sequences' order 327).
+// turns, with one part of the weights, 264 us, in the sequences' order 327).
 __device__ __forceinline__ Fp4Part fp4_block(const Fp4PagedArgs& p, const Fp4Share& share, int x) {
     if (p.items > 0 && p.B <= 64) {
         const int k = share.lane() < p.B ? share.mine.blocks(p) : 0;

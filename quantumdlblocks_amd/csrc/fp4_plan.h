@@ -24,14 +24,15 @@ constexpr int kFp4Narrow = 32;
 constexpr int kFp4AllNarrow = 512;
 constexpr int64_t kFp4AllWork = (int64_t)1 << 24;
 // Workgroups of the narrow kernel that a launch's chunks of keys are made for: two
-// rounds of as many as a compute unit holds, three with one column set, two with two.
-// us with 512, 768, 1024, 1536, 2048: 32 single tokens over long caches 76, 72, 74,
+// rounds of as many as a compute unit holds of bf16 at D128, three with one column
+// set, two with two (one column set of fp16 or fp32 there: two).  us with 512, 768, 1024, 1536, 2048: 32 single tokens over long caches 76, 72, 74,
 // 65, 67; 16 sequences of 5 tokens (two column sets, before chunks of few keys were
 // made fewer) 49, 51, 50, 55, 59.
 constexpr int fp4_wanted(int nc) { return nc == 1 ? 1536 : 1024; }
-// Narrow and wide sequences have a launch each where the keys times key heads are
-// this many and the sequences' rows in the mean fit a narrow workgroup: most are
-// narrow then, and their own launch has three workgroups a compute unit for two.
+// Narrow and wide sequences have a launch each where the keys that the tables have
+// room for (the host knows no lengths), times key heads, are this many and the
+// sequences' rows in the mean fit a narrow workgroup: most are narrow then, and
+// their own launch has three workgroups a compute unit for two.
 // us apart and together, 8 key heads D128, 4 heads each: 64 sequences of 4 tokens
 // over 8192 keys at most 67 and 104; where a few are wide it costs, 31 single
 // tokens beside one of 200 94 and 86, of 512 (mean 68: together) 158 and 127.
@@ -41,7 +42,11 @@ constexpr int64_t kFp4Apart = (int64_t)1 << 20;
 // 2^14 and any number of them: 64 sequences of 1000 keys, 8 key heads, 32 heads,
 // tables of 131072 keys 37, 44, 191; of 16000 keys, tables of 16384, 325, 344, 351.
 constexpr int64_t kFp4Weigh = (int64_t)1 << 12;
-// Sequences that a workgroup looks through to share out the keys.
+// Sequences that a workgroup looks through to share out the keys, which takes every
+// wave two reads of all lengths.  us so and with a chunk a sequence, one token each,
+// 16 heads over 4: 512 sequences of 1000 keys 81 and 48, of 16 to 4000 77 and 63, of
+// 200 and one of 50000 93 and 474; 1024 of them 185 and 89, 183 and 110, 152 and
+// 474; 2048 469 and 171, 460 and 188, 370 and 474.
 constexpr int kFp4Shared = 1024;
 
 // The first key that any of a sequence's nq new tokens sees, of n keys.

@@ -446,21 +446,25 @@ def flash_born_attention_paged_fp4(
 
     ``q`` (N, H, D), H a multiple of the cache's Hkv: one new token per sequence
     (N == B), or several, packed, with ``cu_seqlens`` (B + 1,) the starts of the
-    sequences among them (the first is 0).  Their keys are in the cache already
-    and ``cache_lens`` counts them: a sequence's i-th token of m stands at
-    ``cache_lens - m + i`` and sees the keys up to there, or the last
-    ``window_size`` of them, counted in slots.  The formula, over the stored values:
+    sequences among them (the first is 0), 65536 sequences at most.  Their keys
+    are in the cache already and ``cache_lens`` counts them: a sequence's i-th
+    token of m stands at ``cache_lens - m + i`` and sees the keys up to there, or
+    the last ``window_size`` of them, counted in slots.  The formula, over the
+    stored values:
 
         p_ij = max(0, scale_h q_i . k_j) ** 2,  out_i = sum_j p_ij v_j / (sum_j p_ij + eps)
 
     ``scale``: a float or a tensor of 1 or H values.  ``key_weight`` (B, Hkv, L)
     fp32, only without ``cu_seqlens``: each visible key's weight p_j / (sum p +
     eps), summed over the heads that read it, is added in place at j < L: what
-    ``born_cache_evict_fp4`` goes by; the call's workspace holds B H fp32 values for
-    each of these L keys, or of the table's where it has fewer.  Lengths past the table's pages are cut to
-    them first.  Tokens that see no key get zeros, so do tokens of no sequence,
-    and heads whose (sum p + eps) / scale_h ** 2 lies below fp32's normal range,
-    2^-126; a key that is not a number makes NaN of the rows that see it.
+    ``born_cache_evict_fp4`` goes by; the call's workspace holds B H fp32 values
+    for each of these L keys, or of the table's where it has fewer.  Lengths past
+    the table's pages are cut to them first.  Tokens that see no key get zeros, so
+    do tokens of no sequence, and heads whose (sum p + eps) / scale_h ** 2 lies
+    below fp32's normal range, 2^-126; overlaps q_i . k_j from 2^64 on, whose
+    squares lie past it, are infinite whatever the scale.  A row's precision does
+    not go by the others in the batch.  A key that is not a number makes NaN of
+    the rows that see it.
     """
     if torch.compiler.is_compiling():  # one graph break, as the other operators
         return _call_uncompiled(flash_born_attention_paged_fp4, (q, cache, block_table, cache_lens, scale, cu_seqlens, eps,
@@ -520,7 +524,7 @@ def flash_born_attention_paged_fp4(
     (table, ld), lens = _table(block_table), _index(cache_lens)
     cu = None if cu_seqlens is None else _index(cu_seqlens)
     pages = table.shape[1]
-    size = _paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, w_len if w_ptr else 0)
+    size = _paged_workspace(N, B, H, Hkv, D, pages, page, window, cu is not None, max(w_len, 2) if w_ptr else 0)
     ws = lens.new_empty((size + 3) // 4)
     _run_call(lib.qdl_flash_born_fp4_paged_forward_call, "qdl_flash_born_fp4_paged_forward_call", dev, _native.fp4_paged_call(
         _DTYPE_CODE[dt], N, B, H, Hkv, D, q_c.data_ptr(), st, sh, out.data_ptr(), *fields, table.data_ptr(), pages, ld,

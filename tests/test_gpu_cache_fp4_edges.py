@@ -124,7 +124,8 @@ def test_many_long_sequences_share_the_keys(cuda_device):
 # ---------------------------------------------------------------------------
 # The keys' weights
 # ---------------------------------------------------------------------------
-def test_weights_of_few_keys_over_wide_tables(cuda_device):
+@pytest.mark.parametrize("dtype", list(DT))
+def test_weights_of_few_keys_over_wide_tables(cuda_device, dtype):
     """Tables of 2^20 keys a sequence for 520 sequences of 8 key heads: neither the
     launch nor its workspace goes by them where the weights kept are few."""
     B, Hkv = 520, 8
@@ -132,7 +133,7 @@ def test_weights_of_few_keys_over_wide_tables(cuda_device):
     cache, table, n, _ = ref.make_cache(lens, 256, Hkv, 32, seed=47)
     wide = torch.full((B, 4096), -1, **INT)
     wide[:, : table.shape[1]] = table
-    q = _queries(B, Hkv, 32, torch.bfloat16, 48)
+    q = _queries(B, Hkv, 32, DT[dtype], 48)
     weight = torch.full((B, Hkv, 280), 0.25, device=cuda_device)
     torch.cuda.reset_peak_memory_stats()
     before = torch.cuda.memory_allocated()
