@@ -21,6 +21,8 @@ constexpr int kFp4Narrow = 32;
 // 40, over 30000 of one (2^23.9) 48 and 42, over 8000 of 8 (2^25) 60 and 50, over
 // 30000 of 8 161 and 105; 128 over 30000 of 8 (2^24.9) 58 and 52.  What it is for:
 // 16 sequences of 5 tokens, 4 heads over 4 key heads, 27 and 30, of 8 27 and 34.
+// Beyond 512 rows it is even: one sequence of 1024 rows over 1500 keys of 8 heads 45
+// and 41, 32 of 8 tokens over 1000 keys of 8 heads 30 and 36.
 constexpr int kFp4AllNarrow = 512;
 constexpr int64_t kFp4AllWork = (int64_t)1 << 24;
 // Workgroups of the narrow kernel that a launch's chunks of keys are made for: two
